@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from ctypes import byref  # noqa: F401
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgqk.so")
 
@@ -20,14 +21,17 @@ GQK_FORM_GEMV = 1
 GQK_FORM_GEMM = 2
 GQK_CTR_BYTES = 262144            # the arrival-counter region at the start of every workspace
 GQK_NOALLOC_SCRATCH_BYTES = GQK_CTR_BYTES + (32 << 20)   # gqk_linear_noalloc's per-GPU device array
-GQK_DTYPE_F32, GQK_DTYPE_BF16, GQK_DTYPE_F16 = 0, 1, 2
+GQK_DTYPE_F32, GQK_DTYPE_BF16, GQK_DTYPE_F16, GQK_DTYPE_FP8 = 0, 1, 2, 3
+GQK_ROPE_UNIT_OFFSET, GQK_ROPE_INTERLEAVED = 1, 2
 
 # every entry point include/gguf_hip.h declares
 EXPORTS = ("gqk_last_error", "gqk_version", "gqk_type_info", "gqk_dequantize", "gqk_dequantize_tiles",
            "gqk_tiles_bytes", "gqk_repack", "gqk_unrepack", "gqk_plan", "gqk_linear_workspace_bytes",
            "gqk_gemm_pick", "gqk_workspace_bytes_max", "gqk_linear", "gqk_linear_noalloc", "gqk_ggml_type_size",
            "gqk_gguf_open", "gqk_gguf_close", "gqk_gguf_info", "gqk_gguf_tensor_at", "gqk_gguf_find_tensor",
-           "gqk_gguf_kv_at", "gqk_gguf_find_kv", "gqk_gguf_kv_string", "gqk_gguf_upload_tiles", "gqk_read_floor")
+           "gqk_gguf_kv_at", "gqk_gguf_find_kv", "gqk_gguf_kv_string", "gqk_gguf_upload_tiles", "gqk_read_floor",
+           "gqk_lora_workspace_bytes", "gqk_lora_add", "gqk_qk_norm_rope", "gqk_paged_attention_workspace_bytes",
+           "gqk_paged_attention", "gqk_copy_pages")
 
 
 class GqkShard(ctypes.Structure):
@@ -59,6 +63,18 @@ class GqkGgufKv(ctypes.Structure):
     _fields_ = [("key", ctypes.c_char_p), ("type", ctypes.c_int32), ("array_type", ctypes.c_int32),
                 ("count", ctypes.c_int64), ("i64", ctypes.c_int64), ("f64", ctypes.c_double),
                 ("data", ctypes.c_void_p)]
+
+
+class GqkPages(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_page", ctypes.c_int64), ("k_token", ctypes.c_int64),
+                ("k_head", ctypes.c_int64), ("v_page", ctypes.c_int64), ("v_token", ctypes.c_int64),
+                ("v_head", ctypes.c_int64), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("dtype", ctypes.c_int32), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("dim", ctypes.c_int32)]
+
+
+class GqkHeads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row", ctypes.c_int64), ("head", ctypes.c_int64), ("heads", ctypes.c_int32)]
 
 
 class GqkError(RuntimeError):
@@ -105,6 +121,14 @@ def _load() -> ctypes.CDLL:
         "gqk_gguf_kv_string": (i32, [vp, i64, i64, ctypes.POINTER(ctypes.c_char_p), ctypes.POINTER(ctypes.c_int64)]),
         "gqk_gguf_upload_tiles": (i32, [vp, i64, vp, i64, vp, vp]),
         "gqk_read_floor": (i32, [vp, i64, i32, i32, vp, vp]),
+        "gqk_lora_workspace_bytes": (i64, [i32, i64, i32, i32]),
+        "gqk_lora_add": (i32, [vp, i64, vp, i64, i32, i64, vp, vp, i32, i32, vp, i32, vp, i32, vp, i32, vp, i64, vp, i64, vp]),
+        "gqk_qk_norm_rope": (i32, [vp, vp, vp, i32, i64, i32, vp, i32, vp, i64, i32, vp, vp, i32, ctypes.c_float, i32, vp,
+                                   vp, vp, vp, i32, vp]),
+        "gqk_paged_attention_workspace_bytes": (i64, [i32, i32, i32, i32, i32, i32]),
+        "gqk_paged_attention": (i32, [vp, i64, i64, i32, i32, i32, vp, vp, i64, i32, vp, i32, i32, ctypes.c_float, vp, i64,
+                                      i64, vp, vp, i64, vp]),
+        "gqk_copy_pages": (i32, [vp, i64, i64, i64, i64, i64, vp, vp, i64, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -20,7 +20,8 @@ LIB = os.path.join(PKG, "libgqk.so")
 SOURCES = (("gqk_api.hip", (), "gqk_api.o"), ("gqk_codec.hip", (), "gqk_codec.o"), ("gqk_gemv.hip", (), "gqk_gemv.o"),
            ("gqk_mid.hip", (), "gqk_mid.o"), ("gqk_gemm_plan.hip", (), "gqk_gemm_plan.o"),
            *(("gqk_gemm.hip", (f"-DGQK_GEMM_MB={mb}",), f"gqk_gemm{mb}.o") for mb in (2, 4, 8)),
-           ("gqk_gguf.cpp", (), "gqk_gguf.o"))
+           ("gqk_gguf.cpp", (), "gqk_gguf.o"),
+           *((f"gqk_{n}.hip", (), f"gqk_{n}.o") for n in ("lora", "rope", "attention", "pages")))
 ARCH = os.environ.get("GQK_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -249,6 +249,18 @@ def device_workspace(device: torch.device, need: int = 0) -> torch.Tensor:
     return ws
 
 
+def shared_workspace(device: torch.device) -> torch.Tensor:
+    """The device's shared workspace for a call that was given none; made on the first such call, which a HIP graph
+    capture cannot record."""
+    ws = _WORKSPACES.get(device.index)
+    if ws is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("gguf_hip: the first call on a device makes its workspace (a device allocation), which a "
+                               "HIP graph capture cannot record; prepare a layer or make one eager call before capturing")
+        ws = device_workspace(device)
+    return ws
+
+
 def prepare_grouped_layer(tiles_list: list[torch.Tensor], n_outs: list[int], wtypes: list[int], K: int,
                           target_wgs: int = 0, cus: int = 0) -> GroupedLayer:
     """The loader's step for a run of shards already repacked: one packed buffer (the shards'

@@ -39,6 +39,7 @@ extern "C" {
 #define GQK_DTYPE_F32 0
 #define GQK_DTYPE_BF16 1
 #define GQK_DTYPE_F16 2
+#define GQK_DTYPE_FP8 3 /* OCP e4m3 (pages of a key-value cache) */
 
 /* One shard of a grouped layer: its rows sit at byte `offset` of the packed tile buffer. */
 typedef struct gqk_shard {
@@ -174,6 +175,87 @@ int gqk_linear(const void* packed, const int32_t* desc_dev, const gqk_plan_info*
 #define GQK_NOALLOC_SCRATCH_BYTES (GQK_CTR_BYTES + 33554432)
 int gqk_linear_noalloc(const void* packed, const int32_t* desc_dev, const gqk_plan_info* info, const void* x,
                        int64_t ldx, int M, void* y, int64_t ldy, const void* bias, void* stream);
+
+/* ---- around the linear path: what a decode step does with its outputs ----------------------------
+ * No counterpart in the reference's plugin, which leaves these to the server it is loaded into.
+ * Contents of device arrays are checked where they are read: an index out of its range reads nothing
+ * and makes the token's result NaN (a slot out of range stores nothing). */
+
+/* Low-rank adapters of many requests beside a shared projection, any M rows in one call:
+ *   out[m, n] = y[m, n] + scales[i] * sum_r b[i, n, r] * sum_k a[i, p(n), r, k] * x[m, k],  i = ids[m]
+ * p(n): the part (q, k, v; gate, up) of column n, parts side by side with n_outs[p] columns each.  A row with a
+ * negative id gets y; one with an id >= slots NaN.  y, x, out: bf16 or fp16 (dtype) rows of any stride,
+ * out may be y; a [slots, parts, rank, K] and b [slots, sum(n_outs), rank] of the same type, contiguous, K and
+ * rank multiples of 8, rank <= 256 (adapters of a lower rank are padded with zeros), parts <= 8; ids
+ * int32 [M], or int64 with ids_64; scales fp32 [slots] or NULL (1).  x, a, b are 16-byte aligned.  Products
+ * and sums are in fp32, rounded once to out.  workspace: gqk_lora_workspace_bytes bytes, 256-byte aligned; its
+ * first GQK_CTR_BYTES are left alone, so that a linear layer's workspace serves (calls in stream order). */
+int64_t gqk_lora_workspace_bytes(int M, int64_t K, int parts, int rank);
+int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int M, int64_t K, const void* a,
+                 const void* b, int slots, int parts, const int64_t* n_outs, int rank, const void* ids, int ids_64,
+                 const float* scales, int dtype, void* out, int64_t out_row, void* workspace, int64_t workspace_bytes,
+                 void* stream);
+
+/* The pages of one layer's key-value cache: k and v as [pages, page_size, heads, dim] with any strides
+ * (in elements, multiples of 8; dims side by side), so that a token's heads or a head's tokens may lie together.
+ * dtype: the heads' own type, or GQK_DTYPE_FP8, whose values stand for themselves times k_scale / v_scale
+ * (fp32 [heads] in device memory, NULL: 1).  Pages are aligned to 8 elements. */
+typedef struct gqk_pages {
+  void* k;
+  void* v;
+  int64_t k_page, k_token, k_head;
+  int64_t v_page, v_token, v_head;
+  const float* k_scale;
+  const float* v_scale;
+  int32_t dtype, pages, page_size, heads, dim;
+} gqk_pages;
+
+/* Heads of one token after the other: [tokens, heads, dim] with strides in elements (multiples of 8; data 16-byte
+ * aligned, dims side by side): e.g. a column range of qkv's output. */
+typedef struct gqk_heads {
+  void* data;
+  int64_t row, head;
+  int32_t heads;
+} gqk_heads;
+
+#define GQK_ROPE_UNIT_OFFSET 1 /* norm weights are 1 + w */
+#define GQK_ROPE_INTERLEAVED 2 /* rotated pairs are dims (2 i, 2 i + 1), not (i, i + rot / 2) */
+
+/* RMS norm of each head of q and k (weights [dim] of the heads' type or fp32; NULL: no norm), then the rotation of
+ * its first rot dims by the token's position: table fp32 [table_rows, rot] = cos | sin of each pair's angle.  One
+ * launch; arithmetic in fp32, rounded once.  out_q / out_k may be q / k themselves (or NULL for out_k when the
+ * keys are only stored; k NULL: queries alone).  With pages, token t's keys and values (v, not changed) are stored at slot
+ * slots[t] = page * page_size + place (negative: not stored); in fp8 pages as value / scale, at most 448 in size.
+ * dim: a multiple of 8 up to 256, rot even; positions and slots int32, or int64 where the _64 flag is set.  A position
+ * outside of the table makes the token's heads NaN. */
+int gqk_qk_norm_rope(const gqk_heads* q, const gqk_heads* k, const gqk_heads* v, int dtype, int64_t tokens, int dim,
+                     const void* positions, int positions_64, const float* table, int64_t table_rows, int rot,
+                     const void* q_weight, const void* k_weight, int weight_dtype, float eps, int flags,
+                     const gqk_heads* out_q, const gqk_heads* out_k, const gqk_pages* pages, const void* slots,
+                     int slots_64, void* stream);
+
+/* Attention of one new token per sequence over its pages, split over the length and joined in one launch:
+ *   out[b, h] = sum_j softmax_j(scale * q[b, h] . k_j) v_j,   key j of sequence b in page table[b, j / page_size]
+ * over j in [max(0, lengths[b] - window), lengths[b]) (window 0: all).  No key (a length of zero or less): zeros, lse -inf;
+ * a length above max_length, or a page outside of the cache among the keys: NaN.  Query head h reads key head h / (q_heads / heads).  q, out: bf16 or fp16
+ * [batch, q_heads, dim]; table int32 [batch, table_width] with rows table_row apart; lse: NULL or fp32
+ * [batch, q_heads], log sum_j exp.  Scores, softmax and sums are in fp32; the probabilities that multiply v are rounded to
+ * the heads' type.  workspace: gqk_paged_attention_workspace_bytes bytes, 256-byte aligned, zeroed
+ * before its first use (arrival counters, which every launch leaves at zero, and fp32 partials): a linear
+ * layer's workspace serves (calls in stream order). */
+int64_t gqk_paged_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int dim, int max_length, int window);
+int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype, int batch, int q_heads,
+                        const gqk_pages* pages, const int32_t* table, int64_t table_row, int table_width,
+                        const int32_t* lengths, int max_length, int window, float scale, void* out, int64_t out_row,
+                        int64_t out_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Page src[i] to page dst[i] in each of `planes` planes (a layer's keys, a layer's values, ...), for n pairs: page p of
+ * plane l is the page_bytes bytes at base + l * plane_stride + p * page_stride.  src and dst are host arrays, read
+ * before the call returns (a captured graph copies the pairs of its capture).  A page outside of
+ * the cache, one that is written twice, or one that is both read and written is refused (GQK_ERR_SHAPE, GQK_ERR_ARG) and
+ * nothing is copied. */
+int gqk_copy_pages(void* base, int64_t planes, int64_t plane_stride, int64_t pages, int64_t page_stride,
+                   int64_t page_bytes, const int32_t* src, const int32_t* dst, int64_t n, void* stream);
 
 /* ---- GGUF v3 files: the load path ----------------------------------------------------------
  * The reference's tensors come from vLLM's GGUF loader (gguf-py 0.17.1 GGUFReader,
