@@ -3,6 +3,7 @@
 //   o = sum_j exp(scale q.k_j - m) v_j / sum_j exp(scale q.k_j - m),   m = max_j scale q.k_j
 //
 // over the keys j in [max(0, length - window), length) of the sequence; no key: zeros.
+#include <algorithm>
 #include "gqk_decode.h"
 
 namespace gqk {
@@ -38,6 +39,17 @@ int check_pages(const char* what, const gqk_pages* p, int q_dtype) {
 
 namespace {
 
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;             // waves of a workgroup
+constexpr int kTile = 32;             // keys of a wave's step
+constexpr int kMaxRowWeights = 4096;  // splits x rows of a unit: the joining workgroup keeps their weights in LDS
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
 struct AttnArgs {
   const void* q;
   int64_t q_row, q_head;
@@ -48,58 +60,442 @@ struct AttnArgs {
   void* out;
   int64_t out_row, out_head;
   float* lse;
+  int* counters;
+  float* partials;
   int q_heads, max_length, window;
-  float scale;
+  float scale;          // of a score, in units of log 2
+  int row_waves;        // 16-row tiles of query heads that a workgroup's waves deal among themselves
+  int row_blocks;       // workgroups over the query heads of one key head
+  int chunk, splits;    // keys of a split, and the most splits of a sequence
+  uint32_t magic;       // key / page_size = key * magic >> shift, exact below 2^31
+  int shift;
 };
 
-// One wave per (sequence, query head): 64 keys at a time, a lane per key for the scores, a lane per
-// dim for the values.
-template <typename T, typename C>
-__global__ __launch_bounds__(64) void attention_kernel(AttnArgs a) {
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
-  const int kvh = h / (a.q_heads / a.kv.heads), D = a.kv.dim, ps = a.kv.page_size;
-  const int len = max(0, a.lengths[b]);
-  const float ks = a.kv.k_scale ? a.kv.k_scale[kvh] : 1.f, vs = a.kv.v_scale ? a.kv.v_scale[kvh] : 1.f;
-  const T* q = (const T*)a.q + b * a.q_row + h * a.q_head;
-  __shared__ float sq[256], sp[64];
-  __shared__ int64_t vo[64];
-  for (int d = lane; d < D; d += 64) sq[d] = to_f(q[d]) * (a.scale * ks);
-  __syncthreads();
-  const float kInf = __builtin_huge_valf();
-  float m = -kInf, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  bool bad = len > a.max_length;
-  const int first = a.window > 0 ? max(0, len - a.window) : 0;
-  for (int j0 = first; j0 < len && !bad; j0 += 64) {
-    const int j = min(j0 + lane, len - 1);
-    const int page = a.table[b * a.table_row + j / ps];
-    const bool out = (uint32_t)page >= (uint32_t)a.kv.pages;
-    bad = __any(out);
-    if (bad) break;
-    const C* kp = (const C*)a.kv.k + page * a.kv.k_page + (j % ps) * a.kv.k_token + kvh * a.kv.k_head;
-    float s = 0.f;
-    for (int d = 0; d < D; ++d) s += sq[d] * to_f(kp[d]);
-    if (j0 + lane >= len) s = -kInf;
-    float top = s;
-    for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-    const float mn = fmaxf(m, top), base = mn == -kInf ? 0.f : mn;
-    const float p = __expf(s - base), c = __expf(m - base);
-    float sum = p;
-    for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x);
-    l = l * c + sum;
-    m = mn;
-    __syncthreads();
-    sp[lane] = p;
-    vo[lane] = page * a.kv.v_page + (j % ps) * a.kv.v_token + kvh * a.kv.v_head;
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) o[i] *= c;
-    for (int t = 0; t < min(64, len - j0); ++t)
-      for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < D) o[i] += sp[t] * to_f(((const C*)a.kv.v)[vo[t] + lane + 64 * i]);
+__device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c, bf16_t) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c, f16_t) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// two e4m3 values (bytes 0, 1 or 2, 3 of x) as two values of T, exactly
+template <bool HI> __device__ __forceinline__ uint32_t widen(uint32_t x, bf16_t) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, HI));
+}
+template <bool HI> __device__ __forceinline__ uint32_t widen(uint32_t x, f16_t) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.f, HI));
+}
+template <typename T> __device__ __forceinline__ v4u widen8(uint32_t lo, uint32_t hi) {
+  return v4u{widen<false>(lo, T{}), widen<true>(lo, T{}), widen<false>(hi, T{}), widen<true>(hi, T{})};
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  typedef T v2 __attribute__((ext_vector_type(2)));
+  v2 p;
+  p[0] = (T)lo;
+  p[1] = (T)hi;
+  return __builtin_bit_cast(uint32_t, p);
+}
+
+// max and sum over the four lanes of a query head (lane, lane ^ 16, lane ^ 32, lane ^ 48)
+__device__ __forceinline__ float max4(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum4(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// The exponent's base of a running maximum: nothing was seen yet (-inf) must not become -inf - -inf.
+__device__ __forceinline__ float base_of(float m) { return m == -__builtin_huge_valf() ? 0.f : m; }
+
+// A workgroup takes one split (a.chunk keys) of one sequence's keys of one key head, for up to 16 row_waves query heads
+// that share it; its waves deal the 32-key steps of the split (and the 16-row tiles of the heads) among themselves.
+//
+// Both products run on 16 x 16 x 32 matrix instructions with the keys (then the dims) as the rows and the query
+// heads as the columns, so that a lane holds scores, statistics and sums of one head, and nothing but the maximum
+// crosses lanes:  S^T = K Q^T: lane l = (head n = l % 16, g = l / 16) gets the scores of keys 8 g .. 8 g + 7 of the step (the
+// rows of the two 16-key tiles are dealt so), which is what O^T += V^T P^T wants of it as an operand.  K comes from global
+// memory straight as operands (8 dims of a key per lane).  V's operands hold 8 keys of one dim: a lane loads 8 dims of
+// each of its 8 keys and transposes the 8 x 8 block in registers, one v_perm per pair.  No LDS, no barrier in the loop.
+template <typename T, typename C, int DP, bool FULL, bool P8>
+__global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kernel(AttnArgs a) {
+  constexpr bool F8 = sizeof(C) == 1;
+  constexpr int NM = DP / 32;                 // k-steps of a score
+  constexpr int VD = DP == 64 ? 4 : 8;        // dims of a lane's V load
+  constexpr int NH = DP / (16 * VD);          // V loads of a key per lane
+  constexpr int NT = NH * VD;                 // 16-dim tiles of the output
+  constexpr int KW = F8 ? 2 : 4;              // words of 8 dims
+  constexpr int RS = DP + 4;                  // row stride of the reduction buffer
+  constexpr bool QLDS = DP == 256;
+  __shared__ __align__(16) float red[kWaves * 16 * RS];
+  __shared__ float stat[kWaves * 16][2];
+  __shared__ int flag;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int b = blockIdx.y, split = blockIdx.z;
+  const int kvh = blockIdx.x / a.row_blocks, rb = blockIdx.x % a.row_blocks;
+  const int group = a.q_heads / a.kv.heads, D = a.kv.dim;
+  const int rows_wg = 16 * a.row_waves, row0 = rb * rows_wg, R = min(rows_wg, group - row0);
+  const int len0 = max(0, a.lengths[b]);
+  const bool too_long = len0 > a.max_length;
+  const int len = too_long ? 0 : len0;
+  const int first = a.window > 0 ? max(0, len - a.window) : 0, start = first & ~(kTile - 1);
+  const int ns = max(1, (len - start + a.chunk - 1) / a.chunk);   // splits of this sequence
+  if (split >= ns) return;
+  const int k_begin = start + split * a.chunk, k_end = min(len, k_begin + a.chunk);
+  const float inf = __builtin_huge_valf();
+
+  const int rt = wave % a.row_waves, kw = wave / a.row_waves, nkw = kWaves / a.row_waves;
+  const int row = rt * 16 + n;                                     // of the workgroup's rows
+  const int steps_all = (k_end - k_begin + kTile - 1) / kTile;
+  const int steps = rt * 16 < R && steps_all > kw ? (steps_all - kw + nkw - 1) / nkw : 0;
+  const float scale = a.scale * (a.kv.k_scale ? a.kv.k_scale[kvh] : 1.f);
+
+  v4f acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+  float m = -inf, l = 0.f;
+  bool bad = false;
+
+  if (steps > 0) {
+    const int32_t* table = a.table + (int64_t)b * a.table_row;
+    const char* kb = (const char*)a.kv.k + kvh * a.kv.k_head * (int64_t)sizeof(C);
+    const char* vb = (const char*)a.kv.v + kvh * a.kv.v_head * (int64_t)sizeof(C);
+    const int64_t k_page = a.kv.k_page * (int64_t)sizeof(C), k_tok = a.kv.k_token * (int64_t)sizeof(C);
+    const int64_t v_page = a.kv.v_page * (int64_t)sizeof(C), v_tok = a.kv.v_token * (int64_t)sizeof(C);
+    const int ps = a.kv.page_size, last = len - 1;
+    // first dim of k-step i's operand: 16 bytes of a key per load
+    auto dim_at = [&](int i) { return F8 && FULL ? (i >> 1) * 64 + g * 16 + (i & 1) * 8 : i * 32 + g * 8; };
+    auto page_of = [&](int key) { return (int)(((uint64_t)(uint32_t)key * a.magic) >> a.shift); };
+
+    // Queries stay in registers as operands; at 256 dims, where they would not fit beside K, V and the sums, in the
+    // wave's own part of the reduction buffer, which is free until its loop ends.
+    v4u q[NM];
+    char* const mine = (char*)(red + wave * 16 * RS) + lane * 16;
+    {
+      const bool live = row < R;
+      const T* qp = (const T*)a.q + b * a.q_row + (int64_t)(kvh * group + row0 + (live ? row : 0)) * a.q_head;
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        const int d = dim_at(i);
+        q[i] = *(const v4u*)(qp + (FULL || d < D ? d : 0));
+        if (!live || !(FULL || d < D)) q[i] = v4u{0, 0, 0, 0};
+        if constexpr (QLDS) *(v4u*)(mine + i * 1024) = q[i];
+      }
+    }
+
+    // The keys of a lane: as rows of K's two tiles, group n / 4 of 8 keys, places n % 4 and 4 + n % 4; for V all 8 of
+    // group g.  Keys outside of [first, last] are read as the nearest inside (their weight is 0).
+    struct Pages { int k[P8 ? 1 : 2], v[P8 ? 1 : 8]; };
+    auto key_k = [&](int base, int c) { return min(max(base + (n >> 2) * 8 + c * 4 + (n & 3), first), last); };
+    auto key_v = [&](int base, int j) { return min(max(base + g * 8 + j, first), last); };
+    auto lookup = [&](int base) {
+      Pages p;
+      if constexpr (P8) {   // 8 keys from a multiple of 8 lie in one page; so do those of them that are inside
+        p.k[0] = table[page_of(key_k(base, 0))];
+        p.v[0] = table[page_of(key_v(base, 0))];
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) p.k[c] = table[page_of(key_k(base, c))];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p.v[j] = table[page_of(key_v(base, j))];
+      }
+      return p;
+    };
+    auto checked = [&](int page) {   // a page outside of the cache is not read
+      const bool out = (uint32_t)page >= (uint32_t)a.kv.pages;
+      bad |= out;
+      return out ? 0 : page;
+    };
+    uint32_t kr[2][NM][KW];   // two 16-key tiles of K
+    uint32_t vr[8][NH][VD * (int)sizeof(C) / 4];
+    auto load_k = [&](int base, const Pages& p) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int key = key_k(base, c);
+        const char* at = kb + checked(p.k[P8 ? 0 : c]) * k_page + (key - page_of(key) * ps) * k_tok;
+        if constexpr (F8 && FULL) {
+#pragma unroll
+          for (int i = 0; i < NM; i += 2) {
+            const v4u x = *(const v4u*)(at + dim_at(i));
+            kr[c][i][0] = x.x; kr[c][i][1] = x.y; kr[c][i + 1][0] = x.z; kr[c][i + 1][1] = x.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < NM; ++i) {
+            const int d = dim_at(i);
+            const char* src = at + (FULL || d < D ? d : 0) * (int)sizeof(C);
+            if constexpr (F8) {
+              const v2u x = *(const v2u*)src;
+              kr[c][i][0] = x.x; kr[c][i][1] = x.y;
+            } else {
+              const v4u x = *(const v4u*)src;
+              kr[c][i][0] = x.x; kr[c][i][1] = x.y; kr[c][i][2] = x.z; kr[c][i][3] = x.w;
+            }
+          }
+        }
+      }
+    };
+    auto load_v = [&](int base, const Pages& p) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = key_v(base, j);
+        const char* at = vb + checked(p.v[P8 ? 0 : j]) * v_page + (key - page_of(key) * ps) * v_tok;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const int d = h * 16 * VD + n * VD;
+          const char* src = at + (FULL || d < D ? d : 0) * (int)sizeof(C);
+          if constexpr (VD * sizeof(C) == 16) {
+            const v4u x = *(const v4u*)src;
+            vr[j][h][0] = x.x; vr[j][h][1] = x.y; vr[j][h][2] = x.z; vr[j][h][3] = x.w;
+          } else if constexpr (VD * sizeof(C) == 8) {
+            const v2u x = *(const v2u*)src;
+            vr[j][h][0] = x.x; vr[j][h][1] = x.y;
+          } else {
+            vr[j][h][0] = *(const uint32_t*)src;
+          }
+        }
+      }
+    };
+
+    const int hop = kTile * nkw;
+    int base = k_begin + kTile * kw;
+    Pages now = lookup(base);
+    load_k(base, now);
+    load_v(base, now);
+    Pages next = lookup(base + hop);   // past the split: clamped, still a key of the sequence
+    for (int s = 0; s < steps; ++s, base += hop) {
+      v4f sc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+      int again = 0;
+      if constexpr (QLDS) asm volatile("" : "+v"(again));   // read anew in every step
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        v4u qi;
+        if constexpr (QLDS) qi = *(const v4u*)(mine + again + i * 1024);
+        else qi = q[i];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          v4u x;
+          if constexpr (F8) x = widen8<T>(kr[c][i][0], kr[c][i][1]);
+          else x = v4u{kr[c][i][0], kr[c][i][1], kr[c][i][2], kr[c][i][3]};
+          if constexpr (!FULL) x = dim_at(i) < D ? x : v4u{0, 0, 0, 0};
+          sc[c] = mfma(x, qi, sc[c], T{});
+        }
+      }
+      const bool more = s + 1 < steps;
+      if (more) load_k(base + hop, next);
+      const bool edge = base < first || base + kTile > k_end;
+      float top = -inf;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = base + g * 8 + j;
+        float x = sc[j >> 2][j & 3] * scale;
+        if (edge && (key < first || key >= k_end)) x = -inf;
+        sc[j >> 2][j & 3] = x;
+        top = fmaxf(top, x);
+      }
+      const float mn = fmaxf(m, max4(top)), mb = base_of(mn), c = __builtin_amdgcn_exp2f(m - mb);
+      m = mn;
+      float sum = 0.f, p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(sc[j >> 2][j & 3] - mb);
+        sum += p[j];
+      }
+      l = l * c + sum;
+      const v4u pt{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] *= c;
+      if (edge) {   // a weight of 0 does not silence a value that is not finite
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = base + g * 8 + j;
+          if (key < first || key >= k_end)
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+              for (int w = 0; w < VD * (int)sizeof(C) / 4; ++w) vr[j][h][w] = 0;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int w = 0; w < VD * (int)sizeof(C) / 4; ++w) {
+          if constexpr (F8) {   // four dims of the lane's keys
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi) {
+              uint32_t y[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                y[j] = __builtin_amdgcn_perm(vr[2 * j + 1][h][w], vr[2 * j][h][w], hi ? 0x07030602 : 0x05010400);
+              const int t = h * VD + w * 4 + hi * 2;
+              const v4u lo{widen<false>(y[0], T{}), widen<false>(y[1], T{}), widen<false>(y[2], T{}), widen<false>(y[3], T{})};
+              const v4u up{widen<true>(y[0], T{}), widen<true>(y[1], T{}), widen<true>(y[2], T{}), widen<true>(y[3], T{})};
+              acc[t] = mfma(lo, pt, acc[t], T{});
+              acc[t + 1] = mfma(up, pt, acc[t + 1], T{});
+            }
+          } else {
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi) {
+              v4u x;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                x[j] = __builtin_amdgcn_perm(vr[2 * j + 1][h][w], vr[2 * j][h][w], hi ? 0x07060302 : 0x05040100);
+              acc[h * VD + w * 2 + hi] = mfma(x, pt, acc[h * VD + w * 2 + hi], T{});
+            }
+          }
+        }
+      if (more) {
+        load_v(base + hop, next);
+        next = lookup(base + 2 * hop);
+      }
+    }
+    l = sum4(l);
+    if (__any(bad)) l = __builtin_nanf("");
   }
-  const float nan = __builtin_nanf(""), r = bad ? nan : l > 0.f ? vs / l : l == 0.f ? 0.f : nan;
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < D) ((T*)a.out)[b * a.out_row + h * a.out_head + lane + 64 * i] = from_f<T>(o[i] * r);
-  if (a.lse && lane == 0) a.lse[(int64_t)b * a.q_heads + h] = bad ? nan : l == 0.f ? -kInf : m + __logf(l);
+
+  // the waves' sums, joined: lane (n, g) holds dims h * 16 VD + (4 g + i) VD + t of head n in acc[h VD + t][i]
+  {
+    float* to = red + (wave * 16 + n) * RS;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < VD; t += 4)
+          *(v4f*)(to + h * 16 * VD + (4 * g + i) * VD + t) =
+              v4f{acc[h * VD + t][i], acc[h * VD + t + 1][i], acc[h * VD + t + 2][i], acc[h * VD + t + 3][i]};
+    if (g == 0) {
+      stat[wave * 16 + n][0] = m;
+      stat[wave * 16 + n][1] = l;
+    }
+  }
+  __syncthreads();
+  const float nan = __builtin_nanf("");
+  const float v_scale = a.kv.v_scale ? a.kv.v_scale[kvh] : 1.f;
+  const int64_t unit = (int64_t)b * gridDim.x + blockIdx.x;
+  const int quads = D / 4;
+  // [splits][R][D], then [splits][R][2] (room for a full block's rows in every unit)
+  float* part = a.partials + unit * a.splits * min(rows_wg, group) * (D + 4);
+  float* part_stat = part + (int64_t)a.splits * R * D;
+  auto store = [&](int r, int d, v4f x, float f) {
+    T* to = (T*)a.out + b * a.out_row + (int64_t)(kvh * group + row0 + r) * a.out_head + d;
+    *(v2u*)to = v2u{pack2<T>(x[0] * f, x[1] * f), pack2<T>(x[2] * f, x[3] * f)};
+  };
+  auto store_lse = [&](int r, float M, float L) {
+    a.lse[(int64_t)b * a.q_heads + kvh * group + row0 + r] = L == 0.f ? -inf : (M + __builtin_amdgcn_logf(L)) * kLn2;
+  };
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(part, 0, a.splits * R * (D + 4) * 4, 0x00020000);
+  constexpr int kDevice = 16;   // device-scope cache policy (sc1): through the XCD's L2
+  for (int x = threadIdx.x; x < R * quads; x += 64 * kWaves) {
+    const int r = x / quads, d = (x - r * quads) * 4, tile = r >> 4;
+    float M = -inf;
+    for (int k = 0; k < nkw; ++k) M = fmaxf(M, stat[(tile + k * a.row_waves) * 16 + (r & 15)][0]);
+    const float Mb = base_of(M);
+    v4f o{0.f, 0.f, 0.f, 0.f};
+    float L = 0.f;
+    for (int k = 0; k < nkw; ++k) {
+      const int w = (tile + k * a.row_waves) * 16 + (r & 15);
+      const float f = __builtin_amdgcn_exp2f(stat[w][0] - Mb);
+      L += stat[w][1] * f;
+      o += *(const v4f*)(red + w * RS + d) * f;
+    }
+    if (too_long) L = nan;
+    if (ns == 1) {
+      store(r, d, o, L == 0.f ? 0.f : v_scale / L);
+      if (a.lse && d == 0) store_lse(r, M, L);
+    } else {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, o), rs, ((split * R + r) * D + d) * 4, 0, kDevice);
+      if (d == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(v2u{__builtin_bit_cast(uint32_t, M), __builtin_bit_cast(uint32_t, L)}, rs,
+                                              (a.splits * R * D + (split * R + r) * 2) * 4, 0, kDevice);
+    }
+  }
+  if (ns == 1) return;
+  // The sequence's splits join in the workgroup that arrives last, in split order: partials move through device-coherent
+  // accesses alone; every store is complete before the arrival count.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) flag = __hip_atomic_fetch_add(a.counters + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (flag != ns - 1) return;
+  asm volatile("" ::: "memory");
+  if (threadIdx.x == 0) __hip_atomic_store(a.counters + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // next launch
+  float* weight = red;   // [ns][R][2]: (maximum, sum), then (weight, sum)
+  for (int x = threadIdx.x; x < ns * R; x += 64 * kWaves) {
+    const v2u y = __builtin_amdgcn_raw_buffer_load_b64(rs, (a.splits * R * D + x * 2) * 4, 0, kDevice);
+    *(v2u*)(weight + 2 * x) = y;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < R; r += 64 * kWaves) {
+    float M = -inf, L = 0.f;
+    for (int s = 0; s < ns; ++s) M = fmaxf(M, weight[2 * (s * R + r)]);
+    const float Mb = base_of(M);
+    for (int s = 0; s < ns; ++s) {
+      const float f = __builtin_amdgcn_exp2f(weight[2 * (s * R + r)] - Mb);
+      L += weight[2 * (s * R + r) + 1] * f;
+      weight[2 * (s * R + r)] = f;
+    }
+    stat[r][0] = L == 0.f ? 0.f : v_scale / L;
+    if (a.lse) store_lse(r, M, L);
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < R * quads; x += 64 * kWaves) {
+    const int r = x / quads, d = (x - r * quads) * 4;
+    v4f o{0.f, 0.f, 0.f, 0.f};
+    constexpr int kBatch = 8;
+    for (int s0 = 0; s0 < ns; s0 += kBatch) {
+      v4u y[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        y[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, ((min(s0 + j, ns - 1) * R + r) * D + d) * 4, 0, kDevice);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (s0 + j < ns) o += __builtin_bit_cast(v4f, y[j]) * weight[2 * ((s0 + j) * R + r)];
+    }
+    store(r, d, o, stat[r][0]);
+  }
+}
+
+// How a call is cut: workgroups over the query heads of a key head, and splits of `chunk` keys.
+struct Cut { int row_waves, row_blocks, splits, chunk; };
+
+Cut cut_of(int batch, int q_heads, int kv_heads, int dim, int max_length, int window) {
+  const int group = q_heads / kv_heads, tiles = (group + 15) / 16;
+  Cut c;
+  c.row_waves = tiles >= 3 ? 4 : tiles;
+  c.row_blocks = (tiles + c.row_waves - 1) / c.row_waves;
+  // keys a sequence can have, from a multiple of the step
+  const int64_t span = std::min<int64_t>(max_length, window > 0 ? (int64_t)window + kTile - 1 : max_length);
+  const int64_t units = (int64_t)batch * kv_heads * c.row_blocks, wanted = 4LL * device_cus();
+  const int64_t least = kTile * kWaves;   // keys of the shortest split
+  int64_t splits = std::max<int64_t>(1, std::min((wanted + units - 1) / std::max<int64_t>(1, units), (span + least - 1) / least));
+  splits = std::min<int64_t>(splits, kMaxRowWeights / 2 / (16 * c.row_waves));
+  if (units > GQK_CTR_WORDS) splits = 1;
+  c.chunk = (int)std::max<int64_t>(kTile, ((span + splits - 1) / splits + kTile - 1) / kTile * kTile);
+  c.splits = (int)std::max<int64_t>(1, (span + c.chunk - 1) / c.chunk);
+  return c;
+}
+
+template <typename T, typename C, int DP>
+void launch(const AttnArgs& a, dim3 grid, bool full, hipStream_t st) {
+  const bool p8 = a.kv.page_size % 8 == 0;
+  if (full && p8) attention_kernel<T, C, DP, true, true><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (full) attention_kernel<T, C, DP, true, false><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (p8) attention_kernel<T, C, DP, false, true><<<grid, 64 * kWaves, 0, st>>>(a);
+  else attention_kernel<T, C, DP, false, false><<<grid, 64 * kWaves, 0, st>>>(a);
+}
+
+template <typename T, typename C>
+void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {
+  const int D = a.kv.dim;
+  bool full = D == 64 || D == 128 || D == 256;
+  if (sizeof(C) == 1)   // 16-byte loads of 8-bit keys
+    full = full && !(((uintptr_t)a.kv.k | (uint64_t)a.kv.k_page | (uint64_t)a.kv.k_token | (uint64_t)a.kv.k_head) & 15);
+  if (D <= 64) launch<T, C, 64>(a, grid, full, st);
+  else if (D <= 128) launch<T, C, 128>(a, grid, full, st);
+  else launch<T, C, 256>(a, grid, full, st);
 }
 
 }  // namespace
@@ -111,10 +507,12 @@ extern "C" {
 
 int64_t gqk_paged_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int dim, int max_length, int window) {
   if (batch < 0 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || dim < 8 || dim > 256 || dim % 8 ||
-      max_length < 0 || window < 0)
+      max_length < 0 || max_length > GQK_MAX_KEYS || window < 0)
     return decode_fail(GQK_ERR_SHAPE, "paged_attention: %d sequences, %d / %d heads of %d, max_length %d, window %d", batch,
                        q_heads, kv_heads, dim, max_length, window);
-  return 0;
+  const Cut c = cut_of(batch, q_heads, kv_heads, dim, max_length, window);
+  const int64_t rows = std::min(16 * c.row_waves, q_heads / kv_heads), units = (int64_t)batch * kv_heads * c.row_blocks;
+  return c.splits > 1 ? GQK_CTR_BYTES + units * rows * c.splits * (dim + 4) * 4 : 0;
 }
 
 int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype, int batch, int q_heads,
@@ -125,7 +523,7 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
   if (const int rc = check_pages("paged_attention", pages, dtype)) return rc;
   if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads % pages->heads)
     return decode_fail(GQK_ERR_SHAPE, "paged_attention: %d sequences of %d query heads over %d", batch, q_heads, pages->heads);
-  if (window < 0 || max_length < 0 || table_width < 0 ||
+  if (window < 0 || max_length < 0 || max_length > GQK_MAX_KEYS || table_width < 0 ||
       (int64_t)max_length > (int64_t)table_width * pages->page_size)
     return decode_fail(GQK_ERR_SHAPE, "paged_attention: window %d, lengths up to %d in %d pages of %d tokens", window, max_length,
                        table_width, pages->page_size);
@@ -138,17 +536,30 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace & 255))
     return decode_fail(GQK_ERR_SHAPE, "paged_attention: workspace %lld bytes < %lld (or not 256-byte aligned)",
                        (long long)workspace_bytes, (long long)need);
-  AttnArgs a{q, q_row, q_head, *pages, table, table_row, lengths, out, out_row, out_head, lse, q_heads, max_length, window, scale};
-  const dim3 grid(q_heads, batch);
+  const Cut c = cut_of(batch, q_heads, pages->heads, pages->dim, max_length, window);
+  AttnArgs a{};
+  a.q = q; a.q_row = q_row; a.q_head = q_head; a.kv = *pages; a.table = table; a.table_row = table_row; a.lengths = lengths;
+  a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.q_heads = q_heads; a.max_length = max_length;
+  a.window = window; a.scale = scale * kLog2e; a.row_waves = c.row_waves; a.row_blocks = c.row_blocks; a.chunk = c.chunk;
+  a.splits = c.splits;
+  a.counters = (int*)workspace;
+  a.partials = workspace ? (float*)((char*)workspace + GQK_CTR_BYTES) : nullptr;
+  // key / page_size for keys below 2^31: 2^(31 + bits) / page_size rounded up fits 32 bits, its excess times a key stays
+  // below 2^(31 + bits)
+  int bits = 0;
+  while (((int64_t)1 << bits) < pages->page_size) ++bits;
+  a.shift = 31 + bits;
+  a.magic = (uint32_t)((((uint64_t)1 << a.shift) + pages->page_size - 1) / pages->page_size);
+  const dim3 grid(pages->heads * c.row_blocks, batch, c.splits);
   const hipStream_t st = (hipStream_t)stream;
   const bool bf = dtype == GQK_DTYPE_BF16;
   if (pages->dtype == GQK_DTYPE_FP8) {
-    if (bf) attention_kernel<bf16_t, fp8_t><<<grid, 64, 0, st>>>(a);
-    else attention_kernel<f16_t, fp8_t><<<grid, 64, 0, st>>>(a);
+    if (bf) launch<bf16_t, fp8_t>(a, grid, st);
+    else launch<f16_t, fp8_t>(a, grid, st);
   } else if (bf) {
-    attention_kernel<bf16_t, bf16_t><<<grid, 64, 0, st>>>(a);
+    launch<bf16_t, bf16_t>(a, grid, st);
   } else {
-    attention_kernel<f16_t, f16_t><<<grid, 64, 0, st>>>(a);
+    launch<f16_t, f16_t>(a, grid, st);
   }
   return decode_launched("paged_attention");
 }

@@ -22,6 +22,7 @@ GQK_FORM_GEMM = 2
 GQK_CTR_BYTES = 262144            # the arrival-counter region at the start of every workspace
 GQK_NOALLOC_SCRATCH_BYTES = GQK_CTR_BYTES + (32 << 20)   # gqk_linear_noalloc's per-GPU device array
 GQK_DTYPE_F32, GQK_DTYPE_BF16, GQK_DTYPE_F16, GQK_DTYPE_FP8 = 0, 1, 2, 3
+GQK_MAX_KEYS = 0x7ffffc00
 GQK_ROPE_UNIT_OFFSET, GQK_ROPE_INTERLEAVED = 1, 2
 
 # every entry point include/gguf_hip.h declares
