@@ -4,56 +4,334 @@
 //
 // with i = ids[m] the row's adapter (negative: out = y) and p(n) the part (q, k, v; gate, up) that
 // column n belongs to.  h is kept in 32 bits in the workspace, after its counter region.
+#include <algorithm>
 #include "gqk_decode.h"
 
 namespace gqk {
 namespace {
 
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
 constexpr int kParts = 8;
+constexpr int kDownWaves = 8, kUpWaves = 4;
+constexpr int kBlock = 64;       // rows whose adapters a workgroup sorts out: one per lane
+constexpr int kRankTiles = 4;    // 16-rank tiles of a workgroup of the first kernel
+constexpr int kHPad = 68;        // row stride of its sums in LDS
+constexpr int kNone = -1, kBad = -2;
+
 struct LoraArgs {
   const void *y, *x, *a, *b;
   void* out;
   int64_t y_row, x_row, out_row, K, N;
   const void* ids;
   const float* scales;
-  float* h;
+  float* h;                  // [splits][M][parts * rank]
   int M, slots, parts, rank, wide_ids;
-  int64_t ends[kParts];   // one past each part's last column
+  int splits, chunks;        // splits of K; chunks of 64 ranks
+  int columns;               // of a workgroup of the second kernel
+  int wide_y;                // y and out are 16-byte aligned in every row
+  int64_t ends[kParts];      // one past each part's last column
 };
 
-// a wave per (row, part and rank)
-template <typename T>
-__global__ __launch_bounds__(64) void lora_down_kernel(LoraArgs a) {
-  const int64_t m = blockIdx.y;
-  const int pr = blockIdx.x, lane = threadIdx.x;
-  const int64_t i = index_at(a.ids, a.wide_ids, m);
-  if (i < 0 || i >= a.slots) return;
-  const T* A = (const T*)a.a + (i * a.parts * a.rank + pr) * a.K;
-  const T* x = (const T*)a.x + m * a.x_row;
-  float s = 0.f;
-  for (int64_t k = lane; k < a.K; k += 64) s += to_f(A[k]) * to_f(x[k]);
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if (lane == 0) a.h[(m * a.parts * a.rank) + pr] = s;
+__device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c, bf16_t) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c, f16_t) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// a thread per (row, column)
-template <typename T>
-__global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
-  const int64_t m = blockIdx.y, n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= a.N) return;
-  const int64_t i = index_at(a.ids, a.wide_ids, m);
-  float d = 0.f;
-  if (i >= a.slots) {
-    d = __builtin_nanf("");
-  } else if (i >= 0) {
-    int p = 0;
-    while (n >= a.ends[p]) ++p;
-    const T* B = (const T*)a.b + (i * a.N + n) * a.rank;
-    const float* h = a.h + (m * a.parts + p) * a.rank;
-    for (int r = 0; r < a.rank; ++r) d += to_f(B[r]) * h[r];
-    d *= a.scales ? a.scales[i] : 1.f;
+// Up to 16 TT rows of one block that go with one adapter (or with none, kNone, or a bad id, kBad).
+template <int TT> struct Unit {
+  int adapter, count;
+  int row[TT];   // row of tile t's column lane % 16 (of a column past the count: some row of the unit)
+};
+
+// Unit u of the block's rows: adapters in the order of their first row, each one's rows in order.  A lane holds
+// one row's id; a ballot finds the rows that share it.  False: the block has fewer units.
+template <int TT> __device__ __forceinline__ bool find_unit(const LoraArgs& a, int64_t row0, int u, Unit<TT>& out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t m = row0 + lane;
+  int id = kNone;
+  if (m < a.M) {
+    const int64_t i = index_at(a.ids, a.wide_ids, m);
+    id = i < 0 ? kNone : i >= a.slots ? kBad : (int)i;
   }
-  ((T*)a.out)[m * a.out_row + n] = from_f<T>(to_f(((const T*)a.y)[m * a.y_row + n]) + d);
+  uint64_t left = __ballot(m < a.M);
+  while (left) {
+    const int who = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+    const uint64_t same = __ballot(id == who) & left;
+    const int count = __popcll(same), units = (count + 16 * TT - 1) / (16 * TT);
+    if (u < units) {
+      out.adapter = who;
+      out.count = min(count - u * 16 * TT, 16 * TT);
+      // the lane with place i among them sends its row to lane i; the others' go where nobody looks, or later
+      const int place = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0)) - u * 16 * TT;
+      const bool in = (same >> lane & 1) && place >= 0 && place < out.count;
+      __shared__ int rows[8][kBlock];
+      int* mine = rows[threadIdx.x >> 6];
+      if (in) mine[place] = lane;
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t = 0; t < TT; ++t) out.row[t] = mine[min(t * 16 + (lane & 15), out.count - 1)];
+      return true;
+    }
+    u -= units;
+    left &= ~same;
+  }
+  return false;
+}
+
+// h = A x of one unit's rows, 64 ranks, one split of K: the ranks are the matrix instruction's rows and the batch
+// rows its columns, both operands straight from global memory (8 values along K per lane).  The waves split the split's
+// steps of 32 among themselves and join in LDS, in order.
+template <typename T, int TT>
+__global__ __launch_bounds__(64 * kDownWaves, 2) void lora_down_kernel(LoraArgs a) {
+  constexpr int kDepth = TT == 1 ? 3 : 2;   // steps in flight
+  __shared__ __align__(16) float red[kDownWaves][16][kHPad];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int chunk = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const int64_t row0 = (int64_t)blockIdx.z * kBlock;
+  const int PR = a.parts * a.rank, rank0 = chunk * 16 * kRankTiles, tiles = min(kRankTiles, (PR - rank0 + 15) / 16);
+  const int64_t all = (a.K + 31) / 32, s0 = all * split / a.splits, s1 = all * (split + 1) / a.splits;
+  for (int u = blockIdx.y;; u += gridDim.y) {
+    Unit<TT> unit;
+    if (!find_unit(a, row0, u, unit)) return;
+    if (unit.adapter < 0) continue;
+    const int rows = (unit.count + 15) / 16;   // tiles of rows
+    const T* A[kRankTiles];
+    const T* x[TT];
+#pragma unroll
+    for (int t = 0; t < kRankTiles; ++t)
+      A[t] = (const T*)a.a + ((int64_t)unit.adapter * PR + min(rank0 + t * 16 + n, PR - 1)) * a.K + g * 8;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) x[t] = (const T*)a.x + (row0 + unit.row[t]) * a.x_row + g * 8;
+    v4f acc[kRankTiles][TT];
+#pragma unroll
+    for (int r = 0; r < kRankTiles; ++r)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) acc[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    v4u av[kDepth][kRankTiles], xv[kDepth][TT];
+    auto load = [&](int d, int64_t s) {
+      const int64_t k = s * 32;
+      const bool in = k + g * 8 < a.K;   // K may end inside the step
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+        if (t < rows) xv[d][t] = in ? *(const v4u*)(x[t] + k) : v4u{0, 0, 0, 0};
+#pragma unroll
+      for (int t = 0; t < kRankTiles; ++t)
+        if (t < tiles) av[d][t] = in ? *(const v4u*)(A[t] + k) : v4u{0, 0, 0, 0};
+    };
+    const int64_t steps = s1 - s0 > wave ? (s1 - s0 - wave + kDownWaves - 1) / kDownWaves : 0;
+    const int64_t first = s0 + wave;
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d)
+      if (d < steps) load(d, first + d * kDownWaves);
+    for (int64_t i = 0; i < steps; i += kDepth)
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d)
+        if (i + d < steps) {
+#pragma unroll
+          for (int r = 0; r < kRankTiles; ++r)
+            if (r < tiles)
+#pragma unroll
+              for (int t = 0; t < TT; ++t)
+                if (t < rows) acc[r][t] = mfma(av[d][r], xv[d][t], acc[r][t], T{});
+          if (i + d + kDepth < steps) load(d, first + (i + d + kDepth) * kDownWaves);
+        }
+    // lane (n, g) holds ranks 16 r + 4 g .. + 3 of column n
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      if (t >= rows) break;
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < kRankTiles; ++r)
+        if (r < tiles) *(v4f*)&red[wave][n][r * 16 + g * 4] = acc[r][t];
+      __syncthreads();
+      const int row = threadIdx.x >> 5, c = (threadIdx.x & 31) * 2;   // 16 rows, 2 ranks a thread
+      const int at = __shfl(unit.row[t], row & 15);                   // lane row of this wave holds its number
+      if (t * 16 + row < unit.count && rank0 + c < PR) {
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kDownWaves; ++w) {
+          sum.x += red[w][row][c];
+          sum.y += red[w][row][c + 1];
+        }
+        *(float2*)(a.h + ((int64_t)split * a.M + row0 + at) * PR + rank0 + c) = sum;
+      }
+    }
+  }
+}
+
+// out = y + s B h of one unit's rows and `columns` columns of one part.  The ranks that h has in 32 bits go into the
+// product as two values of T each, h = hi + lo, in one instruction: 16 ranks of hi and the same 16 of lo against B's 16
+// ranks twice (rounding h to T alone would put 2^-9 of the update, for bf16, on top of the output's own rounding; the second
+// half of the instruction would be idle).  fp16 takes h over a power of two near its row's largest, to stay in range.
+template <typename T, int TT>
+__global__ __launch_bounds__(64 * kUpWaves, 2) void lora_up_kernel(LoraArgs a) {
+  constexpr bool kF16 = sizeof(T) == 2 && __is_same(T, f16_t);
+  __shared__ __align__(16) T hs[TT * 16][2][256 + 8];   // [row][hi, lo][rank]
+  __shared__ float factor[TT * 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int64_t row0 = (int64_t)blockIdx.z * kBlock;
+  const int PR = a.parts * a.rank, steps = (a.rank + 15) / 16;
+  // the part and its columns
+  int part = 0, block = blockIdx.x;
+  int64_t begin = 0;
+  for (;;) {
+    const int blocks = (int)((a.ends[part] - begin + a.columns - 1) / a.columns);
+    if (block < blocks) break;
+    block -= blocks;
+    begin = a.ends[part++];
+  }
+  const int64_t c_begin = begin + (int64_t)block * a.columns, c_end = min(a.ends[part], c_begin + a.columns);
+  for (int u = blockIdx.y;; u += gridDim.y) {
+    Unit<TT> unit;
+    if (!find_unit(a, row0, u, unit)) return;
+    if (unit.adapter == kNone && a.out == a.y) continue;
+    const int rows = (unit.count + 15) / 16;
+    if (unit.adapter >= 0) {
+      __syncthreads();   // the last unit's h has been read
+      const float s = a.scales ? a.scales[unit.adapter] : 1.f;
+      // 16 threads a row, 8 ranks each at a time
+      for (int t = 0; t < rows; ++t) {
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < TT; ++k) mine = k == t ? unit.row[k] : mine;
+        const int r = threadIdx.x >> 4, c = threadIdx.x & 15;      // 16 rows of the tile
+        const int64_t m = row0 + __shfl(mine, r);
+        float v[2][8];
+        float top = 0.f;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int rank = (q * 16 + c) * 8;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[q][e] = 0.f;
+          if (rank < a.rank)
+            for (int sp = 0; sp < a.splits; ++sp) {
+              const v4f* from = (const v4f*)(a.h + ((int64_t)sp * a.M + m) * PR + part * a.rank + rank);
+              const v4f lo = from[0], hi = from[1];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[q][e] += lo[e];
+                v[q][4 + e] += hi[e];
+              }
+            }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[q][e]));
+        }
+        float down = 1.f, up = 1.f;
+        if constexpr (kF16) {
+          for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+          if (top > 0.f && top < __builtin_huge_valf()) {
+            const int e = min(max(ilogbf(top), -100), 100);
+            down = ldexpf(1.f, -e);
+            up = ldexpf(1.f, e);
+          }
+        }
+        if (c == 0) factor[t * 16 + r] = s * up;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int rank = (q * 16 + c) * 8;
+          if (rank < steps * 16) {
+            T hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float f = v[q][e] * down;
+              hi[e] = (T)f;
+              const float back = (float)hi[e];
+              lo[e] = fabsf(back) < __builtin_huge_valf() ? (T)(f - back) : (T)0.f;   // inf stays, without inf - inf
+            }
+            __builtin_memcpy(&hs[t * 16 + r][0][rank], hi, 16);
+            __builtin_memcpy(&hs[t * 16 + r][1][rank], lo, 16);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    float f[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) f[t] = unit.adapter >= 0 && t < rows ? factor[t * 16 + n] : 0.f;
+    // 32 columns at a time: as rows of two 16-row tiles dealt so that a lane gets 8 in a row of its batch row
+    for (int64_t c0 = c_begin + wave * 32; c0 < c_end; c0 += 32 * kUpWaves) {
+      v4f acc[2][TT];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[c][t] = v4f{0.f, 0.f, 0.f, 0.f};
+      if (unit.adapter >= 0) {
+        const T* B[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int64_t col = min(c0 + (n >> 2) * 8 + c * 4 + (n & 3), c_end - 1);
+          B[c] = (const T*)a.b + ((int64_t)unit.adapter * a.N + col) * a.rank + (g & 1) * 8;
+        }
+        for (int k = 0; k < steps; ++k) {
+          v4u bv[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) bv[c] = k * 16 + (g & 1) * 8 < a.rank ? *(const v4u*)(B[c] + k * 16) : v4u{0, 0, 0, 0};
+#pragma unroll
+          for (int t = 0; t < TT; ++t)
+            if (t < rows) {
+              const v4u hv = *(const v4u*)&hs[t * 16 + n][g >> 1][k * 16 + (g & 1) * 8];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) acc[c][t] = mfma(bv[c], hv, acc[c][t], T{});
+            }
+        }
+      }
+      const int64_t col = c0 + g * 8;
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        if (t * 16 + n >= unit.count) continue;
+        const int64_t m = row0 + unit.row[t];
+        const T* y = (const T*)a.y + m * a.y_row + col;
+        T* out = (T*)a.out + m * a.out_row + col;
+        auto value = [&](float base, int e) {
+          return unit.adapter >= 0 ? base + acc[e >> 2][t][e & 3] * f[t] : unit.adapter == kNone ? base : __builtin_nanf("");
+        };
+        if (a.wide_y && col + 8 <= c_end) {
+          T v[8];
+          __builtin_memcpy(v, __builtin_assume_aligned(y, 16), 16);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = (T)value((float)v[e], e);
+          __builtin_memcpy(__builtin_assume_aligned(out, 16), v, 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + e < c_end) out[e] = (T)value((float)y[e], e);
+        }
+      }
+    }
+  }
+}
+
+// How a call is cut.  Down: splits of K so that the launch has about 512 workgroups, each wave at least two steps.
+// Rows of a block that share an adapter go 16 to a workgroup up to kBlock rows in all, 64 above.
+struct Cut { int splits, chunks, blocks; };
+
+Cut cut_of(int M, int64_t K, int parts, int rank) {
+  Cut c;
+  c.chunks = (parts * rank + 16 * kRankTiles - 1) / (16 * kRankTiles);
+  c.blocks = (M + kBlock - 1) / kBlock;
+  const int64_t wgs = (int64_t)c.chunks * (M <= kBlock ? std::min(M, 16) : c.blocks);
+  const int64_t steps = (K + 31) / 32;
+  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / wgs, steps / (2 * kDownWaves), 16}));
+  return c;
+}
+
+template <typename T, int TT>
+void launch(const LoraArgs& g, const Cut& c, hipStream_t st) {
+  // units of a block: its adapters, none, bad ids, and what does not fit one unit; the kernels step on over more
+  const int units = TT == 1 ? std::min(g.M, std::min(g.slots, kBlock) + 2 + kBlock / 16) : 2;
+  int64_t blocks = 0, begin = 0;
+  for (int p = 0; p < g.parts; ++p) {
+    blocks += (g.ends[p] - begin + g.columns - 1) / g.columns;
+    begin = g.ends[p];
+  }
+  if (g.slots > 0) lora_down_kernel<T, TT><<<dim3(c.splits * c.chunks, units, c.blocks), 64 * kDownWaves, 0, st>>>(g);
+  lora_up_kernel<T, TT><<<dim3((unsigned)blocks, units, c.blocks), 64 * kUpWaves, 0, st>>>(g);
 }
 
 }  // namespace
@@ -67,7 +345,7 @@ int64_t gqk_lora_workspace_bytes(int M, int64_t K, int parts, int rank) {
   if (M < 0 || K < 0 || parts < 1 || parts > kParts || rank < 8 || rank > 256 || rank % 8)
     return decode_fail(GQK_ERR_SHAPE, "lora: %d rows of %lld, %d parts (at most %d), rank %d (a multiple of 8 in 8..256)", M,
                        (long long)K, parts, kParts, rank);
-  return GQK_CTR_BYTES + (int64_t)M * parts * rank * 4;
+  return M == 0 ? GQK_CTR_BYTES : GQK_CTR_BYTES + (int64_t)cut_of(M, K, parts, rank).splits * M * parts * rank * 4;
 }
 
 int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int M, int64_t K, const void* a, const void* b,
@@ -97,15 +375,22 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
   g.y = y; g.x = x; g.a = a; g.b = b; g.out = out; g.y_row = y_row; g.x_row = x_row; g.out_row = out_row; g.K = K;
   g.ids = ids; g.wide_ids = ids_64; g.scales = scales; g.h = (float*)((char*)workspace + GQK_CTR_BYTES);
   g.M = M; g.slots = slots; g.parts = parts; g.rank = rank;
+  const Cut c = cut_of(M, K, parts, rank);
+  if (c.blocks > 65535) return decode_fail(GQK_ERR_SHAPE, "lora_add: %d rows", M);
+  g.splits = c.splits; g.chunks = c.chunks;
+  g.wide_y = !(((uintptr_t)y | (uintptr_t)out) & 15) && !((y_row | out_row) & 7);
+  for (int p = 0; p + 1 < parts; ++p) g.wide_y &= g.ends[p] % 8 == 0;
+  // columns of a workgroup of the second kernel: 1024, fewer where the launch would have too few of them
+  const int64_t groups = M <= kBlock ? std::min(M, 16) : c.blocks;
+  g.columns = 1024;
+  while (g.columns > 128 && groups * (g.N / g.columns) < 512) g.columns /= 2;
   const hipStream_t st = (hipStream_t)stream;
-  if (M > 65535) return decode_fail(GQK_ERR_SHAPE, "lora_add: %d rows (at most 65535)", M);
-  const dim3 down(parts * rank, M), up((unsigned)((g.N + 255) / 256), M);
   if (dtype == GQK_DTYPE_BF16) {
-    lora_down_kernel<bf16_t><<<down, 64, 0, st>>>(g);
-    lora_up_kernel<bf16_t><<<up, 256, 0, st>>>(g);
+    if (M <= kBlock) launch<bf16_t, 1>(g, c, st);
+    else launch<bf16_t, 4>(g, c, st);
   } else {
-    lora_down_kernel<f16_t><<<down, 64, 0, st>>>(g);
-    lora_up_kernel<f16_t><<<up, 256, 0, st>>>(g);
+    if (M <= kBlock) launch<f16_t, 1>(g, c, st);
+    else launch<f16_t, 4>(g, c, st);
   }
   return decode_launched("lora_add");
 }
