@@ -5,6 +5,7 @@
 //
 // with cos t | sin t of pair i at [position][i] | [position][rot / 2 + i] of a table in 32 bits.  Keys
 // and values of a token with a slot go into its page of the cache.
+#include <algorithm>
 #include "gqk_decode.h"
 
 namespace gqk {
@@ -26,9 +27,9 @@ struct RopeArgs {
   int wide_positions, wide_slots, unit_offset, interleaved, weight_f32, store;
 };
 
-// One wave per (token, head): q heads, k heads, then v heads (stored only).
+// Any even rot: one wave per (token, head), q heads, k heads, then v heads (stored only); the normalized head in LDS.
 template <typename T, typename C>
-__global__ __launch_bounds__(64) void rope_kernel(RopeArgs a) {
+__global__ __launch_bounds__(64) void rope_any_kernel(RopeArgs a) {
   const int h = blockIdx.x, lane = threadIdx.x, D = a.dim;
   const int64_t t = blockIdx.y;
   const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.k_heads;
@@ -73,6 +74,176 @@ __global__ __launch_bounds__(64) void rope_kernel(RopeArgs a) {
       to[d] = from_f<C>(sc ? y / sc[hh] : y);
     }
   }
+}
+
+constexpr int kWaves = 4;
+constexpr int64_t kTokens = 32768;   // of one launch
+
+// x of eight dims
+template <typename T> __device__ __forceinline__ void load8(const T* p, float* x) {
+  T v[8];
+  __builtin_memcpy(v, __builtin_assume_aligned(p, 8 * sizeof(T)), 8 * sizeof(T));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = to_f(v[e]);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float* x) {
+  T v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = from_f<T>(x[e]);
+  __builtin_memcpy(__builtin_assume_aligned(p, 8 * sizeof(T)), v, 8 * sizeof(T));
+}
+template <> __device__ __forceinline__ void store8(fp8_t* p, const float* x) {
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = x[e] != x[e] ? x[e] : fminf(fmaxf(x[e], -kFp8Max), kFp8Max);
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
+  *(int2*)p = make_int2(lo, hi);
+}
+
+template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+// the sum over the 8, 16 or 32 lanes of a head: across pairs, quads, halves of a row and a row by DPP, then over two rows
+template <int LPH> __device__ __forceinline__ float head_sum(float x) {
+  x = dpp_add<0xB1>(x);    // quad_perm 1, 0, 3, 2
+  x = dpp_add<0x4E>(x);    // quad_perm 2, 3, 0, 1
+  x = dpp_add<0x141>(x);   // row_half_mirror
+  if constexpr (LPH >= 16) x = dpp_add<0x140>(x);   // row_mirror
+  if constexpr (LPH >= 32) x += __shfl_xor(x, 16);
+  return x;
+}
+
+// Eight dims to a lane, DP / 8 lanes to a head, so that a wave reads 64 x 16 bytes of neighbouring heads at once; a token's
+// waves go over its heads with the token's cosines and sines and both norms' weights in registers.  Pairs that are
+// rot / 2 apart meet by a shuffle of the normalized values (rot a multiple of 16: a lane's dims have their partners in
+// one other lane); interleaved pairs are a lane's own (rot a multiple of 8).  One pass over the bytes, which bound it.
+template <typename T, typename C, int DP, bool INTER>
+__global__ __launch_bounds__(64 * kWaves) void rope_kernel(RopeArgs a, int waves) {
+  constexpr int LPH = DP / 8, HPW = 64 / LPH;   // lanes of a head, heads of a wave
+  const int64_t item = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int64_t t = item / waves;
+  const int part = (int)(item - t * waves);
+  if (t >= a.tokens) return;
+  const int lane = threadIdx.x & 63, sub = lane & (LPH - 1), d = sub * 8, D = a.dim, half = a.rot >> 1;
+  const bool live = d < D;
+  const int at = live ? d : 0;
+  const float nan = __builtin_nanf("");
+  const int64_t pos = index_at(a.positions, a.wide_positions, t);
+  const bool in = pos >= 0 && pos < a.table_rows;
+  const bool turned = live && d < a.rot, second = d >= half;
+  float cs[8], sn[8], wq[8], wk[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) { cs[e] = 1.f; sn[e] = 0.f; wq[e] = wk[e] = 1.f; }
+  if (turned && in) {
+    if constexpr (INTER) {
+      const float4 c = *(const float4*)(a.table + pos * a.rot + (d >> 1)), s = *(const float4*)(a.table + pos * a.rot + half + (d >> 1));
+      cs[0] = cs[1] = c.x; cs[2] = cs[3] = c.y; cs[4] = cs[5] = c.z; cs[6] = cs[7] = c.w;
+      sn[0] = -s.x; sn[1] = s.x; sn[2] = -s.y; sn[3] = s.y; sn[4] = -s.z; sn[5] = s.z; sn[6] = -s.w; sn[7] = s.w;
+    } else {
+      const float* row = a.table + pos * a.rot + (second ? d - half : d);
+      load8(row, cs);
+      load8(row + half, sn);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sn[e] = second ? sn[e] : -sn[e];
+    }
+  }
+  auto weights = [&](const void* w, float* to) {
+    if (!w) return;
+    if (a.weight_f32) load8((const float*)w + at, to);
+    else load8((const T*)w + at, to);
+    if (a.unit_offset)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[e] += 1.f;
+  };
+  weights(a.q_weight, wq);
+  weights(a.k_weight, wk);
+  int64_t page = 0, place = 0;
+  bool keep = false;
+  if (a.store) {
+    const int64_t slot = index_at(a.slots, a.wide_slots, t);
+    const int64_t room = (int64_t)a.kv.pages * a.kv.page_size;
+    keep = live && slot >= 0 && slot < room;
+    if (keep) {
+      page = room >> 32 ? slot / a.kv.page_size : (uint32_t)slot / (uint32_t)a.kv.page_size;   // a division in 64 bits costs
+      place = slot - page * a.kv.page_size;
+    }
+  }
+  const int heads = a.q_heads + a.k_heads + (a.store ? a.kv.heads : 0), hop = waves * HPW;
+  for (int h = part * HPW + lane / LPH; h - lane / LPH < heads; h += hop) {   // the same for all lanes
+    const bool some = h < heads, is_q = h < a.q_heads, is_v = h >= a.q_heads + a.k_heads;
+    const int hh = !some ? 0 : is_q ? h : is_v ? h - a.q_heads - a.k_heads : h - a.q_heads;
+    const T* from = is_q ? (const T*)a.q + t * a.q_row + hh * a.q_head
+                         : is_v ? (const T*)a.v + t * a.v_row + hh * a.v_head : (const T*)a.k + t * a.k_row + hh * a.k_head;
+    float x[8], y[8];
+    if (some && live) load8(from + at, x);
+    else
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+    ss = head_sum<LPH>(ss);
+    const bool norm = is_q ? a.q_weight != nullptr : a.k_weight != nullptr;
+    const float r = norm && !is_v ? rsqrtf(ss / D + a.eps) : 1.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= is_v ? 1.f : r * (is_q ? wq[e] : wk[e]);
+    if constexpr (INTER) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = x[e] * cs[e] + x[e ^ 1] * sn[e];
+    } else {
+      const int mate = turned ? (second ? lane - half / 8 : lane + half / 8) : lane;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = x[e] * cs[e] + __shfl(x[e], mate) * sn[e];
+    }
+    if (!some || !live) continue;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = is_v || !turned ? x[e] : y[e];   // a partner that is not finite stays out of what is not turned
+    if (!in && !is_v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = nan;
+    if (is_q) store8((T*)a.out_q + t * a.oq_row + hh * a.oq_head + d, y);
+    else if (!is_v && a.out_k) store8((T*)a.out_k + t * a.ok_row + hh * a.ok_head + d, y);
+    if (!is_q && keep) {
+      const float* sc = is_v ? a.kv.v_scale : a.kv.k_scale;
+      C* to = is_v ? (C*)a.kv.v + page * a.kv.v_page + place * a.kv.v_token + hh * a.kv.v_head
+                   : (C*)a.kv.k + page * a.kv.k_page + place * a.kv.k_token + hh * a.kv.k_head;
+      if (sc) {
+        const float s = sc[hh];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] /= s;
+      }
+      store8(to + d, y);
+    }
+  }
+}
+
+template <typename T, typename C, int DP>
+void launch(const RopeArgs& a, bool inter, hipStream_t st) {
+  const int heads = a.q_heads + a.k_heads + (a.store ? a.kv.heads : 0), rounds = (heads + 512 / DP - 1) / (512 / DP);
+  // Waves of a token: one round of heads each until the launch fills the device, then 4
+  const int waves = a.tokens <= 128 ? rounds : std::min(rounds, 4);
+  const dim3 grid((unsigned)(((int64_t)a.tokens * waves + kWaves - 1) / kWaves));
+  if (inter) rope_kernel<T, C, DP, true><<<grid, 64 * kWaves, 0, st>>>(a, waves);
+  else rope_kernel<T, C, DP, false><<<grid, 64 * kWaves, 0, st>>>(a, waves);
+}
+
+template <typename T, typename C>
+void launch(const RopeArgs& a, hipStream_t st) {
+  // whole lanes of pairs, tables and weights that take 16-byte loads: the vector form; else a wave per head
+  const bool inter = a.interleaved;
+  const uint64_t bits = (uintptr_t)a.table | (uintptr_t)a.q_weight | (uintptr_t)a.k_weight;
+  if (a.rot % (inter ? 8 : 16) == 0 && !(bits & 15)) {
+    if (a.dim <= 64) launch<T, C, 64>(a, inter, st);
+    else if (a.dim <= 128) launch<T, C, 128>(a, inter, st);
+    else launch<T, C, 256>(a, inter, st);
+    return;
+  }
+  const int heads = a.q_heads + a.k_heads + (a.store ? a.kv.heads : 0);
+  rope_any_kernel<T, C><<<dim3(heads, (unsigned)a.tokens), 64, 0, st>>>(a);
 }
 
 }  // namespace
@@ -127,21 +298,19 @@ extern "C" int gqk_qk_norm_rope(const gqk_heads* q, const gqk_heads* k, const gq
   if (pages) { a.kv = *pages; a.store = 1; }
   const hipStream_t st = (hipStream_t)stream;
   const bool bf = dtype == GQK_DTYPE_BF16, f8 = pages && pages->dtype == GQK_DTYPE_FP8;
-  const int heads = a.q_heads + a.k_heads + (pages ? pages->heads : 0);
-  for (int64_t t0 = 0; t0 < tokens; t0 += 32768) {   // the grid's second dimension is limited
-    const dim3 grid(heads, (unsigned)(tokens - t0 < 32768 ? tokens - t0 : 32768));
-    if (bf && f8) rope_kernel<bf16_t, fp8_t><<<grid, 64, 0, st>>>(a);
-    else if (bf) rope_kernel<bf16_t, bf16_t><<<grid, 64, 0, st>>>(a);
-    else if (f8) rope_kernel<f16_t, fp8_t><<<grid, 64, 0, st>>>(a);
-    else rope_kernel<f16_t, f16_t><<<grid, 64, 0, st>>>(a);
-    const int64_t step = 32768;
-    a.q = (const char*)a.q + 2 * step * a.q_row;
-    if (a.k) a.k = (const char*)a.k + 2 * step * a.k_row;
-    if (a.v) a.v = (const char*)a.v + 2 * step * a.v_row;
-    a.out_q = (char*)a.out_q + 2 * step * a.oq_row;
-    if (a.out_k) a.out_k = (char*)a.out_k + 2 * step * a.ok_row;
-    a.positions = (const char*)a.positions + step * (positions_64 ? 8 : 4);
-    if (a.slots) a.slots = (const char*)a.slots + step * (slots_64 ? 8 : 4);
+  for (int64_t t0 = 0; t0 < tokens; t0 += kTokens) {   // a grid's dimensions are limited
+    a.tokens = (int)std::min<int64_t>(tokens - t0, kTokens);
+    if (bf && f8) launch<bf16_t, fp8_t>(a, st);
+    else if (bf) launch<bf16_t, bf16_t>(a, st);
+    else if (f8) launch<f16_t, fp8_t>(a, st);
+    else launch<f16_t, f16_t>(a, st);
+    a.q = (const char*)a.q + 2 * kTokens * a.q_row;
+    if (a.k) a.k = (const char*)a.k + 2 * kTokens * a.k_row;
+    if (a.v) a.v = (const char*)a.v + 2 * kTokens * a.v_row;
+    a.out_q = (char*)a.out_q + 2 * kTokens * a.oq_row;
+    if (a.out_k) a.out_k = (char*)a.out_k + 2 * kTokens * a.ok_row;
+    a.positions = (const char*)a.positions + kTokens * (positions_64 ? 8 : 4);
+    if (a.slots) a.slots = (const char*)a.slots + kTokens * (slots_64 ? 8 : 4);
   }
   return decode_launched(what);
 }
