@@ -43,15 +43,16 @@ __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c, f16_t) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// Up to 16 TT rows of one block that go with one adapter (or with none, kNone, or a bad id, kBad).
-template <int TT> struct Unit {
+// Rows of one block that go with one adapter (or with none, kNone, or a bad id, kBad).
+struct Unit {
   int adapter, count;
-  int row[TT];   // row of tile t's column lane % 16 (of a column past the count: some row of the unit)
+  const int* row;   // their numbers within the block
 };
 
-// Unit u of the block's rows: adapters in the order of their first row, each one's rows in order.  A lane holds
-// one row's id; a ballot finds the rows that share it.  False: the block has fewer units.
-template <int TT> __device__ __forceinline__ bool find_unit(const LoraArgs& a, int64_t row0, int u, Unit<TT>& out) {
+// Unit u (of up to `most` rows) of the block's rows: adapters in the order of their first row, each one's rows in order.
+// A lane holds one row's id; a ballot finds the rows that share it, whose numbers go to LDS in order, a list for each
+// wave.  False: the block has fewer units.  All waves find the same.
+__device__ __forceinline__ bool find_unit(const LoraArgs& a, int64_t row0, int u, int most, int* lists, Unit& out) {
   const int lane = threadIdx.x & 63;
   const int64_t m = row0 + lane;
   int id = kNone;
@@ -63,19 +64,15 @@ template <int TT> __device__ __forceinline__ bool find_unit(const LoraArgs& a, i
   while (left) {
     const int who = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
     const uint64_t same = __ballot(id == who) & left;
-    const int count = __popcll(same), units = (count + 16 * TT - 1) / (16 * TT);
+    const int count = __popcll(same), units = (count + most - 1) / most;
     if (u < units) {
       out.adapter = who;
-      out.count = min(count - u * 16 * TT, 16 * TT);
-      // the lane with place i among them sends its row to lane i; the others' go where nobody looks, or later
-      const int place = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0)) - u * 16 * TT;
-      const bool in = (same >> lane & 1) && place >= 0 && place < out.count;
-      __shared__ int rows[8][kBlock];
-      int* mine = rows[threadIdx.x >> 6];
-      if (in) mine[place] = lane;
+      out.count = min(count - u * most, most);
+      const int place = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0)) - u * most;
+      int* mine = lists + (threadIdx.x >> 6) * kBlock;
+      if ((same >> lane & 1) && place >= 0 && place < out.count) mine[place] = lane;
       __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int t = 0; t < TT; ++t) out.row[t] = mine[min(t * 16 + (lane & 15), out.count - 1)];
+      out.row = mine;
       return true;
     }
     u -= units;
@@ -84,61 +81,80 @@ template <int TT> __device__ __forceinline__ bool find_unit(const LoraArgs& a, i
   return false;
 }
 
+// 16 bytes at a byte offset from a base that the whole wave shares; zeros past `bytes`
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)min(bytes, (int64_t)0x7ffffff0), 0x00020000);
+}
+constexpr uint32_t kOutside = 0x80000000u;   // an offset past every buffer
+__device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset, uint32_t shared) {
+  return __builtin_amdgcn_raw_buffer_load_b128(rs, offset, shared, 0);
+}
+
 // h = A x of one unit's rows, 64 ranks, one split of K: the ranks are the matrix instruction's rows and the batch
 // rows its columns, both operands straight from global memory (8 values along K per lane).  The waves split the split's
-// steps of 32 among themselves and join in LDS, in order.
+// steps among themselves and join in LDS, in order.  A step is 64 values of K, so that a wave reads whole 128-byte lines
+// of every row.
 template <typename T, int TT>
 __global__ __launch_bounds__(64 * kDownWaves, 2) void lora_down_kernel(LoraArgs a) {
-  constexpr int kDepth = TT == 1 ? 3 : 2;   // steps in flight
+  constexpr int kDepth = 2;   // steps in flight
   __shared__ __align__(16) float red[kDownWaves][16][kHPad];
+  __shared__ int lists[kDownWaves * kBlock];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int chunk = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
   const int64_t row0 = (int64_t)blockIdx.z * kBlock;
   const int PR = a.parts * a.rank, rank0 = chunk * 16 * kRankTiles, tiles = min(kRankTiles, (PR - rank0 + 15) / 16);
-  const int64_t all = (a.K + 31) / 32, s0 = all * split / a.splits, s1 = all * (split + 1) / a.splits;
+  const int all = (int)((a.K + 63) / 64), s0 = (int)((int64_t)all * split / a.splits), s1 = (int)((int64_t)all * (split + 1) / a.splits);
+  const int K = (int)a.K, tail = K % 64;
   for (int u = blockIdx.y;; u += gridDim.y) {
-    Unit<TT> unit;
-    if (!find_unit(a, row0, u, unit)) return;
+    Unit unit;
+    if (!find_unit(a, row0, u, 16 * TT, lists, unit)) return;
     if (unit.adapter < 0) continue;
     const int rows = (unit.count + 15) / 16;   // tiles of rows
-    const T* A[kRankTiles];
-    const T* x[TT];
+    const T* A = (const T*)a.a + ((int64_t)unit.adapter * PR + rank0) * a.K;
+    const T* X = (const T*)a.x + row0 * a.x_row;
+    const __amdgpu_buffer_rsrc_t ra = buffer_of(A, (int64_t)min(16 * kRankTiles, PR - rank0) * a.K * 2);
+    const __amdgpu_buffer_rsrc_t rx = buffer_of(X, ((int64_t)kBlock * a.x_row) * 2);
+    uint32_t ao[kRankTiles], xo[TT];
 #pragma unroll
-    for (int t = 0; t < kRankTiles; ++t)
-      A[t] = (const T*)a.a + ((int64_t)unit.adapter * PR + min(rank0 + t * 16 + n, PR - 1)) * a.K + g * 8;
+    for (int t = 0; t < kRankTiles; ++t) ao[t] = min(t * 16 + n, PR - rank0 - 1) * (uint32_t)K * 2 + g * 16;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) x[t] = (const T*)a.x + (row0 + unit.row[t]) * a.x_row + g * 8;
+    for (int t = 0; t < TT; ++t) xo[t] = unit.row[min(t * 16 + n, unit.count - 1)] * (uint32_t)a.x_row * 2 + g * 16;
     v4f acc[kRankTiles][TT];
 #pragma unroll
     for (int r = 0; r < kRankTiles; ++r)
 #pragma unroll
       for (int t = 0; t < TT; ++t) acc[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
-    v4u av[kDepth][kRankTiles], xv[kDepth][TT];
-    auto load = [&](int d, int64_t s) {
-      const int64_t k = s * 32;
-      const bool in = k + g * 8 < a.K;   // K may end inside the step
+    v4u av[kDepth][2][kRankTiles], xv[kDepth][2][TT];
+    auto load = [&](int d, int s) {
+      const uint32_t at = s * 128;
+      const bool whole = tail == 0 || s + 1 < all;   // K may end inside the last step
 #pragma unroll
-      for (int t = 0; t < TT; ++t)
-        if (t < rows) xv[d][t] = in ? *(const v4u*)(x[t] + k) : v4u{0, 0, 0, 0};
+      for (int k = 0; k < 2; ++k) {
+        const bool in = whole || k * 32 + g * 8 < tail;
 #pragma unroll
-      for (int t = 0; t < kRankTiles; ++t)
-        if (t < tiles) av[d][t] = in ? *(const v4u*)(A[t] + k) : v4u{0, 0, 0, 0};
+        for (int t = 0; t < TT; ++t)
+          if (t < rows) xv[d][k][t] = load16(rx, in ? xo[t] + k * 64 : kOutside, at);
+#pragma unroll
+        for (int t = 0; t < kRankTiles; ++t)
+          if (t < tiles) av[d][k][t] = load16(ra, in ? ao[t] + k * 64 : kOutside, at);
+      }
     };
-    const int64_t steps = s1 - s0 > wave ? (s1 - s0 - wave + kDownWaves - 1) / kDownWaves : 0;
-    const int64_t first = s0 + wave;
+    const int steps = s1 - s0 > wave ? (s1 - s0 - wave + kDownWaves - 1) / kDownWaves : 0, first = s0 + wave;
 #pragma unroll
     for (int d = 0; d < kDepth; ++d)
       if (d < steps) load(d, first + d * kDownWaves);
-    for (int64_t i = 0; i < steps; i += kDepth)
+    for (int i = 0; i < steps; i += kDepth)
 #pragma unroll
       for (int d = 0; d < kDepth; ++d)
         if (i + d < steps) {
 #pragma unroll
-          for (int r = 0; r < kRankTiles; ++r)
-            if (r < tiles)
+          for (int k = 0; k < 2; ++k)
 #pragma unroll
-              for (int t = 0; t < TT; ++t)
-                if (t < rows) acc[r][t] = mfma(av[d][r], xv[d][t], acc[r][t], T{});
+            for (int r = 0; r < kRankTiles; ++r)
+              if (r < tiles)
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+                  if (t < rows) acc[r][t] = mfma(av[d][k][r], xv[d][k][t], acc[r][t], T{});
           if (i + d + kDepth < steps) load(d, first + (i + d + kDepth) * kDownWaves);
         }
     // lane (n, g) holds ranks 16 r + 4 g .. + 3 of column n
@@ -151,7 +167,6 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void lora_down_kernel(LoraArgs 
         if (r < tiles) *(v4f*)&red[wave][n][r * 16 + g * 4] = acc[r][t];
       __syncthreads();
       const int row = threadIdx.x >> 5, c = (threadIdx.x & 31) * 2;   // 16 rows, 2 ranks a thread
-      const int at = __shfl(unit.row[t], row & 15);                   // lane row of this wave holds its number
       if (t * 16 + row < unit.count && rank0 + c < PR) {
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -159,7 +174,7 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void lora_down_kernel(LoraArgs 
           sum.x += red[w][row][c];
           sum.y += red[w][row][c + 1];
         }
-        *(float2*)(a.h + ((int64_t)split * a.M + row0 + at) * PR + rank0 + c) = sum;
+        *(float2*)(a.h + ((int64_t)split * a.M + row0 + unit.row[t * 16 + row]) * PR + rank0 + c) = sum;
       }
     }
   }
@@ -169,14 +184,20 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void lora_down_kernel(LoraArgs 
 // product as two values of T each, h = hi + lo, in one instruction: 16 ranks of hi and the same 16 of lo against B's 16
 // ranks twice (rounding h to T alone would put 2^-9 of the update, for bf16, on top of the output's own rounding; the second
 // half of the instruction would be idle).  fp16 takes h over a power of two near its row's largest, to stay in range.
+// B and y of a wave's first columns are on their way while h is gathered, those of the next while these are computed.
 template <typename T, int TT>
 __global__ __launch_bounds__(64 * kUpWaves, 2) void lora_up_kernel(LoraArgs a) {
-  constexpr bool kF16 = sizeof(T) == 2 && __is_same(T, f16_t);
-  __shared__ __align__(16) T hs[TT * 16][2][256 + 8];   // [row][hi, lo][rank]
+  constexpr bool kF16 = __is_same(T, f16_t);
+  constexpr int kSteps = 4;                               // 16-rank steps of B that are loaded ahead
+  constexpr int kRowThreads = 64 * kUpWaves / (16 * TT);  // threads that gather one row of h
+  constexpr int kOctets = 32 / kRowThreads;               // octets of ranks of one of them, at most
+  extern __shared__ __align__(16) char lds[];             // h: [16 TT rows][hi, lo][ranks + 8]
   __shared__ float factor[TT * 16];
+  __shared__ int lists[kUpWaves * kBlock];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int64_t row0 = (int64_t)blockIdx.z * kBlock;
-  const int PR = a.parts * a.rank, steps = (a.rank + 15) / 16;
+  const int PR = a.parts * a.rank, steps = (a.rank + 15) / 16, hrow = steps * 16 + 8;
+  T* const hs = (T*)lds;
   // the part and its columns
   int part = 0, block = blockIdx.x;
   int64_t begin = 0;
@@ -186,123 +207,155 @@ __global__ __launch_bounds__(64 * kUpWaves, 2) void lora_up_kernel(LoraArgs a) {
     block -= blocks;
     begin = a.ends[part++];
   }
-  const int64_t c_begin = begin + (int64_t)block * a.columns, c_end = min(a.ends[part], c_begin + a.columns);
+  const int64_t c_begin = begin + (int64_t)block * a.columns;
+  const int width = (int)min(a.ends[part] - c_begin, (int64_t)a.columns);
   for (int u = blockIdx.y;; u += gridDim.y) {
-    Unit<TT> unit;
-    if (!find_unit(a, row0, u, unit)) return;
+    Unit unit;
+    if (!find_unit(a, row0, u, 16 * TT, lists, unit)) return;
+    const bool some = unit.adapter >= 0;
     if (unit.adapter == kNone && a.out == a.y) continue;
     const int rows = (unit.count + 15) / 16;
-    if (unit.adapter >= 0) {
-      __syncthreads();   // the last unit's h has been read
-      const float s = a.scales ? a.scales[unit.adapter] : 1.f;
-      // 16 threads a row, 8 ranks each at a time
-      for (int t = 0; t < rows; ++t) {
-        int mine = 0;
+    const __amdgpu_buffer_rsrc_t rb = buffer_of(
+        (const T*)a.b + ((int64_t)max(unit.adapter, 0) * a.N + c_begin) * a.rank, some ? (int64_t)width * a.rank * 2 : 0);
+    const T* y[TT];
+    T* out[TT];
 #pragma unroll
-        for (int k = 0; k < TT; ++k) mine = k == t ? unit.row[k] : mine;
-        const int r = threadIdx.x >> 4, c = threadIdx.x & 15;      // 16 rows of the tile
-        const int64_t m = row0 + __shfl(mine, r);
-        float v[2][8];
-        float top = 0.f;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int rank = (q * 16 + c) * 8;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[q][e] = 0.f;
-          if (rank < a.rank)
-            for (int sp = 0; sp < a.splits; ++sp) {
-              const v4f* from = (const v4f*)(a.h + ((int64_t)sp * a.M + m) * PR + part * a.rank + rank);
-              const v4f lo = from[0], hi = from[1];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                v[q][e] += lo[e];
-                v[q][4 + e] += hi[e];
-              }
-            }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[q][e]));
-        }
-        float down = 1.f, up = 1.f;
-        if constexpr (kF16) {
-          for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-          if (top > 0.f && top < __builtin_huge_valf()) {
-            const int e = min(max(ilogbf(top), -100), 100);
-            down = ldexpf(1.f, -e);
-            up = ldexpf(1.f, e);
-          }
-        }
-        if (c == 0) factor[t * 16 + r] = s * up;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int rank = (q * 16 + c) * 8;
-          if (rank < steps * 16) {
-            T hi[8], lo[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float f = v[q][e] * down;
-              hi[e] = (T)f;
-              const float back = (float)hi[e];
-              lo[e] = fabsf(back) < __builtin_huge_valf() ? (T)(f - back) : (T)0.f;   // inf stays, without inf - inf
-            }
-            __builtin_memcpy(&hs[t * 16 + r][0][rank], hi, 16);
-            __builtin_memcpy(&hs[t * 16 + r][1][rank], lo, 16);
-          }
-        }
-      }
-      __syncthreads();
+    for (int t = 0; t < TT; ++t) {
+      const int64_t m = row0 + unit.row[min(t * 16 + n, unit.count - 1)];
+      y[t] = (const T*)a.y + m * a.y_row + c_begin + g * 8;
+      out[t] = (T*)a.out + m * a.out_row + c_begin + g * 8;
     }
-    float f[TT];
-#pragma unroll
-    for (int t = 0; t < TT; ++t) f[t] = unit.adapter >= 0 && t < rows ? factor[t * 16 + n] : 0.f;
     // 32 columns at a time: as rows of two 16-row tiles dealt so that a lane gets 8 in a row of its batch row
-    for (int64_t c0 = c_begin + wave * 32; c0 < c_end; c0 += 32 * kUpWaves) {
+    v4u bv[2][kSteps][2], yv[2][TT];
+    auto load_b = [&](v4u (&to)[kSteps][2], int c0, int k0) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t at = min(c0 + (n >> 2) * 8 + c * 4 + (n & 3), width - 1) * (uint32_t)a.rank * 2 + (g & 1) * 16;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+          if (k0 + k < steps) to[k][c] = load16(rb, (k0 + k) * 16 + (g & 1) * 8 < a.rank ? at + k * 32 : kOutside, k0 * 32);
+      }
+    };
+    auto load = [&](int buf, int c0) {
+      if (some) load_b(bv[buf], c0, 0);
+      if (a.wide_y)
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+          if (t * 16 + n < unit.count && c0 + g * 8 + 8 <= width) yv[buf][t] = *(const v4u*)(y[t] + c0);
+    };
+    float f[TT];
+    auto finish = [&](int buf, int c0) {
       v4f acc[2][TT];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int t = 0; t < TT; ++t) acc[c][t] = v4f{0.f, 0.f, 0.f, 0.f};
-      if (unit.adapter >= 0) {
-        const T* B[2];
+      if (some)
+        for (int k0 = 0; k0 < steps; k0 += kSteps) {
+          if (k0 > 0) load_b(bv[buf], c0, k0);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int64_t col = min(c0 + (n >> 2) * 8 + c * 4 + (n & 3), c_end - 1);
-          B[c] = (const T*)a.b + ((int64_t)unit.adapter * a.N + col) * a.rank + (g & 1) * 8;
+          for (int k = 0; k < kSteps; ++k)
+            if (k0 + k < steps)
+#pragma unroll
+              for (int t = 0; t < TT; ++t)
+                if (t < rows) {
+                  const v4u hv = *(const v4u*)(hs + ((t * 16 + n) * 2 + (g >> 1)) * hrow + (k0 + k) * 16 + (g & 1) * 8);
+#pragma unroll
+                  for (int c = 0; c < 2; ++c) acc[c][t] = mfma(bv[buf][k][c], hv, acc[c][t], T{});
+                }
         }
-        for (int k = 0; k < steps; ++k) {
-          v4u bv[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) bv[c] = k * 16 + (g & 1) * 8 < a.rank ? *(const v4u*)(B[c] + k * 16) : v4u{0, 0, 0, 0};
-#pragma unroll
-          for (int t = 0; t < TT; ++t)
-            if (t < rows) {
-              const v4u hv = *(const v4u*)&hs[t * 16 + n][g >> 1][k * 16 + (g & 1) * 8];
-#pragma unroll
-              for (int c = 0; c < 2; ++c) acc[c][t] = mfma(bv[c], hv, acc[c][t], T{});
-            }
-        }
-      }
-      const int64_t col = c0 + g * 8;
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
         if (t * 16 + n >= unit.count) continue;
-        const int64_t m = row0 + unit.row[t];
-        const T* y = (const T*)a.y + m * a.y_row + col;
-        T* out = (T*)a.out + m * a.out_row + col;
         auto value = [&](float base, int e) {
-          return unit.adapter >= 0 ? base + acc[e >> 2][t][e & 3] * f[t] : unit.adapter == kNone ? base : __builtin_nanf("");
+          return some ? base + acc[e >> 2][t][e & 3] * f[t] : unit.adapter == kNone ? base : __builtin_nanf("");
         };
-        if (a.wide_y && col + 8 <= c_end) {
+        if (a.wide_y && c0 + g * 8 + 8 <= width) {
           T v[8];
-          __builtin_memcpy(v, __builtin_assume_aligned(y, 16), 16);
+          __builtin_memcpy(v, &yv[buf][t], 16);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = (T)value((float)v[e], e);
-          __builtin_memcpy(__builtin_assume_aligned(out, 16), v, 16);
+          __builtin_memcpy(__builtin_assume_aligned(out[t] + c0, 16), v, 16);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (col + e < c_end) out[e] = (T)value((float)y[e], e);
+            if (c0 + g * 8 + e < width) out[t][c0 + e] = (T)value((float)y[t][c0 + e], e);
         }
       }
+    };
+    constexpr int hop = 32 * kUpWaves;
+    int c0 = wave * 32;
+    if (c0 < width) load(0, c0);
+    if (some) {
+      __syncthreads();   // the last unit's h has been read
+      const int r = threadIdx.x / kRowThreads, c = threadIdx.x % kRowThreads;
+      const int64_t m = row0 + unit.row[min(r, unit.count - 1)];
+      float v[kOctets][8], top = 0.f;
+#pragma unroll
+      for (int q = 0; q < kOctets; ++q) {
+        const int rank = (q * kRowThreads + c) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[q][e] = 0.f;
+        if (rank < a.rank && r < rows * 16) {
+          const float* from = a.h + m * PR + part * a.rank + rank;
+          const int64_t hop_h = (int64_t)a.M * PR;
+          for (int sp = 0; sp < a.splits; sp += 4) {
+            v4f lo[4], hi[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const v4f* p = (const v4f*)(from + min(sp + j, a.splits - 1) * hop_h);
+              lo[j] = p[0];
+              hi[j] = p[1];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (sp + j < a.splits)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  v[q][e] += lo[j][e];
+                  v[q][4 + e] += hi[j][e];
+                }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[q][e]));
+      }
+      float down = 1.f, up = 1.f;
+      if constexpr (kF16) {
+        for (int o = kRowThreads / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if (top > 0.f && top < __builtin_huge_valf()) {
+          const int e = min(max(ilogbf(top), -100), 100);
+          down = ldexpf(1.f, -e);
+          up = ldexpf(1.f, e);
+        }
+      }
+      if (c == 0) factor[r] = (a.scales ? a.scales[unit.adapter] : 1.f) * up;
+#pragma unroll
+      for (int q = 0; q < kOctets; ++q) {
+        const int rank = (q * kRowThreads + c) * 8;
+        if (rank < steps * 16 && r < rows * 16) {
+          T hi[8], lo[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float x = v[q][e] * down;
+            hi[e] = (T)x;
+            const float back = (float)hi[e];
+            lo[e] = fabsf(back) < __builtin_huge_valf() ? (T)(x - back) : (T)0.f;   // inf stays, without inf - inf
+          }
+          __builtin_memcpy(hs + (r * 2) * hrow + rank, hi, 16);
+          __builtin_memcpy(hs + (r * 2 + 1) * hrow + rank, lo, 16);
+        }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) f[t] = some && t < rows ? factor[t * 16 + n] : 0.f;
+    for (; c0 < width; c0 += 2 * hop) {
+      if (c0 + hop < width) load(1, c0 + hop);
+      finish(0, c0);
+      if (c0 + hop >= width) break;
+      if (c0 + 2 * hop < width) load(0, c0 + 2 * hop);
+      finish(1, c0 + hop);
     }
   }
 }
@@ -316,8 +369,8 @@ Cut cut_of(int M, int64_t K, int parts, int rank) {
   c.chunks = (parts * rank + 16 * kRankTiles - 1) / (16 * kRankTiles);
   c.blocks = (M + kBlock - 1) / kBlock;
   const int64_t wgs = (int64_t)c.chunks * (M <= kBlock ? std::min(M, 16) : c.blocks);
-  const int64_t steps = (K + 31) / 32;
-  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / wgs, steps / (2 * kDownWaves), 16}));
+  const int64_t steps = (K + 63) / 64;
+  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / wgs, steps / kDownWaves, 16}));
   return c;
 }
 
@@ -331,7 +384,8 @@ void launch(const LoraArgs& g, const Cut& c, hipStream_t st) {
     begin = g.ends[p];
   }
   if (g.slots > 0) lora_down_kernel<T, TT><<<dim3(c.splits * c.chunks, units, c.blocks), 64 * kDownWaves, 0, st>>>(g);
-  lora_up_kernel<T, TT><<<dim3((unsigned)blocks, units, c.blocks), 64 * kUpWaves, 0, st>>>(g);
+  const size_t lds = (size_t)16 * TT * 2 * ((g.rank + 15) / 16 * 16 + 8) * sizeof(T);
+  lora_up_kernel<T, TT><<<dim3((unsigned)blocks, units, c.blocks), 64 * kUpWaves, lds, st>>>(g);
 }
 
 }  // namespace
@@ -367,6 +421,8 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
                        (long long)out_row, (long long)x_row, (long long)g.N, (long long)K);
   if (M == 0) return GQK_OK;
   if (!y || !x || !ids || !out || (slots > 0 && (!a || !b))) return decode_fail(GQK_ERR_ARG, "lora_add: null pointer");
+  if (K > GQK_LORA_MAX_K || x_row > GQK_LORA_MAX_K)
+    return decode_fail(GQK_ERR_SHAPE, "lora_add: K %lld or x's row stride %lld above %d", (long long)K, (long long)x_row, GQK_LORA_MAX_K);
   if (((uintptr_t)x | (uintptr_t)a | (uintptr_t)b) & 15 || x_row & 7)
     return decode_fail(GQK_ERR_SHAPE, "lora_add: x, a and b are 16-byte aligned, x's row stride a multiple of 8");
   if (!workspace || workspace_bytes < need || (uintptr_t)workspace & 255)
@@ -380,9 +436,9 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
   g.splits = c.splits; g.chunks = c.chunks;
   g.wide_y = !(((uintptr_t)y | (uintptr_t)out) & 15) && !((y_row | out_row) & 7);
   for (int p = 0; p + 1 < parts; ++p) g.wide_y &= g.ends[p] % 8 == 0;
-  // columns of a workgroup of the second kernel: 1024, fewer where the launch would have too few of them
+  // columns of a workgroup of the second kernel: 512, fewer where the launch would have too few of them
   const int64_t groups = M <= kBlock ? std::min(M, 16) : c.blocks;
-  g.columns = 1024;
+  g.columns = 512;
   while (g.columns > 128 && groups * (g.N / g.columns) < 512) g.columns /= 2;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == GQK_DTYPE_BF16) {

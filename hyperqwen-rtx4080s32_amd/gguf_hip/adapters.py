@@ -14,7 +14,7 @@ from ._lib import check, lib
 from .eager import direct as _direct, stream as _stream
 
 _TYPES = {torch.bfloat16: _lib.GQK_DTYPE_BF16, torch.float16: _lib.GQK_DTYPE_F16}
-MAX_PARTS, MAX_RANK = 8, 256
+MAX_PARTS, MAX_RANK, MAX_K = 8, 256, 1 << 23
 
 
 @lru_cache(maxsize=256)
@@ -94,8 +94,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     for t in (a, b):
         if t.dtype != x.dtype or t.device != x.device or not t.is_contiguous() or not ops._addr_aligned(t, 16):
             raise ValueError(f"{what}: a and b are contiguous, 16-byte aligned {x.dtype} on {x.device}")
-    if K == 0 or K % 8 or a.shape[2] < 8 or a.shape[2] % 8 or a.shape[2] > MAX_RANK:
-        raise ValueError(f"{what}: K {K} and rank {a.shape[2]} must be multiples of 8, the rank at most {MAX_RANK}")
+    if K == 0 or K % 8 or K > MAX_K or a.shape[2] < 8 or a.shape[2] % 8 or a.shape[2] > MAX_RANK:
+        raise ValueError(f"{what}: K {K} and rank {a.shape[2]} must be multiples of 8, the rank at most {MAX_RANK}, K {MAX_K}")
     for t in (y, out):
         if t is not None and (t.shape != (M, N) or t.dtype != x.dtype or t.device != x.device):
             raise ValueError(f"{what}: y and out are {x.dtype} [{M}, {N}] on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -109,7 +109,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     inplace = out is y
     if (N > 1 and y.stride(1) != 1) or (M > 1 and y.stride(0) < N):
         y = y.contiguous()
-    if x.stride(1) != 1 or (M > 1 and (x.stride(0) % 8 or x.stride(0) < K)) or not ops._addr_aligned(x, 16):
+    if x.stride(1) != 1 or (M > 1 and (x.stride(0) % 8 or not K <= x.stride(0) <= MAX_K)) or not ops._addr_aligned(x, 16):
         x = x.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty((M, N), dtype=x.dtype, device=x.device)

@@ -188,8 +188,10 @@ int gqk_linear_noalloc(const void* packed, const int32_t* desc_dev, const gqk_pl
  * out may be y; a [slots, parts, rank, K] and b [slots, sum(n_outs), rank] of the same type, contiguous, K and
  * rank multiples of 8, rank <= 256 (adapters of a lower rank are padded with zeros), parts <= 8; ids
  * int32 [M], or int64 with ids_64; scales fp32 [slots] or NULL (1).  x, a, b are 16-byte aligned.  Products
- * and sums are in fp32, rounded once to out.  workspace: gqk_lora_workspace_bytes bytes, 256-byte aligned; its
+ * and sums are in fp32, rounded once to out.  K and x's row stride (where M > 1) are at most GQK_LORA_MAX_K.
+ * workspace: gqk_lora_workspace_bytes bytes, 256-byte aligned; its
  * first GQK_CTR_BYTES are left alone, so that a linear layer's workspace serves (calls in stream order). */
+#define GQK_LORA_MAX_K 8388608 /* 64 rows stay below 2^30 bytes */
 int64_t gqk_lora_workspace_bytes(int M, int64_t K, int parts, int rank);
 int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int M, int64_t K, const void* a,
                  const void* b, int slots, int parts, const int64_t* n_outs, int rank, const void* ids, int ids_64,
