@@ -30,6 +30,10 @@ int check_pages(const char* what, const gqk_pages* p, int q_dtype) {
   const int64_t strides[6] = {p->k_page, p->k_token, p->k_head, p->v_page, p->v_token, p->v_head};
   for (int64_t s : strides)
     if (s < 0 || s % 8) return decode_fail(GQK_ERR_SHAPE, "%s: page strides are multiples of 8 elements, not %lld", what, (long long)s);
+  if (p->k_token > GQK_MAX_TOKEN_STRIDE || p->v_token > GQK_MAX_TOKEN_STRIDE || p->k_page > GQK_MAX_PAGE_STRIDE ||
+      p->v_page > GQK_MAX_PAGE_STRIDE)
+    return decode_fail(GQK_ERR_SHAPE, "%s: pages further apart than %d elements, or their tokens than %d", what, GQK_MAX_PAGE_STRIDE,
+                       GQK_MAX_TOKEN_STRIDE);
   if ((uintptr_t)p->k % align || (uintptr_t)p->v % align)
     return decode_fail(GQK_ERR_SHAPE, "%s: pages must be %lld-byte aligned", what, (long long)align);
   if ((uintptr_t)p->k_scale % 4 || (uintptr_t)p->v_scale % 4)
@@ -47,7 +51,8 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kWaves = 4;             // waves of a workgroup
 constexpr int kTile = 32;             // keys of a wave's step
-constexpr int kMaxRowWeights = 4096;  // splits x rows of a unit: the joining workgroup keeps their weights in LDS
+constexpr int kJoinSplits = 16;       // splits that the last workgroup of a sequence joins; more go to a launch of their own
+constexpr int kMostSplits = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct AttnArgs {
@@ -67,7 +72,7 @@ struct AttnArgs {
   int row_waves;        // 16-row tiles of query heads that a workgroup's waves deal among themselves
   int row_blocks;       // workgroups over the query heads of one key head
   int chunk, splits;    // keys of a split, and the most splits of a sequence
-  uint32_t magic;       // key / page_size = key * magic >> shift, exact below 2^31
+  uint32_t magic;       // key / page_size = 2 key magic >> 32 >> shift, exact below 2^31
   int shift;
 };
 
@@ -109,6 +114,21 @@ __device__ __forceinline__ float sum4(float x) {
 // The exponent's base of a running maximum: nothing was seen yet (-inf) must not become -inf - -inf.
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_huge_valf() ? 0.f : m; }
 
+// Partial sums over a split's keys, relative to its maximum, added up in order.
+struct Joined {
+  float m = -__builtin_huge_valf(), l = 0.f;
+  v4f o{0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(v2u stat, v4u sums) {
+    float s[2];
+    __builtin_memcpy(s, &stat, 8);
+    const float mn = fmaxf(m, s[0]), mb = base_of(mn);
+    const float f = __builtin_amdgcn_exp2f(m - mb), g = __builtin_amdgcn_exp2f(s[0] - mb);
+    m = mn;
+    l = l * f + s[1] * g;
+    o = o * f + __builtin_bit_cast(v4f, sums) * g;
+  }
+};
+
 // A workgroup takes one split (a.chunk keys) of one sequence's keys of one key head, for up to 16 row_waves query heads
 // that share it; its waves deal the 32-key steps of the split (and the 16-row tiles of the heads) among themselves.
 //
@@ -118,7 +138,7 @@ __device__ __forceinline__ float base_of(float m) { return m == -__builtin_huge_
 // rows of the two 16-key tiles are dealt so), which is what O^T += V^T P^T wants of it as an operand.  K comes from global
 // memory straight as operands (8 dims of a key per lane).  V's operands hold 8 keys of one dim: a lane loads 8 dims of
 // each of its 8 keys and transposes the 8 x 8 block in registers, one v_perm per pair.  No LDS, no barrier in the loop.
-template <typename T, typename C, int DP, bool FULL, bool P8>
+template <typename T, typename C, int DP, bool FULL, bool P8, bool TIGHT>
 __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kernel(AttnArgs a) {
   constexpr bool F8 = sizeof(C) == 1;
   constexpr int NM = DP / 32;                 // k-steps of a score
@@ -126,6 +146,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
   constexpr int NH = DP / (16 * VD);          // V loads of a key per lane
   constexpr int NT = NH * VD;                 // 16-dim tiles of the output
   constexpr int KW = F8 ? 2 : 4;              // words of 8 dims
+  constexpr int RB = DP * (int)sizeof(C);     // bytes of a key (FULL)
   constexpr int RS = DP + 4;                  // row stride of the reduction buffer
   constexpr bool QLDS = DP == 256;
   __shared__ __align__(16) float red[kWaves * 16 * RS];
@@ -162,12 +183,12 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
     const int32_t* table = a.table + (int64_t)b * a.table_row;
     const char* kb = (const char*)a.kv.k + kvh * a.kv.k_head * (int64_t)sizeof(C);
     const char* vb = (const char*)a.kv.v + kvh * a.kv.v_head * (int64_t)sizeof(C);
-    const int64_t k_page = a.kv.k_page * (int64_t)sizeof(C), k_tok = a.kv.k_token * (int64_t)sizeof(C);
-    const int64_t v_page = a.kv.v_page * (int64_t)sizeof(C), v_tok = a.kv.v_token * (int64_t)sizeof(C);
+    const uint32_t k_page = (uint32_t)a.kv.k_page * sizeof(C), k_tok = TIGHT ? RB : (uint32_t)a.kv.k_token * sizeof(C);
+    const uint32_t v_page = (uint32_t)a.kv.v_page * sizeof(C), v_tok = TIGHT ? RB : (uint32_t)a.kv.v_token * sizeof(C);
     const int ps = a.kv.page_size, last = len - 1;
     // first dim of k-step i's operand: 16 bytes of a key per load
     auto dim_at = [&](int i) { return F8 && FULL ? (i >> 1) * 64 + g * 16 + (i & 1) * 8 : i * 32 + g * 8; };
-    auto page_of = [&](int key) { return (int)(((uint64_t)(uint32_t)key * a.magic) >> a.shift); };
+    auto page_of = [&](int key) { return (int)(__umulhi(2u * (uint32_t)key, a.magic) >> a.shift); };
 
     // Queries stay in registers as operands; at 256 dims, where they would not fit beside K, V and the sums, in the
     // wave's own part of the reduction buffer, which is free until its loop ends.
@@ -187,74 +208,109 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
 
     // The keys of a lane: as rows of K's two tiles, group n / 4 of 8 keys, places n % 4 and 4 + n % 4; for V all 8 of
     // group g.  Keys outside of [first, last] are read as the nearest inside (their weight is 0).
-    struct Pages { int k[P8 ? 1 : 2], v[P8 ? 1 : 8]; };
-    auto key_k = [&](int base, int c) { return min(max(base + (n >> 2) * 8 + c * 4 + (n & 3), first), last); };
-    auto key_v = [&](int base, int j) { return min(max(base + g * 8 + j, first), last); };
-    auto lookup = [&](int base) {
-      Pages p;
-      if constexpr (P8) {   // 8 keys from a multiple of 8 lie in one page; so do those of them that are inside
-        p.k[0] = table[page_of(key_k(base, 0))];
-        p.v[0] = table[page_of(key_v(base, 0))];
-      } else {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) p.k[c] = table[page_of(key_k(base, c))];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p.v[j] = table[page_of(key_v(base, j))];
-      }
-      return p;
+    struct Pages { int page, place; };
+    auto find = [&](int key) {
+      const int at = page_of(key);
+      return Pages{table[at], key - at * ps};
     };
-    auto checked = [&](int page) {   // a page outside of the cache is not read
-      const bool out = (uint32_t)page >= (uint32_t)a.kv.pages;
+    auto check = [&](Pages& p) {   // a page outside of the cache is not read
+      const bool out = (uint32_t)p.page >= (uint32_t)a.kv.pages;
       bad |= out;
-      return out ? 0 : page;
+      p.page = out ? 0 : p.page;
+    };
+    auto inside = [&](int base) { return base >= first && base + kTile <= len; };
+    // The page of group g's first key and the place of that key in it: 8 keys from a multiple of 8 lie in one page, and
+    // so do those of them that are inside.  Where pages do not hold whole groups (P8 false), every load finds its own.
+    auto lookup = [&](int base) {
+      if constexpr (!P8) return Pages{0, 0};
+      return find(min(max(base + g * 8, first), last));
     };
     uint32_t kr[2][NM][KW];   // two 16-key tiles of K
     uint32_t vr[8][NH][VD * (int)sizeof(C) / 4];
-    auto load_k = [&](int base, const Pages& p) {
+    auto take_k = [&](int c, const char* row) {
+      if constexpr (F8 && FULL) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int key = key_k(base, c);
-        const char* at = kb + checked(p.k[P8 ? 0 : c]) * k_page + (key - page_of(key) * ps) * k_tok;
-        if constexpr (F8 && FULL) {
+        for (int i = 0; i < NM; i += 2) {
+          const v4u x = *(const v4u*)(row + dim_at(i));
+          kr[c][i][0] = x.x; kr[c][i][1] = x.y; kr[c][i + 1][0] = x.z; kr[c][i + 1][1] = x.w;
+        }
+      } else {
 #pragma unroll
-          for (int i = 0; i < NM; i += 2) {
-            const v4u x = *(const v4u*)(at + dim_at(i));
-            kr[c][i][0] = x.x; kr[c][i][1] = x.y; kr[c][i + 1][0] = x.z; kr[c][i + 1][1] = x.w;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < NM; ++i) {
-            const int d = dim_at(i);
-            const char* src = at + (FULL || d < D ? d : 0) * (int)sizeof(C);
-            if constexpr (F8) {
-              const v2u x = *(const v2u*)src;
-              kr[c][i][0] = x.x; kr[c][i][1] = x.y;
-            } else {
-              const v4u x = *(const v4u*)src;
-              kr[c][i][0] = x.x; kr[c][i][1] = x.y; kr[c][i][2] = x.z; kr[c][i][3] = x.w;
-            }
+        for (int i = 0; i < NM; ++i) {
+          const int d = dim_at(i);
+          const char* src = row + (FULL || d < D ? d : 0) * (int)sizeof(C);
+          if constexpr (F8) {
+            const v2u x = *(const v2u*)src;
+            kr[c][i][0] = x.x; kr[c][i][1] = x.y;
+          } else {
+            const v4u x = *(const v4u*)src;
+            kr[c][i][0] = x.x; kr[c][i][1] = x.y; kr[c][i][2] = x.z; kr[c][i][3] = x.w;
           }
         }
       }
     };
-    auto load_v = [&](int base, const Pages& p) {
+    auto take_v = [&](int j, const char* row) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = key_v(base, j);
-        const char* at = vb + checked(p.v[P8 ? 0 : j]) * v_page + (key - page_of(key) * ps) * v_tok;
+      for (int h = 0; h < NH; ++h) {
+        const int d = h * 16 * VD + n * VD;
+        const char* src = row + (FULL || d < D ? d : 0) * (int)sizeof(C);
+        if constexpr (VD * sizeof(C) == 16) {
+          const v4u x = *(const v4u*)src;
+          vr[j][h][0] = x.x; vr[j][h][1] = x.y; vr[j][h][2] = x.z; vr[j][h][3] = x.w;
+        } else if constexpr (VD * sizeof(C) == 8) {
+          const v2u x = *(const v2u*)src;
+          vr[j][h][0] = x.x; vr[j][h][1] = x.y;
+        } else {
+          vr[j][h][0] = *(const uint32_t*)src;
+        }
+      }
+    };
+    // A row is at base + page * page stride + place * token stride; inside of the sequence a group's rows follow one
+    // another, a constant apart where a page is one run (TIGHT), so that a step's loads share one address.
+    auto load_k = [&](int base, const Pages& p) {
+      if constexpr (P8) {
+        const int src = (n >> 2) * 16;
+        const uint32_t page = __shfl(p.page, src);
+        const int place = __shfl(p.place, src);
+        const char* at = kb + (uint64_t)page * k_page;
+        if (inside(base)) {
+          const char* row = at + (uint64_t)(uint32_t)(place + (n & 3)) * k_tok;
+          take_k(0, row);
+          take_k(1, row + 4 * (TIGHT ? (uint32_t)RB : k_tok));
+        } else {
+          const int own = min(max(base + (n >> 2) * 8, first), last);
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          const int d = h * 16 * VD + n * VD;
-          const char* src = at + (FULL || d < D ? d : 0) * (int)sizeof(C);
-          if constexpr (VD * sizeof(C) == 16) {
-            const v4u x = *(const v4u*)src;
-            vr[j][h][0] = x.x; vr[j][h][1] = x.y; vr[j][h][2] = x.z; vr[j][h][3] = x.w;
-          } else if constexpr (VD * sizeof(C) == 8) {
-            const v2u x = *(const v2u*)src;
-            vr[j][h][0] = x.x; vr[j][h][1] = x.y;
-          } else {
-            vr[j][h][0] = *(const uint32_t*)src;
+          for (int c = 0; c < 2; ++c) {
+            const int key = min(max(base + (n >> 2) * 8 + c * 4 + (n & 3), first), last);
+            take_k(c, at + (uint64_t)(uint32_t)(place + key - own) * k_tok);
           }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          Pages one = find(min(max(base + (n >> 2) * 8 + c * 4 + (n & 3), first), last));
+          check(one);
+          take_k(c, kb + (uint64_t)(uint32_t)one.page * k_page + (uint64_t)(uint32_t)one.place * k_tok);
+        }
+      }
+    };
+    auto load_v = [&](int base, const Pages& p) {
+      if constexpr (P8) {
+        const char* at = vb + (uint64_t)(uint32_t)p.page * v_page + (uint64_t)(uint32_t)p.place * v_tok;
+        if (inside(base)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) take_v(j, at + j * (TIGHT ? (uint32_t)RB : v_tok));
+        } else {
+          const int own = min(max(base + g * 8, first), last);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) take_v(j, at + (uint32_t)(min(max(base + g * 8 + j, first), last) - own) * v_tok);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          Pages one = find(min(max(base + g * 8 + j, first), last));
+          check(one);
+          take_v(j, vb + (uint64_t)(uint32_t)one.page * v_page + (uint64_t)(uint32_t)one.place * v_tok);
         }
       }
     };
@@ -262,6 +318,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
     const int hop = kTile * nkw;
     int base = k_begin + kTile * kw;
     Pages now = lookup(base);
+    check(now);
     load_k(base, now);
     load_v(base, now);
     Pages next = lookup(base + hop);   // past the split: clamped, still a key of the sequence
@@ -284,18 +341,31 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
         }
       }
       const bool more = s + 1 < steps;
-      if (more) load_k(base + hop, next);
+      if (more) {
+        check(next);
+        load_k(base + hop, next);
+      }
       const bool edge = base < first || base + kTile > k_end;
       float top = -inf;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = base + g * 8 + j;
-        float x = sc[j >> 2][j & 3] * scale;
-        if (edge && (key < first || key >= k_end)) x = -inf;
-        sc[j >> 2][j & 3] = x;
-        top = fmaxf(top, x);
+      for (int j = 0; j < 8; ++j) sc[j >> 2][j & 3] *= scale;
+      if (edge) {
+        asm volatile("");   // a branch: most steps have no edge
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = base + g * 8 + j;
+          if (key < first || key >= k_end) sc[j >> 2][j & 3] = -inf;
+        }
       }
-      const float mn = fmaxf(m, max4(top)), mb = base_of(mn), c = __builtin_amdgcn_exp2f(m - mb);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[j >> 2][j & 3]);
+      const float mn = fmaxf(m, max4(top)), mb = base_of(mn);
+      if (__any(mn != m)) {   // rarely, once the first keys were seen
+        const float c = __builtin_amdgcn_exp2f(m - mb);
+        l *= c;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] *= c;
+      }
       m = mn;
       float sum = 0.f, p[8];
 #pragma unroll
@@ -303,10 +373,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
         p[j] = __builtin_amdgcn_exp2f(sc[j >> 2][j & 3] - mb);
         sum += p[j];
       }
-      l = l * c + sum;
+      l += sum;
       const v4u pt{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
-#pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t] *= c;
       if (edge) {   // a weight of 0 does not silence a value that is not finite
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -378,7 +446,6 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
   const int quads = D / 4;
   // [splits][R][D], then [splits][R][2] (room for a full block's rows in every unit)
   float* part = a.partials + unit * a.splits * min(rows_wg, group) * (D + 4);
-  float* part_stat = part + (int64_t)a.splits * R * D;
   auto store = [&](int r, int d, v4f x, float f) {
     T* to = (T*)a.out + b * a.out_row + (int64_t)(kvh * group + row0 + r) * a.out_head + d;
     *(v2u*)to = v2u{pack2<T>(x[0] * f, x[1] * f), pack2<T>(x[2] * f, x[3] * f)};
@@ -412,9 +479,9 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
                                               (a.splits * R * D + (split * R + r) * 2) * 4, 0, kDevice);
     }
   }
-  if (ns == 1) return;
+  if (ns == 1 || a.splits > kJoinSplits) return;
   // The sequence's splits join in the workgroup that arrives last, in split order: partials move through device-coherent
-  // accesses alone; every store is complete before the arrival count.
+  // accesses alone; every store is complete before the arrival count.  All of a value's loads are in flight at once.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) flag = __hip_atomic_fetch_add(a.counters + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -422,40 +489,73 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
   if (flag != ns - 1) return;
   asm volatile("" ::: "memory");
   if (threadIdx.x == 0) __hip_atomic_store(a.counters + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // next launch
-  float* weight = red;   // [ns][R][2]: (maximum, sum), then (weight, sum)
-  for (int x = threadIdx.x; x < ns * R; x += 64 * kWaves) {
-    const v2u y = __builtin_amdgcn_raw_buffer_load_b64(rs, (a.splits * R * D + x * 2) * 4, 0, kDevice);
-    *(v2u*)(weight + 2 * x) = y;
-  }
-  __syncthreads();
-  for (int r = threadIdx.x; r < R; r += 64 * kWaves) {
-    float M = -inf, L = 0.f;
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, weight[2 * (s * R + r)]);
-    const float Mb = base_of(M);
-    for (int s = 0; s < ns; ++s) {
-      const float f = __builtin_amdgcn_exp2f(weight[2 * (s * R + r)] - Mb);
-      L += weight[2 * (s * R + r) + 1] * f;
-      weight[2 * (s * R + r)] = f;
-    }
-    stat[r][0] = L == 0.f ? 0.f : v_scale / L;
-    if (a.lse) store_lse(r, M, L);
-  }
-  __syncthreads();
   for (int x = threadIdx.x; x < R * quads; x += 64 * kWaves) {
     const int r = x / quads, d = (x - r * quads) * 4;
-    v4f o{0.f, 0.f, 0.f, 0.f};
+    v2u st[kJoinSplits];
+    v4u y[kJoinSplits];
+#pragma unroll
+    for (int s = 0; s < kJoinSplits; ++s)
+      if (s < ns) {
+        st[s] = __builtin_amdgcn_raw_buffer_load_b64(rs, (a.splits * R * D + (s * R + r) * 2) * 4, 0, kDevice);
+        y[s] = __builtin_amdgcn_raw_buffer_load_b128(rs, ((s * R + r) * D + d) * 4, 0, kDevice);
+      }
+    Joined j;
+#pragma unroll
+    for (int s = 0; s < kJoinSplits; ++s)
+      if (s < ns) j.add(st[s], y[s]);
+    store(r, d, j.o, j.l == 0.f ? 0.f : v_scale / j.l);
+    if (a.lse && d == 0) store_lse(r, j.m, j.l);
+  }
+}
+
+// The join of more splits than one workgroup takes at once: a workgroup for each query head, its threads over the splits and
+// the dims.  (One workgroup per sequence and key head took 16 us for 64 splits of 5 heads, 39 for 128 of 16.)
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
+  __shared__ __align__(16) float sums[256][4];
+  __shared__ float stat[256][2];
+  const int b = blockIdx.y, h = blockIdx.x, group = a.q_heads / a.kv.heads, kvh = h / group, D = a.kv.dim;
+  const int rows_wg = 16 * a.row_waves, rb = h % group / rows_wg, r = h % group - rb * rows_wg, R = min(rows_wg, group - rb * rows_wg);
+  const int len0 = max(0, a.lengths[b]), len = len0 > a.max_length ? 0 : len0;
+  const int first = a.window > 0 ? max(0, len - a.window) : 0, start = first & ~(kTile - 1);
+  const int ns = max(1, (len - start + a.chunk - 1) / a.chunk);
+  if (ns == 1) return;   // written already
+  const int64_t unit = ((int64_t)b * a.kv.heads + kvh) * a.row_blocks + rb;
+  const float* part = a.partials + unit * a.splits * min(rows_wg, group) * (D + 4);
+  const float* part_stat = part + (int64_t)a.splits * R * D;
+  const int quads = D / 4, lanes = 256 / quads, own = threadIdx.x / quads, d = (threadIdx.x - own * quads) * 4;
+  Joined j;
+  if (own < lanes) {
     constexpr int kBatch = 8;
-    for (int s0 = 0; s0 < ns; s0 += kBatch) {
+    for (int s0 = own; s0 < ns; s0 += kBatch * lanes) {
+      v2u st[kBatch];
       v4u y[kBatch];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        y[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, ((min(s0 + j, ns - 1) * R + r) * D + d) * 4, 0, kDevice);
+      for (int k = 0; k < kBatch; ++k) {
+        const int s = min(s0 + k * lanes, ns - 1);
+        st[k] = *(const v2u*)(part_stat + (s * R + r) * 2);
+        y[k] = *(const v4u*)(part + (s * R + r) * D + d);
+      }
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        if (s0 + j < ns) o += __builtin_bit_cast(v4f, y[j]) * weight[2 * ((s0 + j) * R + r)];
+      for (int k = 0; k < kBatch; ++k)
+        if (s0 + k * lanes < ns) j.add(st[k], y[k]);
     }
-    store(r, d, o, stat[r][0]);
   }
+  *(v4f*)sums[threadIdx.x] = j.o;
+  stat[threadIdx.x][0] = j.m;
+  stat[threadIdx.x][1] = j.l;
+  __syncthreads();
+  if (own > 0) return;
+  Joined all;
+  for (int k = 0; k < lanes; ++k) {
+    const int x = k * quads + threadIdx.x;
+    all.add(*(const v2u*)stat[x], *(const v4u*)sums[x]);
+  }
+  const float f = all.l == 0.f ? 0.f : (a.kv.v_scale ? a.kv.v_scale[kvh] : 1.f) / all.l;
+  T* to = (T*)a.out + b * a.out_row + h * a.out_head + d;
+  *(v2u*)to = v2u{pack2<T>(all.o[0] * f, all.o[1] * f), pack2<T>(all.o[2] * f, all.o[3] * f)};
+  if (a.lse && threadIdx.x == 0)
+    a.lse[(int64_t)b * a.q_heads + h] = all.l == 0.f ? -__builtin_huge_valf() : (all.m + __builtin_amdgcn_logf(all.l)) * kLn2;
 }
 
 // How a call is cut: workgroups over the query heads of a key head, and splits of `chunk` keys.
@@ -471,20 +571,22 @@ Cut cut_of(int batch, int q_heads, int kv_heads, int dim, int max_length, int wi
   const int64_t units = (int64_t)batch * kv_heads * c.row_blocks, wanted = 4LL * device_cus();
   const int64_t least = kTile * kWaves;   // keys of the shortest split
   int64_t splits = std::max<int64_t>(1, std::min((wanted + units - 1) / std::max<int64_t>(1, units), (span + least - 1) / least));
-  splits = std::min<int64_t>(splits, kMaxRowWeights / 2 / (16 * c.row_waves));
+  splits = std::min<int64_t>(splits, kMostSplits);
   if (units > GQK_CTR_WORDS) splits = 1;
   c.chunk = (int)std::max<int64_t>(kTile, ((span + splits - 1) / splits + kTile - 1) / kTile * kTile);
   c.splits = (int)std::max<int64_t>(1, (span + c.chunk - 1) / c.chunk);
   return c;
 }
 
+// The general form takes any head dim up to DP and any page size; whole heads (FULL), pages of a multiple of 8 tokens (P8)
+// and pages that are one run of memory (TIGHT) have fewer addresses to compute, the last one for each step.
 template <typename T, typename C, int DP>
 void launch(const AttnArgs& a, dim3 grid, bool full, hipStream_t st) {
-  const bool p8 = a.kv.page_size % 8 == 0;
-  if (full && p8) attention_kernel<T, C, DP, true, true><<<grid, 64 * kWaves, 0, st>>>(a);
-  else if (full) attention_kernel<T, C, DP, true, false><<<grid, 64 * kWaves, 0, st>>>(a);
-  else if (p8) attention_kernel<T, C, DP, false, true><<<grid, 64 * kWaves, 0, st>>>(a);
-  else attention_kernel<T, C, DP, false, false><<<grid, 64 * kWaves, 0, st>>>(a);
+  const bool p8 = a.kv.page_size % 8 == 0, tight = a.kv.k_token == DP && a.kv.v_token == DP;
+  if (full && p8 && tight) attention_kernel<T, C, DP, true, true, true><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (full && p8) attention_kernel<T, C, DP, true, true, false><<<grid, 64 * kWaves, 0, st>>>(a);
+  else if (p8) attention_kernel<T, C, DP, false, true, false><<<grid, 64 * kWaves, 0, st>>>(a);
+  else attention_kernel<T, C, DP, false, false, false><<<grid, 64 * kWaves, 0, st>>>(a);
 }
 
 template <typename T, typename C>
@@ -548,8 +650,8 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
   // below 2^(31 + bits)
   int bits = 0;
   while (((int64_t)1 << bits) < pages->page_size) ++bits;
-  a.shift = 31 + bits;
-  a.magic = (uint32_t)((((uint64_t)1 << a.shift) + pages->page_size - 1) / pages->page_size);
+  a.shift = bits;
+  a.magic = (uint32_t)((((uint64_t)1 << (31 + bits)) + pages->page_size - 1) / pages->page_size);
   const dim3 grid(pages->heads * c.row_blocks, batch, c.splits);
   const hipStream_t st = (hipStream_t)stream;
   const bool bf = dtype == GQK_DTYPE_BF16;
@@ -560,6 +662,10 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
     launch<bf16_t, bf16_t>(a, grid, st);
   } else {
     launch<f16_t, f16_t>(a, grid, st);
+  }
+  if (c.splits > kJoinSplits) {
+    if (bf) attention_join_kernel<bf16_t><<<dim3(q_heads, batch), 256, 0, st>>>(a);
+    else attention_join_kernel<f16_t><<<dim3(q_heads, batch), 256, 0, st>>>(a);
   }
   return decode_launched("paged_attention");
 }

@@ -199,9 +199,11 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
                  void* stream);
 
 /* The pages of one layer's key-value cache: k and v as [pages, page_size, heads, dim] with any strides
- * (in elements, multiples of 8; dims side by side), so that a token's heads or a head's tokens may lie together.
+ * (in elements, multiples of 8, at most GQK_MAX_PAGE_STRIDE and of tokens GQK_MAX_TOKEN_STRIDE; dims side by side), so that a token's heads or a head's tokens may lie together.
  * dtype: the heads' own type, or GQK_DTYPE_FP8, whose values stand for themselves times k_scale / v_scale
  * (fp32 [heads] in device memory, NULL: 1).  Pages are aligned to 8 elements. */
+#define GQK_MAX_PAGE_STRIDE 2147483640
+#define GQK_MAX_TOKEN_STRIDE 33554432
 typedef struct gqk_pages {
   void* k;
   void* v;
