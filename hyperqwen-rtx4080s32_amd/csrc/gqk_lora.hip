@@ -5,6 +5,7 @@
 // with i = ids[m] the row's adapter (negative: out = y) and p(n) the part (q, k, v; gate, up) that
 // column n belongs to.  h is kept in 32 bits in the workspace, after its counter region.
 #include <algorithm>
+#include <type_traits>
 #include "gqk_decode.h"
 
 namespace gqk {
@@ -16,10 +17,10 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kParts = 8;
-constexpr int kDownWaves = 8, kUpWaves = 4;
+constexpr int kWaves = 4;
+constexpr int kStage = 128;      // values of K that the first kernel takes at a time
 constexpr int kBlock = 64;       // rows whose adapters a workgroup sorts out: one per lane
 constexpr int kRankTiles = 4;    // 16-rank tiles of a workgroup of the first kernel
-constexpr int kHPad = 68;        // row stride of its sums in LDS
 constexpr int kNone = -1, kBad = -2;
 
 struct LoraArgs {
@@ -90,91 +91,93 @@ __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset
   return __builtin_amdgcn_raw_buffer_load_b128(rs, offset, shared, 0);
 }
 
-// h = A x of one unit's rows, 64 ranks, one split of K: the ranks are the matrix instruction's rows and the batch
-// rows its columns, both operands straight from global memory (8 values along K per lane).  The waves split the split's
-// steps among themselves and join in LDS, in order.  A step is 64 values of K, so that a wave reads whole 128-byte lines
-// of every row.
+// h = A x of one unit's rows, 64 ranks, one split of K.  Rows of x and of A are far apart, and a lane of a matrix operand
+// holds 16 bytes of one: loaded like that nothing coalesces (62 L1 accesses a load counted).  So 256 bytes of each row at a
+// time come in as rows, 16 lanes to one, go through LDS with their 16-byte pieces swapped by the row's number (16 rows'
+// pieces of one k-step in different banks), and are read as operands: ranks as the instruction's rows, batch rows as its
+// columns.  Loads run kDepth stages ahead in registers; two LDS buffers, one barrier a stage.  A wave takes one 16-row tile and all
+// ranks (TT = 4), or all 16 rows and one 16-rank tile (TT = 1).
 template <typename T, int TT>
-__global__ __launch_bounds__(64 * kDownWaves, 2) void lora_down_kernel(LoraArgs a) {
-  constexpr int kDepth = 2;   // steps in flight
-  __shared__ __align__(16) float red[kDownWaves][16][kHPad];
-  __shared__ int lists[kDownWaves * kBlock];
+__global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
+  constexpr int kDepth = TT == 1 ? 4 : 2;
+  constexpr int kRows = 16 * TT, kAcc = TT == 1 ? 1 : kRankTiles;
+  __shared__ __align__(16) char buf[2][(kRows + 16 * kRankTiles) * 256];
+  __shared__ int lists[kWaves * kBlock];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int chunk = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
   const int64_t row0 = (int64_t)blockIdx.z * kBlock;
   const int PR = a.parts * a.rank, rank0 = chunk * 16 * kRankTiles, tiles = min(kRankTiles, (PR - rank0 + 15) / 16);
-  const int all = (int)((a.K + 63) / 64), s0 = (int)((int64_t)all * split / a.splits), s1 = (int)((int64_t)all * (split + 1) / a.splits);
-  const int K = (int)a.K, tail = K % 64;
+  const int all = (int)((a.K + kStage - 1) / kStage);
+  const int s0 = (int)((int64_t)all * split / a.splits), stages = (int)((int64_t)all * (split + 1) / a.splits) - s0;
+  const int K = (int)a.K, row = threadIdx.x >> 4, piece = threadIdx.x & 15;
   for (int u = blockIdx.y;; u += gridDim.y) {
     Unit unit;
-    if (!find_unit(a, row0, u, 16 * TT, lists, unit)) return;
+    if (!find_unit(a, row0, u, kRows, lists, unit)) return;
     if (unit.adapter < 0) continue;
     const int rows = (unit.count + 15) / 16;   // tiles of rows
-    const T* A = (const T*)a.a + ((int64_t)unit.adapter * PR + rank0) * a.K;
-    const T* X = (const T*)a.x + row0 * a.x_row;
-    const __amdgpu_buffer_rsrc_t ra = buffer_of(A, (int64_t)min(16 * kRankTiles, PR - rank0) * a.K * 2);
-    const __amdgpu_buffer_rsrc_t rx = buffer_of(X, ((int64_t)kBlock * a.x_row) * 2);
+    const __amdgpu_buffer_rsrc_t ra = buffer_of((const T*)a.a + ((int64_t)unit.adapter * PR + rank0) * a.K,
+                                                (int64_t)min(16 * kRankTiles, PR - rank0) * a.K * 2);
+    const __amdgpu_buffer_rsrc_t rx = buffer_of((const T*)a.x + row0 * a.x_row, (int64_t)kBlock * a.x_row * 2);
     uint32_t ao[kRankTiles], xo[TT];
 #pragma unroll
-    for (int t = 0; t < kRankTiles; ++t) ao[t] = min(t * 16 + n, PR - rank0 - 1) * (uint32_t)K * 2 + g * 16;
+    for (int t = 0; t < kRankTiles; ++t) ao[t] = min(t * 16 + row, PR - rank0 - 1) * (uint32_t)K * 2 + piece * 16;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) xo[t] = unit.row[min(t * 16 + n, unit.count - 1)] * (uint32_t)a.x_row * 2 + g * 16;
-    v4f acc[kRankTiles][TT];
-#pragma unroll
-    for (int r = 0; r < kRankTiles; ++r)
-#pragma unroll
-      for (int t = 0; t < TT; ++t) acc[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
-    v4u av[kDepth][2][kRankTiles], xv[kDepth][2][TT];
+    for (int t = 0; t < TT; ++t) xo[t] = unit.row[min(t * 16 + row, unit.count - 1)] * (uint32_t)a.x_row * 2 + piece * 16;
+    v4u av[kDepth][kRankTiles], xv[kDepth][TT];
     auto load = [&](int d, int s) {
-      const uint32_t at = s * 128;
-      const bool whole = tail == 0 || s + 1 < all;   // K may end inside the last step
+      const bool in = s * kStage + piece * 8 < K;   // K may end inside the last stage
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const bool in = whole || k * 32 + g * 8 < tail;
+      for (int t = 0; t < TT; ++t)
+        if (t < rows) xv[d][t] = load16(rx, in ? xo[t] : kOutside, s * (2 * kStage));
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
-          if (t < rows) xv[d][k][t] = load16(rx, in ? xo[t] + k * 64 : kOutside, at);
-#pragma unroll
-        for (int t = 0; t < kRankTiles; ++t)
-          if (t < tiles) av[d][k][t] = load16(ra, in ? ao[t] + k * 64 : kOutside, at);
-      }
+      for (int t = 0; t < kRankTiles; ++t)
+        if (t < tiles) av[d][t] = load16(ra, in ? ao[t] : kOutside, s * (2 * kStage));
     };
-    const int steps = s1 - s0 > wave ? (s1 - s0 - wave + kDownWaves - 1) / kDownWaves : 0, first = s0 + wave;
+    v4f acc[kAcc];
+#pragma unroll
+    for (int r = 0; r < kAcc; ++r) acc[r] = v4f{0.f, 0.f, 0.f, 0.f};
+    const bool busy = wave < (TT == 1 ? tiles : rows);
 #pragma unroll
     for (int d = 0; d < kDepth; ++d)
-      if (d < steps) load(d, first + d * kDownWaves);
-    for (int i = 0; i < steps; i += kDepth)
+      if (d < stages) load(d, s0 + d);
+    __syncthreads();   // the last unit's stages have been read
+    for (int i = 0; i < stages; i += kDepth)
 #pragma unroll
       for (int d = 0; d < kDepth; ++d)
-        if (i + d < steps) {
+        if (i + d < stages) {
+          char* const to = buf[d & 1];   // kDepth is even
+          char* const at = to + row * 256 + (piece ^ row) * 16;
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
+          for (int t = 0; t < TT; ++t)
+            if (t < rows) *(v4u*)(at + t * 4096) = xv[d][t];
 #pragma unroll
-            for (int r = 0; r < kRankTiles; ++r)
-              if (r < tiles)
+          for (int t = 0; t < kRankTiles; ++t)
+            if (t < tiles) *(v4u*)(at + (TT + t) * 4096) = av[d][t];
+          if (i + d + kDepth < stages) load(d, s0 + i + d + kDepth);
+          __syncthreads();
+          if (busy)
 #pragma unroll
-                for (int t = 0; t < TT; ++t)
-                  if (t < rows) acc[r][t] = mfma(av[d][k][r], xv[d][k][t], acc[r][t], T{});
-          if (i + d + kDepth < steps) load(d, first + (i + d + kDepth) * kDownWaves);
+            for (int k = 0; k < kStage / 32; ++k) {
+              const char* from = to + n * 256 + ((k * 4 + g) ^ n) * 16;
+              const v4u xop = *(const v4u*)(from + (TT == 1 ? 0 : wave) * 4096);
+              if constexpr (TT == 1) {
+                acc[0] = mfma(*(const v4u*)(from + (TT + wave) * 4096), xop, acc[0], T{});
+              } else {
+                // of tiles that the chunk does not have too: sums that nobody reads cost less than the copies that a branch
+                // around each instruction takes (64 moves a product counted)
+#pragma unroll
+                for (int r = 0; r < kRankTiles; ++r) acc[r] = mfma(*(const v4u*)(from + (TT + r) * 4096), xop, acc[r], T{});
+              }
+            }
         }
-    // lane (n, g) holds ranks 16 r + 4 g .. + 3 of column n
+    // lane (n, g) holds ranks 4 g .. + 3 of a tile for row n
+    const int r_at = (TT == 1 ? 0 : wave) * 16 + n;
+    if (busy && r_at < unit.count) {
+      float* to = a.h + ((int64_t)split * a.M + row0 + unit.row[r_at]) * PR;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      if (t >= rows) break;
-      __syncthreads();
-#pragma unroll
-      for (int r = 0; r < kRankTiles; ++r)
-        if (r < tiles) *(v4f*)&red[wave][n][r * 16 + g * 4] = acc[r][t];
-      __syncthreads();
-      const int row = threadIdx.x >> 5, c = (threadIdx.x & 31) * 2;   // 16 rows, 2 ranks a thread
-      if (t * 16 + row < unit.count && rank0 + c < PR) {
-        float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kDownWaves; ++w) {
-          sum.x += red[w][row][c];
-          sum.y += red[w][row][c + 1];
-        }
-        *(float2*)(a.h + ((int64_t)split * a.M + row0 + unit.row[t * 16 + row]) * PR + rank0 + c) = sum;
+      for (int r = 0; r < kAcc; ++r) {
+        const int rank = rank0 + (TT == 1 ? wave : r) * 16 + g * 4;
+        if ((TT == 1 || r < tiles) && rank < PR) *(v4f*)(to + rank) = acc[r];
       }
     }
   }
@@ -184,20 +187,29 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void lora_down_kernel(LoraArgs 
 // product as two values of T each, h = hi + lo, in one instruction: 16 ranks of hi and the same 16 of lo against B's 16
 // ranks twice (rounding h to T alone would put 2^-9 of the update, for bf16, on top of the output's own rounding; the second
 // half of the instruction would be idle).  fp16 takes h over a power of two near its row's largest, to stay in range.
-// B and y of a wave's first columns are on their way while h is gathered, those of the next while these are computed.
-template <typename T, int TT>
-__global__ __launch_bounds__(64 * kUpWaves, 2) void lora_up_kernel(LoraArgs a) {
+//
+// A wave takes 64 columns at a time by itself: their rows of B come in as one run of memory (EACH 16-byte pieces of
+// a column, 8 EACH ranks at a time) and turn into operands in the wave's LDS, and the update goes back through the same LDS to
+// meet y in whole lines (128 bytes of a row to 8 lanes).  B and y are on their way while h is gathered.  What lies outside of
+// the columns or ranks is an offset past the buffer: zeros, no branch.
+template <typename T, int TT, int EACH>
+__global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
   constexpr bool kF16 = __is_same(T, f16_t);
-  constexpr int kSteps = 4;                               // 16-rank steps of B that are loaded ahead
-  constexpr int kRowThreads = 64 * kUpWaves / (16 * TT);  // threads that gather one row of h
-  constexpr int kOctets = 32 / kRowThreads;               // octets of ranks of one of them, at most
-  extern __shared__ __align__(16) char lds[];             // h: [16 TT rows][hi, lo][ranks + 8]
-  __shared__ float factor[TT * 16];
-  __shared__ int lists[kUpWaves * kBlock];
+  constexpr int kRows = 16 * TT;
+  constexpr int kRowThreads = 64 * kWaves / kRows;  // threads that gather one row of h
+  constexpr int kRanks = 8 * EACH;                  // of a pass over B
+  constexpr int kBRow = 2 * kRanks + 16;            // LDS bytes of a column
+  constexpr int kDRow = 68;                         // LDS floats of a row's update
+  constexpr int kStrip = 64 * kBRow > 16 * kDRow * 4 ? 64 * kBRow : 16 * kDRow * 4;
+  extern __shared__ __align__(16) char lds[];       // h: [hi, lo][rows][ranks + 8]
+  __shared__ __align__(16) char strip[kWaves][kStrip];   // B, then the update, of a wave's columns
+  __shared__ float factor[kRows];
+  __shared__ int lists[kWaves * kBlock];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int64_t row0 = (int64_t)blockIdx.z * kBlock;
-  const int PR = a.parts * a.rank, steps = (a.rank + 15) / 16, hrow = steps * 16 + 8;
+  const int rank = a.rank, PR = a.parts * rank, padded = (rank + kRanks - 1) / kRanks * kRanks, hrow = padded + 8;
   T* const hs = (T*)lds;
+  char* const mine = strip[wave];
   // the part and its columns
   int part = 0, block = blockIdx.x;
   int64_t begin = 0;
@@ -209,159 +221,206 @@ __global__ __launch_bounds__(64 * kUpWaves, 2) void lora_up_kernel(LoraArgs a) {
   }
   const int64_t c_begin = begin + (int64_t)block * a.columns;
   const int width = (int)min(a.ends[part] - c_begin, (int64_t)a.columns);
+  const T* const ybase = (const T*)a.y + row0 * a.y_row + c_begin;
+  T* const obase = (T*)a.out + row0 * a.out_row + c_begin;
   for (int u = blockIdx.y;; u += gridDim.y) {
     Unit unit;
-    if (!find_unit(a, row0, u, 16 * TT, lists, unit)) return;
-    const bool some = unit.adapter >= 0;
-    if (unit.adapter == kNone && a.out == a.y) continue;
-    const int rows = (unit.count + 15) / 16;
-    const __amdgpu_buffer_rsrc_t rb = buffer_of(
-        (const T*)a.b + ((int64_t)max(unit.adapter, 0) * a.N + c_begin) * a.rank, some ? (int64_t)width * a.rank * 2 : 0);
-    const T* y[TT];
-    T* out[TT];
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const int64_t m = row0 + unit.row[min(t * 16 + n, unit.count - 1)];
-      y[t] = (const T*)a.y + m * a.y_row + c_begin + g * 8;
-      out[t] = (T*)a.out + m * a.out_row + c_begin + g * 8;
+    if (!find_unit(a, row0, u, kRows, lists, unit)) return;
+    if (unit.adapter < 0) {   // rows as they are, or NaN
+      if (unit.adapter == kNone && a.out == a.y) continue;
+      for (int x = threadIdx.x; x < unit.count * width; x += 64 * kWaves) {
+        const int r = x / width, c = x - r * width;
+        const int64_t m = unit.row[r];
+        obase[m * a.out_row + c] = unit.adapter == kNone ? ybase[m * a.y_row + c] : (T)__builtin_nanf("");
+      }
+      continue;
     }
-    // 32 columns at a time: as rows of two 16-row tiles dealt so that a lane gets 8 in a row of its batch row
-    v4u bv[2][kSteps][2], yv[2][TT];
-    auto load_b = [&](v4u (&to)[kSteps][2], int c0, int k0) {
+    const int rows = (unit.count + 15) / 16;
+    const __amdgpu_buffer_rsrc_t rb = buffer_of((const T*)a.b + ((int64_t)unit.adapter * a.N + c_begin) * rank, (int64_t)width * rank * 2);
+    const __amdgpu_buffer_rsrc_t ry = buffer_of(ybase, kBlock * a.y_row * 2), ro = buffer_of(obase, kBlock * a.out_row * 2);
+    // lane's place in y: rows t * 16 + i * 8 + lane / 8, columns (lane % 8) * 8 .. + 7 of the wave's
+    const int c8 = (lane & 7) * 8;
+    uint32_t yo[TT][2], oo[TT][2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t at = min(c0 + (n >> 2) * 8 + c * 4 + (n & 3), width - 1) * (uint32_t)a.rank * 2 + (g & 1) * 16;
+    for (int t = 0; t < TT; ++t)
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-          if (k0 + k < steps) to[k][c] = load16(rb, (k0 + k) * 16 + (g & 1) * 8 < a.rank ? at + k * 32 : kOutside, k0 * 32);
+      for (int i = 0; i < 2; ++i) {
+        const int r = t * 16 + i * 8 + (lane >> 3);
+        const uint32_t at = unit.row[min(r, unit.count - 1)];
+        yo[t][i] = r < unit.count ? (at * (uint32_t)a.y_row + c8) * 2 : kOutside;
+        oo[t][i] = r < unit.count ? (at * (uint32_t)a.out_row + c8) * 2 : kOutside;
+      }
+    v4u bv[EACH], yv[TT][2];
+    auto load_b = [&](int c0, int k0) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int col = i * (64 / EACH) + lane / EACH, r = k0 + lane % EACH * 8;
+        bv[i] = load16(rb, c0 + col < width && r < rank ? ((c0 + col) * (uint32_t)rank + r) * 2 : kOutside, 0);
       }
     };
-    auto load = [&](int buf, int c0) {
-      if (some) load_b(bv[buf], c0, 0);
-      if (a.wide_y)
+    auto load_y = [&](int c0) {
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
-          if (t * 16 + n < unit.count && c0 + g * 8 + 8 <= width) yv[buf][t] = *(const v4u*)(y[t] + c0);
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) yv[t][i] = load16(ry, c0 + c8 < width ? yo[t][i] : kOutside, c0 * 2);
     };
-    float f[TT];
-    auto finish = [&](int buf, int c0) {
-      v4f acc[2][TT];
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int t = 0; t < TT; ++t) acc[c][t] = v4f{0.f, 0.f, 0.f, 0.f};
-      if (some)
-        for (int k0 = 0; k0 < steps; k0 += kSteps) {
-          if (k0 > 0) load_b(bv[buf], c0, k0);
-#pragma unroll
-          for (int k = 0; k < kSteps; ++k)
-            if (k0 + k < steps)
-#pragma unroll
-              for (int t = 0; t < TT; ++t)
-                if (t < rows) {
-                  const v4u hv = *(const v4u*)(hs + ((t * 16 + n) * 2 + (g >> 1)) * hrow + (k0 + k) * 16 + (g & 1) * 8);
-#pragma unroll
-                  for (int c = 0; c < 2; ++c) acc[c][t] = mfma(bv[buf][k][c], hv, acc[c][t], T{});
-                }
-        }
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        if (t * 16 + n >= unit.count) continue;
-        auto value = [&](float base, int e) {
-          return some ? base + acc[e >> 2][t][e & 3] * f[t] : unit.adapter == kNone ? base : __builtin_nanf("");
-        };
-        if (a.wide_y && c0 + g * 8 + 8 <= width) {
-          T v[8];
-          __builtin_memcpy(v, &yv[buf][t], 16);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = (T)value((float)v[e], e);
-          __builtin_memcpy(__builtin_assume_aligned(out[t] + c0, 16), v, 16);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (c0 + g * 8 + e < width) out[t][c0 + e] = (T)value((float)y[t][c0 + e], e);
-        }
-      }
-    };
-    constexpr int hop = 32 * kUpWaves;
-    int c0 = wave * 32;
-    if (c0 < width) load(0, c0);
-    if (some) {
+    constexpr int hop = 64 * kWaves;
+    int c0 = wave * 64;
+    load_b(c0, 0);
+    if (a.wide_y) load_y(c0);
+    {
       __syncthreads();   // the last unit's h has been read
       const int r = threadIdx.x / kRowThreads, c = threadIdx.x % kRowThreads;
       const int64_t m = row0 + unit.row[min(r, unit.count - 1)];
-      float v[kOctets][8], top = 0.f;
+      const float* const from = a.h + m * PR + part * rank;
+      const int octets = (padded / 8 + kRowThreads - 1) / kRowThreads;   // of this thread: q * kRowThreads + c
+      auto gather = [&](int q, float (&v)[8]) {   // the splits of eight ranks, added in order
+        const int at = (q * kRowThreads + c) * 8;
 #pragma unroll
-      for (int q = 0; q < kOctets; ++q) {
-        const int rank = (q * kRowThreads + c) * 8;
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        if (at >= rank || r >= rows * 16) return;
+        constexpr int kBatch = TT == 1 ? 8 : 4;
+        for (int sp = 0; sp < a.splits; sp += kBatch) {
+          v4f lo[kBatch], hi[kBatch];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[q][e] = 0.f;
-        if (rank < a.rank && r < rows * 16) {
-          const float* from = a.h + m * PR + part * a.rank + rank;
-          const int64_t hop_h = (int64_t)a.M * PR;
-          for (int sp = 0; sp < a.splits; sp += 4) {
-            v4f lo[4], hi[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const v4f* p = (const v4f*)(from + min(sp + j, a.splits - 1) * hop_h);
+          for (int j = 0; j < kBatch; ++j)
+            if (sp + j < a.splits) {
+              const v4f* p = (const v4f*)(from + (int64_t)(sp + j) * a.M * PR + at);
               lo[j] = p[0];
               hi[j] = p[1];
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (sp + j < a.splits)
+          for (int j = 0; j < kBatch; ++j)
+            if (sp + j < a.splits)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  v[q][e] += lo[j][e];
-                  v[q][4 + e] += hi[j][e];
-                }
+              for (int e = 0; e < 4; ++e) {
+                v[e] += lo[j][e];
+                v[4 + e] += hi[j][e];
+              }
+        }
+      };
+      float down = 1.f, up = 1.f, top = 0.f;
+      auto seen = [&](const float (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+      };
+      auto fit = [&]() {   // a power of two near the row's largest
+        if constexpr (kF16) {
+          for (int o = kRowThreads / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+          if (top > 0.f && top < __builtin_huge_valf()) {
+            const int e = min(max(ilogbf(top), -100), 100);
+            down = ldexpf(1.f, -e);
+            up = ldexpf(1.f, e);
           }
         }
+      };
+      auto put = [&](int q, const float (&v)[8]) {
+        const int at = (q * kRowThreads + c) * 8;
+        if (at >= padded) return;
+        T hi[8], lo[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[q][e]));
-      }
-      float down = 1.f, up = 1.f;
-      if constexpr (kF16) {
-        for (int o = kRowThreads / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        if (top > 0.f && top < __builtin_huge_valf()) {
-          const int e = min(max(ilogbf(top), -100), 100);
-          down = ldexpf(1.f, -e);
-          up = ldexpf(1.f, e);
+        for (int e = 0; e < 8; ++e) {
+          const float x = v[e] * down;
+          hi[e] = (T)x;
+          const float back = (float)hi[e];
+          lo[e] = fabsf(back) < __builtin_huge_valf() ? (T)(x - back) : (T)0.f;   // inf stays, without inf - inf
+        }
+        __builtin_memcpy(hs + r * hrow + at, hi, 16);
+        __builtin_memcpy(hs + (kRows + r) * hrow + at, lo, 16);
+      };
+      if (octets <= 2) {
+        float v[2][8];
+        gather(0, v[0]);
+        gather(1, v[1]);
+        seen(v[0]);
+        seen(v[1]);
+        fit();
+        put(0, v[0]);
+        put(1, v[1]);
+      } else {   // more than registers hold: fp16 gathers twice
+        float v[8];
+        if constexpr (kF16)
+          for (int q = 0; q < octets; ++q) {
+            gather(q, v);
+            seen(v);
+          }
+        fit();
+        for (int q = 0; q < octets; ++q) {
+          gather(q, v);
+          put(q, v);
         }
       }
       if (c == 0) factor[r] = (a.scales ? a.scales[unit.adapter] : 1.f) * up;
-#pragma unroll
-      for (int q = 0; q < kOctets; ++q) {
-        const int rank = (q * kRowThreads + c) * 8;
-        if (rank < steps * 16 && r < rows * 16) {
-          T hi[8], lo[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = v[q][e] * down;
-            hi[e] = (T)x;
-            const float back = (float)hi[e];
-            lo[e] = fabsf(back) < __builtin_huge_valf() ? (T)(x - back) : (T)0.f;   // inf stays, without inf - inf
-          }
-          __builtin_memcpy(hs + (r * 2) * hrow + rank, hi, 16);
-          __builtin_memcpy(hs + (r * 2 + 1) * hrow + rank, lo, 16);
-        }
-      }
       __syncthreads();
     }
+    for (; c0 < width; c0 += hop) {
+      v4f acc[4][TT];
 #pragma unroll
-    for (int t = 0; t < TT; ++t) f[t] = some && t < rows ? factor[t * 16 + n] : 0.f;
-    for (; c0 < width; c0 += 2 * hop) {
-      if (c0 + hop < width) load(1, c0 + hop);
-      finish(0, c0);
-      if (c0 + hop >= width) break;
-      if (c0 + 2 * hop < width) load(0, c0 + 2 * hop);
-      finish(1, c0 + hop);
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[c][t] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int k0 = 0; k0 < padded; k0 += kRanks) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+          *(v4u*)(mine + (i * (64 / EACH) + lane / EACH) * kBRow + lane % EACH * 16) = bv[i];
+        const bool next = k0 + kRanks >= padded;
+        load_b(next ? c0 + hop : c0, next ? 0 : k0 + kRanks);
+#pragma unroll
+        for (int k = 0; k < EACH / 2; ++k) {
+          v4u bop[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) bop[c] = *(const v4u*)(mine + (c * 16 + n) * kBRow + k * 32 + (g & 1) * 16);
+#pragma unroll
+          for (int t = 0; t < TT; ++t) {   // of tiles that the unit does not have too, as above
+            const v4u hv = *(const v4u*)(hs + ((g >> 1) * kRows + t * 16 + n) * hrow + k0 + k * 16 + (g & 1) * 8);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c][t] = mfma(bop[c], hv, acc[c][t], T{});
+          }
+        }
+      }
+      // lane (n, g) holds columns 16 c + 4 g .. + 3 of row n; through LDS to 8 columns of rows lane / 8 and 8 + lane / 8
+      float* const turn = (float*)mine;
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const float f = factor[t * 16 + n];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) *(v4f*)(turn + n * kDRow + c * 16 + g * 4) = acc[c][t] * f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float* d = turn + (i * 8 + (lane >> 3)) * kDRow + c8;
+          if (a.wide_y) {
+            const v4f d0 = *(const v4f*)d, d1 = *(const v4f*)(d + 4);
+            T v[8];
+            v4u w;
+            __builtin_memcpy(v, &yv[t][i], 16);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (T)((float)v[e] + (e < 4 ? d0[e & 3] : d1[e & 3]));
+            __builtin_memcpy(&w, v, 16);
+            __builtin_amdgcn_raw_buffer_store_b128(w, ro, c0 + c8 < width ? oo[t][i] : kOutside, c0 * 2, 0);
+          } else {
+            const int r = t * 16 + i * 8 + (lane >> 3);
+            const int64_t m = unit.row[min(r, unit.count - 1)];
+            const T* from = ybase + m * a.y_row + c0 + c8;
+            T* to = obase + m * a.out_row + c0 + c8;
+            if (r < unit.count && c0 + c8 + 8 <= width) {
+              T v[8];
+              __builtin_memcpy(v, from, 16);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = (T)((float)v[e] + d[e]);
+              __builtin_memcpy(to, v, 16);
+            } else if (r < unit.count) {
+              for (int e = 0; c0 + c8 + e < width; ++e) to[e] = (T)((float)from[e] + d[e]);
+            }
+          }
+        }
+      }
+      if (a.wide_y) load_y(c0 + hop);
     }
   }
 }
 
-// How a call is cut.  Down: splits of K so that the launch has about 512 workgroups, each wave at least two steps.
-// Rows of a block that share an adapter go 16 to a workgroup up to kBlock rows in all, 64 above.
+// How a call is cut.  Rows of a block that share an adapter go 16 to a workgroup up to kBlock rows in all, 64 above.  K is
+// split so that the first launch has about two workgroups a CU, each at least two stages.
 struct Cut { int splits, chunks, blocks; };
 
 Cut cut_of(int M, int64_t K, int parts, int rank) {
@@ -369,8 +428,8 @@ Cut cut_of(int M, int64_t K, int parts, int rank) {
   c.chunks = (parts * rank + 16 * kRankTiles - 1) / (16 * kRankTiles);
   c.blocks = (M + kBlock - 1) / kBlock;
   const int64_t wgs = (int64_t)c.chunks * (M <= kBlock ? std::min(M, 16) : c.blocks);
-  const int64_t steps = (K + 63) / 64;
-  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / wgs, steps / kDownWaves, 16}));
+  const int64_t stages = (K + kStage - 1) / kStage;
+  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / wgs, stages / 2, 16}));
   return c;
 }
 
@@ -383,9 +442,15 @@ void launch(const LoraArgs& g, const Cut& c, hipStream_t st) {
     blocks += (g.ends[p] - begin + g.columns - 1) / g.columns;
     begin = g.ends[p];
   }
-  if (g.slots > 0) lora_down_kernel<T, TT><<<dim3(c.splits * c.chunks, units, c.blocks), 64 * kDownWaves, 0, st>>>(g);
-  const size_t lds = (size_t)16 * TT * 2 * ((g.rank + 15) / 16 * 16 + 8) * sizeof(T);
-  lora_up_kernel<T, TT><<<dim3((unsigned)blocks, units, c.blocks), 64 * kUpWaves, lds, st>>>(g);
+  if (g.slots > 0) lora_down_kernel<T, TT><<<dim3(c.splits * c.chunks, units, c.blocks), 64 * kWaves, 0, st>>>(g);
+  auto up = [&](auto each) {
+    constexpr int kEach = decltype(each)::value, kRanks = 8 * kEach;
+    const size_t lds = (size_t)16 * TT * 2 * ((g.rank + kRanks - 1) / kRanks * kRanks + 8) * sizeof(T);
+    lora_up_kernel<T, TT, kEach><<<dim3((unsigned)blocks, units, c.blocks), 64 * kWaves, lds, st>>>(g);
+  };
+  if (g.rank <= 16) up(std::integral_constant<int, 2>{});
+  else if (g.rank <= 32) up(std::integral_constant<int, 4>{});
+  else up(std::integral_constant<int, 8>{});
 }
 
 }  // namespace
@@ -434,12 +499,14 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
   const Cut c = cut_of(M, K, parts, rank);
   if (c.blocks > 65535) return decode_fail(GQK_ERR_SHAPE, "lora_add: %d rows", M);
   g.splits = c.splits; g.chunks = c.chunks;
-  g.wide_y = !(((uintptr_t)y | (uintptr_t)out) & 15) && !((y_row | out_row) & 7);
-  for (int p = 0; p + 1 < parts; ++p) g.wide_y &= g.ends[p] % 8 == 0;
-  // columns of a workgroup of the second kernel: 512, fewer where the launch would have too few of them
+  // whole 16-byte pieces in every row, and rows that 32-bit offsets reach
+  g.wide_y = !(((uintptr_t)y | (uintptr_t)out) & 15) && !((y_row | out_row) & 7) && y_row <= (1 << 23) && out_row <= (1 << 23);
+  for (int p = 0; p < parts; ++p) g.wide_y &= g.ends[p] % 8 == 0;
+  // columns of a workgroup of the second kernel, which gathers h once for them: 64 for each wave, more where the launch
+  // has workgroups enough
   const int64_t groups = M <= kBlock ? std::min(M, 16) : c.blocks;
-  g.columns = 512;
-  while (g.columns > 128 && groups * (g.N / g.columns) < 512) g.columns /= 2;
+  g.columns = 64 * kWaves;
+  while (g.columns < 1024 && groups * (g.N / g.columns) > 2048) g.columns *= 2;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == GQK_DTYPE_BF16) {
     if (M <= kBlock) launch<bf16_t, 1>(g, c, st);
