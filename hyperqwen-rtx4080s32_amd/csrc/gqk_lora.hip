@@ -19,7 +19,11 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 constexpr int kParts = 8;
 constexpr int kWaves = 4;
 constexpr int kStage = 128;      // values of K that the first kernel takes at a time
-constexpr int kBlock = 64;       // rows whose adapters a workgroup sorts out: one per lane
+constexpr int kList = 64;        // rows of a unit, at most
+// A workgroup sorts out the adapters of a block of 64 Q rows, Q ids to a lane.  Batches of up to kSmall rows are one block (Q 1
+// or 4), so that each adapter is read once for its rows wherever they are, in units of 16; longer ones (prompts, whose
+// rows come in runs) go by 64 rows and units of up to 64.
+constexpr int kSmall = 256;
 constexpr int kRankTiles = 4;    // 16-rank tiles of a workgroup of the first kernel
 constexpr int kNone = -1, kBad = -2;
 
@@ -50,35 +54,56 @@ struct Unit {
   const int* row;   // their numbers within the block
 };
 
-// Unit u (of up to `most` rows) of the block's rows: adapters in the order of their first row, each one's rows in order.
-// A lane holds one row's id; a ballot finds the rows that share it, whose numbers go to LDS in order, a list for each
-// wave.  False: the block has fewer units.  All waves find the same.
+// Unit u (of up to `most` rows) of a block of 64 Q rows: adapters in the order of their first row, each one's rows in
+// order.  A lane holds the ids of Q rows; ballots find the rows that share one, whose numbers go to LDS in order, a list for
+// each wave.  False: the block has fewer units.  All waves find the same.
+template <int Q>
 __device__ __forceinline__ bool find_unit(const LoraArgs& a, int64_t row0, int u, int most, int* lists, Unit& out) {
   const int lane = threadIdx.x & 63;
-  const int64_t m = row0 + lane;
-  int id = kNone;
-  if (m < a.M) {
-    const int64_t i = index_at(a.ids, a.wide_ids, m);
-    id = i < 0 ? kNone : i >= a.slots ? kBad : (int)i;
-  }
-  uint64_t left = __ballot(m < a.M);
-  while (left) {
-    const int who = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-    const uint64_t same = __ballot(id == who) & left;
-    const int count = __popcll(same), units = (count + most - 1) / most;
-    if (u < units) {
-      out.adapter = who;
-      out.count = min(count - u * most, most);
-      const int place = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0)) - u * most;
-      int* mine = lists + (threadIdx.x >> 6) * kBlock;
-      if ((same >> lane & 1) && place >= 0 && place < out.count) mine[place] = lane;
-      __builtin_amdgcn_wave_barrier();
-      out.row = mine;
-      return true;
+  int id[Q];
+  uint64_t left[Q];
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    const int64_t m = row0 + q * 64 + lane;
+    id[q] = kNone;
+    if (m < a.M) {
+      const int64_t i = index_at(a.ids, a.wide_ids, m);
+      id[q] = i < 0 ? kNone : i >= a.slots ? kBad : (int)i;
     }
-    u -= units;
-    left &= ~same;
+    left[q] = __ballot(m < a.M);
   }
+#pragma unroll
+  for (int f = 0; f < Q; ++f)   // the first row that is left lies in part f
+    while (left[f]) {
+      const int who = __builtin_amdgcn_readlane(id[f], __builtin_ctzll(left[f]));
+      uint64_t same[Q];
+      int count = 0;
+#pragma unroll
+      for (int q = f; q < Q; ++q) {
+        same[q] = __ballot(id[q] == who) & left[q];
+        count += __popcll(same[q]);
+      }
+      const int units = (count + most - 1) / most;
+      if (u < units) {
+        out.adapter = who;
+        out.count = min(count - u * most, most);
+        int* mine = lists + (threadIdx.x >> 6) * kList;
+        int before = -u * most;   // rows of the adapter in earlier parts, from the unit's first
+#pragma unroll
+        for (int q = f; q < Q; ++q) {
+          const int place =
+              before + __builtin_amdgcn_mbcnt_hi((uint32_t)(same[q] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same[q], 0));
+          if ((same[q] >> lane & 1) && place >= 0 && place < out.count) mine[place] = q * 64 + lane;
+          before += __popcll(same[q]);
+        }
+        __builtin_amdgcn_wave_barrier();
+        out.row = mine;
+        return true;
+      }
+      u -= units;
+#pragma unroll
+      for (int q = f; q < Q; ++q) left[q] &= ~same[q];
+    }
   return false;
 }
 
@@ -86,9 +111,10 @@ __device__ __forceinline__ bool find_unit(const LoraArgs& a, int64_t row0, int u
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)min(bytes, (int64_t)0x7ffffff0), 0x00020000);
 }
-constexpr uint32_t kOutside = 0x80000000u;   // an offset past every buffer
-__device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset, uint32_t shared) {
-  return __builtin_amdgcn_raw_buffer_load_b128(rs, offset, shared, 0);
+// An offset past every buffer, with what is added to it too: a row of x or A is below 2^23 bytes, columns below 2^12.
+constexpr uint32_t kOutside = 0x80000000u;
+__device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(rs, offset, 0, 0);
 }
 
 // h = A x of one unit's rows, 64 ranks, one split of K.  Rows of x and of A are far apart, and a lane of a matrix operand
@@ -97,14 +123,15 @@ __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset
 // pieces of one k-step in different banks), and are read as operands: ranks as the instruction's rows, batch rows as its
 // columns.  Loads run kDepth stages ahead in registers; two LDS buffers, one barrier a stage.  A wave takes one 16-row tile and all
 // ranks (TT = 4), or all 16 rows and one 16-rank tile (TT = 1).
-template <typename T, int TT>
+template <typename T, int TT, int Q>
 __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
   constexpr int kDepth = TT == 1 ? 4 : 2;
   constexpr int kRows = 16 * TT, kAcc = TT == 1 ? 1 : kRankTiles;
   __shared__ __align__(16) char buf[2][(kRows + 16 * kRankTiles) * 256];
-  __shared__ int lists[kWaves * kBlock];
+  __shared__ int lists[kWaves * kList];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int chunk = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  constexpr int kBlock = 64 * Q;
   const int64_t row0 = (int64_t)blockIdx.z * kBlock;
   const int PR = a.parts * a.rank, rank0 = chunk * 16 * kRankTiles, tiles = min(kRankTiles, (PR - rank0 + 15) / 16);
   const int all = (int)((a.K + kStage - 1) / kStage);
@@ -112,34 +139,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
   const int K = (int)a.K, row = threadIdx.x >> 4, piece = threadIdx.x & 15;
   for (int u = blockIdx.y;; u += gridDim.y) {
     Unit unit;
-    if (!find_unit(a, row0, u, kRows, lists, unit)) return;
+    if (!find_unit<Q>(a, row0, u, kRows, lists, unit)) return;
     if (unit.adapter < 0) continue;
     const int rows = (unit.count + 15) / 16;   // tiles of rows
     const __amdgpu_buffer_rsrc_t ra = buffer_of((const T*)a.a + ((int64_t)unit.adapter * PR + rank0) * a.K,
                                                 (int64_t)min(16 * kRankTiles, PR - rank0) * a.K * 2);
     const __amdgpu_buffer_rsrc_t rx = buffer_of((const T*)a.x + row0 * a.x_row, (int64_t)kBlock * a.x_row * 2);
     uint32_t ao[kRankTiles], xo[TT];
+    // ranks and rows that are not there are offsets past the buffers: zeros, no branch
 #pragma unroll
-    for (int t = 0; t < kRankTiles; ++t) ao[t] = min(t * 16 + row, PR - rank0 - 1) * (uint32_t)K * 2 + piece * 16;
+    for (int t = 0; t < kRankTiles; ++t)
+      ao[t] = t * 16 + row < PR - rank0 ? (t * 16 + row) * (uint32_t)K * 2 + piece * 16 : kOutside;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) xo[t] = unit.row[min(t * 16 + row, unit.count - 1)] * (uint32_t)a.x_row * 2 + piece * 16;
+    for (int t = 0; t < TT; ++t)
+      xo[t] = t * 16 + row < unit.count ? unit.row[t * 16 + row] * (uint32_t)a.x_row * 2 + piece * 16 : kOutside;
     v4u av[kDepth][kRankTiles], xv[kDepth][TT];
     auto load = [&](int d, int s) {
-      const bool in = s * kStage + piece * 8 < K;   // K may end inside the last stage
+      const bool in = s < s0 + stages && s * kStage + piece * 8 < K;   // K may end inside the last stage
 #pragma unroll
-      for (int t = 0; t < TT; ++t)
-        if (t < rows) xv[d][t] = load16(rx, in ? xo[t] : kOutside, s * (2 * kStage));
+      for (int t = 0; t < TT; ++t) xv[d][t] = load16(rx, in ? xo[t] + s * (2 * kStage) : kOutside);
 #pragma unroll
-      for (int t = 0; t < kRankTiles; ++t)
-        if (t < tiles) av[d][t] = load16(ra, in ? ao[t] : kOutside, s * (2 * kStage));
+      for (int t = 0; t < kRankTiles; ++t) av[d][t] = load16(ra, in ? ao[t] + s * (2 * kStage) : kOutside);
     };
     v4f acc[kAcc];
 #pragma unroll
     for (int r = 0; r < kAcc; ++r) acc[r] = v4f{0.f, 0.f, 0.f, 0.f};
     const bool busy = wave < (TT == 1 ? tiles : rows);
 #pragma unroll
-    for (int d = 0; d < kDepth; ++d)
-      if (d < stages) load(d, s0 + d);
+    for (int d = 0; d < kDepth; ++d) load(d, s0 + d);
     __syncthreads();   // the last unit's stages have been read
     for (int i = 0; i < stages; i += kDepth)
 #pragma unroll
@@ -148,12 +175,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
           char* const to = buf[d & 1];   // kDepth is even
           char* const at = to + row * 256 + (piece ^ row) * 16;
 #pragma unroll
-          for (int t = 0; t < TT; ++t)
-            if (t < rows) *(v4u*)(at + t * 4096) = xv[d][t];
+          for (int t = 0; t < TT; ++t) *(v4u*)(at + t * 4096) = xv[d][t];
 #pragma unroll
-          for (int t = 0; t < kRankTiles; ++t)
-            if (t < tiles) *(v4u*)(at + (TT + t) * 4096) = av[d][t];
-          if (i + d + kDepth < stages) load(d, s0 + i + d + kDepth);
+          for (int t = 0; t < kRankTiles; ++t) *(v4u*)(at + (TT + t) * 4096) = av[d][t];
+          load(d, s0 + i + d + kDepth);
           __syncthreads();
           if (busy)
 #pragma unroll
@@ -163,8 +188,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
               if constexpr (TT == 1) {
                 acc[0] = mfma(*(const v4u*)(from + (TT + wave) * 4096), xop, acc[0], T{});
               } else {
-                // of tiles that the chunk does not have too: sums that nobody reads cost less than the copies that a branch
-                // around each instruction takes (64 moves a product counted)
+                // of tiles that the chunk does not have too: zeros cost less than the copies that a branch around each
+                // instruction takes (64 moves a product counted)
 #pragma unroll
                 for (int r = 0; r < kRankTiles; ++r) acc[r] = mfma(*(const v4u*)(from + (TT + r) * 4096), xop, acc[r], T{});
               }
@@ -192,7 +217,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
 // a column, 8 EACH ranks at a time) and turn into operands in the wave's LDS, and the update goes back through the same LDS to
 // meet y in whole lines (128 bytes of a row to 8 lanes).  B and y are on their way while h is gathered.  What lies outside of
 // the columns or ranks is an offset past the buffer: zeros, no branch.
-template <typename T, int TT, int EACH>
+template <typename T, int TT, int Q, int EACH>
 __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
   constexpr bool kF16 = __is_same(T, f16_t);
   constexpr int kRows = 16 * TT;
@@ -204,8 +229,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
   extern __shared__ __align__(16) char lds[];       // h: [hi, lo][rows][ranks + 8]
   __shared__ __align__(16) char strip[kWaves][kStrip];   // B, then the update, of a wave's columns
   __shared__ float factor[kRows];
-  __shared__ int lists[kWaves * kBlock];
+  __shared__ int lists[kWaves * kList];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  constexpr int kBlock = 64 * Q;
   const int64_t row0 = (int64_t)blockIdx.z * kBlock;
   const int rank = a.rank, PR = a.parts * rank, padded = (rank + kRanks - 1) / kRanks * kRanks, hrow = padded + 8;
   T* const hs = (T*)lds;
@@ -225,7 +251,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
   T* const obase = (T*)a.out + row0 * a.out_row + c_begin;
   for (int u = blockIdx.y;; u += gridDim.y) {
     Unit unit;
-    if (!find_unit(a, row0, u, kRows, lists, unit)) return;
+    if (!find_unit<Q>(a, row0, u, kRows, lists, unit)) return;
     if (unit.adapter < 0) {   // rows as they are, or NaN
       if (unit.adapter == kNone && a.out == a.y) continue;
       for (int x = threadIdx.x; x < unit.count * width; x += 64 * kWaves) {
@@ -255,14 +281,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int col = i * (64 / EACH) + lane / EACH, r = k0 + lane % EACH * 8;
-        bv[i] = load16(rb, c0 + col < width && r < rank ? ((c0 + col) * (uint32_t)rank + r) * 2 : kOutside, 0);
+        bv[i] = load16(rb, c0 + col < width && r < rank ? ((c0 + col) * (uint32_t)rank + r) * 2 : kOutside);
       }
     };
     auto load_y = [&](int c0) {
 #pragma unroll
       for (int t = 0; t < TT; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) yv[t][i] = load16(ry, c0 + c8 < width ? yo[t][i] : kOutside, c0 * 2);
+        for (int i = 0; i < 2; ++i) yv[t][i] = load16(ry, c0 + c8 < width ? yo[t][i] + c0 * 2 : kOutside);
     };
     constexpr int hop = 64 * kWaves;
     int c0 = wave * 64;
@@ -273,25 +299,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
       const int r = threadIdx.x / kRowThreads, c = threadIdx.x % kRowThreads;
       const int64_t m = row0 + unit.row[min(r, unit.count - 1)];
       const float* const from = a.h + m * PR + part * rank;
-      const int octets = (padded / 8 + kRowThreads - 1) / kRowThreads;   // of this thread: q * kRowThreads + c
-      auto gather = [&](int q, float (&v)[8]) {   // the splits of eight ranks, added in order
-        const int at = (q * kRowThreads + c) * 8;
+      const int octets = (padded / 8 + kRowThreads - 1) / kRowThreads;   // of this thread
+      auto gather = [&](int at, int sp0, int by, float (&v)[8]) {   // splits sp0, sp0 + by, .. of eight ranks, added in order
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.f;
         if (at >= rank || r >= rows * 16) return;
-        constexpr int kBatch = TT == 1 ? 8 : 4;
-        for (int sp = 0; sp < a.splits; sp += kBatch) {
+        constexpr int kBatch = 4;
+        for (int sp = sp0; sp < a.splits; sp += kBatch * by) {
           v4f lo[kBatch], hi[kBatch];
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j)
-            if (sp + j < a.splits) {
-              const v4f* p = (const v4f*)(from + (int64_t)(sp + j) * a.M * PR + at);
-              lo[j] = p[0];
-              hi[j] = p[1];
-            }
+          for (int j = 0; j < kBatch; ++j) {
+            const v4f* p = (const v4f*)(from + (int64_t)min(sp + j * by, a.splits - 1) * a.M * PR + at);
+            lo[j] = p[0];
+            hi[j] = p[1];
+          }
 #pragma unroll
           for (int j = 0; j < kBatch; ++j)
-            if (sp + j < a.splits)
+            if (sp + j * by < a.splits)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 v[e] += lo[j][e];
@@ -314,8 +338,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
           }
         }
       };
-      auto put = [&](int q, const float (&v)[8]) {
-        const int at = (q * kRowThreads + c) * 8;
+      auto put = [&](int at, const float (&v)[8]) {
         if (at >= padded) return;
         T hi[8], lo[8];
 #pragma unroll
@@ -328,26 +351,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
         __builtin_memcpy(hs + r * hrow + at, hi, 16);
         __builtin_memcpy(hs + (kRows + r) * hrow + at, lo, 16);
       };
-      if (octets <= 2) {
+      auto at = [&](int q) { return (q * kRowThreads + c) * 8; };
+      constexpr int kGroups = kRowThreads / EACH;   // threads of a row that share eight ranks' splits
+      if (kGroups > 1 && padded == kRanks) {
+        float v[8];
+        gather(c % EACH * 8, c / EACH, kGroups, v);
+#pragma unroll
+        for (int o = EACH; o < kRowThreads; o *= 2)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += __shfl_xor(v[e], o);
+        seen(v);
+        fit();
+        if (c < EACH) put(c * 8, v);
+      } else if (octets <= 2) {
         float v[2][8];
-        gather(0, v[0]);
-        gather(1, v[1]);
+        gather(at(0), 0, 1, v[0]);
+        gather(at(1), 0, 1, v[1]);
         seen(v[0]);
         seen(v[1]);
         fit();
-        put(0, v[0]);
-        put(1, v[1]);
+        put(at(0), v[0]);
+        put(at(1), v[1]);
       } else {   // more than registers hold: fp16 gathers twice
         float v[8];
         if constexpr (kF16)
           for (int q = 0; q < octets; ++q) {
-            gather(q, v);
+            gather(at(q), 0, 1, v);
             seen(v);
           }
         fit();
         for (int q = 0; q < octets; ++q) {
-          gather(q, v);
-          put(q, v);
+          gather(at(q), 0, 1, v);
+          put(at(q), v);
         }
       }
       if (c == 0) factor[r] = (a.scales ? a.scales[unit.adapter] : 1.f) * up;
@@ -396,7 +431,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = (T)((float)v[e] + (e < 4 ? d0[e & 3] : d1[e & 3]));
             __builtin_memcpy(&w, v, 16);
-            __builtin_amdgcn_raw_buffer_store_b128(w, ro, c0 + c8 < width ? oo[t][i] : kOutside, c0 * 2, 0);
+            __builtin_amdgcn_raw_buffer_store_b128(w, ro, c0 + c8 < width ? oo[t][i] + c0 * 2 : kOutside, 0, 0);
           } else {
             const int r = t * 16 + i * 8 + (lane >> 3);
             const int64_t m = unit.row[min(r, unit.count - 1)];
@@ -419,34 +454,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
   }
 }
 
-// How a call is cut.  Rows of a block that share an adapter go 16 to a workgroup up to kBlock rows in all, 64 above.  K is
-// split so that the first launch has about two workgroups a CU, each at least two stages.
+// How a call is cut.  K is split so that the first launch has about a workgroup a CU, each at least two stages
+// (4096 rows of 17408 values: 512 workgroups 43 us, 256 40; the second launch reads fewer partial sums).
 struct Cut { int splits, chunks, blocks; };
 
 Cut cut_of(int M, int64_t K, int parts, int rank) {
   Cut c;
   c.chunks = (parts * rank + 16 * kRankTiles - 1) / (16 * kRankTiles);
-  c.blocks = (M + kBlock - 1) / kBlock;
-  const int64_t wgs = (int64_t)c.chunks * (M <= kBlock ? std::min(M, 16) : c.blocks);
+  c.blocks = M <= kSmall ? 1 : (M + 63) / 64;
+  const int64_t wgs = (int64_t)c.chunks * (M <= kSmall ? std::min(M, 16) : c.blocks);
   const int64_t stages = (K + kStage - 1) / kStage;
-  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / wgs, stages / 2, 16}));
+  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / wgs, stages / 2, 16}));
   return c;
 }
 
-template <typename T, int TT>
+template <typename T, int TT, int Q>
 void launch(const LoraArgs& g, const Cut& c, hipStream_t st) {
   // units of a block: its adapters, none, bad ids, and what does not fit one unit; the kernels step on over more
-  const int units = TT == 1 ? std::min(g.M, std::min(g.slots, kBlock) + 2 + kBlock / 16) : 2;
+  const int units = TT == 1 ? std::min(g.M, std::min(g.slots, kSmall) + 2 + g.M / 16) : 2;
   int64_t blocks = 0, begin = 0;
   for (int p = 0; p < g.parts; ++p) {
     blocks += (g.ends[p] - begin + g.columns - 1) / g.columns;
     begin = g.ends[p];
   }
-  if (g.slots > 0) lora_down_kernel<T, TT><<<dim3(c.splits * c.chunks, units, c.blocks), 64 * kWaves, 0, st>>>(g);
+  if (g.slots > 0) lora_down_kernel<T, TT, Q><<<dim3(c.splits * c.chunks, units, c.blocks), 64 * kWaves, 0, st>>>(g);
   auto up = [&](auto each) {
     constexpr int kEach = decltype(each)::value, kRanks = 8 * kEach;
     const size_t lds = (size_t)16 * TT * 2 * ((g.rank + kRanks - 1) / kRanks * kRanks + 8) * sizeof(T);
-    lora_up_kernel<T, TT, kEach><<<dim3((unsigned)blocks, units, c.blocks), 64 * kWaves, lds, st>>>(g);
+    lora_up_kernel<T, TT, Q, kEach><<<dim3((unsigned)blocks, units, c.blocks), 64 * kWaves, lds, st>>>(g);
   };
   if (g.rank <= 16) up(std::integral_constant<int, 2>{});
   else if (g.rank <= 32) up(std::integral_constant<int, 4>{});
@@ -500,20 +535,22 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
   if (c.blocks > 65535) return decode_fail(GQK_ERR_SHAPE, "lora_add: %d rows", M);
   g.splits = c.splits; g.chunks = c.chunks;
   // whole 16-byte pieces in every row, and rows that 32-bit offsets reach
-  g.wide_y = !(((uintptr_t)y | (uintptr_t)out) & 15) && !((y_row | out_row) & 7) && y_row <= (1 << 23) && out_row <= (1 << 23);
+  g.wide_y = !(((uintptr_t)y | (uintptr_t)out) & 15) && !((y_row | out_row) & 7) && y_row < (1 << 22) && out_row < (1 << 22);
   for (int p = 0; p < parts; ++p) g.wide_y &= g.ends[p] % 8 == 0;
   // columns of a workgroup of the second kernel, which gathers h once for them: 64 for each wave, more where the launch
   // has workgroups enough
-  const int64_t groups = M <= kBlock ? std::min(M, 16) : c.blocks;
+  const int64_t groups = M <= kSmall ? std::min(M, 16) : c.blocks;
   g.columns = 64 * kWaves;
-  while (g.columns < 1024 && groups * (g.N / g.columns) > 2048) g.columns *= 2;
+  while (g.columns < 1024 && groups * (g.N / g.columns) > 256) g.columns *= 2;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == GQK_DTYPE_BF16) {
-    if (M <= kBlock) launch<bf16_t, 1>(g, c, st);
-    else launch<bf16_t, 4>(g, c, st);
+    if (M <= 64) launch<bf16_t, 1, 1>(g, c, st);
+    else if (M <= kSmall) launch<bf16_t, 1, kSmall / 64>(g, c, st);
+    else launch<bf16_t, 4, 1>(g, c, st);
   } else {
-    if (M <= kBlock) launch<f16_t, 1>(g, c, st);
-    else launch<f16_t, 4>(g, c, st);
+    if (M <= 64) launch<f16_t, 1, 1>(g, c, st);
+    else if (M <= kSmall) launch<f16_t, 1, kSmall / 64>(g, c, st);
+    else launch<f16_t, 4, 1>(g, c, st);
   }
   return decode_launched("lora_add");
 }

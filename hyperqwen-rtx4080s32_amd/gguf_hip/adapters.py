@@ -14,7 +14,7 @@ from ._lib import check, lib
 from .eager import direct as _direct, stream as _stream
 
 _TYPES = {torch.bfloat16: _lib.GQK_DTYPE_BF16, torch.float16: _lib.GQK_DTYPE_F16}
-MAX_PARTS, MAX_RANK, MAX_K = 8, 256, 1 << 23
+MAX_PARTS, MAX_RANK, MAX_K = 8, 256, (1 << 22) - 8
 
 
 @lru_cache(maxsize=256)

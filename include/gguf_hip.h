@@ -191,7 +191,7 @@ int gqk_linear_noalloc(const void* packed, const int32_t* desc_dev, const gqk_pl
  * and sums are in fp32, rounded once to out.  K and x's row stride (where M > 1) are at most GQK_LORA_MAX_K.
  * workspace: gqk_lora_workspace_bytes bytes, 256-byte aligned; its
  * first GQK_CTR_BYTES are left alone, so that a linear layer's workspace serves (calls in stream order). */
-#define GQK_LORA_MAX_K 8388608 /* 64 rows stay below 2^30 bytes */
+#define GQK_LORA_MAX_K 4194296 /* 256 rows stay below 2^31 bytes */
 int64_t gqk_lora_workspace_bytes(int M, int64_t K, int parts, int rank);
 int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int M, int64_t K, const void* a,
                  const void* b, int slots, int parts, const int64_t* n_outs, int rank, const void* ids, int ids_64,
