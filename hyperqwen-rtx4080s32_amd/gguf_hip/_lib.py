@@ -9,6 +9,8 @@ import ctypes
 import os
 from ctypes import byref  # noqa: F401
 
+import torch  # noqa: F401
+
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgqk.so")
 
 GQK_OK = 0
@@ -139,6 +141,11 @@ def _load() -> ctypes.CDLL:
 
 
 lib = _load()
+try:
+    from . import _fast  # noqa: E402,F401  (needs torch loaded: the package imports it first)
+except ImportError as e:
+    raise ImportError(f"gguf_hip: the module _fast.so of the eager calls does not load ({e}); run `python -m gguf_hip.build` "
+                      "(or __graft_entry__.build()) first.") from e
 
 
 def check(rc: int, what: str) -> int:

@@ -10,8 +10,8 @@ from functools import lru_cache
 import torch
 
 from . import _lib, ops
-from ._lib import check, lib
-from .eager import direct as _direct, stream as _stream
+from ._lib import _fast, check, lib
+from .eager import direct as _direct, stream as _stream, unwatched as _unwatched
 
 _TYPES = {torch.bfloat16: _lib.GQK_DTYPE_BF16, torch.float16: _lib.GQK_DTYPE_F16}
 MAX_PARTS, MAX_RANK, MAX_K = 8, 256, (1 << 22) - 8
@@ -80,6 +80,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     Returns a new tensor, or ``out`` (a [M, N] view with unit column stride), which may be y itself.
     ``workspace``: as mul_mat_grouped's (its own for calls on concurrent streams)."""
     what = "lora_add"
+    if _unwatched():
+        got = _fast.lora_add(y, x, a, b, ids, scales, n_outs, out, workspace)
+        if got is not None:
+            return got
     ops._require_gpu(x, what)
     n_outs = tuple(int(n) for n in n_outs)
     if x.dtype not in _TYPES or x.dim() != 2:

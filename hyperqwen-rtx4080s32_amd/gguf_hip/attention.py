@@ -13,8 +13,8 @@ import math
 import torch
 
 from . import _lib, ops
-from ._lib import GqkHeads, GqkPages, check, lib
-from .eager import direct as _direct, stream as _stream
+from ._lib import GqkHeads, GqkPages, _fast, check, lib
+from .eager import direct as _direct, stream as _stream, unwatched as _unwatched
 
 _TYPES = {torch.bfloat16: _lib.GQK_DTYPE_BF16, torch.float16: _lib.GQK_DTYPE_F16}
 _PAGE_TYPES = {**_TYPES, torch.float8_e4m3fn: _lib.GQK_DTYPE_FP8}
@@ -134,6 +134,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Returns out [batch, query heads, dim], with ``return_lse`` also the log-sum-exp of its scores (fp32 [batch,
     query heads], -inf without a key), which joins attention over separate caches.  ``workspace``: as
     mul_mat_grouped's (its own for calls on concurrent streams)."""
+    if _unwatched():
+        got = _fast.paged_attention(q, k_pages, v_pages, block_table, lengths, scale, window, k_scale, v_scale, max_length, out,
+                                    return_lse, workspace)
+        if got is not None:
+            return got
     ops._require_gpu(q, "paged_attention")
     if q.dtype not in _TYPES:
         raise ValueError(f"paged_attention: q is bf16 or fp16, not {q.dtype}")
@@ -279,6 +284,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     Returns (queries, keys): new tensors, or out_q / out_k, which may be q and k themselves; with pages the keys are
     returned (and written beside the pages) only into an out_k that is given."""
     what = "qk_norm_rope"
+    flags = (_lib.GQK_ROPE_UNIT_OFFSET if unit_offset else 0) | (_lib.GQK_ROPE_INTERLEAVED if interleaved else 0)
+    if _unwatched():
+        got = _fast.qk_norm_rope(q, k, positions, table, q_weight, k_weight, eps, flags, v, k_pages, v_pages, slots, k_scale,
+                                 v_scale, out_q, out_k)
+        if got is not None:
+            return got
     ops._require_gpu(q, what)
     if q.dtype not in _TYPES:
         raise ValueError(f"{what}: heads are bf16 or fp16, not {q.dtype}")
@@ -319,7 +330,6 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         _out_heads(out_k, k, what)
     elif k is not None and k_pages is None:
         out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    flags = (_lib.GQK_ROPE_UNIT_OFFSET if unit_offset else 0) | (_lib.GQK_ROPE_INTERLEAVED if interleaved else 0)
     args = (_heads_view(q, what), None if k is None else _heads_view(k, what), None if v is None else _heads_view(v, what),
             positions, table, q_weight, k_weight, float(eps), flags, slots, k_scale, v_scale, out_q, out_k, k_pages, v_pages)
     if _direct(q, k, v, positions, table, q_weight, k_weight, slots, out_q, out_k, k_pages, v_pages):

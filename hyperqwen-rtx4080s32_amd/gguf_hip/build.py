@@ -24,6 +24,7 @@ SOURCES = (("gqk_api.hip", (), "gqk_api.o"), ("gqk_codec.hip", (), "gqk_codec.o"
            *((f"gqk_{n}.hip", (), f"gqk_{n}.o") for n in ("lora", "rope", "attention", "pages")))
 ARCH = os.environ.get("GQK_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+MODULE = os.path.join(PKG, "_fast.so")   # the CPython module of the eager calls (gqk_torch.cpp)
 FLAGS = [
     "-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}",
     "-I", os.path.join(REPO, "include"), "-I", CSRC,
@@ -40,8 +41,26 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError(f"hipcc failed ({p.returncode}): {' '.join(cmd)}\n{p.stderr[-6000:]}")
 
 
+def _module_commands() -> tuple[list[str], list[str]]:
+    """Compile and link of the eager calls' module against torch and the library beside it."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    obj = os.path.join(BUILD, "gqk_torch.o")
+    compile_ = [HIPCC, "-x", "c++", "-O2", "-fPIC", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(REPO, "include"),
+                *(x for d in [*include_paths(), "/opt/rocm/include", sysconfig.get_paths()["include"]] for x in ("-isystem", d)),
+                "-c", os.path.join(CSRC, "gqk_torch.cpp"), "-o", obj]
+    link = [HIPCC, "-shared", "-o", MODULE + ".tmp", obj, "-L", PKG, "-lgqk", "-Wl,-rpath,$ORIGIN",
+            *(x for d in library_paths() for x in ("-L", d)), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+    return compile_, link
+
+
 def build(jobs: int | None = None) -> str:
-    """Compile every source (HIP kernels; the host-only GGUF reader) and link libgqk.so (always rebuilds); returns the library path."""
+    """Compile every source (HIP kernels; the host-only GGUF reader; the eager calls' module) and link libgqk.so and _fast.so (always
+    rebuilds); returns the library path."""
     os.makedirs(BUILD, exist_ok=True)
     objs = []
     cmds = []
@@ -49,11 +68,15 @@ def build(jobs: int | None = None) -> str:
         obj = os.path.join(BUILD, name)
         objs.append(obj)
         cmds.append([HIPCC, *FLAGS, *extra, "-c", os.path.join(CSRC, src), "-o", obj])
+    compile_module, link_module = _module_commands()
+    cmds.append(compile_module)
     with ThreadPoolExecutor(max_workers=jobs or min(len(cmds), os.cpu_count() or 4)) as ex:
         list(ex.map(_run, cmds))
     tmp = LIB + ".tmp"
     _run([HIPCC, "-shared", f"--offload-arch={ARCH}", "-o", tmp, *objs])
     os.replace(tmp, LIB)
+    _run(link_module)
+    os.replace(MODULE + ".tmp", MODULE)
     return LIB
 
 

@@ -18,6 +18,11 @@ except AttributeError:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def unwatched() -> bool:
+    """Whether a call may try the module of the eager calls, which sees everything else for itself (gqk_torch.cpp)."""
+    return not torch.compiler.is_compiling() and getattr(forward_ad, "_current_level", 0) < 0
+
+
 def stream(device: torch.device) -> int:
     """The device's current stream as a raw handle (no Stream object is made)."""
     return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)

@@ -246,6 +246,7 @@ def device_workspace(device: torch.device, need: int = 0) -> torch.Tensor:
             size = max(need, check(lib.gqk_workspace_bytes_max(), "workspace_bytes_max"))
         ws = torch.zeros((size + 3) // 4, dtype=torch.int32, device=torch.device("cuda", idx))
         _WORKSPACES[idx] = ws
+        _lib._fast.set_workspace(idx, ws)
     return ws
 
 

@@ -8,8 +8,8 @@ import numpy as np
 import torch
 
 from . import ops
-from ._lib import check, lib
-from .eager import stream as _stream
+from ._lib import _fast, check, lib
+from .eager import stream as _stream, unwatched as _unwatched
 
 
 def _pairs(t, what: str) -> np.ndarray:
@@ -36,6 +36,8 @@ def copy_pages(pages: torch.Tensor, src, dst, dim: int = 0) -> None:
     arrays or CPU tensors); a page outside of the cache, written twice, or both read and written raises ValueError and
     nothing is copied.  Under HIP graph capture the pairs of the capture are recorded."""
     what = "copy_pages"
+    if _unwatched() and _fast.copy_pages(pages, src, dst, dim):
+        return
     ops._require_gpu(pages, what)
     dim = dim + pages.dim() if dim < 0 else dim
     if not 0 <= dim < pages.dim():

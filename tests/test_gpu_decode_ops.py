@@ -680,3 +680,91 @@ def test_copy_pages_views_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert (store[:, 8:] == step + 1).all() and torch.equal(store[:, 2:8], want[:, 2:8])
+
+
+# ---- the eager way ---------------------------------------------------------------------------
+
+def _eager_calls():
+    """Arguments of each function of the eager calls' module, as the Python functions pass them."""
+    gen = _gen(1)
+    k, v, table = _cache(gen, [70, 40], 16, 2, 64, BF, "heads", poison=False)
+    q = _randn(gen, 2, 8, 64, dtype=BF)
+    n = torch.tensor([70, 40], dtype=torch.int32, device="cuda")
+    attend = [q, k, v, table, n, None, 0, None, None, None, None, True, None]
+    hq, hk, hv, rt, pos, wq, wk = _rope_case(gen, 3, 4, 2, 64, BF, 64, BF)
+    rope = [hq, hk, pos, rt, wq, wk, 1e-6, 0, hv, k, v, torch.tensor([0, 1, 2], device="cuda"), None, None, None, None]
+    y, x, a, b, scales = _lora_case(gen, 5, 64, (16, 24), 8, 2, F16)
+    lora = [y, x, a, b, torch.tensor([0, 1, -1, 0, 1], device="cuda"), scales, (16, 24), None, None]
+    return {"paged_attention": attend, "qk_norm_rope": rope, "lora_add": lora, "copy_pages": [k.transpose(1, 2), [0], [1], 0]}
+
+
+@pytest.mark.parametrize("name", ["paged_attention", "qk_norm_rope", "lora_add", "copy_pages"])
+def test_eager_calls_are_taken_and_step_aside(name):
+    """A plain call is served without the Python path; a subclass, lazy negation, autograd, a mode, a profiler or a
+    functorch transform sends it there (None, and nothing written)."""
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from gguf_hip import _lib, ops
+
+    ops.shared_workspace(torch.device("cuda", 0))
+    args = _eager_calls()[name]
+    call = getattr(_lib._fast, name)
+    assert call(*args) is not None
+    before = args[0].clone()
+
+    class Sub(torch.Tensor):
+        pass
+
+    class Function(TorchFunctionMode):
+        pass
+
+    class Dispatch(TorchDispatchMode):
+        pass
+
+    assert call(args[0].as_subclass(Sub), *args[1:]) is None
+    assert call(torch._neg_view(args[0]), *args[1:]) is None
+    assert call(args[0].cpu(), *args[1:]) is None and call(None, *args[1:]) is None
+    assert call(args[0].detach().requires_grad_(), *args[1:]) is None
+    with torch.no_grad():
+        assert call(args[0].detach().requires_grad_(), *args[1:]) is not None
+    for mode in (Function(), Dispatch(), torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU])):
+        with mode:
+            assert call(*args) is None
+    seen = []
+    torch.func.vmap(lambda t: seen.append(call(*args)) or t)(torch.zeros(2, 1, device="cuda"))
+    assert seen == [None]
+    with torch.inference_mode():
+        assert call(*args) is not None
+    assert call(*args[:-1]) is None                          # another number of arguments
+    assert call(*args) is not None
+    if name == "copy_pages":
+        assert call(args[0], [0], [0], 0) is None and call(args[0], [0, 2], [1, 1], 0) is None and call(args[0], [0], [99], 0) is None
+    assert torch.equal(before, args[0])
+
+
+def test_eager_calls_agree_with_the_ops():
+    """The same bits through the eager module, the Python path and the registered ops; versions are bumped."""
+    from gguf_hip import adapters, attention
+
+    e = _eager_calls()
+    q, k, v, table, n = e["paged_attention"][:5]
+    out, lse = gguf_hip.paged_attention(q, k, v, table, n, return_lse=True)
+    o2, l2 = torch.empty_like(out), torch.empty_like(lse)
+    attention._attention_op(q, k, v, table, n, 0.125, 0, None, None, 80, o2, l2, None)
+    assert torch.equal(out, o2) and torch.equal(lse, l2)
+    o3 = torch.empty_like(out)
+    version = o3._version
+    gguf_hip.paged_attention(q, k, v, table, n, out=o3)
+    assert o3._version > version and torch.equal(o3, out)
+    y, x, a, b, ids, scales, outs = e["lora_add"][:7]
+    out = gguf_hip.lora_add(y, x, a, b, ids, scales, outs)
+    o2 = torch.empty_like(out)
+    adapters._lora_op(y, x, a, b, ids, scales, list(outs), o2, None)
+    assert torch.equal(out, o2)
+    hq, hk, pos, rt, wq, wk = e["qk_norm_rope"][:6]
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        through_op = gguf_hip.qk_norm_rope(hq, hk, pos, rt, wq, wk)
+    assert any("qk_norm_rope" in ev.key for ev in prof.key_averages())
+    eager = gguf_hip.qk_norm_rope(hq, hk, pos, rt, wq, wk)
+    assert torch.equal(eager[0], through_op[0]) and torch.equal(eager[1], through_op[1])
