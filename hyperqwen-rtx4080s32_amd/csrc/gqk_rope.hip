@@ -117,27 +117,47 @@ template <int LPH> __device__ __forceinline__ float head_sum(float x) {
   return x;
 }
 
-// Eight dims to a lane, DP / 8 lanes to a head, so that a wave reads 64 x 16 bytes of neighbouring heads at once; a token's
-// waves go over its heads with the token's cosines and sines and both norms' weights in registers.  Pairs that are
-// rot / 2 apart meet by a shuffle of the normalized values (rot a multiple of 16: a lane's dims have their partners in
-// one other lane); interleaved pairs are a lane's own (rot a multiple of 8).  One pass over the bytes, which bound it.
+// Eight dims to a lane, DP / 8 lanes to a head, so that a wave reads 64 x 16 bytes of neighbouring heads at once.  A round
+// is 64 LPH heads of one kind (queries, keys, values), the same for the whole wave; a token's waves deal its rounds.
+// The rotation of a normalized head is  y = r (x A + x' B)  with x' the other dim of the pair, A = w cos and B = -+ w' sin:
+// A and B are made once for a token and kept in registers, and r is the head's own.  Pairs that are rot / 2 apart meet
+// by a shuffle of the packed values (rot a multiple of 16: a lane's dims have their partners in one other lane);
+// interleaved pairs are a lane's own (rot a multiple of 8).  One pass over the bytes, which bound it.
 template <typename T, typename C, int DP, bool INTER>
 __global__ __launch_bounds__(64 * kWaves) void rope_kernel(RopeArgs a, int waves) {
-  constexpr int LPH = DP / 8, HPW = 64 / LPH;   // lanes of a head, heads of a wave
-  const int64_t item = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  constexpr int LPH = DP / 8, HPW = 64 / LPH;   // lanes of a head, heads of a round
+  struct alignas(16) Raw { uint32_t w[4]; };
+  const int64_t item = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t = item / waves;
   const int part = (int)(item - t * waves);
   if (t >= a.tokens) return;
-  const int lane = threadIdx.x & 63, sub = lane & (LPH - 1), d = sub * 8, D = a.dim, half = a.rot >> 1;
+  const int lane = threadIdx.x & 63, sub = lane & (LPH - 1), own = lane / LPH, d = sub * 8, D = a.dim, half = a.rot >> 1;
   const bool live = d < D;
   const int at = live ? d : 0;
   const float nan = __builtin_nanf("");
+  const int rq = (a.q_heads + HPW - 1) / HPW, rk = (a.k_heads + HPW - 1) / HPW;
+  const int rounds = rq + rk + (a.store ? (a.kv.heads + HPW - 1) / HPW : 0);
+  // round i: the kind, the lane's head of it, whether there is one
+  auto kind_of = [&](int i) { return i < rq ? 0 : i < rq + rk ? 1 : 2; };
+  auto head_of = [&](int i, int kind) { return (kind == 0 ? i : kind == 1 ? i - rq : i - rq - rk) * HPW + own; };
+  auto count_of = [&](int kind) { return kind == 0 ? a.q_heads : kind == 1 ? a.k_heads : a.kv.heads; };
+  auto load = [&](int i) {
+    Raw x{};
+    const int kind = kind_of(i), h = head_of(i, kind);
+    const T* base = kind == 0 ? (const T*)a.q + t * a.q_row : kind == 1 ? (const T*)a.k + t * a.k_row : (const T*)a.v + t * a.v_row;
+    const int64_t stride = kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head;
+    if (live && h < count_of(kind)) x = *(const Raw*)(base + h * stride + d);
+    return x;
+  };
+  Raw next{};
+  if (part < rounds) next = load(part);   // on its way while the angles are looked up
   const int64_t pos = index_at(a.positions, a.wide_positions, t);
   const bool in = pos >= 0 && pos < a.table_rows;
-  const bool turned = live && d < a.rot, second = d >= half;
-  float cs[8], sn[8], wq[8], wk[8];
+  const bool turned = live && d < a.rot, second = !INTER && d >= half;
+  const int mate = INTER || !turned ? lane : second ? lane - half / 8 : lane + half / 8;
+  float cs[8], sn[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) { cs[e] = 1.f; sn[e] = 0.f; wq[e] = wk[e] = 1.f; }
+  for (int e = 0; e < 8; ++e) { cs[e] = in ? 1.f : nan; sn[e] = 0.f; }   // a position that is not in the table: NaN
   if (turned && in) {
     if constexpr (INTER) {
       const float4 c = *(const float4*)(a.table + pos * a.rot + (d >> 1)), s = *(const float4*)(a.table + pos * a.rot + half + (d >> 1));
@@ -151,68 +171,82 @@ __global__ __launch_bounds__(64 * kWaves) void rope_kernel(RopeArgs a, int waves
       for (int e = 0; e < 8; ++e) sn[e] = second ? sn[e] : -sn[e];
     }
   }
-  auto weights = [&](const void* w, float* to) {
-    if (!w) return;
-    if (a.weight_f32) load8((const float*)w + at, to);
-    else load8((const T*)w + at, to);
-    if (a.unit_offset)
+  float A[2][8], B[2][8];   // of queries and of keys
 #pragma unroll
-      for (int e = 0; e < 8; ++e) to[e] += 1.f;
-  };
-  weights(a.q_weight, wq);
-  weights(a.k_weight, wk);
+  for (int k = 0; k < 2; ++k) {
+    // the wave's first round that is not before the kind's
+    const int begin = k ? rq : 0, end = k ? rq + rk : rq, i = begin <= part ? part : part + (begin - part + waves - 1) / waves * waves;
+    if (i >= end) continue;   // none of the kind
+    const void* w = k ? a.k_weight : a.q_weight;
+    float own_w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) own_w[e] = 1.f;
+    if (w) {
+      if (a.weight_f32) load8((const float*)w + at, own_w);
+      else load8((const T*)w + at, own_w);
+      if (a.unit_offset)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) own_w[e] += 1.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      A[k][e] = own_w[e] * cs[e];
+      B[k][e] = (INTER ? own_w[e ^ 1] : __shfl(own_w[e], mate)) * sn[e];
+    }
+  }
   int64_t page = 0, place = 0;
   bool keep = false;
   if (a.store) {
     const int64_t slot = index_at(a.slots, a.wide_slots, t);
     const int64_t room = (int64_t)a.kv.pages * a.kv.page_size;
-    keep = live && slot >= 0 && slot < room;
+    keep = slot >= 0 && slot < room;
     if (keep) {
       page = room >> 32 ? slot / a.kv.page_size : (uint32_t)slot / (uint32_t)a.kv.page_size;   // a division in 64 bits costs
       place = slot - page * a.kv.page_size;
     }
   }
-  const int heads = a.q_heads + a.k_heads + (a.store ? a.kv.heads : 0), hop = waves * HPW;
-  for (int h = part * HPW + lane / LPH; h - lane / LPH < heads; h += hop) {   // the same for all lanes
-    const bool some = h < heads, is_q = h < a.q_heads, is_v = h >= a.q_heads + a.k_heads;
-    const int hh = !some ? 0 : is_q ? h : is_v ? h - a.q_heads - a.k_heads : h - a.q_heads;
-    const T* from = is_q ? (const T*)a.q + t * a.q_row + hh * a.q_head
-                         : is_v ? (const T*)a.v + t * a.v_row + hh * a.v_head : (const T*)a.k + t * a.k_row + hh * a.k_head;
-    float x[8], y[8];
-    if (some && live) load8(from + at, x);
-    else
+  for (int i = part; i < rounds; i += waves) {
+    const Raw raw = next;
+    if (i + waves < rounds) next = load(i + waves);   // no head is written by another's round, in place either
+    const int kind = kind_of(i), h = head_of(i, kind);
+    float y[8];
+    T v[8];
+    __builtin_memcpy(v, &raw, 16);
+    if (kind == 2) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-    ss = head_sum<LPH>(ss);
-    const bool norm = is_q ? a.q_weight != nullptr : a.k_weight != nullptr;
-    const float r = norm && !is_v ? rsqrtf(ss / D + a.eps) : 1.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= is_v ? 1.f : r * (is_q ? wq[e] : wk[e]);
-    if constexpr (INTER) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = x[e] * cs[e] + x[e ^ 1] * sn[e];
+      for (int e = 0; e < 8; ++e) y[e] = to_f(v[e]);
     } else {
-      const int mate = turned ? (second ? lane - half / 8 : lane + half / 8) : lane;
+      Raw other = raw;
+      if constexpr (!INTER)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = x[e] * cs[e] + __shfl(x[e], mate) * sn[e];
+        for (int w = 0; w < 4; ++w) other.w[w] = turned ? __shfl(raw.w[w], mate) : 0;
+      T o[8];
+      __builtin_memcpy(o, &other, 16);
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += to_f(v[e]) * to_f(v[e]);
+      ss = head_sum<LPH>(ss);
+      const float r = (kind ? a.k_weight : a.q_weight) ? rsqrtf(ss / D + a.eps) : 1.f;
+      auto turn = [&](const float (&fa)[8], const float (&fb)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // what is not turned has no other: not 0 times one that is not finite
+          const float z = INTER ? (turned ? to_f(v[e ^ 1]) : 0.f) : to_f(o[e]);
+          y[e] = r * (to_f(v[e]) * fa[e] + z * fb[e]);
+        }
+      };
+      if (kind == 0) turn(A[0], B[0]);
+      else turn(A[1], B[1]);
     }
-    if (!some || !live) continue;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = is_v || !turned ? x[e] : y[e];   // a partner that is not finite stays out of what is not turned
-    if (!in && !is_v)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = nan;
-    if (is_q) store8((T*)a.out_q + t * a.oq_row + hh * a.oq_head + d, y);
-    else if (!is_v && a.out_k) store8((T*)a.out_k + t * a.ok_row + hh * a.ok_head + d, y);
-    if (!is_q && keep) {
-      const float* sc = is_v ? a.kv.v_scale : a.kv.k_scale;
-      C* to = is_v ? (C*)a.kv.v + page * a.kv.v_page + place * a.kv.v_token + hh * a.kv.v_head
-                   : (C*)a.kv.k + page * a.kv.k_page + place * a.kv.k_token + hh * a.kv.k_head;
+    if (!live || h >= count_of(kind)) continue;
+    if (kind == 0) store8((T*)a.out_q + t * a.oq_row + h * a.oq_head + d, y);
+    else if (kind == 1 && a.out_k) store8((T*)a.out_k + t * a.ok_row + h * a.ok_head + d, y);
+    if (kind > 0 && keep) {
+      const float* sc = kind == 2 ? a.kv.v_scale : a.kv.k_scale;
+      C* to = kind == 2 ? (C*)a.kv.v + page * a.kv.v_page + place * a.kv.v_token + h * a.kv.v_head
+                        : (C*)a.kv.k + page * a.kv.k_page + place * a.kv.k_token + h * a.kv.k_head;
       if (sc) {
-        const float s = sc[hh];
+        const float s = sc[h];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] /= s;
       }
@@ -223,9 +257,12 @@ __global__ __launch_bounds__(64 * kWaves) void rope_kernel(RopeArgs a, int waves
 
 template <typename T, typename C, int DP>
 void launch(const RopeArgs& a, bool inter, hipStream_t st) {
-  const int heads = a.q_heads + a.k_heads + (a.store ? a.kv.heads : 0), rounds = (heads + 512 / DP - 1) / (512 / DP);
-  // Waves of a token: one round of heads each until the launch fills the device, then 4
-  const int waves = a.tokens <= 128 ? rounds : std::min(rounds, 4);
+  constexpr int HPW = 512 / DP;   // heads of a round
+  auto of = [](int heads) { return (heads + HPW - 1) / HPW; };
+  const int rounds = of(a.q_heads) + of(a.k_heads) + (a.store ? of(a.kv.heads) : 0);
+  // Waves of a token: one for each round until the launch has 4096 (16 a CU), then as many as make that, as a wave spends as
+  // long on looking up a token's angles as on some rounds (8191 tokens of 14 rounds: 1 wave 60 us, 2 63, 4 75, 14 123)
+  const int waves = std::max(1, std::min(rounds, 4096 / a.tokens));
   const dim3 grid((unsigned)(((int64_t)a.tokens * waves + kWaves - 1) / kWaves));
   if (inter) rope_kernel<T, C, DP, true><<<grid, 64 * kWaves, 0, st>>>(a, waves);
   else rope_kernel<T, C, DP, false><<<grid, 64 * kWaves, 0, st>>>(a, waves);
