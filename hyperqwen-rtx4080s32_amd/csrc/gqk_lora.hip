@@ -168,33 +168,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) load(d, s0 + d);
     __syncthreads();   // the last unit's stages have been read
-    for (int i = 0; i < stages; i += kDepth)
+    auto stage = [&](int d, int s) {
+      char* const to = buf[d & 1];   // kDepth is even
+      char* const at = to + row * 256 + (piece ^ row) * 16;
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d)
-        if (i + d < stages) {
-          char* const to = buf[d & 1];   // kDepth is even
-          char* const at = to + row * 256 + (piece ^ row) * 16;
+      for (int t = 0; t < TT; ++t) *(v4u*)(at + t * 4096) = xv[d][t];
 #pragma unroll
-          for (int t = 0; t < TT; ++t) *(v4u*)(at + t * 4096) = xv[d][t];
+      for (int t = 0; t < kRankTiles; ++t) *(v4u*)(at + (TT + t) * 4096) = av[d][t];
+      load(d, s + kDepth);
+      __syncthreads();
+      if (busy)
 #pragma unroll
-          for (int t = 0; t < kRankTiles; ++t) *(v4u*)(at + (TT + t) * 4096) = av[d][t];
-          load(d, s0 + i + d + kDepth);
-          __syncthreads();
-          if (busy)
+        for (int k = 0; k < kStage / 32; ++k) {
+          const char* from = to + n * 256 + ((k * 4 + g) ^ n) * 16;
+          const v4u xop = *(const v4u*)(from + (TT == 1 ? 0 : wave) * 4096);
+          if constexpr (TT == 1) {
+            acc[0] = mfma(*(const v4u*)(from + (TT + wave) * 4096), xop, acc[0], T{});
+          } else {
+            // of tiles that the chunk does not have too: zeros cost less than the copies that a branch around each
+            // instruction takes (64 moves a product counted)
 #pragma unroll
-            for (int k = 0; k < kStage / 32; ++k) {
-              const char* from = to + n * 256 + ((k * 4 + g) ^ n) * 16;
-              const v4u xop = *(const v4u*)(from + (TT == 1 ? 0 : wave) * 4096);
-              if constexpr (TT == 1) {
-                acc[0] = mfma(*(const v4u*)(from + (TT + wave) * 4096), xop, acc[0], T{});
-              } else {
-                // of tiles that the chunk does not have too: zeros cost less than the copies that a branch around each
-                // instruction takes (64 moves a product counted)
-#pragma unroll
-                for (int r = 0; r < kRankTiles; ++r) acc[r] = mfma(*(const v4u*)(from + (TT + r) * 4096), xop, acc[r], T{});
-              }
-            }
+            for (int r = 0; r < kRankTiles; ++r) acc[r] = mfma(*(const v4u*)(from + (TT + r) * 4096), xop, acc[r], T{});
+          }
         }
+    };
+    // whole rounds of kDepth without a branch: the loads of the next stages stay on their way through a wait
+    int i = 0;
+    for (; i + kDepth <= stages; i += kDepth)
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) stage(d, s0 + i + d);
+#pragma unroll
+    for (int d = 0; d < kDepth - 1; ++d)
+      if (i + d < stages) stage(d, s0 + i + d);
     // lane (n, g) holds ranks 4 g .. + 3 of a tile for row n
     const int r_at = (TT == 1 ? 0 : wave) * 16 + n;
     if (busy && r_at < unit.count) {
