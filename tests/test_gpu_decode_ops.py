@@ -768,3 +768,20 @@ def test_eager_calls_agree_with_the_ops():
     assert any("qk_norm_rope" in ev.key for ev in prof.key_averages())
     eager = gguf_hip.qk_norm_rope(hq, hk, pos, rt, wq, wk)
     assert torch.equal(eager[0], through_op[0]) and torch.equal(eager[1], through_op[1])
+
+
+# ---- all together ----------------------------------------------------------------------------
+
+def test_decode_step_example():
+    """examples/decode_step.py: prompts, steps by a graph, a fork, a compaction.  Per layer a token's value is rounded at most eight
+    times on its way (projection, adapter, heads, cache, probabilities, attention, projection, adapter), weights once, each at
+    most 2^-8 of it: two layers stay within 18 * 2^-8."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "decode_step.py")
+    spec = importlib.util.spec_from_file_location("decode_step", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    got = module.run(steps=6)
+    assert sorted(got["errors"]) == ["a", "b", "c", "d"] and got["moved"] > 0
+    assert max(got["errors"].values()) < 18 * 2.0 ** -8, got
