@@ -38,6 +38,7 @@ struct LoraArgs {
   int M, slots, parts, rank, wide_ids;
   int splits, chunks, blocks;   // splits of K; chunks of 64 ranks; blocks of rows
   int columns;               // of a workgroup of the second kernel
+  int half_units;            // the second kernel takes long batches by 32 rows, not 64
   int wide_y;                // y and out are 16-byte aligned in every row
   int64_t ends[kParts];      // one past each part's last column
 };
@@ -114,8 +115,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64
 }
 // An offset past every buffer, with what is added to it too: a row of x or A is below 2^23 bytes, columns below 2^12.
 constexpr uint32_t kOutside = 0x80000000u;
+constexpr int kOnce = 2;   // a load's cache policy: its lines leave the cache first
+template <int POLICY = 0>
 __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset) {
-  return __builtin_amdgcn_raw_buffer_load_b128(rs, offset, 0, 0);
+  return __builtin_amdgcn_raw_buffer_load_b128(rs, offset, 0, POLICY);
 }
 
 // h = A x of one unit's rows, 64 ranks, one split of K.  Rows of x and of A are far apart, and a lane of a matrix operand
@@ -123,7 +126,8 @@ __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset
 // time come in as rows, 16 lanes to one, go through LDS with their 16-byte pieces swapped by the row's number (16 rows'
 // pieces of one k-step in different banks), and are read as operands: ranks as the instruction's rows, batch rows as its
 // columns.  Loads run kDepth stages ahead in registers; two LDS buffers, one barrier a stage.  A wave takes one 16-row tile and all
-// ranks (TT = 4), or all 16 rows and one 16-rank tile (TT = 1).
+// ranks (TT = 4), or all 16 rows and one 16-rank tile (TT = 1).  x goes by once and leaves the caches first, so that A, which every
+// block of rows reads again, stays (4096 rows of 17408 values 82.4 -> 78.1 us, both launches).
 template <typename T, int TT, int Q>
 __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
   constexpr int kDepth = TT == 1 ? 4 : 2;
@@ -158,7 +162,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
     auto load = [&](int d, int s) {
       const bool in = s < s0 + stages && s * kStage + piece * 8 < K;   // K may end inside the last stage
 #pragma unroll
-      for (int t = 0; t < TT; ++t) xv[d][t] = load16(rx, in ? xo[t] + s * (2 * kStage) : kOutside);
+      for (int t = 0; t < TT; ++t) xv[d][t] = load16<kOnce>(rx, in ? xo[t] + s * (2 * kStage) : kOutside);
 #pragma unroll
       for (int t = 0; t < kRankTiles; ++t) av[d][t] = load16(ra, in ? ao[t] + s * (2 * kStage) : kOutside);
     };
@@ -491,14 +495,23 @@ void launch(const LoraArgs& g, const Cut& c, hipStream_t st) {
   }
   const int near = std::min(c.blocks, kXcds);
   if (g.slots > 0) lora_down_kernel<T, TT, Q><<<dim3(c.splits * c.chunks, units, c.blocks), 64 * kWaves, 0, st>>>(g);
-  auto up = [&](auto each) {
-    constexpr int kEach = decltype(each)::value, kRanks = 8 * kEach;
-    const size_t lds = (size_t)16 * TT * 2 * ((g.rank + kRanks - 1) / kRanks * kRanks + 8) * sizeof(T);
-    lora_up_kernel<T, TT, Q, kEach><<<dim3((unsigned)(blocks * near), units, (c.blocks + near - 1) / near), 64 * kWaves, lds, st>>>(g);
+  auto up = [&](auto each, auto tiles) {
+    constexpr int kEach = decltype(each)::value, kRanks = 8 * kEach, UT = decltype(tiles)::value;
+    const size_t lds = (size_t)16 * UT * 2 * ((g.rank + kRanks - 1) / kRanks * kRanks + 8) * sizeof(T);
+    lora_up_kernel<T, UT, Q, kEach><<<dim3((unsigned)(blocks * near), TT == 1 ? units : 1 + 4 / UT, (c.blocks + near - 1) / near),
+                                      64 * kWaves, lds, st>>>(g);
   };
-  if (g.rank <= 16) up(std::integral_constant<int, 2>{});
-  else if (g.rank <= 32) up(std::integral_constant<int, 4>{});
-  else up(std::integral_constant<int, 8>{});
+  auto by_rank = [&](auto tiles) {
+    if (g.rank <= 16) up(std::integral_constant<int, 2>{}, tiles);
+    else if (g.rank <= 32) up(std::integral_constant<int, 4>{}, tiles);
+    else up(std::integral_constant<int, 8>{}, tiles);
+  };
+  if constexpr (TT == 1) {
+    by_rank(std::integral_constant<int, 1>{});
+  } else {
+    if (g.half_units) by_rank(std::integral_constant<int, 2>{});
+    else by_rank(std::integral_constant<int, 4>{});
+  }
 }
 
 }  // namespace
@@ -552,6 +565,9 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
   for (int p = 0; p < parts; ++p) g.wide_y &= g.ends[p] % 8 == 0;
   // columns of a workgroup of the second kernel, which gathers h once for them: 64 for each wave, more where the launch
   // has workgroups enough
+  // Units of 32 rows where 64 would leave too few workgroups for the chip (us for 64 and 32: 5120 columns of rank 64, 512 rows
+  // 27.8 and 22.6, 1024 rows 38.9 and 31.7, 4096 rows 78.2 and 79.9; 34816 columns, 300 rows 39.4 and 29.9, 512 rows 28.0 and 30.0).
+  g.half_units = M > kSmall && c.blocks * (g.N / 256) <= 1024;
   const int64_t groups = M <= kSmall ? std::min(M, 16) : c.blocks;
   g.columns = 64 * kWaves;
   while (g.columns < 1024 && groups * (g.N / g.columns) > 256) g.columns *= 2;
