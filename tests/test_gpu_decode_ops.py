@@ -510,6 +510,15 @@ def test_lora_rows_and_depth(M, K):
     _lora_check(M + K, M, K, (200, 56), 16, 9, BF)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("rank", [8, 24, 32, 72, 256])
+@pytest.mark.parametrize("n_outs", [(264, 3), (53_000, 7_000)])
+def test_lora_prompts(dtype, rank, n_outs):
+    """Long batches of few and of many columns, whose rows come mixed or in runs."""
+    _lora_check(rank, 300, 136, n_outs, rank, 4, dtype)
+    _lora_check(rank, 300, 136, n_outs, rank, 4, dtype, torch.arange(300, device="cuda") // 90)
+
+
 def test_lora_batches():
     """One adapter for all rows, none for any, all rows different, runs of rows, ids of either width, no scales."""
     dev = "cuda"
