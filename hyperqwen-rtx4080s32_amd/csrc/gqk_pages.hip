@@ -15,11 +15,16 @@ struct CopyArgs {
   int32_t src[kPairs], dst[kPairs];
 };
 
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+// A workgroup copies one page of one plane; nothing is computed, memory bounds it.  Lines on their way through leave the
+// caches first (400 pages of 16 KiB in 128 planes: 325 -> 306 us, 5.5 TB/s read and written together).
 template <typename W>
 __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
   const W* from = (const W*)(a.base + blockIdx.y * a.plane + a.src[blockIdx.x] * a.page);
   W* to = (W*)(a.base + blockIdx.y * a.plane + a.dst[blockIdx.x] * a.page);
-  for (int64_t i = threadIdx.x; i < a.bytes / (int64_t)sizeof(W); i += 256) to[i] = from[i];
+  for (int64_t i = threadIdx.x; i < a.bytes / (int64_t)sizeof(W); i += 256)
+    __builtin_nontemporal_store(__builtin_nontemporal_load(from + i), to + i);
 }
 
 }  // namespace
@@ -62,7 +67,7 @@ extern "C" int gqk_copy_pages(void* base, int64_t planes, int64_t plane_stride, 
       const int c = (int)(n - i0 < kPairs ? n - i0 : kPairs);
       for (int i = 0; i < c; ++i) a.src[i] = src[i0 + i], a.dst[i] = dst[i0 + i];
       const dim3 grid(c, (unsigned)(planes - p0 < 32768 ? planes - p0 : 32768));
-      if (!(bits & 15)) copy_kernel<uint4><<<grid, 256, 0, st>>>(a);
+      if (!(bits & 15)) copy_kernel<v4u><<<grid, 256, 0, st>>>(a);
       else if (!(bits & 3)) copy_kernel<uint32_t><<<grid, 256, 0, st>>>(a);
       else copy_kernel<uint8_t><<<grid, 256, 0, st>>>(a);
     }

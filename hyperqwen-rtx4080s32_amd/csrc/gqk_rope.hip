@@ -76,6 +76,7 @@ __global__ __launch_bounds__(64) void rope_any_kernel(RopeArgs a) {
   }
 }
 
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int64_t kTokens = 32768;   // of one launch
 
@@ -146,7 +147,10 @@ __global__ __launch_bounds__(64 * kWaves) void rope_kernel(RopeArgs a, int waves
     const int kind = kind_of(i), h = head_of(i, kind);
     const T* base = kind == 0 ? (const T*)a.q + t * a.q_row : kind == 1 ? (const T*)a.k + t * a.k_row : (const T*)a.v + t * a.v_row;
     const int64_t stride = kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head;
-    if (live && h < count_of(kind)) x = *(const Raw*)(base + h * stride + d);
+    if (live && h < count_of(kind)) {
+      const v4u z = __builtin_nontemporal_load((const v4u*)(base + h * stride + d));   // read once: 56.6 -> 55.2 us (8191 tokens)
+      __builtin_memcpy(&x, &z, 16);
+    }
     return x;
   };
   Raw next{};
