@@ -137,7 +137,17 @@ struct Joined {
 // crosses lanes:  S^T = K Q^T: lane l = (head n = l % 16, g = l / 16) gets the scores of keys 8 g .. 8 g + 7 of the step (the
 // rows of the two 16-key tiles are dealt so), which is what O^T += V^T P^T wants of it as an operand.  K comes from global
 // memory straight as operands (8 dims of a key per lane).  V's operands hold 8 keys of one dim: a lane loads 8 dims of
-// each of its 8 keys and transposes the 8 x 8 block in registers, one v_perm per pair.  No LDS, no barrier in the loop.
+// each of its 8 keys and transposes the 8 x 8 block in registers, one v_perm per pair.  No barrier in the loop, and no LDS but for
+// the queries of 256 dims.
+//
+// Scores, statistics and sums are in 32 bits; the probabilities become T for the second product (at most 2^-9 of each for bf16, as
+// random as the output's own rounding: 1.9e-3 of error against 64 bits where the output's rounding alone has 1.7e-3), two terms
+// of T would need twice the instructions.  8-bit keys and values widen to T exactly, their scales go
+// into the score's and the output's factor.
+//
+// Memory bounds it: 2.6 GB of bf16 keys and values (128 sequences of up to 8000) 406 us, 6.5 TB/s; 330 MB (32 of up to 4000)
+// 61.8 us, 5.3 TB/s; fp16 heads of 256 dims under a window, 1.5 GB, 253 us, 5.8 TB/s; 268 MB of 8-bit pages of one sequence
+// 47 us and 6 for the join.  A sequence of 61 keys takes 4.8 us: a launch, and lengths, table and keys read one after the other.
 template <typename T, typename C, int DP, bool FULL, bool P8, bool TIGHT>
 __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kernel(AttnArgs a) {
   constexpr bool F8 = sizeof(C) == 1;
@@ -512,7 +522,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
 }
 
 // The join of more splits than one workgroup takes at once: a workgroup for each query head, its threads over the splits and
-// the dims.  (One workgroup per sequence and key head took 16 us for 64 splits of 5 heads, 39 for 128 of 16.)
+// the dims.  (One workgroup per sequence and key head took 16 us for 64 splits of 5 heads, 39 for 128 of 16.)  96 splits of 40 heads: 5.8 us,
+// of which a launch that waits for another takes about half.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
   __shared__ __align__(16) float sums[256][4];
@@ -564,8 +575,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
 // How a call is cut: workgroups over the query heads of a key head, and splits of `chunk` keys.
 struct Cut { int row_waves, row_blocks, splits, chunk; };
 
-// About as many workgroups as stay resident, of 256 keys at least (32 x 4000 tokens in bf16: 3 a CU 73.9 us, 4 66.8, 6 70.4,
-// 8 68.5; in fp8 40.9, 43.9, 42.2, 43.1; 8 x 2000 in splits of 128 keys or more 16.5, of 256 13.6).
+// About as many workgroups as stay resident, of 256 keys at least (32 x 4000 tokens in bf16: 3 a CU 69.9 us, 4 62.4, 6 66.3,
+// 8 64.2; 64 x 3000 of 256 dims in fp8: 3 a CU 50.2, 4 58.3, 5 55.6; 8 x 2000 in splits of 128 keys or more 16.5, of 256 13.6).
 Cut cut_of(int batch, int q_heads, int kv_heads, int size, int max_length, int window) {
   const int group = q_heads / kv_heads, tiles = (group + 15) / 16;
   Cut c;

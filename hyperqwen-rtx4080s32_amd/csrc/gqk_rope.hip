@@ -27,7 +27,8 @@ struct RopeArgs {
   int wide_positions, wide_slots, unit_offset, interleaved, weight_f32, store;
 };
 
-// Any even rot: one wave per (token, head), q heads, k heads, then v heads (stored only); the normalized head in LDS.
+// Any even rot, and tables or weights off 16 bytes: one wave per (token, head), q heads, k heads, then v heads (stored only); the
+// normalized head in LDS.  The general form, not the fast one: it looks up a token's angles again for each head.
 template <typename T, typename C>
 __global__ __launch_bounds__(64) void rope_any_kernel(RopeArgs a) {
   const int h = blockIdx.x, lane = threadIdx.x, D = a.dim;
@@ -123,7 +124,9 @@ template <int LPH> __device__ __forceinline__ float head_sum(float x) {
 // The rotation of a normalized head is  y = r (x A + x' B)  with x' the other dim of the pair, A = w cos and B = -+ w' sin:
 // A and B are made once for a token and kept in registers, and r is the head's own.  Pairs that are rot / 2 apart meet
 // by a shuffle of the packed values (rot a multiple of 16: a lane's dims have their partners in one other lane);
-// interleaved pairs are a lane's own (rot a multiple of 8).  One pass over the bytes, which bound it.
+// interleaved pairs are a lane's own (rot a multiple of 8).  Arithmetic is in 32 bits, rounded once.  One pass over the bytes, which
+// bound it: 8191 tokens of 40 + 8 + 8 heads of 128 dims, keys kept and stored, 256 MB in 55 us (4.6 TB/s, a copy's rate); one
+// token 3.7 us, a launch and three dependent loads.
 template <typename T, typename C, int DP, bool INTER>
 __global__ __launch_bounds__(64 * kWaves) void rope_kernel(RopeArgs a, int waves) {
   constexpr int LPH = DP / 8, HPW = 64 / LPH;   // lanes of a head, heads of a round
@@ -265,7 +268,7 @@ void launch(const RopeArgs& a, bool inter, hipStream_t st) {
   auto of = [](int heads) { return (heads + HPW - 1) / HPW; };
   const int rounds = of(a.q_heads) + of(a.k_heads) + (a.store ? of(a.kv.heads) : 0);
   // Waves of a token: one for each round until the launch has 4096 (16 a CU), then as many as make that, as a wave spends as
-  // long on looking up a token's angles as on some rounds (8191 tokens of 14 rounds: 1 wave 60 us, 2 63, 4 75, 14 123)
+  // long on looking up a token's angles as on some rounds (8191 tokens of 14 rounds: 1 wave 55 us, 2 63, 4 75, 14 123)
   const int waves = std::max(1, std::min(rounds, 4096 / a.tokens));
   const dim3 grid((unsigned)(((int64_t)a.tokens * waves + kWaves - 1) / kWaves));
   if (inter) rope_kernel<T, C, DP, true><<<grid, 64 * kWaves, 0, st>>>(a, waves);

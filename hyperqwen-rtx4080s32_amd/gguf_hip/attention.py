@@ -1,7 +1,8 @@
 """Attention around the linear path: the heads that qkv's output holds, normalized, rotated and stored into
 the pages of a key-value cache (``qk_norm_rope``), and the attention of each new token over those pages
-(``paged_attention``).  Both are one launch on the current stream, allocate their outputs alone, do not
-synchronise the host and can be captured in a HIP graph; under tracing they are custom ops with fakes.
+(``paged_attention``).  Both run on the current stream (one launch; a second where a
+sequence's keys are cut into more than 16 splits), allocate their outputs alone, do not synchronise the host
+and can be captured in a HIP graph; under tracing they are custom ops with fakes.
 
 Layouts: heads are [tokens, heads, dim] views with any strides (column ranges of qkv's output as they are);
 pages are [pages, page_size, heads, dim] with any strides, so a cache may keep a token's heads or a head's tokens
