@@ -226,6 +226,28 @@ def test_lora_add_shapes_and_refusals():
                 gguf_hip.lora_add(**_lora_args(**bad))
 
 
+def test_make_fx_traces_the_ops():
+    """A traced decode step holds each operator as one opaque call, and no view or copy of the caches."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(q, k, v, positions, table, k_pages, v_pages, slots, block_table, lengths, y, x, a, b, ids):
+        q, _ = gguf_hip.qk_norm_rope(q, k, positions, table, v=v, k_pages=k_pages, v_pages=v_pages, slots=slots)
+        o = gguf_hip.paged_attention(q, k_pages, v_pages, block_table, lengths)
+        return o, gguf_hip.lora_add(y, x, a, b, ids, None, [32, 16]), gguf_hip.lora_add(y, x, a, b, ids, None, [32, 16], out=y)
+
+    with FakeTensorMode():
+        heads, pages, i32 = _fake((3, 2, 64)), _fake((9, 16, 2, 64)), _fake((3,), torch.int32)
+        lo = _lora_args()
+        g = make_fx(step)(_fake((3, 8, 64)), heads, _fake((3, 2, 64)), i32, _fake((100, 64), torch.float32), pages,
+                          _fake((9, 16, 2, 64)), _fake((3,), torch.int32), _fake((3, 4), torch.int32), _fake((3,), torch.int32),
+                          lo["y"], lo["x"], lo["a"], lo["b"], lo["ids"])
+    ops = torch.ops.gguf_hip
+    calls = [n.target for n in g.graph.nodes if n.op == "call_function"]
+    ours = [c for c in calls if str(c).startswith("gguf_hip")]
+    assert ours == [ops.qk_norm_rope.default, ops.paged_attention.default, ops.lora_add.default, ops.lora_add_.default], calls
+    assert all(c in ours or "empty" in str(c) for c in calls), calls
+
+
 def test_pack_adapters():
     g = torch.Generator().manual_seed(1)
     A, B = torch.randn(5, 32, generator=g), torch.randn(12, 5, generator=g)
