@@ -26,6 +26,19 @@ template <> __device__ __forceinline__ fp8_t from_f(float v) {
   return fp8_t{(uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false)};
 }
 
+template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+// the sum over 8, 16 or 32 neighbouring lanes: across pairs, quads, halves of a row and a row by DPP, then over two rows
+template <int LPH> __device__ __forceinline__ float lane_sum(float x) {
+  x = dpp_add<0xB1>(x);    // quad_perm 1, 0, 3, 2
+  x = dpp_add<0x4E>(x);    // quad_perm 2, 3, 0, 1
+  x = dpp_add<0x141>(x);   // row_half_mirror
+  if constexpr (LPH >= 16) x = dpp_add<0x140>(x);   // row_mirror
+  if constexpr (LPH >= 32) x += __shfl_xor(x, 16);
+  return x;
+}
+
 // element i of an index array of 32-bit or 64-bit integers
 __device__ __forceinline__ int64_t index_at(const void* p, int wide, int64_t i) {
   return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];

@@ -25,6 +25,8 @@ constexpr int kList = 64;        // rows of a unit, at most
 // rows come in runs) go by 64 rows and units of up to 64.
 constexpr int kSmall = 256;
 constexpr int kRankTiles = 4;    // 16-rank tiles of a workgroup of the first kernel
+constexpr int kRowColumns = 64 * kWaves;
+constexpr int64_t kRowBytes = 1 << 18;   // of a part's A, that a workgroup of a row reads by itself
 constexpr int kXcds = 8;         // workgroups go to them in turn
 constexpr int kNone = -1, kBad = -2;
 
@@ -478,6 +480,93 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
   }
 }
 
+// A row by itself, in one launch: a workgroup takes 256 columns of one part and works out h of that part.  A wave takes RW
+// ranks: each lane 8 values of K at a time of every rank's row and of x (whole runs of 1 KiB), products and sums in 32
+// bits, the 64 lanes' sums through LDS in fours.  Then a thread has a column: B's row of it, read at the start, times h in 32
+// bits.  A is read by every workgroup of its part, from the caches, which is cheap while a launch leaves CUs idle anyway; it saves
+// the second launch and its wait for the first.  One row of 5120 values to q, k and v, rank 16: 6.9 us (two launches 9.4), of which
+// a launch takes 2 and 164 KiB of A through one CU 3.
+template <typename T, int RW>
+__global__ __launch_bounds__(64 * kWaves, 2) void lora_row_kernel(LoraArgs a) {
+  constexpr int kDepth = 40 / RW;
+  constexpr int kRun = 512;   // values of K that a wave takes at a time
+  __shared__ __align__(16) float sums[RW * kWaves][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t m = blockIdx.y, id = index_at(a.ids, a.wide_ids, m);
+  const int rank = a.rank, K = (int)a.K;
+  int part = 0, block = blockIdx.x;
+  int64_t begin = 0;
+  for (;;) {
+    const int blocks = (int)((a.ends[part] - begin + kRowColumns - 1) / kRowColumns);
+    if (block < blocks) break;
+    block -= blocks;
+    begin = a.ends[part++];
+  }
+  const int64_t c_begin = begin + (int64_t)block * kRowColumns;
+  const int width = (int)min(a.ends[part] - c_begin, (int64_t)kRowColumns), n = threadIdx.x;
+  T* const out = (T*)a.out + m * a.out_row + c_begin + n;
+  const float old = n < width ? to_f(((const T*)a.y)[m * a.y_row + c_begin + n]) : 0.f;
+  if (id < 0 || id >= a.slots) {   // the row as it is, or NaN
+    if (n < width && !(id < 0 && a.out == a.y)) *out = id < 0 ? (T)old : (T)__builtin_nanf("");
+    return;
+  }
+  const __amdgpu_buffer_rsrc_t rx = buffer_of((const T*)a.x + m * a.x_row, (int64_t)K * 2);
+  const __amdgpu_buffer_rsrc_t ra = buffer_of((const T*)a.a + (id * a.parts + part) * rank * K, (int64_t)rank * K * 2);
+  const __amdgpu_buffer_rsrc_t rb = buffer_of((const T*)a.b + (id * a.N + c_begin) * rank, (int64_t)width * rank * 2);
+  uint32_t ao[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) ao[r] = wave * RW + r < rank ? ((wave * RW + r) * (uint32_t)K + lane * 8) * 2 : kOutside;
+  v4u av[kDepth][RW], xv[kDepth];
+  auto load = [&](int d, int j) {
+    const bool in = j * kRun + lane * 8 < K;   // K may end inside the last run
+    xv[d] = load16(rx, in ? (j * kRun + lane * 8) * 2 : kOutside);
+#pragma unroll
+    for (int r = 0; r < RW; ++r) av[d][r] = load16(ra, in ? ao[r] + j * (2 * kRun) : kOutside);
+  };
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) load(d, d);
+  v4u bv[RW / 2];
+#pragma unroll
+  for (int i = 0; i < RW / 2; ++i) bv[i] = load16(rb, n < width && i * 8 < rank ? (n * (uint32_t)rank + i * 8) * 2 : kOutside);
+  const float scale = a.scales ? a.scales[id] : 1.f;
+  float acc[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) acc[r] = 0.f;
+  for (int j = 0; j * kRun < K; j += kDepth)   // past K: zeros
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      T xs[8];
+      __builtin_memcpy(xs, &xv[d], 16);
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        T as[8];
+        __builtin_memcpy(as, &av[d][r], 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[r] += to_f(as[e]) * to_f(xs[e]);
+      }
+      load(d, j + d + kDepth);
+    }
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const float s = lane_sum<16>(acc[r]);
+    if ((lane & 15) == 0) sums[wave * RW + r][lane >> 4] = s;
+  }
+  __syncthreads();
+  float update = 0.f;
+#pragma unroll
+  for (int i = 0; i < RW / 2; ++i) {
+    T bs[8];
+    __builtin_memcpy(bs, &bv[i], 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i * 8 < rank) {
+        const v4f h = *(const v4f*)sums[i * 8 + e];
+        update += to_f(bs[e]) * ((h[0] + h[1]) + (h[2] + h[3]));
+      }
+  }
+  if (n < width) *out = (T)(old + scale * update);
+}
+
 // How a call is cut.  K is split so that the first launch has about a workgroup a CU, each at least two stages
 // (4096 rows of 17408 values: 512 workgroups 69.2 us, 256 66.6, both launches: the second reads fewer partial sums).
 struct Cut { int splits, chunks, blocks; };
@@ -492,15 +581,28 @@ Cut cut_of(int M, int64_t K, int parts, int rank) {
   return c;
 }
 
+// Workgroups of `columns` columns over all parts.
+int64_t column_blocks(const LoraArgs& g, int columns) {
+  int64_t blocks = 0, begin = 0;
+  for (int p = 0; p < g.parts; ++p) {
+    blocks += (g.ends[p] - begin + columns - 1) / columns;
+    begin = g.ends[p];
+  }
+  return blocks;
+}
+
+template <typename T>
+void launch_rows(const LoraArgs& g, hipStream_t st) {
+  const dim3 grid((unsigned)column_blocks(g, kRowColumns), g.M);
+  if (g.rank <= 16) lora_row_kernel<T, 4><<<grid, 64 * kWaves, 0, st>>>(g);
+  else lora_row_kernel<T, 8><<<grid, 64 * kWaves, 0, st>>>(g);
+}
+
 template <typename T, int TT, int Q>
 void launch(const LoraArgs& g, const Cut& c, hipStream_t st) {
   // units of a block: its adapters, none, bad ids, and what does not fit one unit; the kernels step on over more
   const int units = TT == 1 ? std::min(g.M, std::min(g.slots, kSmall) + 2 + g.M / 16) : 2;
-  int64_t blocks = 0, begin = 0;
-  for (int p = 0; p < g.parts; ++p) {
-    blocks += (g.ends[p] - begin + g.columns - 1) / g.columns;
-    begin = g.ends[p];
-  }
+  const int64_t blocks = column_blocks(g, g.columns);
   const int near = std::min(c.blocks, kXcds);
   // units last: workgroups go to the XCDs in turn, and with units before blocks the second ones, mostly empty, fell on the
   // same XCDs every time (4096 rows of 17408 values 78.1 -> 66.6 us, both launches)
@@ -582,7 +684,13 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
   g.columns = 64 * kWaves;
   while (g.columns < 1024 && groups * (g.N / g.columns) > 256) g.columns *= 2;
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == GQK_DTYPE_BF16) {
+  // Rows by themselves, in one launch, while a workgroup for each 256 columns of each row finds a CU of its own and A is short (us
+  // of two launches and of this: 8 rows of 5120 to 5120 columns, rank 16, 160 workgroups 10.6 and 7.0; to q, k and v, 224 workgroups 10.9
+  // and 8.7, 16 rows 12.5 and 12.1, 24 rows 12.8 and 17.6; one row of 8192 (256 KiB of A) 9.6 and 9.1, of 17408 10.6 and 13.4).
+  if (rank <= 32 && (int64_t)rank * K * 2 <= kRowBytes && M * column_blocks(g, kRowColumns) <= device_cus()) {
+    if (dtype == GQK_DTYPE_BF16) launch_rows<bf16_t>(g, st);
+    else launch_rows<f16_t>(g, st);
+  } else if (dtype == GQK_DTYPE_BF16) {
     if (M <= 64) launch<bf16_t, 1, 1>(g, c, st);
     else if (M <= kSmall) launch<bf16_t, 1, kSmall / 64>(g, c, st);
     else launch<bf16_t, 4, 1>(g, c, st);

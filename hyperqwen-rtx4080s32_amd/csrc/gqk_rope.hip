@@ -106,19 +106,6 @@ template <> __device__ __forceinline__ void store8(fp8_t* p, const float* x) {
   *(int2*)p = make_int2(lo, hi);
 }
 
-template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
-  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
-}
-// the sum over the 8, 16 or 32 lanes of a head: across pairs, quads, halves of a row and a row by DPP, then over two rows
-template <int LPH> __device__ __forceinline__ float head_sum(float x) {
-  x = dpp_add<0xB1>(x);    // quad_perm 1, 0, 3, 2
-  x = dpp_add<0x4E>(x);    // quad_perm 2, 3, 0, 1
-  x = dpp_add<0x141>(x);   // row_half_mirror
-  if constexpr (LPH >= 16) x = dpp_add<0x140>(x);   // row_mirror
-  if constexpr (LPH >= 32) x += __shfl_xor(x, 16);
-  return x;
-}
-
 // Eight dims to a lane, DP / 8 lanes to a head, so that a wave reads 64 x 16 bytes of neighbouring heads at once.  A round
 // is 64 LPH heads of one kind (queries, keys, values), the same for the whole wave; a token's waves deal its rounds.
 // The rotation of a normalized head is  y = r (x A + x' B)  with x' the other dim of the pair, A = w cos and B = -+ w' sin:
@@ -232,7 +219,7 @@ __global__ __launch_bounds__(64 * kWaves) void rope_kernel(RopeArgs a, int waves
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += to_f(v[e]) * to_f(v[e]);
-      ss = head_sum<LPH>(ss);
+      ss = lane_sum<LPH>(ss);
       const float r = (kind ? a.k_weight : a.q_weight) ? rsqrtf(ss / D + a.eps) : 1.f;
       auto turn = [&](const float (&fa)[8], const float (&fb)[8]) {
 #pragma unroll

@@ -1,6 +1,6 @@
 """Low-rank adapters of many requests beside a shared projection: ``lora_add`` adds to a layer's output
 (``mul_mat_grouped``, ``GGUFLinearMethod.apply``) what each row's own adapter contributes.  Two launches on the current
-stream; which rows go with which adapter is found on the GPU from the row's index, so a batch may change between
+stream (one for a few rows); which rows go with which adapter is found on the GPU from the row's index, so a batch may change between
 the replays of a HIP graph."""
 from __future__ import annotations
 

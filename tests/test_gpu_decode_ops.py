@@ -519,6 +519,36 @@ def test_lora_prompts(dtype, rank, n_outs):
     _lora_check(rank, 300, 136, n_outs, rank, 4, dtype, torch.arange(300, device="cuda") // 90)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("rank", [8, 16, 24, 32])
+@pytest.mark.parametrize("M", [7, 17, 63, 64, 65, 200])
+def test_lora_many_columns(dtype, rank, M):
+    """Rows that share adapters, and more columns than a row alone would take."""
+    _lora_check(M, M, 520, (9000, 805), rank, 6, dtype)
+    dev = "cuda"
+    for ids in (torch.zeros(M, dtype=torch.int32, device=dev), torch.full((M,), -1, device=dev),
+                torch.arange(M, device=dev).flip(0) % 6, torch.arange(M, device=dev) // 20 % 6):
+        _lora_check(M, M, 520, (9000, 805), rank, 6, dtype, ids)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("M,K,n_outs,rank", [(1, 8192, (1000,), 16), (1, 8200, (1000,), 16), (1, 4096, (300, 7, 1), 32), (5, 504, (257,), 8),
+                                             (4, 1024, (256, 1), 32), (3, 16384, (511,), 8), (120, 8, (513,), 16)])
+def test_lora_few_rows(dtype, M, K, n_outs, rank):
+    """Rows by themselves: K that ends inside a run, columns that end inside a workgroup, every kind of id, strides."""
+    y, x, a, b, ids, scales, out = _lora_check(M + K, M, K, n_outs, rank, 3, dtype)
+    N = sum(n_outs)
+    wide = torch.full((M, N + 40), 7.0, dtype=dtype, device="cuda")
+    wide[:, 3:N + 3] = y
+    wx = torch.zeros((M, K + 16), dtype=dtype, device="cuda")
+    wx[:, 8:K + 8] = x
+    got = wide[:, 3:N + 3]
+    gguf_hip.lora_add(got, wx[:, 8:K + 8], a, b, ids, scales, n_outs, out=got)
+    assert torch.equal(got, out) and (wide[:, :3] == 7).all() and (wide[:, N + 3:] == 7).all()
+    bad = gguf_hip.lora_add(y, x, a, b, torch.full((M,), 3, device="cuda"), scales, n_outs)
+    assert bad.isnan().all()
+
+
 def test_lora_batches():
     """One adapter for all rows, none for any, all rows different, runs of rows, ids of either width, no scales."""
     dev = "cuda"
