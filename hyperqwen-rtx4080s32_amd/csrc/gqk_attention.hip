@@ -51,7 +51,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kWaves = 4;             // waves of a workgroup
 constexpr int kTile = 32;             // keys of a wave's step
-constexpr int kJoinSplits = 16;       // splits that the last workgroup of a sequence joins; more go to a launch of their own
+constexpr int kJoinSplits = 16;       // splits that the last workgroup of a sequence joins, at most
 constexpr int kMostSplits = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
@@ -74,6 +74,7 @@ struct AttnArgs {
   int chunk, splits;    // keys of a split, and the most splits of a sequence
   uint32_t magic;       // key / page_size = 2 key magic >> 32 >> shift, exact below 2^31
   int shift;
+  int join_apart;       // the splits are joined by a launch of their own
 };
 
 __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c, bf16_t) {
@@ -492,7 +493,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
                                               (a.splits * R * D + (split * R + r) * 2) * 4, 0, kDevice);
     }
   }
-  if (ns == 1 || a.splits > kJoinSplits) return;
+  if (ns == 1 || a.join_apart) return;
   // The sequence's splits join in the workgroup that arrives last, in split order: partials move through device-coherent
   // accesses alone; every store is complete before the arrival count.  All of a value's loads are in flight at once.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -576,7 +577,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
 struct Cut { int row_waves, row_blocks, splits, chunk; };
 
 // About as many workgroups as stay resident, of 256 keys at least (32 x 4000 tokens in bf16: 3 a CU 69.9 us, 4 62.4, 6 66.3,
-// 8 64.2; 64 x 3000 of 256 dims in fp8: 3 a CU 50.2, 4 58.3, 5 55.6; 8 x 2000 in splits of 128 keys or more 16.5, of 256 13.6).
+// 8 64.2; 64 x 3000 of 256 dims in fp8: 3 a CU 50.2, 4 58.3, 5 55.6; 8 x 2000 in splits of 128 keys or more 16.5, of 256 13.6; of 32
+// heads that share one of keys, whose waves see more of a split each, 8 x 4000 13.3 and 15.6, of 128 heads 4 x 4000 17.7 and 22.9).
 Cut cut_of(int batch, int q_heads, int kv_heads, int size, int max_length, int window) {
   const int group = q_heads / kv_heads, tiles = (group + 15) / 16;
   Cut c;
@@ -585,7 +587,7 @@ Cut cut_of(int batch, int q_heads, int kv_heads, int size, int max_length, int w
   // keys a sequence can have, from a multiple of the step
   const int64_t span = std::min<int64_t>(max_length, window > 0 ? (int64_t)window + kTile - 1 : max_length);
   const int64_t units = (int64_t)batch * kv_heads * c.row_blocks, wanted = (size == 1 ? 3LL : 4LL) * device_cus();
-  const int64_t least = 2 * kTile * kWaves;   // keys of the shortest split
+  const int64_t least = (c.row_waves == 1 ? 2 * kWaves : 4) * kTile;   // keys of the shortest split
   int64_t splits = std::max<int64_t>(1, std::min((wanted + units - 1) / std::max<int64_t>(1, units), (span + least - 1) / least));
   splits = std::min<int64_t>(splits, kMostSplits);
   if (units > GQK_CTR_WORDS) splits = 1;
@@ -669,6 +671,10 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
   while (((int64_t)1 << bits) < pages->page_size) ++bits;
   a.shift = bits;
   a.magic = (uint32_t)((((uint64_t)1 << (31 + bits)) + pages->page_size - 1) / pages->page_size);
+  // one workgroup joins up to 16 splits, of heads that its threads go over twice at most (in a launch of their own and in it: 32 heads
+  // of 128 dims over one, 8 x 4000, 15.7 us and 21.3; 16 heads, two rounds, 16 x 2000, 17.9 and 16.6)
+  a.join_apart = c.splits > kJoinSplits ||
+                 (c.splits > 1 && std::min(16 * c.row_waves, q_heads / pages->heads) * (pages->dim / 4) > 2 * 64 * kWaves);
   const dim3 grid(pages->heads * c.row_blocks, batch, c.splits);
   const hipStream_t st = (hipStream_t)stream;
   const bool bf = dtype == GQK_DTYPE_BF16;
@@ -680,7 +686,7 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
   } else {
     launch<f16_t, f16_t>(a, grid, st);
   }
-  if (c.splits > kJoinSplits) {
+  if (a.join_apart) {
     if (bf) attention_join_kernel<bf16_t><<<dim3(q_heads, batch), 256, 0, st>>>(a);
     else attention_join_kernel<f16_t><<<dim3(q_heads, batch), 256, 0, st>>>(a);
   }

@@ -1,7 +1,7 @@
 """Attention around the linear path: the heads that qkv's output holds, normalized, rotated and stored into
 the pages of a key-value cache (``qk_norm_rope``), and the attention of each new token over those pages
 (``paged_attention``).  Both run on the current stream (one launch; a second where a
-sequence's keys are cut into more than 16 splits), allocate their outputs alone, do not synchronise the host
+sequence's keys are cut into more than 16 splits, or heads that share one of keys are many), allocate their outputs alone, do not synchronise the host
 and can be captured in a HIP graph; under tracing they are custom ops with fakes.
 
 Layouts: heads are [tokens, heads, dim] views with any strides (column ranges of qkv's output as they are);

@@ -239,7 +239,7 @@ int gqk_qk_norm_rope(const gqk_heads* q, const gqk_heads* k, const gqk_heads* v,
                      int slots_64, void* stream);
 
 /* Attention of one new token per sequence over its pages, split over the length (one launch; a second one joins more than
- * 16 splits of a sequence):
+ * 16 splits of a sequence, or those of many heads that share one of keys):
  *   out[b, h] = sum_j softmax_j(scale * q[b, h] . k_j) v_j,   key j of sequence b in page table[b, j / page_size]
  * over j in [max(0, lengths[b] - window), lengths[b]) (window 0: all).  No key (a length of zero or less): zeros, lse -inf;
  * a length above max_length, or a page outside of the cache among the keys: NaN.  Query head h reads key head h / (q_heads / heads).  q, out: bf16 or fp16
