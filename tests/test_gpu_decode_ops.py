@@ -126,6 +126,15 @@ def test_attention_shared_heads(hq, hkv):
     _attend_check(hq, [130, 5, 0, 700], hq, hkv, 64, 16, BF, BF)
 
 
+@pytest.mark.parametrize("qt,ct", [(BF, BF), (F16, F16), (BF, F8)])
+@pytest.mark.parametrize("hq,hkv,dim", [(33, 1, 128), (96, 2, 64), (128, 1, 128), (20, 1, 256)])
+def test_attention_many_heads_in_splits(qt, ct, hq, hkv, dim):
+    """Many heads over one of keys, cut into few and into many splits, beside sequences that are not cut."""
+    _attend_check(hq, [1500, 128, 0, 129, 1], hq, hkv, dim, 16, qt, ct, scaled=ct == F8)
+    _attend_check(hq, [9000], hq, hkv, dim, 16, qt, ct, window=7777, scaled=ct == F8)
+
+
+
 @pytest.mark.parametrize("page", [1, 2, 7, 8, 16, 24, 33, 48, 64, 256])
 @pytest.mark.parametrize("layout", ["heads", "tokens"])
 def test_attention_page_sizes(page, layout):
