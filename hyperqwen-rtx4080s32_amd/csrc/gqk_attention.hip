@@ -525,10 +525,10 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
 // The join of more splits than one workgroup takes at once: a workgroup for each query head, its threads over the splits and
 // the dims.  (One workgroup per sequence and key head took 16 us for 64 splits of 5 heads, 39 for 128 of 16.)  96 splits of 40 heads: 5.8 us,
 // of which a launch that waits for another takes about half.
-template <typename T>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
-  __shared__ __align__(16) float sums[256][4];
-  __shared__ float stat[256][2];
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void attention_join_kernel(AttnArgs a) {
+  __shared__ __align__(16) float sums[THREADS][4];
+  __shared__ float stat[THREADS][2];
   const int b = blockIdx.y, h = blockIdx.x, group = a.q_heads / a.kv.heads, kvh = h / group, D = a.kv.dim;
   const int rows_wg = 16 * a.row_waves, rb = h % group / rows_wg, r = h % group - rb * rows_wg, R = min(rows_wg, group - rb * rows_wg);
   const int len0 = max(0, a.lengths[b]), len = len0 > a.max_length ? 0 : len0;
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
   const int64_t unit = ((int64_t)b * a.kv.heads + kvh) * a.row_blocks + rb;
   const float* part = a.partials + unit * a.splits * min(rows_wg, group) * (D + 4);
   const float* part_stat = part + (int64_t)a.splits * R * D;
-  const int quads = D / 4, lanes = 256 / quads, own = threadIdx.x / quads, d = (threadIdx.x - own * quads) * 4;
+  const int quads = D / 4, lanes = THREADS / quads, own = threadIdx.x / quads, d = (threadIdx.x - own * quads) * 4;
   Joined j;
   if (own < lanes) {
     constexpr int kBatch = 8;
@@ -687,8 +687,14 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
     launch<f16_t, f16_t>(a, grid, st);
   }
   if (a.join_apart) {
-    if (bf) attention_join_kernel<bf16_t><<<dim3(q_heads, batch), 256, 0, st>>>(a);
-    else attention_join_kernel<f16_t><<<dim3(q_heads, batch), 256, 0, st>>>(a);
+    const dim3 all(q_heads, batch);
+    if (c.splits > 128) {   // more threads cost more to bring together (us of 256 and 512: 256 splits 22.7 and 21.1, 16 13.2 and 14.0)
+      if (bf) attention_join_kernel<bf16_t, 512><<<all, 512, 0, st>>>(a);
+      else attention_join_kernel<f16_t, 512><<<all, 512, 0, st>>>(a);
+    } else {
+      if (bf) attention_join_kernel<bf16_t, 256><<<all, 256, 0, st>>>(a);
+      else attention_join_kernel<f16_t, 256><<<all, 256, 0, st>>>(a);
+    }
   }
   return decode_launched("paged_attention");
 }

@@ -132,6 +132,7 @@ def test_attention_many_heads_in_splits(qt, ct, hq, hkv, dim):
     """Many heads over one of keys, cut into few and into many splits, beside sequences that are not cut."""
     _attend_check(hq, [1500, 128, 0, 129, 1], hq, hkv, dim, 16, qt, ct, scaled=ct == F8)
     _attend_check(hq, [9000], hq, hkv, dim, 16, qt, ct, window=7777, scaled=ct == F8)
+    _attend_check(hq, [40_000], hq, hkv, dim, 16, qt, ct, scaled=ct == F8)
 
 
 
