@@ -104,7 +104,7 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_de
 // the call's workspace: its own, or the device's
 bool workspace_of(const Tensor* own, const Tensor& ref, void** at, int64_t* bytes) {
   const Tensor* t = own ? own : g_workspace[ref.get_device()];
-  if (!t || !same_device(ref, t)) return false;
+  if (!t || !same_device(ref, t) || !t->is_contiguous()) return false;
   *at = t->data_ptr();
   *bytes = t->numel() * t->element_size();
   return true;

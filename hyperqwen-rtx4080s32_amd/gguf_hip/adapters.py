@@ -108,6 +108,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     if scales is not None and (scales.dtype != torch.float32 or scales.shape != (a.shape[0],) or scales.device != x.device
                                or not scales.is_contiguous()):
         raise ValueError(f"{what}: scales is contiguous fp32 [{a.shape[0]}] on {x.device}")
+    ops.check_workspace(workspace, x.device, what)
     if out is not None and out.numel() and ((N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N)):
         raise ValueError(f"{what}: out's columns must lie side by side, got strides {out.stride()}")
     inplace = out is y

@@ -154,6 +154,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if (lengths.dtype != torch.int32 or lengths.shape != (batch,) or lengths.device != q.device
             or not lengths.is_contiguous()):
         raise ValueError(f"paged_attention: lengths is contiguous int32 [{batch}] on {q.device}")
+    ops.check_workspace(workspace, q.device, "paged_attention")
     room = min(block_table.shape[1] * k_pages.shape[1], _lib.GQK_MAX_KEYS)
     max_length = room if max_length is None else int(max_length)
     if not 0 <= max_length <= room or window < 0:

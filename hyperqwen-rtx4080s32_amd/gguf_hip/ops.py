@@ -262,6 +262,12 @@ def shared_workspace(device: torch.device) -> torch.Tensor:
     return ws
 
 
+def check_workspace(workspace: torch.Tensor | None, device: torch.device, what: str) -> None:
+    """A workspace of the call's own: one run of memory on the call's device."""
+    if workspace is not None and (workspace.device != device or not workspace.is_contiguous()):
+        raise ValueError(f"{what}: workspace is contiguous on {device}, got strides {workspace.stride()} on {workspace.device}")
+
+
 def prepare_grouped_layer(tiles_list: list[torch.Tensor], n_outs: list[int], wtypes: list[int], K: int,
                           target_wgs: int = 0, cus: int = 0) -> GroupedLayer:
     """The loader's step for a run of shards already repacked: one packed buffer (the shards'

@@ -226,6 +226,17 @@ def test_lora_add_shapes_and_refusals():
                 gguf_hip.lora_add(**_lora_args(**bad))
 
 
+def test_workspaces_that_are_refused():
+    with FakeTensorMode():
+        apart = _fake((1 << 20, 2), torch.int32)[:, 0]
+        spread = _fake((1,), torch.int32).expand(1 << 24)
+        for ws in (apart, spread, torch.empty(1 << 24, dtype=torch.int32)):
+            with pytest.raises(ValueError, match="workspace"):
+                gguf_hip.paged_attention(**_attend_args(), workspace=ws)
+            with pytest.raises(ValueError, match="workspace"):
+                gguf_hip.lora_add(**_lora_args(), workspace=ws)
+
+
 def test_make_fx_traces_the_ops():
     """A traced decode step holds each operator as one opaque call, and no view or copy of the caches."""
     from torch.fx.experimental.proxy_tensor import make_fx
