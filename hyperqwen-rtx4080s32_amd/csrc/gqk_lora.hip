@@ -687,7 +687,10 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
   // Rows by themselves, in one launch, while a workgroup for each 256 columns of each row finds a CU of its own and A is short (us
   // of two launches and of this: 8 rows of 5120 to 5120 columns, rank 16, 160 workgroups 10.6 and 7.0; to q, k and v, 224 workgroups 10.9
   // and 8.7, 16 rows 12.5 and 12.1, 24 rows 12.8 and 17.6; one row of 8192 (256 KiB of A) 9.6 and 9.1, of 17408 10.6 and 13.4).
-  if (rank <= 32 && (int64_t)rank * K * 2 <= kRowBytes && M * column_blocks(g, kRowColumns) <= device_cus()) {
+  // They read x while others write out, which must lie apart.
+  const uintptr_t x0 = (uintptr_t)x, x1 = x0 + ((M - 1) * x_row + K) * 2, o0 = (uintptr_t)out, o1 = o0 + ((M - 1) * out_row + g.N) * 2;
+  const bool apart = x1 <= o0 || o1 <= x0;
+  if (apart && rank <= 32 && (int64_t)rank * K * 2 <= kRowBytes && M * column_blocks(g, kRowColumns) <= device_cus()) {
     if (dtype == GQK_DTYPE_BF16) launch_rows<bf16_t>(g, st);
     else launch_rows<f16_t>(g, st);
   } else if (dtype == GQK_DTYPE_BF16) {

@@ -77,7 +77,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     one part: [N]), their sum N; a [adapters, parts, rank, K] and b [adapters, N, rank] as ``pack_adapters`` makes
     them, of x's and y's type (bf16 or fp16), contiguous, K and rank multiples of 8, rank up to 256; scales fp32 [adapters] or None (1); ids
     int32 or int64 [M], negative for a row without an adapter (one beyond the adapters gives a row of NaN).
-    Returns a new tensor, or ``out`` (a [M, N] view with unit column stride), which may be y itself.
+    Returns a new tensor, or ``out`` (a [M, N] view with unit column stride), which may be y itself, or x.
     ``workspace``: as mul_mat_grouped's (its own for calls on concurrent streams)."""
     what = "lora_add"
     if _unwatched():

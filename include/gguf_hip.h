@@ -185,7 +185,7 @@ int gqk_linear_noalloc(const void* packed, const int32_t* desc_dev, const gqk_pl
  *   out[m, n] = y[m, n] + scales[i] * sum_r b[i, n, r] * sum_k a[i, p(n), r, k] * x[m, k],  i = ids[m]
  * p(n): the part (q, k, v; gate, up) of column n, parts side by side with n_outs[p] columns each.  A row with a
  * negative id gets y; one with an id >= slots NaN.  y, x, out: bf16 or fp16 (dtype) rows of any stride,
- * out may be y; a [slots, parts, rank, K] and b [slots, sum(n_outs), rank] of the same type, contiguous, K and
+ * out may be y or x; a [slots, parts, rank, K] and b [slots, sum(n_outs), rank] of the same type, contiguous, K and
  * rank multiples of 8, rank <= 256 (adapters of a lower rank are padded with zeros), parts <= 8; ids
  * int32 [M], or int64 with ids_64; scales fp32 [slots] or NULL (1).  x, a, b are 16-byte aligned.  Products
  * and sums are in fp32, rounded once to out.  K and x's row stride (where M > 1) are at most GQK_LORA_MAX_K.

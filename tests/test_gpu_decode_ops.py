@@ -559,6 +559,19 @@ def test_lora_few_rows(dtype, M, K, n_outs, rank):
     assert bad.isnan().all()
 
 
+@pytest.mark.parametrize("M", [1, 3, 40, 300])
+def test_lora_into_its_input(M):
+    """out may be y, and where the sizes allow it x."""
+    y, x, a, b, ids, scales, out = _lora_check(M, M, 1024, (1000, 24), 16, 3, BF)
+    want, tol = _lora_exact(y, x, a, b, ids, scales, (1000, 24))
+    mine = x.clone()
+    gguf_hip.lora_add(y, mine, a, b, ids, scales, (1000, 24), out=mine)
+    _within(mine, want, tol, "into x")   # its sums may go in another order
+    mine = y.clone()
+    gguf_hip.lora_add(mine, x, a, b, ids, scales, (1000, 24), out=mine)
+    assert torch.equal(mine, out)
+
+
 def test_lora_batches():
     """One adapter for all rows, none for any, all rows different, runs of rows, ids of either width, no scales."""
     dev = "cuda"
