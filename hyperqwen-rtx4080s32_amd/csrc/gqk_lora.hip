@@ -39,6 +39,7 @@ struct LoraArgs {
   float* h;                  // [splits][M][parts * rank]
   int M, slots, parts, rank, wide_ids;
   int splits, chunks, blocks;   // splits of K; chunks of 64 ranks; blocks of rows
+  int finer;                 // parts of each split, for the units after a block's first
   int columns;               // of a workgroup of the second kernel
   int half_units;            // the second kernel takes long batches by 32 rows, not 64
   int wide_y;                // y and out are 16-byte aligned in every row
@@ -56,6 +57,7 @@ __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c, f16_t) {
 struct Unit {
   int adapter, count;
   const int* row;   // their numbers within the block
+  bool lead;        // of the block's first row's adapter
 };
 
 // Unit u (of up to `most` rows) of a block of 64 Q rows: adapters in the order of their first row, each one's rows in
@@ -90,6 +92,7 @@ __device__ __forceinline__ bool find_unit(const LoraArgs& a, int64_t row0, int u
       const int units = (count + most - 1) / most;
       if (u < units) {
         out.adapter = who;
+        out.lead = who == __builtin_amdgcn_readlane(id[0], 0);
         out.count = min(count - u * most, most);
         int* mine = lists + (threadIdx.x >> 6) * kList;
         int before = -u * most;   // rows of the adapter in earlier parts, from the unit's first
@@ -142,14 +145,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
   __shared__ __align__(16) char buf[2][(kRows + 16 * kRankTiles) * 256];
   __shared__ int lists[kWaves * kList];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  const int chunk = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const int chunk = blockIdx.x / a.splits;
+  // Long batches: a block's first unit by splits, which give every CU a workgroup; the later ones (a second prompt begins inside of
+  // the block) by parts of them, as each shares a CU with another and would otherwise end last (us for one, two and four
+  // parts, 4096 rows of 17408 values of three adapters: 70.9, 70.1, 66.7, both launches).
+  const bool later = TT > 1 && blockIdx.z > 0;
+  const int splits = later ? a.splits * a.finer : a.splits;
+  const int split = later ? blockIdx.x % a.splits * a.finer + blockIdx.z - 1 : blockIdx.x % a.splits;
   constexpr int kBlock = 64 * Q;
   const int64_t row0 = (int64_t)blockIdx.y * kBlock;
   const int PR = a.parts * a.rank, rank0 = chunk * 16 * kRankTiles, tiles = min(kRankTiles, (PR - rank0 + 15) / 16);
   const int all = (int)((a.K + kStage - 1) / kStage);
-  const int s0 = (int)((int64_t)all * split / a.splits), stages = (int)((int64_t)all * (split + 1) / a.splits) - s0;
+  const int s0 = (int)((int64_t)all * split / splits), stages = (int)((int64_t)all * (split + 1) / splits) - s0;
   const int K = (int)a.K, row = threadIdx.x >> 4, piece = threadIdx.x & 15;
-  for (int u = blockIdx.z;; u += gridDim.z) {
+  const int step = TT == 1 ? gridDim.z : later ? 1 : 1 << 20;
+  for (int u = TT == 1 ? blockIdx.z : later;; u += step) {
     Unit unit;
     if (!find_unit<Q>(a, row0, u, kRows, lists, unit)) return;
     if (unit.adapter < 0) continue;
@@ -287,7 +297,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
       }
       continue;
     }
-    const int rows = (unit.count + 15) / 16;
+    const int rows = (unit.count + 15) / 16, splits = unit.lead ? a.splits : a.splits * a.finer;
     const __amdgpu_buffer_rsrc_t rb = buffer_of((const T*)a.b + ((int64_t)unit.adapter * a.N + c_begin) * rank, (int64_t)width * rank * 2);
     const __amdgpu_buffer_rsrc_t ry = buffer_of(ybase, kBlock * a.y_row * 2), ro = buffer_of(obase, kBlock * a.out_row * 2);
     // lane's place in y: rows t * 16 + i * 8 + lane / 8, columns (lane % 8) * 8 .. + 7 of the wave's
@@ -331,17 +341,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
         for (int e = 0; e < 8; ++e) v[e] = 0.f;
         if (at >= rank || r >= rows * 16) return;
         constexpr int kBatch = 4;
-        for (int sp = sp0; sp < a.splits; sp += kBatch * by) {
+        for (int sp = sp0; sp < splits; sp += kBatch * by) {
           v4f lo[kBatch], hi[kBatch];
 #pragma unroll
           for (int j = 0; j < kBatch; ++j) {
-            const v4f* p = (const v4f*)(from + (int64_t)min(sp + j * by, a.splits - 1) * a.M * PR + at);
+            const v4f* p = (const v4f*)(from + (int64_t)min(sp + j * by, splits - 1) * a.M * PR + at);
             lo[j] = p[0];
             hi[j] = p[1];
           }
 #pragma unroll
           for (int j = 0; j < kBatch; ++j)
-            if (sp + j * by < a.splits)
+            if (sp + j * by < splits)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 v[e] += lo[j][e];
@@ -569,7 +579,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_row_kernel(LoraArgs a) {
 
 // How a call is cut.  K is split so that the first launch has about a workgroup a CU, each at least two stages
 // (4096 rows of 17408 values: 512 workgroups 69.2 us, 256 66.6, both launches: the second reads fewer partial sums).
-struct Cut { int splits, chunks, blocks; };
+struct Cut { int splits, chunks, blocks, finer; };
 
 Cut cut_of(int M, int64_t K, int parts, int rank) {
   Cut c;
@@ -578,6 +588,8 @@ Cut cut_of(int M, int64_t K, int parts, int rank) {
   const int64_t wgs = (int64_t)c.chunks * (M <= kSmall ? std::min(M, 16) : c.blocks);
   const int64_t stages = (K + kStage - 1) / kStage;
   c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / wgs, stages / 2, 16}));
+  // partial sums that the second kernel adds: at most 16
+  c.finer = M <= kSmall || c.splits == 1 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({4, 16 / c.splits, stages / (2 * c.splits)}));
   return c;
 }
 
@@ -606,7 +618,7 @@ void launch(const LoraArgs& g, const Cut& c, hipStream_t st) {
   const int near = std::min(c.blocks, kXcds);
   // units last: workgroups go to the XCDs in turn, and with units before blocks the second ones, mostly empty, fell on the
   // same XCDs every time (4096 rows of 17408 values 78.1 -> 66.6 us, both launches)
-  if (g.slots > 0) lora_down_kernel<T, TT, Q><<<dim3(c.splits * c.chunks, c.blocks, units), 64 * kWaves, 0, st>>>(g);
+  if (g.slots > 0) lora_down_kernel<T, TT, Q><<<dim3(c.splits * c.chunks, c.blocks, TT == 1 ? units : 1 + c.finer), 64 * kWaves, 0, st>>>(g);
   auto up = [&](auto each, auto tiles) {
     constexpr int kEach = decltype(each)::value, kRanks = 8 * kEach, UT = decltype(tiles)::value;
     const size_t lds = (size_t)16 * UT * 2 * ((g.rank + kRanks - 1) / kRanks * kRanks + 8) * sizeof(T);
@@ -637,7 +649,9 @@ int64_t gqk_lora_workspace_bytes(int M, int64_t K, int parts, int rank) {
   if (M < 0 || K < 0 || parts < 1 || parts > kParts || rank < 8 || rank > 256 || rank % 8)
     return decode_fail(GQK_ERR_SHAPE, "lora: %d rows of %lld, %d parts (at most %d), rank %d (a multiple of 8 in 8..256)", M,
                        (long long)K, parts, kParts, rank);
-  return M == 0 ? GQK_CTR_BYTES : GQK_CTR_BYTES + (int64_t)cut_of(M, K, parts, rank).splits * M * parts * rank * 4;
+  if (M == 0) return GQK_CTR_BYTES;
+  const Cut c = cut_of(M, K, parts, rank);
+  return GQK_CTR_BYTES + (int64_t)c.splits * c.finer * M * parts * rank * 4;
 }
 
 int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int M, int64_t K, const void* a, const void* b,
@@ -671,7 +685,7 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
   g.M = M; g.slots = slots; g.parts = parts; g.rank = rank;
   const Cut c = cut_of(M, K, parts, rank);
   if (c.blocks > 65535) return decode_fail(GQK_ERR_SHAPE, "lora_add: %d rows", M);
-  g.splits = c.splits; g.chunks = c.chunks; g.blocks = c.blocks;
+  g.splits = c.splits; g.finer = c.finer; g.chunks = c.chunks; g.blocks = c.blocks;
   // whole 16-byte pieces in every row, and rows that 32-bit offsets reach
   g.wide_y = !(((uintptr_t)y | (uintptr_t)out) & 15) && !((y_row | out_row) & 7) && y_row < (1 << 22) && out_row < (1 << 22);
   for (int p = 0; p < parts; ++p) g.wide_y &= g.ends[p] % 8 == 0;
