@@ -572,6 +572,17 @@ def test_lora_into_its_input(M):
     assert torch.equal(mine, out)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("M,K,n_outs,rank", [(2100, 5120, (200, 56), 16), (4100, 2600, (136,), 64), (4097, 1296, (70_000,), 8),
+                                             (8200, 1024, (40, 40, 8), 40)])
+def test_lora_long_prompts(dtype, M, K, n_outs, rank):
+    """Blocks of rows that begin with one adapter or with none and hold one or more others, cut over K in two ways."""
+    _lora_check(M, M, K, n_outs, rank, 5, dtype)
+    for ids in (torch.arange(M, device="cuda") // 700 % 5, torch.arange(M, device="cuda") // 31 % 6 - 1,
+                (torch.arange(M, device="cuda") % 64 == 63).long() * 2 - 1):
+        _lora_check(M, M, K, n_outs, rank, 5, dtype, ids)
+
+
 def test_lora_batches():
     """One adapter for all rows, none for any, all rows different, runs of rows, ids of either width, no scales."""
     dev = "cuda"
