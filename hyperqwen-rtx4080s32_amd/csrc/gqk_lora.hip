@@ -28,7 +28,6 @@ constexpr int kRankTiles = 4;    // 16-rank tiles of a workgroup of the first ke
 constexpr int kRowColumns = 64 * kWaves;
 constexpr int64_t kRowBytes = 1 << 18;   // of a part's A, that a workgroup of a row reads by itself
 constexpr int kXcds = 8;         // workgroups go to them in turn
-constexpr int down_waves(int TT) { return TT == 1 ? kWaves : 2 * kWaves; }   // of a workgroup of the first kernel
 constexpr int kNone = -1, kBad = -2;
 
 struct LoraArgs {
@@ -131,9 +130,8 @@ __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset
 // holds 16 bytes of one: loaded like that nothing coalesces (62 L1 accesses a load counted).  So 256 bytes of each row at a
 // time come in as rows, 16 lanes to one, go through LDS with their 16-byte pieces swapped by the row's number (16 rows'
 // pieces of one k-step in different banks), and are read as operands: ranks as the instruction's rows, batch rows as its
-// columns.  Loads run kDepth stages ahead in registers; two LDS buffers, one barrier a stage.  A wave takes one 16-row tile, all
-// ranks and half of each stage (TT = 4: eight waves, whose halves are added at the end; with four and whole stages 66.7 us where eight
-// take 64.6), or all 16 rows and one 16-rank tile (TT = 1).  x goes by once and leaves the caches first, so that A, which every
+// columns.  Loads run kDepth stages ahead in registers; two LDS buffers, one barrier a stage.  A wave takes one 16-row tile and all
+// ranks (TT = 4), or all 16 rows and one 16-rank tile (TT = 1).  x goes by once and leaves the caches first, so that A, which every
 // block of rows reads again, stays (4096 rows of 17408 values 82.4 -> 78.1 us, both launches).
 //
 // 4096 rows of 17408 values, rank 64: 39.6 us, 3.6 TB/s of x.  Without any load it takes 27.6: LDS, the barriers and the
@@ -141,16 +139,12 @@ __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset
 // a CU 69.2, blocks of 128 rows 76.7).  48 rows of 5120, 12 adapters of rank 32: 6.7 us, a launch, ids, one trip to memory,
 // partial sums out.
 template <typename T, int TT, int Q>
-__global__ __launch_bounds__(64 * down_waves(TT), 2) void lora_down_kernel(LoraArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
   constexpr int kDepth = TT == 1 ? 4 : 2;
-  constexpr int kW = down_waves(TT), kPass = 4 * kW;   // rows that the workgroup loads at once
   constexpr int kRows = 16 * TT, kAcc = TT == 1 ? 1 : kRankTiles;
-  constexpr int kX = kRows / kPass, kA = 16 * kRankTiles / kPass;
-  constexpr int kShare = TT == 1 ? 1 : kW / TT, kSteps = kStage / 32 / kShare;   // waves that share a row tile, each one's k-steps
   __shared__ __align__(16) char buf[2][(kRows + 16 * kRankTiles) * 256];
-  __shared__ int lists[kW * kList];
+  __shared__ int lists[kWaves * kList];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  const int tile = TT == 1 ? 0 : wave % TT, k_first = TT == 1 ? 0 : wave / TT * kSteps;
   const int chunk = blockIdx.x / a.splits;
   // Long batches: a block's first unit by splits, which give every CU a workgroup; the later ones (a second prompt begins inside of
   // the block) by parts of them, as each shares a CU with another and would otherwise end last (us for one, two and four
@@ -173,43 +167,43 @@ __global__ __launch_bounds__(64 * down_waves(TT), 2) void lora_down_kernel(LoraA
     const __amdgpu_buffer_rsrc_t ra = buffer_of((const T*)a.a + ((int64_t)unit.adapter * PR + rank0) * a.K,
                                                 (int64_t)min(16 * kRankTiles, PR - rank0) * a.K * 2);
     const __amdgpu_buffer_rsrc_t rx = buffer_of((const T*)a.x + row0 * a.x_row, (int64_t)kBlock * a.x_row * 2);
-    uint32_t ao[kA], xo[kX];
+    uint32_t ao[kRankTiles], xo[TT];
     // ranks and rows that are not there are offsets past the buffers: zeros, no branch
 #pragma unroll
-    for (int t = 0; t < kA; ++t)
-      ao[t] = t * kPass + row < PR - rank0 ? (t * kPass + row) * (uint32_t)K * 2 + piece * 16 : kOutside;
+    for (int t = 0; t < kRankTiles; ++t)
+      ao[t] = t * 16 + row < PR - rank0 ? (t * 16 + row) * (uint32_t)K * 2 + piece * 16 : kOutside;
 #pragma unroll
-    for (int t = 0; t < kX; ++t)
-      xo[t] = t * kPass + row < unit.count ? unit.row[t * kPass + row] * (uint32_t)a.x_row * 2 + piece * 16 : kOutside;
-    v4u av[kDepth][kA], xv[kDepth][kX];
+    for (int t = 0; t < TT; ++t)
+      xo[t] = t * 16 + row < unit.count ? unit.row[t * 16 + row] * (uint32_t)a.x_row * 2 + piece * 16 : kOutside;
+    v4u av[kDepth][kRankTiles], xv[kDepth][TT];
     auto load = [&](int d, int s) {
       const bool in = s < s0 + stages && s * kStage + piece * 8 < K;   // K may end inside the last stage
 #pragma unroll
-      for (int t = 0; t < kX; ++t) xv[d][t] = load16<kOnce>(rx, in ? xo[t] + s * (2 * kStage) : kOutside);
+      for (int t = 0; t < TT; ++t) xv[d][t] = load16<kOnce>(rx, in ? xo[t] + s * (2 * kStage) : kOutside);
 #pragma unroll
-      for (int t = 0; t < kA; ++t) av[d][t] = load16(ra, in ? ao[t] + s * (2 * kStage) : kOutside);
+      for (int t = 0; t < kRankTiles; ++t) av[d][t] = load16(ra, in ? ao[t] + s * (2 * kStage) : kOutside);
     };
     v4f acc[kAcc];
 #pragma unroll
     for (int r = 0; r < kAcc; ++r) acc[r] = v4f{0.f, 0.f, 0.f, 0.f};
-    const bool busy = TT == 1 ? wave < tiles : tile < rows;
+    const bool busy = wave < (TT == 1 ? tiles : rows);
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) load(d, s0 + d);
     __syncthreads();   // the last unit's stages have been read
     auto stage = [&](int d, int s) {
       char* const to = buf[d & 1];   // kDepth is even
-      char* const at = to + row * 256 + (piece ^ (row & 15)) * 16;
+      char* const at = to + row * 256 + (piece ^ row) * 16;
 #pragma unroll
-      for (int t = 0; t < kX; ++t) *(v4u*)(at + t * kPass * 256) = xv[d][t];
+      for (int t = 0; t < TT; ++t) *(v4u*)(at + t * 4096) = xv[d][t];
 #pragma unroll
-      for (int t = 0; t < kA; ++t) *(v4u*)(at + (kRows + t * kPass) * 256) = av[d][t];
+      for (int t = 0; t < kRankTiles; ++t) *(v4u*)(at + (TT + t) * 4096) = av[d][t];
       load(d, s + kDepth);
       __syncthreads();
       if (busy)
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          const char* from = to + n * 256 + (((k_first + k) * 4 + g) ^ n) * 16;
-          const v4u xop = *(const v4u*)(from + tile * 4096);
+        for (int k = 0; k < kStage / 32; ++k) {
+          const char* from = to + n * 256 + ((k * 4 + g) ^ n) * 16;
+          const v4u xop = *(const v4u*)(from + (TT == 1 ? 0 : wave) * 4096);
           if constexpr (TT == 1) {
             acc[0] = mfma(*(const v4u*)(from + (TT + wave) * 4096), xop, acc[0], T{});
           } else {
@@ -228,18 +222,8 @@ __global__ __launch_bounds__(64 * down_waves(TT), 2) void lora_down_kernel(LoraA
 #pragma unroll
     for (int d = 0; d < kDepth - 1; ++d)
       if (i + d < stages) stage(d, s0 + i + d);
-    if constexpr (kShare == 2) {   // the two halves of each stage, added: through the buffer that the last stage did not use
-      char* const other = buf[stages & 1] + (tile * kAcc * 64 + lane) * 16;
-      if (wave >= TT)
-#pragma unroll
-        for (int r = 0; r < kAcc; ++r) *(v4f*)(other + r * 1024) = acc[r];
-      __syncthreads();
-      if (wave >= TT) continue;
-#pragma unroll
-      for (int r = 0; r < kAcc; ++r) acc[r] += *(const v4f*)(other + r * 1024);
-    }
     // lane (n, g) holds ranks 4 g .. + 3 of a tile for row n
-    const int r_at = tile * 16 + n;
+    const int r_at = (TT == 1 ? 0 : wave) * 16 + n;
     if (busy && r_at < unit.count) {
       float* to = a.h + ((int64_t)split * a.M + row0 + unit.row[r_at]) * PR;
 #pragma unroll
@@ -634,7 +618,7 @@ void launch(const LoraArgs& g, const Cut& c, hipStream_t st) {
   const int near = std::min(c.blocks, kXcds);
   // units last: workgroups go to the XCDs in turn, and with units before blocks the second ones, mostly empty, fell on the
   // same XCDs every time (4096 rows of 17408 values 78.1 -> 66.6 us, both launches)
-  if (g.slots > 0) lora_down_kernel<T, TT, Q><<<dim3(c.splits * c.chunks, c.blocks, TT == 1 ? units : 1 + c.finer), 64 * down_waves(TT), 0, st>>>(g);
+  if (g.slots > 0) lora_down_kernel<T, TT, Q><<<dim3(c.splits * c.chunks, c.blocks, TT == 1 ? units : 1 + c.finer), 64 * kWaves, 0, st>>>(g);
   auto up = [&](auto each, auto tiles) {
     constexpr int kEach = decltype(each)::value, kRanks = 8 * kEach, UT = decltype(tiles)::value;
     const size_t lds = (size_t)16 * UT * 2 * ((g.rank + kRanks - 1) / kRanks * kRanks + 8) * sizeof(T);
