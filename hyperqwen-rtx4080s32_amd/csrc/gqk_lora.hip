@@ -134,9 +134,9 @@ __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset
 // ranks (TT = 4), or all 16 rows and one 16-rank tile (TT = 1).  x goes by once and leaves the caches first, so that A, which every
 // block of rows reads again, stays (4096 rows of 17408 values 82.4 -> 78.1 us, both launches).
 //
-// 4096 rows of 17408 values, rank 64: 39.6 us, 3.6 TB/s of x.  Without any load it takes 27.6: LDS, the barriers and the
-// issue of each stage, which hide the loads in part only (66.6 us for both launches; loads 4 stages ahead 68.0, two workgroups
-// a CU 69.2, blocks of 128 rows 76.7).  48 rows of 5120, 12 adapters of rank 32: 6.7 us, a launch, ids, one trip to memory,
+// 4096 rows of 17408 values, rank 64: 34 us, 4.2 TB/s of x.  Without any load it takes 24: LDS, the barriers and the
+// issue of each stage, which hide the loads in part only (loads 4 stages ahead cost 1.4 us more, two workgroups a CU 2.6, blocks of
+// 128 rows 9; eight waves with half of each stage change nothing).  48 rows of 5120, 12 adapters of rank 32: 6.7 us, a launch, ids, one trip to memory,
 // partial sums out.
 template <typename T, int TT, int Q>
 __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
@@ -147,8 +147,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int chunk = blockIdx.x / a.splits;
   // Long batches: a block's first unit by splits, which give every CU a workgroup; the later ones (a second prompt begins inside of
-  // the block) by parts of them, as each shares a CU with another and would otherwise end last (us for one, two and four
-  // parts, 4096 rows of 17408 values of three adapters: 70.9, 70.1, 66.7, both launches).
+  // the block) by parts of them, as each shares a CU with another and would otherwise end last (us for one to four
+  // parts, 4096 rows of 17408 values of three adapters: 70.9, 68.5, 67.7, 66.5, both launches).
   const bool later = TT > 1 && blockIdx.z > 0;
   const int splits = later ? a.splits * a.finer : a.splits;
   const int split = later ? blockIdx.x % a.splits * a.finer + blockIdx.z - 1 : blockIdx.x % a.splits;
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
 // one XCD and near in time (dealt by columns: 4096 rows of 17408 values 83.9 -> 81.9 us, 8192 of 5120 to three parts 93.0 -> 85.7,
 // both launches).
 //
-// 4096 rows of 5120 columns, rank 64: 27.8 us for 84 MB of y and out; 18 us of it go by at memory's rate, the first 9 are the
+// 4096 rows of 5120 columns, rank 64: 30 us for 84 MB of y and out; 18 us of it go by at memory's rate, the first 9 to 12 are the
 // launch, the ids and h on their way.  48 rows of 34816 columns, 12 adapters of rank 32: 14.2 us, of which B, y and out (33 MB) take 6.
 template <typename T, int TT, int Q, int EACH>
 __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
