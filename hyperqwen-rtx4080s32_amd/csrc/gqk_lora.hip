@@ -134,8 +134,8 @@ __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset
 // ranks (TT = 4), or all 16 rows and one 16-rank tile (TT = 1).  x goes by once and leaves the caches first, so that A, which every
 // block of rows reads again, stays (4096 rows of 17408 values 82.4 -> 78.1 us, both launches).
 //
-// 4096 rows of 17408 values, rank 64: 34 us, 4.2 TB/s of x.  Without any load it takes 24: LDS, the barriers and the
-// issue of each stage, which hide the loads in part only (loads 4 stages ahead cost 1.4 us more, two workgroups a CU 2.6, blocks of
+// 4096 rows of 17408 values, rank 64: 34 us, 4.2 TB/s of x, near what a copy reaches (4.75).  Without any load it takes
+// 21: LDS, the barriers and the issue of each stage, beside which the loads go on (loads 4 stages ahead cost 1.4 us more, two workgroups a CU 2.6, blocks of
 // 128 rows 9; eight waves with half of each stage change nothing).  48 rows of 5120, 12 adapters of rank 32: 6.7 us, a launch, ids, one trip to memory,
 // partial sums out.
 template <typename T, int TT, int Q>
