@@ -112,6 +112,9 @@ __device__ __forceinline__ float sum4(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+// Splits of `chunk` keys of the keys [start, len), one at least.  (len - start + chunk can pass 31 bits where the sequence is long.)
+__device__ __forceinline__ int splits_of(int start, int len, int chunk) { return len > start ? (len - start - 1) / chunk + 1 : 1; }
+
 // The exponent's base of a running maximum: nothing was seen yet (-inf) must not become -inf - -inf.
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_huge_valf() ? 0.f : m; }
 
@@ -173,9 +176,9 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
   const bool too_long = len0 > a.max_length;
   const int len = too_long ? 0 : len0;
   const int first = a.window > 0 ? max(0, len - a.window) : 0, start = first & ~(kTile - 1);
-  const int ns = max(1, (len - start + a.chunk - 1) / a.chunk);   // splits of this sequence
+  const int ns = splits_of(start, len, a.chunk);   // of this sequence
   if (split >= ns) return;
-  const int k_begin = start + split * a.chunk, k_end = min(len, k_begin + a.chunk);
+  const int k_begin = start + split * a.chunk, k_end = k_begin + min(a.chunk, len - k_begin);
   const float inf = __builtin_huge_valf();
 
   const int rt = wave % a.row_waves, kw = wave / a.row_waves, nkw = kWaves / a.row_waves;
@@ -533,7 +536,7 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(AttnArgs a) {
   const int rows_wg = 16 * a.row_waves, rb = h % group / rows_wg, r = h % group - rb * rows_wg, R = min(rows_wg, group - rb * rows_wg);
   const int len0 = max(0, a.lengths[b]), len = len0 > a.max_length ? 0 : len0;
   const int first = a.window > 0 ? max(0, len - a.window) : 0, start = first & ~(kTile - 1);
-  const int ns = max(1, (len - start + a.chunk - 1) / a.chunk);
+  const int ns = splits_of(start, len, a.chunk);
   if (ns == 1) return;   // written already
   const int64_t unit = ((int64_t)b * a.kv.heads + kvh) * a.row_blocks + rb;
   const float* part = a.partials + unit * a.splits * min(rows_wg, group) * (D + 4);
