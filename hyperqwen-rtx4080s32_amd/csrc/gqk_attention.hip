@@ -53,6 +53,10 @@ constexpr int kWaves = 4;             // waves of a workgroup
 constexpr int kTile = 32;             // keys of a wave's step
 constexpr int kJoinSplits = 16;       // splits that the last workgroup of a sequence joins, at most
 constexpr int kMostSplits = 256;
+// A weight is 2^(score - maximum + kLift): fp16 uses its whole range, so that weights keep their relative precision down to 2^-29 of
+// the heaviest and none is lost above 2^-40 (not lifted they do to 2^-14, and a long flat tail of them, each lighter than that, lost
+// up to all of its weight).  bf16 has fp32's exponents.
+template <typename T> constexpr float kLift = __is_same(T, f16_t) ? 15.f : 0.f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct AttnArgs {
@@ -118,7 +122,7 @@ __device__ __forceinline__ int splits_of(int start, int len, int chunk) { return
 // The exponent's base of a running maximum: nothing was seen yet (-inf) must not become -inf - -inf.
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_huge_valf() ? 0.f : m; }
 
-// Partial sums over a split's keys, relative to its maximum, added up in order.
+// Partial sums over a split's keys, relative to its maximum (both lifted alike), added up in order.
 struct Joined {
   float m = -__builtin_huge_valf(), l = 0.f;
   v4f o{0.f, 0.f, 0.f, 0.f};
@@ -385,9 +389,10 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
       }
       m = mn;
       float sum = 0.f, p[8];
+      const float pb = mb - kLift<T>;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(sc[j >> 2][j & 3] - mb);
+        p[j] = __builtin_amdgcn_exp2f(sc[j >> 2][j & 3] - pb);
         sum += p[j];
       }
       l += sum;
@@ -468,7 +473,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
     *(v2u*)to = v2u{pack2<T>(x[0] * f, x[1] * f), pack2<T>(x[2] * f, x[3] * f)};
   };
   auto store_lse = [&](int r, float M, float L) {
-    a.lse[(int64_t)b * a.q_heads + kvh * group + row0 + r] = L == 0.f ? -inf : (M + __builtin_amdgcn_logf(L)) * kLn2;
+    a.lse[(int64_t)b * a.q_heads + kvh * group + row0 + r] = L == 0.f ? -inf : (M - kLift<T> + __builtin_amdgcn_logf(L)) * kLn2;
   };
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(part, 0, a.splits * R * (D + 4) * 4, 0x00020000);
   constexpr int kDevice = 16;   // device-scope cache policy (sc1): through the XCD's L2
@@ -573,7 +578,7 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(AttnArgs a) {
   T* to = (T*)a.out + b * a.out_row + h * a.out_head + d;
   *(v2u*)to = v2u{pack2<T>(all.o[0] * f, all.o[1] * f), pack2<T>(all.o[2] * f, all.o[3] * f)};
   if (a.lse && threadIdx.x == 0)
-    a.lse[(int64_t)b * a.q_heads + h] = all.l == 0.f ? -__builtin_huge_valf() : (all.m + __builtin_amdgcn_logf(all.l)) * kLn2;
+    a.lse[(int64_t)b * a.q_heads + h] = all.l == 0.f ? -__builtin_huge_valf() : (all.m - kLift<T> + __builtin_amdgcn_logf(all.l)) * kLn2;
 }
 
 // How a call is cut: workgroups over the query heads of a key head, and splits of `chunk` keys.

@@ -56,3 +56,29 @@ def test_attention_at_the_limit_of_keys(length, window):
     _within(out, want.cuda().expand(1, 1, dim), tol.cuda(), (length, window))
     want_l = (light + heavy).log()
     _within(lse, want_l.cuda().expand(1, 1), chain + 2.0 ** -16 + 4 * E32 * (want_l + 20).cuda(), "lse")
+
+
+@pytest.mark.parametrize("qt,ct,dim", [(F16, F16, 64), (F16, F16, 128), (F16, F16, 256), (F16, F8, 128), (BF, BF, 128)])
+@pytest.mark.parametrize("batch,pages", [(1, 40), (1100, 1)])
+@pytest.mark.parametrize("late", [False, True])
+def test_attention_flat_tail(qt, ct, dim, batch, pages, late):
+    """Four heavy keys of value 0 to a page, one for each wave, first or last of it; 4092 others of 2^-25.2 of their weight each,
+    which are all of the result.  A weight keeps its relative precision down there: half a step of the type."""
+    page = 4096
+    k, v = (torch.zeros((1, page, 1, dim), device="cuda") for _ in range(2))
+    k[..., 0], v[:] = -14.0, 256.0
+    heavy = torch.arange(0, 128, 32, device="cuda") + (page - 128 if late else 0)
+    k[:, heavy], v[:, heavy] = 0.0, 0.0
+    k, v = k.to(ct), v.to(ct)
+    q = torch.zeros((batch, 2, dim), dtype=qt, device="cuda")
+    q[..., 0] = 1.25                                         # scores of 0 and -17.5
+    table = torch.zeros((batch, pages), dtype=torch.int32, device="cuda")
+    n = torch.full((batch,), pages * page, dtype=torch.int32, device="cuda")
+    out, lse = gguf_hip.paged_attention(q, k, v, table, n, scale=1.0, return_lse=True)
+    light = (page - 4) * torch.tensor(-17.5, dtype=torch.float64).exp().item()
+    want = 256 * light / (4 + light)
+    # a score's error (one product, two factors, its exponential) and up to 2^7 steps a wave with two sums each
+    e = 2.0 ** -18 + 2.0 ** 9 * E32
+    _within(out, torch.full_like(out, want, dtype=torch.float64), (2 * U[qt] + 2 * e) * want + 2.0 ** -25, "out")
+    want_l = torch.tensor((4 + light) * pages, dtype=torch.float64).log().item()
+    _within(lse, torch.full_like(lse, want_l, dtype=torch.float64), 2 * e + 4 * E32 * (want_l + 40), "lse")
