@@ -593,6 +593,15 @@ Cut cut_of(int M, int64_t K, int parts, int rank) {
   return c;
 }
 
+// The same with at most as many partial sums of h as the workspace holds; false: not even one.
+bool fit(Cut& c, int64_t bytes, int64_t h_bytes) {
+  const int64_t most = (bytes - GQK_CTR_BYTES) / h_bytes;
+  if (bytes < GQK_CTR_BYTES || most < 1) return false;
+  c.splits = (int)std::min<int64_t>(c.splits, most);
+  c.finer = (int)std::min<int64_t>(c.finer, most / c.splits);
+  return true;
+}
+
 // Workgroups of `columns` columns over all parts.
 int64_t column_blocks(const LoraArgs& g, int columns) {
   int64_t blocks = 0, begin = 0;
@@ -677,13 +686,14 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
     return decode_fail(GQK_ERR_SHAPE, "lora_add: K %lld or x's row stride %lld above %d", (long long)K, (long long)x_row, GQK_LORA_MAX_K);
   if (((uintptr_t)x | (uintptr_t)a | (uintptr_t)b) & 15 || x_row & 7)
     return decode_fail(GQK_ERR_SHAPE, "lora_add: x, a and b are 16-byte aligned, x's row stride a multiple of 8");
-  if (!workspace || workspace_bytes < need || (uintptr_t)workspace & 255)
+  Cut c = cut_of(M, K, parts, rank);
+  const int64_t h_bytes = (int64_t)M * parts * rank * 4;
+  if (!workspace || !fit(c, workspace_bytes, h_bytes) || (uintptr_t)workspace & 255)
     return decode_fail(GQK_ERR_SHAPE, "lora_add: workspace %lld bytes < %lld (or not 256-byte aligned)", (long long)workspace_bytes,
-                       (long long)need);
+                       (long long)(GQK_CTR_BYTES + h_bytes));
   g.y = y; g.x = x; g.a = a; g.b = b; g.out = out; g.y_row = y_row; g.x_row = x_row; g.out_row = out_row; g.K = K;
   g.ids = ids; g.wide_ids = ids_64; g.scales = scales; g.h = (float*)((char*)workspace + GQK_CTR_BYTES);
   g.M = M; g.slots = slots; g.parts = parts; g.rank = rank;
-  const Cut c = cut_of(M, K, parts, rank);
   if (c.blocks > 65535) return decode_fail(GQK_ERR_SHAPE, "lora_add: %d rows", M);
   g.splits = c.splits; g.finer = c.finer; g.chunks = c.chunks; g.blocks = c.blocks;
   // whole 16-byte pieces in every row, and rows that 32-bit offsets reach

@@ -35,7 +35,8 @@ def _lora_into(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     have = ws.numel() * ws.element_size()
     slots, parts, rank, _ = a.shape
     wide, size = ids.dtype == torch.int64, ids.element_size()
-    # rows are independent: what does not fit the workspace at once goes in turns
+    # rows are independent: what does not fit the workspace at once goes in turns (a last, shorter one that would like more room
+    # than the others gets fewer splits of K)
     rows = M
     while rows > 1 and check(lib.gqk_lora_workspace_bytes(rows, K, parts, rank), "lora_add") > have:
         rows = (rows + 1) // 2

@@ -189,8 +189,9 @@ int gqk_linear_noalloc(const void* packed, const int32_t* desc_dev, const gqk_pl
  * rank multiples of 8, rank <= 256 (adapters of a lower rank are padded with zeros), parts <= 8; ids
  * int32 [M], or int64 with ids_64; scales fp32 [slots] or NULL (1).  x, a, b are 16-byte aligned.  Products
  * and sums are in fp32, rounded once to out.  K and x's row stride (where M > 1) are at most GQK_LORA_MAX_K.
- * workspace: gqk_lora_workspace_bytes bytes, 256-byte aligned; its
- * first GQK_CTR_BYTES are left alone, so that a linear layer's workspace serves (calls in stream order). */
+ * workspace: gqk_lora_workspace_bytes bytes, 256-byte aligned (fewer rows may want more: K is cut finer); in a smaller one, down to
+ * GQK_CTR_BYTES + 4 M parts rank, K is cut into fewer splits.  Its first GQK_CTR_BYTES are left alone, so that a linear layer's
+ * workspace serves (calls in stream order). */
 #define GQK_LORA_MAX_K 4194296 /* 256 rows stay below 2^31 bytes */
 int64_t gqk_lora_workspace_bytes(int M, int64_t K, int parts, int rank);
 int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int M, int64_t K, const void* a,

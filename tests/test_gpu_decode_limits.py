@@ -2,6 +2,8 @@
 little weight each, workspaces smaller than a call would like, batches beyond one launch.  Each against its definition in 64
 bits, with bounds from the roundings that the operators are allowed: u is half a step of a type (2^-8 of a bf16 value, 2^-11 of an
 fp16 one), sums and products are fp32 (2^-24 of each)."""
+import ctypes
+
 import pytest
 import torch
 
@@ -82,3 +84,64 @@ def test_attention_flat_tail(qt, ct, dim, batch, pages, late):
     _within(out, torch.full_like(out, want, dtype=torch.float64), (2 * U[qt] + 2 * e) * want + 2.0 ** -25, "out")
     want_l = torch.tensor((4 + light) * pages, dtype=torch.float64).log().item()
     _within(lse, torch.full_like(lse, want_l, dtype=torch.float64), 2 * e + 4 * E32 * (want_l + 40), "lse")
+
+
+# ---- adapters --------------------------------------------------------------------------------
+
+def _lora_case(gen, M, K, n_outs, rank, slots, dtype):
+    y, x = _randn(gen, M, sum(n_outs), dtype=dtype), _randn(gen, M, K, dtype=dtype)
+    a = (_randn(gen, slots, len(n_outs), rank, K) * K ** -0.5).to(dtype)
+    b = _randn(gen, slots, sum(n_outs), rank, dtype=dtype)
+    return y, x, a, b, torch.randint(-1, slots, (M,), device="cuda", generator=gen)
+
+
+def _lora_exact(y, x, a, b, ids, n_outs):
+    """(out, its bound) in 64 bits: h's K products in fp32, kept to 2^-16, rank products in fp32, one rounding."""
+    out, tol = y.double(), torch.zeros(y.shape, dtype=torch.float64, device="cuda")
+    K, rank = x.shape[1], a.shape[2]
+    for i in range(a.shape[0]):
+        rows = (ids == i).nonzero()[:, 0]
+        X, col = x[rows].double(), 0
+        for p, n in enumerate(n_outs):
+            A, B = a[i, p].double(), b[i, col:col + n].double()
+            h, ha = X @ A.t(), X.abs() @ A.abs().t()
+            out[rows, col:col + n] += h @ B.t()
+            e = (2.0 ** -16 + (rank + 4) * E32) * h.abs() + K * E32 * ha
+            tol[rows, col:col + n] = e @ B.abs().t()
+            col += n
+    u = U[y.dtype]
+    return out, (1 + u) * (tol + 2 * E32 * y.double().abs()) + u * out.abs() + 2.0 ** -25
+
+
+@pytest.mark.parametrize("into", ["y", "new"])
+def test_lora_turns_whose_last_is_the_smallest(into):
+    """4867 rows in a workspace made for 15520 go in turns of 1217; the last, of 1216, would like more splits of K, and
+    so more room, than the others.  It must not be refused once they are written."""
+    K, n_outs = 17408, (24,)
+    need = _lib.lib.gqk_lora_workspace_bytes
+    size = need(15520, K, 1, 16)
+    assert need(1217, K, 1, 16) <= size < need(1216, K, 1, 16)
+    y, x, a, b, ids = _lora_case(_gen(1), 4867, K, n_outs, 16, 2, BF)
+    want, tol = _lora_exact(y, x, a, b, ids, n_outs)
+    ws = torch.zeros(size // 4, dtype=torch.int32, device="cuda")
+    out = gguf_hip.lora_add(y, x, a, b, ids, None, n_outs, out=y if into == "y" else None, workspace=ws)
+    _within(out, want, tol, into)
+
+
+@pytest.mark.parametrize("rows", [8192, 4096, 2047, 300, 256, 40])
+def test_lora_workspace_of_more_rows_serves_fewer(rows):
+    """The C entry in a workspace sized for 16384 rows, and in the least that it takes; nothing is written past it or in the counters."""
+    K, n, rank = 17408, 16, 64
+    y, x, a, b, ids = _lora_case(_gen(rows), rows, K, (n,), rank, 2, BF)
+    want, tol = _lora_exact(y, x, a, b, ids, (n,))
+    cols = (ctypes.c_int64 * 1)(n)
+    for size in (_lib.lib.gqk_lora_workspace_bytes(16384, K, 1, rank), _lib.GQK_CTR_BYTES + rows * rank * 4):
+        whole = torch.zeros(size // 4 + 4096, dtype=torch.int32, device="cuda")
+        out = torch.empty_like(y)
+        args = [y.data_ptr(), n, x.data_ptr(), K, rows, K, a.data_ptr(), b.data_ptr(), 2, 1, cols, rank, ids.data_ptr(), 1, None,
+                _lib.GQK_DTYPE_BF16, out.data_ptr(), n, whole.data_ptr(), size, torch.cuda.current_stream().cuda_stream]
+        assert _lib.lib.gqk_lora_add(*args) == 0, _lib.lib.gqk_last_error()
+        _within(out, want, tol, (rows, size))
+        assert not whole[size // 4:].any() and not whole[:_lib.GQK_CTR_BYTES // 4].any()
+    args[-2] = size - 4
+    assert _lib.lib.gqk_lora_add(*args) == _lib.GQK_ERR_SHAPE
