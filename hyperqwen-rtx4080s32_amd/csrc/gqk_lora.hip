@@ -694,7 +694,7 @@ int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int
   g.y = y; g.x = x; g.a = a; g.b = b; g.out = out; g.y_row = y_row; g.x_row = x_row; g.out_row = out_row; g.K = K;
   g.ids = ids; g.wide_ids = ids_64; g.scales = scales; g.h = (float*)((char*)workspace + GQK_CTR_BYTES);
   g.M = M; g.slots = slots; g.parts = parts; g.rank = rank;
-  if (c.blocks > 65535) return decode_fail(GQK_ERR_SHAPE, "lora_add: %d rows", M);
+  if (M > GQK_LORA_MAX_ROWS) return decode_fail(GQK_ERR_SHAPE, "lora_add: %d rows, more than %d", M, GQK_LORA_MAX_ROWS);
   g.splits = c.splits; g.finer = c.finer; g.chunks = c.chunks; g.blocks = c.blocks;
   // whole 16-byte pieces in every row, and rows that 32-bit offsets reach
   g.wide_y = !(((uintptr_t)y | (uintptr_t)out) & 15) && !((y_row | out_row) & 7) && y_row < (1 << 22) && out_row < (1 << 22);

@@ -15,6 +15,7 @@ from .eager import direct as _direct, stream as _stream, unwatched as _unwatched
 
 _TYPES = {torch.bfloat16: _lib.GQK_DTYPE_BF16, torch.float16: _lib.GQK_DTYPE_F16}
 MAX_PARTS, MAX_RANK, MAX_K = 8, 256, (1 << 22) - 8
+MAX_ROWS = 65535 * 64   # of one launch
 
 
 @lru_cache(maxsize=256)
@@ -38,7 +39,7 @@ def _lora_into(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     # rows are independent: what does not fit the workspace at once goes in turns (a last, shorter one that would like more room
     # than the others gets fewer splits of K)
     rows = M
-    while rows > 1 and check(lib.gqk_lora_workspace_bytes(rows, K, parts, rank), "lora_add") > have:
+    while rows > MAX_ROWS or rows > 1 and check(lib.gqk_lora_workspace_bytes(rows, K, parts, rank), "lora_add") > have:
         rows = (rows + 1) // 2
     ys, xs, os = (t.stride(0) if M > 1 else t.shape[1] for t in (y, x, out))   # of one row alone it means nothing
     for r in range(0, M, rows):

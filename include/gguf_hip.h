@@ -181,7 +181,7 @@ int gqk_linear_noalloc(const void* packed, const int32_t* desc_dev, const gqk_pl
  * Contents of device arrays are checked where they are read: an index out of its range reads nothing
  * and makes the token's result NaN (a slot out of range stores nothing). */
 
-/* Low-rank adapters of many requests beside a shared projection, any M rows in one call:
+/* Low-rank adapters of many requests beside a shared projection, M rows (at most GQK_LORA_MAX_ROWS):
  *   out[m, n] = y[m, n] + scales[i] * sum_r b[i, n, r] * sum_k a[i, p(n), r, k] * x[m, k],  i = ids[m]
  * p(n): the part (q, k, v; gate, up) of column n, parts side by side with n_outs[p] columns each.  A row with a
  * negative id gets y; one with an id >= slots NaN.  y, x, out: bf16 or fp16 (dtype) rows of any stride,
@@ -193,6 +193,7 @@ int gqk_linear_noalloc(const void* packed, const int32_t* desc_dev, const gqk_pl
  * GQK_CTR_BYTES + 4 M parts rank, K is cut into fewer splits.  Its first GQK_CTR_BYTES are left alone, so that a linear layer's
  * workspace serves (calls in stream order). */
 #define GQK_LORA_MAX_K 4194296 /* 256 rows stay below 2^31 bytes */
+#define GQK_LORA_MAX_ROWS 4194240 /* 65535 blocks of 64 */
 int64_t gqk_lora_workspace_bytes(int M, int64_t K, int parts, int rank);
 int gqk_lora_add(const void* y, int64_t y_row, const void* x, int64_t x_row, int M, int64_t K, const void* a,
                  const void* b, int slots, int parts, const int64_t* n_outs, int rank, const void* ids, int ids_64,

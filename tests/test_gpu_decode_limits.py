@@ -145,3 +145,11 @@ def test_lora_workspace_of_more_rows_serves_fewer(rows):
         assert not whole[size // 4:].any() and not whole[:_lib.GQK_CTR_BYTES // 4].any()
     args[-2] = size - 4
     assert _lib.lib.gqk_lora_add(*args) == _lib.GQK_ERR_SHAPE
+
+
+def test_lora_more_rows_than_a_launch_takes():
+    """Rows beyond 65535 blocks of 64 go in turns."""
+    M = 65535 * 64 + 77
+    y, x, a, b, ids = _lora_case(_gen(2), M, 8, (8,), 8, 2, BF)
+    want, tol = _lora_exact(y, x, a, b, ids, (8,))
+    _within(gguf_hip.lora_add(y, x, a, b, ids, None, (8,)), want, tol, M)
