@@ -587,7 +587,8 @@ struct Cut { int row_waves, row_blocks, splits, chunk; };
 // About as many workgroups as stay resident, of 256 keys at least (32 x 4000 tokens in bf16: 3 a CU 69.9 us, 4 62.4, 6 66.3,
 // 8 64.2; 64 x 3000 of 256 dims in fp8: 3 a CU 50.2, 4 58.3, 5 55.6; 8 x 2000 in splits of 128 keys or more 16.5, of 256 13.6; of 32
 // heads that share one of keys, whose waves see more of a split each, 8 x 4000 13.3 and 15.6, of 128 heads 4 x 4000 17.7 and 22.9).
-Cut cut_of(int batch, int q_heads, int kv_heads, int size, int max_length, int window) {
+// The splits' partial sums lie in the workspace: as many splits as it holds, one (which needs none) in any.
+Cut cut_of(int batch, int q_heads, int kv_heads, int dim, int size, int max_length, int window, int64_t workspace_bytes) {
   const int group = q_heads / kv_heads, tiles = (group + 15) / 16;
   Cut c;
   c.row_waves = tiles >= 3 ? 4 : tiles;
@@ -598,7 +599,9 @@ Cut cut_of(int batch, int q_heads, int kv_heads, int size, int max_length, int w
   const int64_t least = (c.row_waves == 1 ? 2 * kWaves : 4) * kTile;   // keys of the shortest split
   int64_t splits = std::max<int64_t>(1, std::min((wanted + units - 1) / std::max<int64_t>(1, units), (span + least - 1) / least));
   splits = std::min<int64_t>(splits, kMostSplits);
-  if (units > GQK_CTR_WORDS) splits = 1;
+  const int64_t each = units * std::min(16 * c.row_waves, group) * (dim + 4) * 4;   // bytes of one split of all units
+  if (units > GQK_CTR_WORDS || workspace_bytes < GQK_CTR_BYTES) splits = 1;
+  else if (each > 0) splits = std::max<int64_t>(1, std::min(splits, (workspace_bytes - GQK_CTR_BYTES) / each));
   c.chunk = (int)std::max<int64_t>(kTile, ((span + splits - 1) / splits + kTile - 1) / kTile * kTile);
   c.splits = (int)std::max<int64_t>(1, (span + c.chunk - 1) / c.chunk);
   return c;
@@ -639,7 +642,7 @@ int64_t gqk_paged_attention_workspace_bytes(int batch, int q_heads, int kv_heads
     return decode_fail(GQK_ERR_SHAPE, "paged_attention: %d sequences, %d / %d heads of %d, max_length %d, window %d", batch,
                        q_heads, kv_heads, dim, max_length, window);
   // of either size of pages: the larger
-  const Cut c = cut_of(batch, q_heads, kv_heads, 2, max_length, window);
+  const Cut c = cut_of(batch, q_heads, kv_heads, dim, 2, max_length, window, INT64_MAX);
   const int64_t rows = std::min(16 * c.row_waves, q_heads / kv_heads), units = (int64_t)batch * kv_heads * c.row_blocks;
   return c.splits > 1 ? GQK_CTR_BYTES + units * rows * c.splits * (dim + 4) * 4 : 0;
 }
@@ -660,12 +663,10 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
   if (!q || !out || !lengths || (!table && max_length > 0)) return decode_fail(GQK_ERR_ARG, "paged_attention: null pointer");
   if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_row | q_head | out_row | out_head) & 7)
     return decode_fail(GQK_ERR_SHAPE, "paged_attention: q and out are 16-byte aligned with strides that are multiples of 8");
-  const int64_t need = gqk_paged_attention_workspace_bytes(batch, q_heads, pages->heads, pages->dim, max_length, window);
-  if (need < 0) return (int)need;
-  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace & 255))
-    return decode_fail(GQK_ERR_SHAPE, "paged_attention: workspace %lld bytes < %lld (or not 256-byte aligned)",
-                       (long long)workspace_bytes, (long long)need);
-  const Cut c = cut_of(batch, q_heads, pages->heads, pages->dtype == GQK_DTYPE_FP8 ? 1 : 2, max_length, window);
+  const Cut c = cut_of(batch, q_heads, pages->heads, pages->dim, pages->dtype == GQK_DTYPE_FP8 ? 1 : 2, max_length, window,
+                       workspace ? workspace_bytes : 0);
+  if (c.splits > 1 && (uintptr_t)workspace & 255)
+    return decode_fail(GQK_ERR_SHAPE, "paged_attention: workspace is not 256-byte aligned");
   AttnArgs a{};
   a.q = q; a.q_row = q_row; a.q_head = q_head; a.kv = *pages; a.table = table; a.table_row = table_row; a.lengths = lengths;
   a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.q_heads = q_heads; a.max_length = max_length;

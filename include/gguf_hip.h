@@ -248,8 +248,8 @@ int gqk_qk_norm_rope(const gqk_heads* q, const gqk_heads* k, const gqk_heads* v,
  * [batch, q_heads, dim]; table int32 [batch, table_width] with rows table_row apart; lse: NULL or fp32
  * [batch, q_heads], log sum_j exp.  Scores, softmax and sums are in fp32; the probabilities that multiply v are rounded to
  * the heads' type.  workspace: gqk_paged_attention_workspace_bytes bytes, 256-byte aligned, zeroed
- * before its first use (arrival counters, which every launch leaves at zero, and fp32 partials): a linear
- * layer's workspace serves (calls in stream order). */
+ * before its first use (arrival counters, which every launch leaves at zero, and fp32 partials); in a smaller one (or none: NULL)
+ * the length is cut into fewer splits.  A linear layer's workspace serves (calls in stream order). */
 #define GQK_MAX_KEYS 0x7ffffc00 /* the largest max_length */
 int64_t gqk_paged_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int dim, int max_length, int window);
 int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype, int batch, int q_heads,

@@ -86,6 +86,61 @@ def test_attention_flat_tail(qt, ct, dim, batch, pages, late):
     _within(lse, torch.full_like(lse, want_l, dtype=torch.float64), 2 * e + 4 * E32 * (want_l + 40), "lse")
 
 
+def _attend(q, k, v, table, lens, scale):
+    """(out, its bound) in 64 bits, for lengths that all sequences share or not, one page to a sequence."""
+    B, H, D = q.shape
+    hkv = k.shape[2]
+    kk, vv = (t[table[:, 0].long()].double().transpose(1, 2) for t in (k, v))           # [B, hkv, page, D]
+    qq = q.double().view(B, hkv, H // hkv, D)
+    live = torch.arange(k.shape[1], device="cuda")[None] < lens[:, None]
+    s = (qq @ kk.transpose(2, 3).contiguous() * scale).masked_fill(~live[:, None, None], float("-inf"))
+    size = (qq.abs() @ kk.abs().transpose(2, 3).contiguous() * scale).masked_fill(~live[:, None, None], 0).amax(-1, keepdim=True)
+    top = s.amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(top.isinf(), 0.0, top))
+    p = p / p.sum(-1, keepdim=True).clamp_min(1e-300)
+    o, abs_o = p @ vv, p @ vv.abs()
+    es = (D + 8) * E32 * size + 2.0 ** -19
+    tol = U[q.dtype] * o.abs() + (1 + U[q.dtype]) * (U[q.dtype] + 2 * es + 2.0 ** -18) * abs_o + 2.0 ** -25
+    return o.view(B, H, D), tol.view(B, H, D)
+
+
+@pytest.mark.parametrize("batch,heads", [(1005, 64), (1020, 64), (1023, 64), (511, 128)])
+def test_attention_of_many_rows_on_the_shared_workspace(batch, heads):
+    """Just under as many workgroups as stay resident, of many wide heads each: two splits of all would not fit the workspace."""
+    gen = _gen(batch)
+    k, v = (_randn(gen, 5, 64, 1, 256, dtype=BF) for _ in range(2))
+    q = _randn(gen, batch, heads, 256, dtype=BF)
+    table = torch.randint(0, 5, (batch, 1), device="cuda", generator=gen).int()
+    lens = torch.randint(0, 65, (batch,), device="cuda", generator=gen).int()
+    wide = torch.full((batch, 128), -1, dtype=torch.int32, device="cuda")               # 8192 keys: the bound that the call goes by
+    wide[:, :1] = table
+    out = gguf_hip.paged_attention(q, k, v, wide, lens)
+    want, tol = _attend(q, k, v, table, lens, 256 ** -0.5)
+    _within(out, want, tol, batch)
+
+
+@pytest.mark.parametrize("batch,heads,hkv,dim", [(1, 8, 2, 64), (3, 40, 8, 128), (2, 40, 1, 256)])
+def test_attention_in_small_workspaces(batch, heads, hkv, dim):
+    """A workspace that holds all, some, two or none of the splits that the call would like; its counters stay at zero, and
+    nothing is written past its end."""
+    gen = _gen(heads)
+    k, v = (_randn(gen, 3, 4096, hkv, dim, dtype=BF) for _ in range(2))
+    q = _randn(gen, batch, heads, dim, dtype=BF)
+    table = torch.arange(batch, device="cuda").int()[:, None]
+    lens = torch.tensor([4096, 4001, 0][:batch], device="cuda").int()
+    want, tol = _attend(q, k, v, table, lens, dim ** -0.5)
+    need = _lib.lib.gqk_paged_attention_workspace_bytes(batch, heads, hkv, dim, 4096, 0)
+    split = batch * heads * (dim + 4) * 4
+    assert need >= _lib.GQK_CTR_BYTES + 4 * split
+    for size in (need, need - 4, _lib.GQK_CTR_BYTES + 3 * split, _lib.GQK_CTR_BYTES + 2 * split, _lib.GQK_CTR_BYTES + 2 * split - 4,
+                 _lib.GQK_CTR_BYTES, 256):
+        whole = torch.zeros(size // 4 + 1024, dtype=torch.int32, device="cuda")
+        ws = whole[:size // 4]
+        _within(gguf_hip.paged_attention(q, k, v, table, lens, workspace=ws), want, tol, size)
+        assert not whole[size // 4:].any() and not ws[:_lib.GQK_CTR_BYTES // 4].any(), size
+        _within(gguf_hip.paged_attention(q, k, v, table, lens, workspace=ws), want, tol, size)
+
+
 # ---- adapters --------------------------------------------------------------------------------
 
 def _lora_case(gen, M, K, n_outs, rank, slots, dtype):
