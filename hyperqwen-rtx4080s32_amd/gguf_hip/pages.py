@@ -9,7 +9,7 @@ import torch
 
 from . import ops
 from ._lib import _fast, check, lib
-from .eager import stream as _stream, unwatched as _unwatched
+from .eager import direct as _direct, stream as _stream, unwatched as _unwatched
 
 
 def _pairs(t, what: str) -> np.ndarray:
@@ -29,6 +29,48 @@ def _pairs(t, what: str) -> np.ndarray:
     return np.ascontiguousarray(a)
 
 
+def _layout(pages: torch.Tensor, dim: int) -> tuple[int, int, int, int, int]:
+    """(planes, elements from one to the next, pages, elements from one to the next, elements of a page)."""
+    what = "copy_pages"
+    shape, stride = pages.shape, pages.stride()
+    n = 1
+    for m, st in zip(reversed(shape[dim + 1:]), reversed(stride[dim + 1:])):
+        if m != 1 and st != n:
+            raise ValueError(f"{what}: a page's own dimensions must be contiguous, got strides {stride}")
+        n *= m
+    planes, plane = 1, 0
+    for m, st in zip(reversed(shape[:dim]), reversed(stride[:dim])):
+        if m == 1:
+            continue
+        if planes > 1 and st != plane * planes:
+            raise ValueError(f"{what}: the dimensions before the pages must be evenly spaced, got strides {stride}")
+        plane = st if planes == 1 else plane
+        planes *= m
+    if pages.numel() == 0:
+        planes = 0
+    return planes, plane, shape[dim], stride[dim] if shape[dim] > 1 else n, n
+
+
+def _copy_into(pages: torch.Tensor, src: np.ndarray, dst: np.ndarray, dim: int) -> None:
+    if pages.device.index != torch.cuda.current_device():
+        with torch.cuda.device(pages.device):
+            return _copy_into(pages, src, dst, dim)
+    planes, plane, count, page, n = _layout(pages, dim)
+    size = pages.element_size()
+    check(lib.gqk_copy_pages(pages.data_ptr(), planes, plane * size, count, page * size, n * size, src.ctypes.data, dst.ctypes.data,
+                             src.size, _stream(pages.device)), "copy_pages")
+
+
+@torch.library.custom_op("gguf_hip::copy_pages", mutates_args=("pages",))
+def _copy_op(pages: torch.Tensor, src: list[int], dst: list[int], dim: int) -> None:
+    _copy_into(pages, np.array(src, np.int32), np.array(dst, np.int32), dim)
+
+
+@_copy_op.register_fake
+def _(pages, src, dst, dim):
+    return None
+
+
 def copy_pages(pages: torch.Tensor, src, dst, dim: int = 0) -> None:
     """pages[..., dst[i], ...] = pages[..., src[i], ...] for every i along dimension ``dim``, in place, in one launch:
     ``pages`` is a cache's whole storage (any type), the page's own dimensions after ``dim`` contiguous, the dimensions
@@ -45,29 +87,14 @@ def copy_pages(pages: torch.Tensor, src, dst, dim: int = 0) -> None:
     s, d = _pairs(src, what), _pairs(dst, what)
     if s.size != d.size:
         raise ValueError(f"{what}: {s.size} sources for {d.size} destinations")
-    shape, stride, size = pages.shape, pages.stride(), pages.element_size()
-    n = 1
-    for m, st in zip(reversed(shape[dim + 1:]), reversed(stride[dim + 1:])):
-        if m != 1 and st != n:
-            raise ValueError(f"{what}: a page's own dimensions must be contiguous, got strides {stride}")
-        n *= m
-    planes, plane = 1, 0
-    for m, st in zip(reversed(shape[:dim]), reversed(stride[:dim])):
-        if m == 1:
-            continue
-        if planes > 1 and st != plane * planes:
-            raise ValueError(f"{what}: the dimensions before the pages must be evenly spaced, got strides {stride}")
-        plane = st if planes == 1 else plane
-        planes *= m
-    if pages.numel() == 0:
-        planes = 0
-    if pages.device.index != torch.cuda.current_device():
-        with torch.cuda.device(pages.device):
-            return copy_pages(pages, s, d, dim)
-    page = stride[dim] if shape[dim] > 1 else n
-    check(lib.gqk_copy_pages(pages.data_ptr(), planes, plane * size, shape[dim], page * size, n * size,
-                             s.ctypes.data, d.ctypes.data, s.size, _stream(pages.device)), what)
-    torch.autograd.graph.increment_version(pages)
+    _, _, count, page, n = _layout(pages, dim)
+    if _direct(pages):
+        _copy_into(pages, s, d, dim)
+        torch.autograd.graph.increment_version(pages)
+    else:
+        # of no plane: the pairs are looked at, and nothing is launched
+        check(lib.gqk_copy_pages(None, 0, 0, count, page, n, s.ctypes.data, d.ctypes.data, s.size, None), what)
+        _copy_op(pages, s.tolist(), d.tolist(), dim)
 
 
 class PagePool:

@@ -208,3 +208,29 @@ def test_lora_more_rows_than_a_launch_takes():
     y, x, a, b, ids = _lora_case(_gen(2), M, 8, (8,), 8, 2, BF)
     want, tol = _lora_exact(y, x, a, b, ids, (8,))
     _within(gguf_hip.lora_add(y, x, a, b, ids, None, (8,)), want, tol, M)
+
+
+# ---- page copies -----------------------------------------------------------------------------
+
+def test_copy_pages_traced_and_watched():
+    """A trace records the copy and does not make it; the recorded call, the op that a profiler sees and the eager call agree."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def fork(pages):
+        gguf_hip.copy_pages(pages, [3, 4], [7, 8], dim=1)
+        return pages[:, 7] + 1
+
+    pages = _randn(_gen(1), 3, 9, 16, 64, dtype=BF)
+    want = pages.clone()
+    want[:, [7, 8]] = want[:, [3, 4]]
+    g = make_fx(fork, tracing_mode="fake")(pages)
+    assert not torch.equal(pages, want)
+    mine = pages.clone()
+    assert torch.equal(g(mine), want[:, 7] + 1) and torch.equal(mine, want)
+    mine = pages.clone()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        gguf_hip.copy_pages(mine, [3, 4], [7, 8], dim=1)
+    assert torch.equal(mine, want) and any("copy_pages" in ev.key for ev in prof.key_averages())
+    version = pages._version
+    gguf_hip.copy_pages(pages, [3, 4], [7, 8], dim=1)
+    assert torch.equal(pages, want) and pages._version > version
