@@ -230,12 +230,14 @@ class GroupedLayer:
 
 # one workspace per device, shared by every grouped layer prepared on it
 _WORKSPACES: dict[int, torch.Tensor] = {}
+# those that a larger one replaced: a captured call that no layer stands behind (lora_add, paged_attention) may hold their address
+_REPLACED: list[torch.Tensor] = []
 
 
 def device_workspace(device: torch.device, need: int = 0) -> torch.Tensor:
     """The device's shared workspace: zero-filled int32, at least ``gqk_workspace_bytes_max()``
     bytes (every GEMM plan at any M) and ``need`` (a layer's GEMV plans).  It is made at a layer's
-    preparation and never resized or freed while a layer holds it, so the apply path allocates
+    preparation and never resized or freed, so the apply path allocates
     nothing and a captured graph's pointer stays valid.  Only a layer whose GEMV plans need more
     (a very large custom wave target) gets a larger one, which then serves the layers prepared
     after it; earlier layers keep theirs."""
@@ -244,6 +246,8 @@ def device_workspace(device: torch.device, need: int = 0) -> torch.Tensor:
     if ws is None or ws.numel() * ws.element_size() < need:
         with torch.cuda.device(idx):
             size = max(need, check(lib.gqk_workspace_bytes_max(), "workspace_bytes_max"))
+        if ws is not None:
+            _REPLACED.append(ws)
         ws = torch.zeros((size + 3) // 4, dtype=torch.int32, device=torch.device("cuda", idx))
         _WORKSPACES[idx] = ws
         _lib._fast.set_workspace(idx, ws)

@@ -3,6 +3,7 @@ little weight each, workspaces smaller than a call would like, batches beyond on
 bits, with bounds from the roundings that the operators are allowed: u is half a step of a type (2^-8 of a bf16 value, 2^-11 of an
 fp16 one), sums and products are fp32 (2^-24 of each)."""
 import ctypes
+import weakref
 
 import pytest
 import torch
@@ -234,3 +235,19 @@ def test_copy_pages_traced_and_watched():
     version = pages._version
     gguf_hip.copy_pages(pages, [3, 4], [7, 8], dim=1)
     assert torch.equal(pages, want) and pages._version > version
+
+
+# ---- the shared workspace --------------------------------------------------------------------
+
+def test_shared_workspace_outlives_a_larger_one(monkeypatch):
+    """A captured call keeps the address of the workspace that it was captured with: where a layer's plans need a larger one, the
+    old one's memory is not given to others."""
+    from gguf_hip import ops
+
+    device = torch.device("cuda", 0)
+    monkeypatch.setattr(ops, "_WORKSPACES", {})
+    old = ops.shared_workspace(device)
+    alive, size = weakref.ref(old), old.numel() * 4
+    del old
+    assert ops.device_workspace(device, size + 4096).numel() * 4 == size + 4096
+    assert alive() is not None
