@@ -11,7 +11,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import _fast, check, lib
-from .eager import direct as _direct, stream as _stream, unwatched as _unwatched
+from .eager import direct as _direct, no_backward, stream as _stream, unwatched as _unwatched
 
 _TYPES = {torch.bfloat16: _lib.GQK_DTYPE_BF16, torch.float16: _lib.GQK_DTYPE_F16}
 MAX_PARTS, MAX_RANK, MAX_K = 8, 256, (1 << 22) - 8
@@ -79,7 +79,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     one part: [N]), their sum N; a [adapters, parts, rank, K] and b [adapters, N, rank] as ``pack_adapters`` makes
     them, of x's and y's type (bf16 or fp16), contiguous, K and rank multiples of 8, rank up to 256; scales fp32 [adapters] or None (1); ids
     int32 or int64 [M], negative for a row without an adapter (one beyond the adapters gives a row of NaN).
-    Returns a new tensor, or ``out`` (a [M, N] view with unit column stride), which may be y itself, or x.
+    Returns a new tensor, or ``out`` (a [M, N] view with unit column stride), which may be y itself, or x.  No backward pass.
     ``workspace``: as mul_mat_grouped's (its own for calls on concurrent streams)."""
     what = "lora_add"
     if _unwatched():
@@ -127,6 +127,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         _lora_inplace_op(out, x, a, b, ids, scales, list(n_outs), workspace)
     else:
         _lora_op(y, x, a, b, ids, scales, list(n_outs), out, workspace)
+    no_backward(what, out, y, x, a, b, scales)
     return out
 
 

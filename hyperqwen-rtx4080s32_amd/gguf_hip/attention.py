@@ -15,7 +15,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import GqkHeads, GqkPages, _fast, check, lib
-from .eager import direct as _direct, stream as _stream, unwatched as _unwatched
+from .eager import direct as _direct, no_backward, stream as _stream, unwatched as _unwatched
 
 _TYPES = {torch.bfloat16: _lib.GQK_DTYPE_BF16, torch.float16: _lib.GQK_DTYPE_F16}
 _PAGE_TYPES = {**_TYPES, torch.float8_e4m3fn: _lib.GQK_DTYPE_FP8}
@@ -134,7 +134,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     is split by it, so a tight one is faster.  A sequence above it, or with a page outside of the cache, gets NaN.
     Returns out [batch, query heads, dim], with ``return_lse`` also the log-sum-exp of its scores (fp32 [batch,
     query heads], -inf without a key), which joins attention over separate caches.  ``workspace``: as
-    mul_mat_grouped's (its own for calls on concurrent streams)."""
+    mul_mat_grouped's (its own for calls on concurrent streams).  No backward pass."""
     if _unwatched():
         got = _fast.paged_attention(q, k_pages, v_pages, block_table, lengths, scale, window, k_scale, v_scale, max_length, out,
                                     return_lse, workspace)
@@ -171,6 +171,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         torch.autograd.graph.increment_version(out)
     else:
         _attention_op(*args)
+    for t in (out, lse):
+        no_backward("paged_attention", t, q, k_pages, v_pages, k_scale, v_scale)
     return (out, lse) if return_lse else out
 
 
@@ -284,7 +286,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     slots of one call must differ), in float8_e4m3fn pages divided by ``k_scale`` / ``v_scale`` (fp32 [heads]) and
     held to +-448.  positions and slots: int32 or int64 [tokens]; a position outside of the table gives NaN.
     Returns (queries, keys): new tensors, or out_q / out_k, which may be q and k themselves; with pages the keys are
-    returned (and written beside the pages) only into an out_k that is given."""
+    returned (and written beside the pages) only into an out_k that is given.  No backward pass, and what is stored in pages is
+    cut from any graph."""
     what = "qk_norm_rope"
     flags = (_lib.GQK_ROPE_UNIT_OFFSET if unit_offset else 0) | (_lib.GQK_ROPE_INTERLEAVED if interleaved else 0)
     if _unwatched():
@@ -341,4 +344,6 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
                 torch.autograd.graph.increment_version(t)
     else:
         _rope_op(*args)
+    no_backward(what, out_q, q, q_weight, table)
+    no_backward(what, out_k, k, k_weight, table)
     return out_q, out_k

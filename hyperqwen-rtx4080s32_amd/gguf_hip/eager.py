@@ -46,3 +46,23 @@ def direct(*tensors: torch.Tensor | None) -> bool:
                               or t._is_zerotensor() or _functional(t) or (grad and t.requires_grad)):
             return False
     return True
+
+
+class _NoBackward(torch.autograd.Function):
+    """Marks a result that was written into out: a gradient that gets there is an error, not silence."""
+
+    @staticmethod
+    def forward(ctx, what, out, *inputs):
+        ctx.what = what
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError(f"{ctx.what} has no backward pass; call it under torch.no_grad(), or on detached tensors")
+
+
+def no_backward(what: str, out: torch.Tensor | None, *inputs: torch.Tensor | None) -> None:
+    """Where a call's inputs (or out's old values) belong to a graph, so does its result, whose backward raises."""
+    if out is not None and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (out, *inputs)):
+        _NoBackward.apply(what, out, *(t for t in inputs if t is not None and t is not out))

@@ -251,3 +251,26 @@ def test_shared_workspace_outlives_a_larger_one(monkeypatch):
     del old
     assert ops.device_workspace(device, size + 4096).numel() * 4 == size + 4096
     assert alive() is not None
+
+
+# ---- gradients -------------------------------------------------------------------------------
+
+def test_gradients_raise_and_values_stay():
+    gen = _gen(1)
+    y, x, a, b, ids = _lora_case(gen, 20, 64, (40,), 8, 2, BF)
+    k, v = (_randn(gen, 3, 16, 2, 64, dtype=BF) for _ in range(2))
+    table, lens = torch.zeros((4, 1), dtype=torch.int32, device="cuda"), torch.full((4,), 9, dtype=torch.int32, device="cuda")
+    q, pos, rope = _randn(gen, 4, 8, 64, dtype=BF), torch.arange(4, device="cuda"), gguf_hip.rope_table(64, 9, device="cuda")
+    for call, t in ((lambda t: gguf_hip.lora_add(y, x, t, b, ids, None, (40,)), a),
+                    (lambda t: gguf_hip.lora_add(t * 1, x, a, b, ids, None, (40,)), y),
+                    (lambda t: gguf_hip.paged_attention(t, k, v, table, lens), q),
+                    (lambda t: gguf_hip.qk_norm_rope(q, None, pos, rope, t)[0], _randn(gen, 64, dtype=BF))):
+        want = call(t)
+        leaf = torch.nn.Parameter(t)
+        got = call(leaf)
+        assert got.requires_grad and not want.requires_grad and torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="no backward"):
+            got.float().sum().backward()
+        with torch.no_grad():
+            got = call(leaf)
+        assert not got.requires_grad and torch.equal(got, want)
