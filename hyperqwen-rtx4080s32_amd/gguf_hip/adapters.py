@@ -82,7 +82,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     Returns a new tensor, or ``out`` (a [M, N] view with unit column stride), which may be y itself, or x.  No backward pass.
     ``workspace``: as mul_mat_grouped's (its own for calls on concurrent streams)."""
     what = "lora_add"
-    if _unwatched():
+    if _fast is not None and _unwatched():
         got = _fast.lora_add(y, x, a, b, ids, scales, n_outs, out, workspace)
         if got is not None:
             return got

@@ -135,7 +135,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Returns out [batch, query heads, dim], with ``return_lse`` also the log-sum-exp of its scores (fp32 [batch,
     query heads], -inf without a key), which joins attention over separate caches.  ``workspace``: as
     mul_mat_grouped's (its own for calls on concurrent streams).  No backward pass."""
-    if _unwatched():
+    if _fast is not None and _unwatched():
         got = _fast.paged_attention(q, k_pages, v_pages, block_table, lengths, scale, window, k_scale, v_scale, max_length, out,
                                     return_lse, workspace)
         if got is not None:
@@ -290,7 +290,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     cut from any graph."""
     what = "qk_norm_rope"
     flags = (_lib.GQK_ROPE_UNIT_OFFSET if unit_offset else 0) | (_lib.GQK_ROPE_INTERLEAVED if interleaved else 0)
-    if _unwatched():
+    if _fast is not None and _unwatched():
         got = _fast.qk_norm_rope(q, k, positions, table, q_weight, k_weight, eps, flags, v, k_pages, v_pages, slots, k_scale,
                                  v_scale, out_q, out_k)
         if got is not None:

@@ -250,7 +250,8 @@ def device_workspace(device: torch.device, need: int = 0) -> torch.Tensor:
             _REPLACED.append(ws)
         ws = torch.zeros((size + 3) // 4, dtype=torch.int32, device=torch.device("cuda", idx))
         _WORKSPACES[idx] = ws
-        _lib._fast.set_workspace(idx, ws)
+        if _lib._fast is not None:
+            _lib._fast.set_workspace(idx, ws)
     return ws
 
 

@@ -78,7 +78,7 @@ def copy_pages(pages: torch.Tensor, src, dst, dim: int = 0) -> None:
     arrays or CPU tensors); a page outside of the cache, written twice, or both read and written raises ValueError and
     nothing is copied.  Under HIP graph capture the pairs of the capture are recorded."""
     what = "copy_pages"
-    if _unwatched() and _fast.copy_pages(pages, src, dst, dim):
+    if _fast is not None and _unwatched() and _fast.copy_pages(pages, src, dst, dim):
         return
     ops._require_gpu(pages, what)
     dim = dim + pages.dim() if dim < 0 else dim

@@ -90,3 +90,32 @@ def test_gradients_of_results_that_are_written_into_a_tensor():
         gguf_hip.qk_norm_rope(**{**ro, "k": ro["k"].detach().clone().requires_grad_()}, v=_fake((5, 2, 64)), k_pages=cache,
                               v_pages=_fake((9, 16, 2, 64)), slots=_fake((5,), torch.int32))
         assert not cache.requires_grad
+
+
+def test_a_torch_that_does_not_load_the_module():
+    """The eager calls' module is built for one torch; without it the package is all there, with a warning."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import sys, warnings
+sys.modules["gguf_hip._fast"] = None                         # its import raises ImportError
+with warnings.catch_warnings(record=True) as seen:
+    warnings.simplefilter("always")
+    import gguf_hip
+assert [w.category for w in seen if "_fast" in str(w.message)] == [RuntimeWarning], seen
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+with FakeTensorMode():
+    e = lambda *s, dtype=torch.bfloat16: torch.empty(s, dtype=dtype, device="cuda")
+    i32 = lambda *s: e(*s, dtype=torch.int32)
+    assert gguf_hip.paged_attention(e(3, 8, 64), e(9, 16, 2, 64), e(9, 16, 2, 64), i32(3, 4), i32(3)).shape == (3, 8, 64)
+    assert gguf_hip.lora_add(e(4, 48), e(4, 64), e(3, 1, 16, 64), e(3, 48, 16), i32(4), None, [48]).shape == (4, 48)
+    assert gguf_hip.qk_norm_rope(e(5, 8, 64), None, i32(5), e(100, 32, dtype=torch.float32))[0].shape == (5, 8, 64)
+    gguf_hip.copy_pages(e(3, 9, 16), [0], [1], dim=1)
+print("done")
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100,
+                         env={**os.environ, "PYTHONPATH": os.pathsep.join(p for p in sys.path if p)})
+    assert run.returncode == 0 and run.stdout.strip() == "done", run.stderr[-2000:]

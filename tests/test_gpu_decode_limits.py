@@ -274,3 +274,27 @@ def test_gradients_raise_and_values_stay():
         with torch.no_grad():
             got = call(leaf)
         assert not got.requires_grad and torch.equal(got, want)
+
+
+# ---- without the eager calls' module ---------------------------------------------------------
+
+def test_calls_without_the_eager_module(monkeypatch):
+    """The same bits by way of Python."""
+    from gguf_hip import adapters, attention, pages as pages_py
+
+    gen = _gen(2)
+    y, x, a, b, ids = _lora_case(gen, 20, 64, (40,), 8, 2, BF)
+    k, v = (_randn(gen, 3, 16, 2, 64, dtype=BF) for _ in range(2))
+    table, lens = torch.zeros((4, 1), dtype=torch.int32, device="cuda"), torch.full((4,), 9, dtype=torch.int32, device="cuda")
+    q, pos, rope = _randn(gen, 4, 8, 64, dtype=BF), torch.arange(4, device="cuda"), gguf_hip.rope_table(64, 9, device="cuda")
+
+    def calls():
+        mine = k.clone()
+        gguf_hip.copy_pages(mine, [0], [2])
+        return (gguf_hip.lora_add(y, x, a, b, ids, None, (40,)), gguf_hip.paged_attention(q, k, v, table, lens),
+                gguf_hip.qk_norm_rope(q, None, pos, rope)[0], mine)
+
+    want = calls()
+    for module in (adapters, attention, pages_py, _lib):
+        monkeypatch.setattr(module, "_fast", None)
+    assert all(torch.equal(g, w) for g, w in zip(calls(), want)) and torch.equal(want[3][2], k[0])
