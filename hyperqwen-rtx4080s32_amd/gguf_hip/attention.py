@@ -337,7 +337,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
     args = (_heads_view(q, what), None if k is None else _heads_view(k, what), None if v is None else _heads_view(v, what),
             positions, table, q_weight, k_weight, float(eps), flags, slots, k_scale, v_scale, out_q, out_k, k_pages, v_pages)
-    if _direct(q, k, v, positions, table, q_weight, k_weight, slots, out_q, out_k, k_pages, v_pages):
+    if _direct(q, k, v, positions, table, q_weight, k_weight, slots, k_scale, v_scale, out_q, out_k, k_pages, v_pages):
         _rope_into(*args)
         for t in (out_q, out_k, k_pages, v_pages):
             if t is not None:

@@ -142,6 +142,24 @@ def test_attention_in_small_workspaces(batch, heads, hkv, dim):
         _within(gguf_hip.paged_attention(q, k, v, table, lens, workspace=ws), want, tol, size)
 
 
+# ---- norm, rotation, store -------------------------------------------------------------------
+
+def test_rope_scales_that_are_negated_lazily():
+    """Tensors whose memory is not their value go through the op, the pages' scales among them."""
+    gen = _gen(3)
+    q, k, v = (_randn(gen, 4, 2, 64, dtype=BF) for _ in range(3))
+    pos, rope = torch.arange(4, device="cuda"), gguf_hip.rope_table(64, 9, device="cuda")
+    ks, vs = torch.tensor([0.5, 2.0], device="cuda"), torch.tensor([0.25, 4.0], device="cuda")
+
+    def stored(ks, vs):
+        kp, vp = (torch.zeros((1, 4, 2, 64), dtype=F8, device="cuda") for _ in range(2))
+        gguf_hip.qk_norm_rope(q, k, pos, rope, v=v, k_pages=kp, v_pages=vp, slots=pos, k_scale=ks, v_scale=vs)
+        return kp.view(torch.uint8), vp.view(torch.uint8)
+
+    for got, want in zip(stored(torch._neg_view(-ks), torch._neg_view(-vs)), stored(ks, vs)):
+        assert torch.equal(got, want)
+
+
 # ---- adapters --------------------------------------------------------------------------------
 
 def _lora_case(gen, M, K, n_outs, rank, slots, dtype):
