@@ -53,6 +53,15 @@ __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c, f16_t) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// x without what T has no bits for
+__device__ __forceinline__ bf16_t toward_zero(float x, bf16_t) {
+  return __builtin_bit_cast(bf16_t, (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16 | (x != x ? 0x40 : 0)));   // NaN stays
+}
+__device__ __forceinline__ f16_t toward_zero(float x, f16_t) { return (f16_t)__builtin_amdgcn_cvt_pkrtz(x, x)[0]; }
+// what T still holds beside a value, and which adds nothing to it that shows (0 beside 0); fp16 values are below 2 here
+__device__ __forceinline__ float least_beside(float x, bf16_t) { return fabsf(x) * 0x1p-20f; }
+__device__ __forceinline__ float least_beside(float x, f16_t) { return fminf(fabsf(x) * 0x1p30f, 0x1p-24f); }
+
 // Rows of one block that go with one adapter (or with none, kNone, or a bad id, kBad).
 struct Unit {
   int adapter, count;
@@ -237,8 +246,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
 
 // out = y + s B h of one unit's rows and `columns` columns of one part.  The ranks that h has in 32 bits go into the
 // product as two values of T each, h = hi + lo, in one instruction: 16 ranks of hi and the same 16 of lo against B's 16
-// ranks twice (rounding h to T alone would put 2^-9 of the update, for bf16, on top of the output's own rounding; the second
-// half of the instruction would be idle).  fp16 takes h over a power of two near its row's largest, to stay in range.
+// ranks twice (rounding h to T alone would put up to 2^-8 of the update, for bf16, on top of the output's own rounding; the second
+// half of the instruction would be idle).  hi is cut off, not rounded, so that both have h's sign, which costs lo a bit: what is left of h's
+// error is 2^-16 for bf16, 2^-22 for fp16.  fp16 takes h over a power of two near its row's largest, to stay in range.
 //
 // A wave takes 64 columns at a time by itself: their rows of B come in as one run of memory (EACH 16-byte pieces of
 // a column, 8 EACH ranks at a time) and turn into operands in the wave's LDS, and the update goes back through the same LDS to
@@ -362,12 +372,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
       float down = 1.f, up = 1.f, top = 0.f;
       auto seen = [&](const float (&v)[8]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]) < __builtin_huge_valf() ? fabsf(v[e]) : 0.f);
       };
-      auto fit = [&]() {   // a power of two near the row's largest
+      auto fit = [&]() {   // a power of two near the row's largest finite one
         if constexpr (kF16) {
           for (int o = kRowThreads / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-          if (top > 0.f && top < __builtin_huge_valf()) {
+          if (top > 0.f) {
             const int e = min(max(ilogbf(top), -100), 100);
             down = ldexpf(1.f, -e);
             up = ldexpf(1.f, e);
@@ -380,9 +390,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float x = v[e] * down;
-          hi[e] = (T)x;
+          hi[e] = toward_zero(x, T{});
           const float back = (float)hi[e];
-          lo[e] = fabsf(back) < __builtin_huge_valf() ? (T)(x - back) : (T)0.f;   // inf stays, without inf - inf
+          // of x's sign and not 0 where x is not: an infinite weight times both is one infinity, and so is a weight times infinite ones
+          const float rest = fabsf(back) < __builtin_huge_valf() ? x - back : back;
+          lo[e] = (T)copysignf(fmaxf(fabsf(rest), least_beside(back, T{})), x);
         }
         __builtin_memcpy(hs + r * hrow + at, hi, 16);
         __builtin_memcpy(hs + (kRows + r) * hrow + at, lo, 16);

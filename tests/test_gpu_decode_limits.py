@@ -229,6 +229,39 @@ def test_lora_more_rows_than_a_launch_takes():
     _within(gguf_hip.lora_add(y, x, a, b, ids, None, (8,)), want, tol, M)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("rows", [1, 20, 300])
+@pytest.mark.parametrize("rank", [8, 32, 72, 256])
+def test_lora_infinite_weights(dtype, rows, rank):
+    """An infinity in B reaches its column with its sign times h's, whatever h's value rounds to: no inf - inf of h's two terms."""
+    gen = _gen(rows)
+    y, x, a, b, ids = _lora_case(gen, rows, 64, (40,), rank, 2, dtype)
+    ids[:] = 0
+    x[0] = 0
+    x[0, 0] = 1.0
+    a[:, :, :, 0] = 0.5                                      # row 0's h is 0.5 exactly: one term holds it
+    b[0, 3, 2], b[0, 7, rank - 1] = float("inf"), float("-inf")
+    out = gguf_hip.lora_add(y, x, a, b, ids, None, (40,))
+    want, tol = _lora_exact(y, x, a, b, ids, (40,))
+    whole = [c for c in range(40) if c not in (3, 7)]
+    assert want[:, [3, 7]].isinf().all() and torch.equal(out[:, [3, 7]].double(), want[:, [3, 7]])
+    _within(out[:, whole], want[:, whole], tol[:, whole], rows)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("rows", [1, 20, 300])
+@pytest.mark.parametrize("rank", [8, 32, 72, 256])
+def test_lora_an_infinite_rank_beside_large_ones(dtype, rows, rank):
+    """One rank's h is infinite, the others' are finite and beyond fp16: they do not cancel it."""
+    y, x, a, b, ids = _lora_case(_gen(rows), rows, 64, (40,), rank, 2, dtype)
+    ids[:] = 0
+    x, a = x * 1000, a * 1000
+    a[0, 0, 3, 5] = float("inf")
+    out = gguf_hip.lora_add(y, x, a, b, ids, None, (40,))
+    want, _ = _lora_exact(y, x, a, b, ids, (40,))
+    assert want.isinf().all() and torch.equal(out.double(), want)
+
+
 # ---- page copies -----------------------------------------------------------------------------
 
 def test_copy_pages_traced_and_watched():
