@@ -148,14 +148,14 @@ struct Joined {
 // each of its 8 keys and transposes the 8 x 8 block in registers, one v_perm per pair.  No barrier in the loop, and no LDS but for
 // the queries of 256 dims.
 //
-// Scores, statistics and sums are in 32 bits; the probabilities become T for the second product (at most 2^-9 of each for bf16, as
+// Scores, statistics and sums are in 32 bits; the probabilities become T for the second product (up to 2^-8 of each for bf16, as
 // random as the output's own rounding: 1.9e-3 of error against 64 bits where the output's rounding alone has 1.7e-3), two terms
 // of T would need twice the instructions.  8-bit keys and values widen to T exactly, their scales go
 // into the score's and the output's factor.
 //
 // Memory bounds it: 2.6 GB of bf16 keys and values (128 sequences of up to 8000) 406 us, 6.5 TB/s; 330 MB (32 of up to 4000)
-// 61.8 us, 5.3 TB/s; fp16 heads of 256 dims under a window, 1.5 GB, 253 us, 5.8 TB/s; 268 MB of 8-bit pages of one sequence
-// 47 us and 6 for the join.  A sequence of 61 keys takes 4.8 us: a launch, and lengths, table and keys read one after the other.
+// 61.8 us, 5.3 TB/s; fp16 heads of 256 dims under a window, 1.5 GB, 245 us, 6.0 TB/s; 268 MB of 8-bit pages of one sequence
+// 47 us and 6 for the join.  A sequence of 61 keys takes 5.3 us: a launch, and lengths, table and keys read one after the other.
 template <typename T, typename C, int DP, bool FULL, bool P8, bool TIGHT>
 __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kernel(AttnArgs a) {
   constexpr bool F8 = sizeof(C) == 1;
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
 }
 
 // The join of more splits than one workgroup takes at once: a workgroup for each query head, its threads over the splits and
-// the dims.  (One workgroup per sequence and key head took 16 us for 64 splits of 5 heads, 39 for 128 of 16.)  96 splits of 40 heads: 5.8 us,
+// the dims.  (One workgroup per sequence and key head took 16 us for 64 splits of 5 heads, 39 for 128 of 16.)  96 splits of 40 heads: 6.1 us,
 // of which a launch that waits for another takes about half.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void attention_join_kernel(AttnArgs a) {
@@ -608,7 +608,8 @@ Cut cut_of(int batch, int q_heads, int kv_heads, int dim, int size, int max_leng
 }
 
 // The general form takes any head dim up to DP and any page size; whole heads (FULL), pages of a multiple of 8 tokens (P8)
-// and pages that are one run of memory (TIGHT) have fewer addresses to compute, the last one for each step.
+// and pages that are one run of memory (TIGHT) have fewer addresses to compute, the last one for each step.  Bound by memory like them:
+// 32 x 4000 of 80 dims 45.8 us (4.5 TB/s), of 192 dims 106 us (4.6); of 128 dims in pages of 7 tokens 63.9, of 16 61.8.
 template <typename T, typename C, int DP>
 void launch(const AttnArgs& a, dim3 grid, bool full, hipStream_t st) {
   const bool p8 = a.kv.page_size % 8 == 0, tight = a.kv.k_token == DP && a.kv.v_token == DP;

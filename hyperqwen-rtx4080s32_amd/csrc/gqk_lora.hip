@@ -22,7 +22,8 @@ constexpr int kStage = 128;      // values of K that the first kernel takes at a
 constexpr int kList = 64;        // rows of a unit, at most
 // A workgroup sorts out the adapters of a block of 64 Q rows, Q ids to a lane.  Batches of up to kSmall rows are one block (Q 1
 // or 4), so that each adapter is read once for its rows wherever they are, in units of 16; longer ones (prompts, whose
-// rows come in runs) go by 64 rows and units of up to 64.
+// rows come in runs) go by 64 rows and units of up to 64.  Long batches whose rows come mixed are right but slow, as a block's units after the
+// first wait for one another: to q, k and v of 5120 values, 32 adapters of rank 16, 256 rows 39 us, 257 158, 512 205, but 36 sorted by adapter.
 constexpr int kSmall = 256;
 constexpr int kRankTiles = 4;    // 16-rank tiles of a workgroup of the first kernel
 constexpr int kRowColumns = 64 * kWaves;
@@ -143,9 +144,9 @@ __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset
 // ranks (TT = 4), or all 16 rows and one 16-rank tile (TT = 1).  x goes by once and leaves the caches first, so that A, which every
 // block of rows reads again, stays (4096 rows of 17408 values 82.4 -> 78.1 us, both launches).
 //
-// 4096 rows of 17408 values, rank 64: 34 us, 4.2 TB/s of x, near what a copy reaches (4.75).  Without any load it takes
+// 4096 rows of 17408 values, rank 64: 35 us, 4.1 TB/s of x, near what a copy reaches (4.75).  Without any load it takes
 // 21: LDS, the barriers and the issue of each stage, beside which the loads go on (loads 4 stages ahead cost 1.4 us more, two workgroups a CU 2.6, blocks of
-// 128 rows 9; eight waves with half of each stage change nothing).  48 rows of 5120, 12 adapters of rank 32: 6.7 us, a launch, ids, one trip to memory,
+// 128 rows 9; eight waves with half of each stage change nothing).  48 rows of 5120, 12 adapters of rank 32: 6.6 us, a launch, ids, one trip to memory,
 // partial sums out.
 template <typename T, int TT, int Q>
 __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
@@ -259,8 +260,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_down_kernel(LoraArgs a) {
 // one XCD and near in time (dealt by columns: 4096 rows of 17408 values 83.9 -> 81.9 us, 8192 of 5120 to three parts 93.0 -> 85.7,
 // both launches).
 //
-// 4096 rows of 5120 columns, rank 64: 30 us for 84 MB of y and out; 18 us of it go by at memory's rate, the first 9 to 12 are the
-// launch, the ids and h on their way.  48 rows of 34816 columns, 12 adapters of rank 32: 14.2 us, of which B, y and out (33 MB) take 6.
+// 4096 rows of 5120 columns, rank 64: 32 us for 84 MB of y and out; 18 us of it go by at memory's rate, the first 9 to 14 are the
+// launch, the ids and h on their way.  48 rows of 34816 columns, 12 adapters of rank 32: 14.4 us, of which B, y and out (33 MB) take 7 at a copy's
+// rate; before them go the ids, the ballots and the gather of h, and each wave then has four strips of 64 columns in turn, one on its way.
 template <typename T, int TT, int Q, int EACH>
 __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
   constexpr bool kF16 = __is_same(T, f16_t);
@@ -506,7 +508,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void lora_up_kernel(LoraArgs a) {
 // ranks: each lane 8 values of K at a time of every rank's row and of x (whole runs of 1 KiB), products and sums in 32
 // bits, the 64 lanes' sums through LDS in fours.  Then a thread has a column: B's row of it, read at the start, times h in 32
 // bits.  A is read by every workgroup of its part, from the caches, which is cheap while a launch leaves CUs idle anyway; it saves
-// the second launch and its wait for the first.  One row of 5120 values to q, k and v, rank 16: 6.9 us (two launches 9.4), of which
+// the second launch and its wait for the first.  One row of 5120 values to q, k and v, rank 16: 7.2 us (two launches 9.4), of which
 // a launch takes 2 and 164 KiB of A through one CU 3.
 template <typename T, int RW>
 __global__ __launch_bounds__(64 * kWaves, 2) void lora_row_kernel(LoraArgs a) {

@@ -1,5 +1,5 @@
 // gqk_pages.hip - copies of a cache's pages: in every plane (each layer's keys and values), page
-// src[i] to page dst[i], all pairs in one launch.
+// src[i] to page dst[i], one launch for each 448 pairs (and each 32768 planes).
 #include <new>
 #include <vector>
 #include "gqk_decode.h"

@@ -1,5 +1,5 @@
 """The pages of a key-value cache: which are free, shared or a sequence's own (``PagePool``, on the host), and the
-copies between them on the GPU (``copy_pages``, one launch for all pairs and all layers)."""
+copies between them on the GPU (``copy_pages``, one launch for each 448 pairs, of all layers)."""
 from __future__ import annotations
 
 import heapq
@@ -72,7 +72,7 @@ def _(pages, src, dst, dim):
 
 
 def copy_pages(pages: torch.Tensor, src, dst, dim: int = 0) -> None:
-    """pages[..., dst[i], ...] = pages[..., src[i], ...] for every i along dimension ``dim``, in place, in one launch:
+    """pages[..., dst[i], ...] = pages[..., src[i], ...] for every i along dimension ``dim``, in place, one launch for each 448 pairs:
     ``pages`` is a cache's whole storage (any type), the page's own dimensions after ``dim`` contiguous, the dimensions
     before it (layers; keys and values) evenly spaced.  src and dst are page numbers on the host (lists,
     arrays or CPU tensors); a page outside of the cache, written twice, or both read and written raises ValueError and
