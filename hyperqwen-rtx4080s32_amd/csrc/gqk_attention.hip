@@ -4,7 +4,7 @@
 //
 // over the keys j in [max(0, length - window), length) of the sequence; no key: zeros.
 #include <algorithm>
-#include "gqk_decode.h"
+#include "gqk_attend.h"
 
 namespace gqk {
 
@@ -43,28 +43,16 @@ int check_pages(const char* what, const gqk_pages* p, int q_dtype) {
 
 namespace {
 
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-
 constexpr int kWaves = 4;             // waves of a workgroup
 constexpr int kTile = 32;             // keys of a wave's step
 constexpr int kJoinSplits = 16;       // splits that the last workgroup of a sequence joins, at most
 constexpr int kMostSplits = 256;
-// A weight is 2^(score - maximum + kLift): fp16 uses its whole range, so that weights keep their relative precision down to 2^-29 of
-// the heaviest and none is lost above 2^-40 (not lifted they do to 2^-14, and a long flat tail of them, each lighter than that, lost
-// up to all of its weight).  bf16 has fp32's exponents.
-template <typename T> constexpr float kLift = __is_same(T, f16_t) ? 15.f : 0.f;
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-
 struct AttnArgs {
   const void* q;
   int64_t q_row, q_head;
   gqk_pages kv;
   const int32_t* table;
-  int64_t table_row;
+  int64_t table_row, table_head;   // (0: one table for all heads)
   const int32_t* lengths;
   void* out;
   int64_t out_row, out_head;
@@ -88,24 +76,6 @@ __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c, f16_t) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// two e4m3 values (bytes 0, 1 or 2, 3 of x) as two values of T, exactly
-template <bool HI> __device__ __forceinline__ uint32_t widen(uint32_t x, bf16_t) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, HI));
-}
-template <bool HI> __device__ __forceinline__ uint32_t widen(uint32_t x, f16_t) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.f, HI));
-}
-template <typename T> __device__ __forceinline__ v4u widen8(uint32_t lo, uint32_t hi) {
-  return v4u{widen<false>(lo, T{}), widen<true>(lo, T{}), widen<false>(hi, T{}), widen<true>(hi, T{})};
-}
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  typedef T v2 __attribute__((ext_vector_type(2)));
-  v2 p;
-  p[0] = (T)lo;
-  p[1] = (T)hi;
-  return __builtin_bit_cast(uint32_t, p);
-}
-
 // max and sum over the four lanes of a query head (lane, lane ^ 16, lane ^ 32, lane ^ 48)
 __device__ __forceinline__ float max4(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
@@ -115,27 +85,6 @@ __device__ __forceinline__ float sum4(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
 }
-
-// Splits of `chunk` keys of the keys [start, len), one at least.  (len - start + chunk can pass 31 bits where the sequence is long.)
-__device__ __forceinline__ int splits_of(int start, int len, int chunk) { return len > start ? (len - start - 1) / chunk + 1 : 1; }
-
-// The exponent's base of a running maximum: nothing was seen yet (-inf) must not become -inf - -inf.
-__device__ __forceinline__ float base_of(float m) { return m == -__builtin_huge_valf() ? 0.f : m; }
-
-// Partial sums over a split's keys, relative to its maximum (both lifted alike), added up in order.
-struct Joined {
-  float m = -__builtin_huge_valf(), l = 0.f;
-  v4f o{0.f, 0.f, 0.f, 0.f};
-  __device__ __forceinline__ void add(v2u stat, v4u sums) {
-    float s[2];
-    __builtin_memcpy(s, &stat, 8);
-    const float mn = fmaxf(m, s[0]), mb = base_of(mn);
-    const float f = __builtin_amdgcn_exp2f(m - mb), g = __builtin_amdgcn_exp2f(s[0] - mb);
-    m = mn;
-    l = l * f + s[1] * g;
-    o = o * f + __builtin_bit_cast(v4f, sums) * g;
-  }
-};
 
 // A workgroup takes one split (a.chunk keys) of one sequence's keys of one key head, for up to 16 row_waves query heads
 // that share it; its waves deal the 32-key steps of the split (and the 16-row tiles of the heads) among themselves.
@@ -198,7 +147,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 2 : 3) void attention_kern
   bool bad = false;
 
   if (steps > 0) {
-    const int32_t* table = a.table + (int64_t)b * a.table_row;
+    const int32_t* table = a.table + (int64_t)b * a.table_row + kvh * a.table_head;
     const char* kb = (const char*)a.kv.k + kvh * a.kv.k_head * (int64_t)sizeof(C);
     const char* vb = (const char*)a.kv.v + kvh * a.kv.v_head * (int64_t)sizeof(C);
     const uint32_t k_page = (uint32_t)a.kv.k_page * sizeof(C), k_tok = TIGHT ? RB : (uint32_t)a.kv.k_token * sizeof(C);
@@ -648,10 +597,10 @@ int64_t gqk_paged_attention_workspace_bytes(int batch, int q_heads, int kv_heads
   return c.splits > 1 ? GQK_CTR_BYTES + units * rows * c.splits * (dim + 4) * 4 : 0;
 }
 
-int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype, int batch, int q_heads,
-                        const gqk_pages* pages, const int32_t* table, int64_t table_row, int table_width,
-                        const int32_t* lengths, int max_length, int window, float scale, void* out, int64_t out_row,
-                        int64_t out_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+int gqk_paged_attention_heads(const void* q, int64_t q_row, int64_t q_head, int dtype, int batch, int q_heads,
+                              const gqk_pages* pages, const int32_t* table, int64_t table_row, int64_t table_head, int table_width,
+                              const int32_t* lengths, int max_length, int window, float scale, void* out, int64_t out_row,
+                              int64_t out_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   if (dtype != GQK_DTYPE_BF16 && dtype != GQK_DTYPE_F16) return decode_fail(GQK_ERR_ARG, "paged_attention: dtype %d", dtype);
   if (const int rc = check_pages("paged_attention", pages, dtype)) return rc;
   if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads % pages->heads)
@@ -669,18 +618,15 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
   if (c.splits > 1 && (uintptr_t)workspace & 255)
     return decode_fail(GQK_ERR_SHAPE, "paged_attention: workspace is not 256-byte aligned");
   AttnArgs a{};
-  a.q = q; a.q_row = q_row; a.q_head = q_head; a.kv = *pages; a.table = table; a.table_row = table_row; a.lengths = lengths;
+  a.q = q; a.q_row = q_row; a.q_head = q_head; a.kv = *pages; a.table = table; a.table_row = table_row; a.table_head = table_head; a.lengths = lengths;
   a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.q_heads = q_heads; a.max_length = max_length;
   a.window = window; a.scale = scale * kLog2e; a.row_waves = c.row_waves; a.row_blocks = c.row_blocks; a.chunk = c.chunk;
   a.splits = c.splits;
   a.counters = (int*)workspace;
   a.partials = workspace ? (float*)((char*)workspace + GQK_CTR_BYTES) : nullptr;
-  // key / page_size for keys below 2^31: 2^(31 + bits) / page_size rounded up fits 32 bits, its excess times a key stays
-  // below 2^(31 + bits)
-  int bits = 0;
-  while (((int64_t)1 << bits) < pages->page_size) ++bits;
-  a.shift = bits;
-  a.magic = (uint32_t)((((uint64_t)1 << (31 + bits)) + pages->page_size - 1) / pages->page_size);
+  const PageDivisor by = page_divisor(pages->page_size);
+  a.magic = by.magic;
+  a.shift = by.shift;
   // one workgroup joins up to 16 splits, of heads that its threads go over twice at most (in a launch of their own and in it: 32 heads
   // of 128 dims over one, 8 x 4000, 15.7 us and 21.3; 16 heads, two rounds, 16 x 2000, 17.9 and 16.6)
   a.join_apart = c.splits > kJoinSplits ||
@@ -707,6 +653,14 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
     }
   }
   return decode_launched("paged_attention");
+}
+
+int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype, int batch, int q_heads,
+                        const gqk_pages* pages, const int32_t* table, int64_t table_row, int table_width,
+                        const int32_t* lengths, int max_length, int window, float scale, void* out, int64_t out_row,
+                        int64_t out_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  return gqk_paged_attention_heads(q, q_row, q_head, dtype, batch, q_heads, pages, table, table_row, 0, table_width, lengths, max_length,
+                                   window, scale, out, out_row, out_head, lse, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -98,6 +98,28 @@ bool index_of(const Tensor& t, int64_t n, const Tensor& ref) {
          same_device(ref, &t);
 }
 
+// contiguous int32 [n]
+bool i32_of(const Tensor& t, int64_t n, const Tensor& ref) {
+  return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous() && same_device(ref, &t);
+}
+
+// a page table of so many dimensions: int32, its columns side by side
+bool table_of(const Tensor& t, int64_t dims, int64_t batch, const Tensor& ref) {
+  return t.scalar_type() == at::kInt && t.dim() == dims && t.size(0) == batch && same_device(ref, &t) && t.size(-1) <= 0x7fffffff &&
+         (t.size(-1) <= 1 || t.stride(-1) == 1);
+}
+
+// a Python integer of 0 .. 2^31 - 1
+bool int_of(PyObject* o, int64_t* to) {
+  if (!PyLong_CheckExact(o)) return false;
+  *to = PyLong_AsLongLong(o);
+  if (PyErr_Occurred()) {   // beyond 64 bits
+    PyErr_Clear();
+    return false;
+  }
+  return *to >= 0 && *to <= 0x7fffffff;
+}
+
 bool here(const Tensor& t) { return t.get_device() < kDevices && c10::hip::current_device() == t.get_device(); }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
@@ -130,11 +152,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (type < 0 || !here(*q) || !heads_of(q, &qh) || !pages_of(*k, *v, ks, vs, *q, &p)) return none();
   const int64_t batch = q->size(0), heads = q->size(1), dim = q->size(2);
   if (batch < 1 || batch > 65535 || heads < 1 || heads % p.heads) return none();
-  if (table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) != batch || !same_device(*q, table) ||
-      (table->size(1) > 1 && table->stride(1) != 1) || table->size(1) > 0x7fffffff || lengths->scalar_type() != at::kInt ||
-      lengths->dim() != 1 || lengths->size(0) != batch || !lengths->is_contiguous() || !same_device(*q, lengths))
-    return none();
-  const int64_t room = std::min<int64_t>(table->size(1) * p.page_size, GQK_MAX_KEYS);
+  const bool by_head = table->dim() == 3;   // a table for each of the pages' heads
+  if (by_head && table->size(1) != p.heads) return none();
+  if (!table_of(*table, by_head ? 3 : 2, batch, *q) || !i32_of(*lengths, batch, *q)) return none();
+  const int64_t width = table->size(-1), room = std::min<int64_t>(width * p.page_size, GQK_MAX_KEYS);
   int64_t window = 0, most = room;
   double scale = 1.0 / sqrt(static_cast<double>(dim));
   if (!PyLong_CheckExact(a[6])) return none();
@@ -162,16 +183,212 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const bool with_lse = a[11] == Py_True;
   if (with_lse) lse = at::empty({batch, heads}, q->options().dtype(at::kFloat));
-  const int rc = gqk_paged_attention(qh.data, qh.row, qh.head, type, static_cast<int>(batch), static_cast<int>(heads), &p,
-                                     table->data_ptr<int>(), table->stride(0), static_cast<int>(table->size(1)),
-                                     lengths->data_ptr<int>(), static_cast<int>(most), static_cast<int>(window),
-                                     static_cast<float>(scale), oh.data, oh.row, oh.head, with_lse ? lse.data_ptr<float>() : nullptr,
-                                     space, bytes, stream_of(*q));
+  const int rc = gqk_paged_attention_heads(
+      qh.data, qh.row, qh.head, type, static_cast<int>(batch), static_cast<int>(heads), &p, table->data_ptr<int>(), table->stride(0),
+      by_head ? table->stride(1) : 0, static_cast<int>(width), lengths->data_ptr<int>(), static_cast<int>(most), static_cast<int>(window),
+      static_cast<float>(scale), oh.data, oh.row, oh.head, with_lse ? lse.data_ptr<float>() : nullptr, space, bytes, stream_of(*q));
   if (rc) return none();   // nothing was launched: the Python path says why
   PyObject* result = out ? (Py_INCREF(a[10]), a[10]) : THPVariable_Wrap(made);
   written(out ? *out : made);
   if (!with_lse) return result;
   return Py_BuildValue("(NN)", result, THPVariable_Wrap(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// tree_attention(q, k_pages, v_pages, block_table, lengths, starts, mask, scale, window, k_scale, v_scale, max_length, max_tokens, out,
+// return_lse, workspace)
+PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *q, *k, *v, *table, *lengths, *starts, *mask, *ks, *vs, *out, *ws;
+  if (n != 16 || !plain_world() || !plain(a[0], &q) || !plain(a[1], &k) || !plain(a[2], &v) || !plain(a[3], &table) ||
+      !plain(a[4], &lengths) || !plain(a[5], &starts) || !plain_or_none(a[6], &mask) || !plain_or_none(a[9], &ks) ||
+      !plain_or_none(a[10], &vs) || !plain_or_none(a[13], &out) || !plain_or_none(a[15], &ws))
+    return none();
+  gqk_heads qh, oh;
+  gqk_pages p;
+  const int type = heads_type(q->scalar_type());
+  if (type < 0 || !here(*q) || !heads_of(q, &qh) || !pages_of(*k, *v, ks, vs, *q, &p) || lengths->dim() != 1) return none();
+  const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), batch = lengths->size(0);
+  if (batch < 1 || batch > 65535 || tokens < 1 || tokens > GQK_MAX_TOKENS || heads < 1 || heads % p.heads || heads / p.heads > GQK_MAX_GROUP)
+    return none();
+  if (!table_of(*table, 2, batch, *q) || !i32_of(*lengths, batch, *q) || !i32_of(*starts, batch + 1, *q)) return none();
+  if (mask && (mask->scalar_type() != at::kInt || mask->dim() != 2 || mask->size(0) != tokens || mask->size(1) < 1 ||
+               mask->size(1) > 0x7fffffff || !mask->is_contiguous() || !same_device(*q, mask)))
+    return none();
+  const int64_t room = std::min<int64_t>(table->size(1) * p.page_size, GQK_MAX_KEYS);
+  int64_t window, most = room, most_tokens = tokens;
+  double scale = 1.0 / sqrt(static_cast<double>(dim));
+  if (!int_of(a[8], &window) || (a[11] != Py_None && !int_of(a[11], &most)) || most > room ||
+      (a[12] != Py_None && !int_of(a[12], &most_tokens)))
+    return none();
+  most_tokens = std::min(most_tokens, tokens);
+  if (a[7] != Py_None) {
+    if (!PyFloat_CheckExact(a[7])) return none();
+    scale = PyFloat_AS_DOUBLE(a[7]);
+  }
+  void* space;
+  int64_t bytes;
+  if (!workspace_of(ws, *q, &space, &bytes) || (out && (!like(*out, *q) || !heads_of(out, &oh)))) return none();
+  Tensor made, lse;
+  if (!out) {
+    made = at::empty({tokens, heads, dim}, q->options());
+    heads_of(&made, &oh);
+  }
+  const bool with_lse = a[14] == Py_True;
+  if (with_lse) lse = at::empty({tokens, heads}, q->options().dtype(at::kFloat));
+  const int rc = gqk_tree_attention(
+      qh.data, qh.row, qh.head, type, static_cast<int>(tokens), static_cast<int>(batch), static_cast<int>(heads), &p, table->data_ptr<int>(),
+      table->stride(0), static_cast<int>(table->size(1)), lengths->data_ptr<int>(), starts->data_ptr<int>(),
+      mask ? mask->data_ptr<int>() : nullptr, mask ? static_cast<int>(mask->size(1)) : 0, static_cast<int>(most),
+      static_cast<int>(most_tokens), static_cast<int>(window), static_cast<float>(scale), oh.data, oh.row, oh.head,
+      with_lse ? lse.data_ptr<float>() : nullptr, space, bytes, stream_of(*q));
+  if (rc) return none();
+  PyObject* result = out ? (Py_INCREF(a[13]), a[13]) : THPVariable_Wrap(made);
+  written(out ? *out : made);
+  if (!with_lse) return result;
+  return Py_BuildValue("(NN)", result, THPVariable_Wrap(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// add_rms_norm(x, residual, weight, eps, flags, f8, group, out, out_residual): (out, residual), or with f8 (out, scale, residual)
+PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *r, *w, *out, *rout;
+  int64_t group;
+  if (n != 9 || !plain_world() || !plain(a[0], &x) || !plain_or_none(a[1], &r) || !plain_or_none(a[2], &w) || !PyFloat_CheckExact(a[3]) ||
+      !PyLong_CheckExact(a[4]) || !int_of(a[6], &group) || !plain_or_none(a[7], &out) || !plain_or_none(a[8], &rout))
+    return none();
+  const int type = heads_type(x->scalar_type());
+  const bool f8 = a[5] == Py_True;
+  if (type < 0 || !here(*x) || x->dim() != 2 || (f8 && out)) return none();   // (an 8-bit out may share memory: the Python path looks)
+  const int64_t rows = x->size(0), dim = x->size(1);
+  if (rows < 1 || rows > 0x7fffffff || dim < 1 || dim > GQK_NORM_MAX_DIM || (group && dim % group) || (!r && rout)) return none();
+  for (const Tensor* t : {x, r, out, rout})
+    if (t && (!like(*t, *x) || (dim > 1 && t->stride(1) != 1) || (rows > 1 && t->stride(0) < dim))) return none();
+  if (w && (w->dim() != 1 || w->size(0) != dim || (w->scalar_type() != x->scalar_type() && w->scalar_type() != at::kFloat) ||
+            !w->is_contiguous() || !same_device(*x, w)))
+    return none();
+  Tensor made, scale, made_r;
+  if (!out) made = at::empty({rows, dim}, f8 ? x->options().dtype(at::kFloat8_e4m3fn) : x->options());
+  if (f8) scale = at::empty({rows, group ? dim / group : 1}, x->options().dtype(at::kFloat));
+  if (r && !rout) made_r = at::empty({rows, dim}, x->options());
+  auto row = [&](const Tensor* t) { return rows > 1 ? t->stride(0) : dim; };
+  const Tensor *to = out ? out : &made, *to_r = rout ? rout : r ? &made_r : nullptr;
+  const int rc = gqk_add_rms_norm(x->data_ptr(), row(x), r ? r->data_ptr() : nullptr, r ? row(r) : 0, type, rows, static_cast<int>(dim),
+                                  w ? w->data_ptr() : nullptr, w && w->scalar_type() == at::kFloat ? GQK_DTYPE_F32 : type,
+                                  static_cast<float>(PyFloat_AS_DOUBLE(a[3])), static_cast<int>(PyLong_AsLong(a[4])), to->data_ptr(),
+                                  row(to), f8 ? GQK_DTYPE_FP8 : type, f8 ? scale.data_ptr<float>() : nullptr, static_cast<int>(group),
+                                  to_r ? to_r->data_ptr() : nullptr, to_r ? row(to_r) : 0, stream_of(*x));
+  if (rc) return none();
+  for (const Tensor* t : {out, rout})
+    if (t) written(*t);
+  PyObject* first = out ? (Py_INCREF(a[7]), a[7]) : THPVariable_Wrap(made);
+  PyObject* last = rout ? (Py_INCREF(a[8]), a[8]) : r ? THPVariable_Wrap(made_r) : none();
+  if (!f8) return Py_BuildValue("(NN)", first, last);
+  return Py_BuildValue("(NNN)", first, THPVariable_Wrap(scale), last);
+  END_HANDLE_TH_ERRORS
+}
+
+// step_tables(page_lists, requests, lengths, counts, tokens, page_size, parents, tree): StepTables' fields
+PyObject* tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *lists, *requests, *lengths, *counts, *parents;
+  int64_t tokens, page_size, tree;
+  if (n != 8 || !plain_world() || !plain(a[0], &lists) || !plain(a[1], &requests) || !plain(a[2], &lengths) || !plain(a[3], &counts) ||
+      !int_of(a[4], &tokens) || !int_of(a[5], &page_size) || !plain_or_none(a[6], &parents) || !int_of(a[7], &tree))
+    return none();
+  if (!here(*lists) || lists->scalar_type() != at::kInt || lists->dim() != 2 || lists->size(0) > 0x7fffffff || lists->size(1) > 0x7fffffff ||
+      (lists->size(1) > 1 && lists->stride(1) != 1) || (lists->size(0) > 1 && lists->stride(0) < lists->size(1)) || requests->dim() != 1)
+    return none();
+  const int64_t batch = requests->size(0), width = lists->size(1);
+  if (batch > 65535 || !index_of(*requests, batch, *lists) || !i32_of(*lengths, batch, *lists) || !i32_of(*counts, batch, *lists) ||
+      (parents && !i32_of(*parents, tokens, *lists)) || (parents != nullptr) != (tree > 0) || tree > GQK_MAX_TREE)
+    return none();
+  const auto i32 = lists->options();
+  Tensor table = at::empty({batch, width}, i32), totals = at::empty({batch}, i32), starts = at::empty({batch + 1}, i32),
+         sequences = at::empty({tokens}, i32), positions = at::empty({tokens}, i32), slots = at::empty({tokens}, i32.dtype(at::kLong)), mask;
+  if (tree) mask = at::empty({tokens, (tree + 31) / 32}, i32);
+  const int rc = gqk_step_tables(lists->data_ptr<int>(), lists->size(0) > 1 ? lists->stride(0) : width, static_cast<int>(lists->size(0)),
+                                 static_cast<int>(width), requests->data_ptr(), requests->scalar_type() == at::kLong,
+                                 lengths->data_ptr<int>(), counts->data_ptr<int>(), static_cast<int>(batch), static_cast<int>(tokens),
+                                 static_cast<int>(page_size), parents ? parents->data_ptr<int>() : nullptr, static_cast<int>(tree),
+                                 table.data_ptr<int>(), totals.data_ptr<int>(), starts.data_ptr<int>(), sequences.data_ptr<int>(),
+                                 positions.data_ptr<int>(), slots.data_ptr<int64_t>(), tree ? mask.data_ptr<int>() : nullptr,
+                                 stream_of(*lists));
+  if (rc) return none();
+  return Py_BuildValue("(NNNNNNN)", THPVariable_Wrap(table), THPVariable_Wrap(totals), THPVariable_Wrap(starts), THPVariable_Wrap(sequences),
+                       THPVariable_Wrap(positions), THPVariable_Wrap(slots), tree ? THPVariable_Wrap(mask) : none());
+  END_HANDLE_TH_ERRORS
+}
+
+// page_bounds(k_pages, block_table, lengths, bounds, count): True when done
+PyObject* bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *k, *table, *lengths, *to;
+  int64_t count;
+  if (n != 5 || !plain_world() || !plain(a[0], &k) || !plain(a[1], &table) || !plain(a[2], &lengths) || !plain(a[3], &to) ||
+      !int_of(a[4], &count) || !here(*k) || k->dim() != 4 || k->numel() == 0 || k->stride(3) != 1 || lengths->dim() != 1)
+    return none();
+  const int type = k->scalar_type() == at::kFloat8_e4m3fn ? GQK_DTYPE_FP8 : heads_type(k->scalar_type());
+  const int64_t batch = lengths->size(0);
+  if (type < 0 || batch > 65535 || !table_of(*table, 2, batch, *k) || !i32_of(*lengths, batch, *k) || to->scalar_type() != k->scalar_type() ||
+      !same_device(*k, to) || !to->is_contiguous() || to->dim() != 4 || to->size(0) != k->size(0) || to->size(1) != 2 ||
+      to->size(2) != k->size(2) || to->size(3) != k->size(3))
+    return none();
+  for (int i = 0; i < 4; ++i)
+    if (k->size(i) > 0x7fffffff) return none();
+  auto stride = [&](int i) { return k->size(i) > 1 ? k->stride(i) : 0; };
+  gqk_pages p{};
+  p.k = k->data_ptr();
+  p.k_page = stride(0);
+  p.k_token = stride(1);
+  p.k_head = stride(2);
+  p.dtype = type;
+  p.pages = static_cast<int32_t>(k->size(0));
+  p.page_size = static_cast<int32_t>(k->size(1));
+  p.heads = static_cast<int32_t>(k->size(2));
+  p.dim = static_cast<int32_t>(k->size(3));
+  if (gqk_page_bounds(&p, table->data_ptr<int>(), table->stride(0), static_cast<int>(table->size(1)), lengths->data_ptr<int>(),
+                      static_cast<int>(batch), static_cast<int>(count), to->data_ptr(), stream_of(*k)))
+    return none();
+  written(*to);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// select_pages(q, bounds, block_table, lengths, keep, page_size, sink, recent, max_length, workspace): (table, lengths)
+PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *q, *from, *table, *lengths, *ws;
+  int64_t keep, page_size, sink, recent, most = 0;
+  if (n != 10 || !plain_world() || !plain(a[0], &q) || !plain(a[1], &from) || !plain(a[2], &table) || !plain(a[3], &lengths) ||
+      !int_of(a[4], &keep) || !int_of(a[5], &page_size) || !int_of(a[6], &sink) || !int_of(a[7], &recent) ||
+      (a[8] != Py_None && !int_of(a[8], &most)) || !plain_or_none(a[9], &ws))
+    return none();
+  gqk_heads qh;
+  const int type = heads_type(q->scalar_type());
+  if (type < 0 || !here(*q) || !heads_of(q, &qh)) return none();
+  const int64_t batch = q->size(0), heads = q->size(1), dim = q->size(2);
+  if (from->dim() != 4 || from->size(1) != 2 || from->size(3) != dim || from->size(0) < 1 || from->size(0) > 0x7fffffff ||
+      from->size(2) < 1 || from->size(2) > heads || (from->scalar_type() != q->scalar_type() && from->scalar_type() != at::kFloat8_e4m3fn) ||
+      !from->is_contiguous() || !same_device(*q, from))
+    return none();
+  if (batch < 1 || batch > 65535 || keep < 1 || page_size < 1 || !table_of(*table, 2, batch, *q) || !i32_of(*lengths, batch, *q)) return none();
+  const int64_t room = std::min<int64_t>(table->size(1) * page_size, GQK_MAX_KEYS);
+  if (a[8] == Py_None) most = room;
+  if (most > room) return none();
+  void* space;
+  int64_t bytes;
+  if (!workspace_of(ws, *q, &space, &bytes)) return none();
+  Tensor chosen = at::empty({batch, from->size(2), keep}, table->options()), kept = at::empty({batch}, table->options());
+  if (gqk_select_pages(qh.data, qh.row, qh.head, type, static_cast<int>(batch), static_cast<int>(heads), from->data_ptr(),
+                       from->scalar_type() == at::kFloat8_e4m3fn ? GQK_DTYPE_FP8 : type, static_cast<int>(from->size(0)),
+                       static_cast<int>(from->size(2)), static_cast<int>(dim), table->data_ptr<int>(), table->stride(0),
+                       static_cast<int>(table->size(1)), lengths->data_ptr<int>(), static_cast<int>(most), static_cast<int>(page_size),
+                       static_cast<int>(keep), static_cast<int>(sink), static_cast<int>(recent), chosen.data_ptr<int>(),
+                       kept.data_ptr<int>(), space, bytes, stream_of(*q)))
+    return none();
+  return Py_BuildValue("(NN)", THPVariable_Wrap(chosen), THPVariable_Wrap(kept));
   END_HANDLE_TH_ERRORS
 }
 
@@ -381,6 +598,11 @@ PyObject* set_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
 PyMethodDef methods[] = {{"paged_attention", FAST(attention), METH_FASTCALL, nullptr},
                          {"qk_norm_rope", FAST(rope), METH_FASTCALL, nullptr},
+                         {"tree_attention", FAST(tree), METH_FASTCALL, nullptr},
+                         {"add_rms_norm", FAST(norm), METH_FASTCALL, nullptr},
+                         {"step_tables", FAST(tables), METH_FASTCALL, nullptr},
+                         {"page_bounds", FAST(bounds), METH_FASTCALL, nullptr},
+                         {"select_pages", FAST(select), METH_FASTCALL, nullptr},
                          {"lora_add", FAST(lora), METH_FASTCALL, nullptr},
                          {"copy_pages", FAST(copy), METH_FASTCALL, nullptr},
                          {"set_workspace", FAST(set_workspace), METH_FASTCALL, nullptr},

@@ -1,0 +1,587 @@
+// gqk_tree.hip - attention of several new tokens per sequence over a paged key-value cache: the tokens of a drafted tree, of a
+// chain, or of a chunk of a prompt.
+//
+//   o_i = sum_j exp(scale q_i.k_j - m_i) v_j / sum_j exp(scale q_i.k_j - m_i),   m_i = max_j scale q_i.k_j
+//
+// over the keys j that new token i sees: those before the new ones, and of the new ones' those that its mask names (without a
+// mask: its own and the earlier ones'); with a window the last `window` of them.  No key: zeros.
+#include <algorithm>
+#include "gqk_attend.h"
+
+namespace gqk {
+namespace {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+constexpr int kMostSplits = 256;
+
+struct TreeArgs {
+  const void* q;
+  int64_t q_row, q_head;
+  gqk_pages kv;
+  const int32_t* table;
+  int64_t table_row;
+  const int32_t *lengths, *starts, *mask;
+  void* out;
+  int64_t out_row, out_head;
+  float* lse;
+  float* partials;
+  int tokens, batch, q_heads, words, max_length, max_tokens, window;
+  float scale;          // of a score, in units of log 2, not negative: the queries take its sign
+  uint32_t sign;
+  int chunk, splits;    // keys of a split, and the most splits of a row tile
+  int slots;            // places for row tiles
+  uint32_t magic;       // key / page_size = 2 key magic >> 32 >> shift, exact below 2^31
+  int shift;
+};
+
+__device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c, bf16_t) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c, f16_t) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// A row tile: `rows` (token, query head) pairs of one sequence and key head, tokens outermost, from row row0 of the sequence's on.
+struct Tile {
+  int b, start, tokens;   // the sequence, its first row of q, its new tokens
+  int row0, rows;
+  int context, length;    // keys before the new tokens', and with them
+  int begin, end;         // the keys that its rows can see lie in [begin, end)
+  bool bad;               // lengths or a mask that cannot be: NaN
+};
+
+// The tile at place `slot`.  Sequence b's tiles take the places from starts[b] group / ROWS + b on, which are enough for them, so that
+// a launch knows its size without reading the lengths.  False: the place has none.
+template <int ROWS> __device__ __forceinline__ bool tile_at(const TreeArgs& a, int slot, int lane, Tile& t) {
+  const int group = a.q_heads / a.kv.heads;
+  auto place = [&](int b) { return (int64_t)max(0, a.starts[b]) * group / ROWS + b; };
+  int lo = 0, n = a.batch;   // the last sequence whose first place is not behind: 64 candidates a step
+  while (n > 1) {
+    const int stride = (n + 63) / 64, b = lo + lane * stride;
+    const bool before = lane * stride < n && place(b) <= slot;
+    const int at = max(0, __popcll(__ballot(before)) - 1);
+    lo += at * stride;
+    n = min(stride, n - at * stride);
+  }
+  t.b = lo;
+  t.start = a.starts[lo];
+  const int stop = a.starts[lo + 1];
+  if (t.start < 0 || stop > a.tokens || stop <= t.start) return false;
+  t.tokens = stop - t.start;
+  const int64_t own = slot - place(lo), all = (int64_t)t.tokens * group;
+  if (own < 0 || own * ROWS >= all) return false;
+  t.row0 = (int)(own * ROWS);
+  t.rows = (int)min((int64_t)ROWS, all - t.row0);
+  const int len = a.lengths[lo];
+  t.bad = len < t.tokens || len > a.max_length || t.tokens > a.max_tokens || (a.mask && (int64_t)a.words * 32 < t.tokens);
+  t.length = t.bad ? t.tokens : len;
+  t.context = t.length - t.tokens;
+  const int first = t.row0 / group, last = (t.row0 + t.rows - 1) / group;
+  const int sees = a.mask ? t.context : t.context + first + 1;   // the least keys of a row (a mask may name none of the new ones)
+  t.begin = (a.window > 0 ? max(0, sees - a.window) : 0) & ~31;
+  t.end = t.bad ? 0 : a.mask ? t.length : t.context + last + 1;
+  if (t.bad) t.begin = 0;
+  return true;
+}
+
+// The first key that a row sees under the window, and its mask.
+struct Row {
+  int token, first;
+  const int32_t* mask;
+};
+__device__ __forceinline__ Row row_of(const TreeArgs& a, const Tile& t, int row) {
+  Row r{row / (a.q_heads / a.kv.heads), 0, nullptr};
+  if (a.mask) r.mask = a.mask + (int64_t)(t.start + r.token) * a.words;
+  if (a.window > 0 && !t.bad) {
+    if (!a.mask) {
+      r.first = max(0, t.context + r.token + 1 - a.window);
+    } else {   // of the new tokens' keys that it sees, the last ones first
+      int left = a.window;
+      for (int w = (t.tokens - 1) >> 5; w >= 0 && left > 0; --w) {
+        uint32_t bits = r.mask[w];
+        if (w == (t.tokens - 1) >> 5 && t.tokens & 31) bits &= (1u << (t.tokens & 31)) - 1;
+        const int c = __popc(bits);
+        if (c < left) { left -= c; continue; }
+        for (int over = c - left; over > 0; --over) bits &= bits - 1;   // the lowest of them are too far back
+        r.first = t.context + w * 32 + __ffs(bits) - 1;
+        left = 0;
+      }
+      if (left > 0) r.first = max(0, t.context - left);
+    }
+  }
+  return r;
+}
+
+// Which of the keys base .. base + 31 a row sees.
+__device__ __forceinline__ uint32_t seen_of(const TreeArgs& a, const Tile& t, const Row& r, int base) {
+  auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; };   // the first n
+  uint32_t seen = below((a.mask ? t.length : t.context + r.token + 1) - base);
+  if (a.mask && base + 32 > t.context) {
+    const int at = base - t.context;
+    uint32_t bits;
+    if (at >= 0) {
+      const int w = at >> 5, s = at & 31;
+      bits = w < a.words ? (uint32_t)r.mask[w] >> s : 0u;
+      if (s && w + 1 < a.words) bits |= (uint32_t)r.mask[w + 1] << (32 - s);
+    } else {
+      bits = (uint32_t)r.mask[0] << -at | below(-at);
+    }
+    seen &= bits;
+  }
+  return seen & ~below(r.first - base);
+}
+
+// Where 16-byte chunk c of a key lies in its row of LDS: a wave that reads one chunk of 32 keys, or two 16-dim runs of eight, finds them in
+// different banks.
+template <int DP> __device__ __forceinline__ int place_of(int key, int c) {
+  return DP == 64 ? c ^ ((key >> 1 & 1) << 2 | (key >> 2 & 3)) : c ^ ((key & 3) << 2 | (key >> 2 & 3));
+}
+
+// A workgroup takes one row tile of one key head and one split of its keys.  Its four waves are 4 / KW groups of 32 rows by KW
+// groups of 32 keys of each step; keys and values of a step of KT keys go through LDS (the next step's are on their way in registers
+// meanwhile), so that a page's row is read once by the workgroup, in whole lines, whatever its type and layout.
+//
+// Both products run on 32 x 32 x 16 matrix instructions with the keys (then the dims) as the rows and the tile's rows as the
+// columns: S^T = K Q^T, lane l has row l % 32's scores of keys 8 (i / 4) + 4 (l / 32) + i % 4 of 32, and as O^T += V^T P^T may take the
+// keys in any order, these are its operand as they are; V's operand comes transposed out of LDS in the same order.  Only the
+// maximum crosses lanes.
+//
+// Scores, statistics and sums are in 32 bits; the weights become T for the second product, as in the attention of single tokens.
+template <typename T, typename C, int DP, int KW, int KT>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {
+  constexpr bool F8 = sizeof(C) == 1;
+  constexpr int RW = 4 / KW, ROWS = 32 * RW;
+  constexpr int NM = DP / 16, ND = DP / 32, CPK = DP / 8;
+  constexpr int NCH = KT * CPK / 256;            // chunks of a thread's share of a step
+  constexpr int KPR = 256 / CPK;                 // keys of a round of them
+  constexpr int KB = KT / 32 / KW;               // 32-key blocks of a wave
+  constexpr int TB = KT * DP * 2;                // bytes of a step's keys, or values
+  constexpr int RS = DP + 4;                     // row stride of the sums
+  constexpr int LDS = std::max(4 * TB, 4 * 32 * RS * 4);
+  __shared__ __align__(16) char lds[LDS];
+  __shared__ float stat[4 * 32][2];
+  __shared__ uint32_t odd[3][KT / 32];           // of three steps: keys with a value that is not finite
+  __shared__ int wrong;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % a.kv.heads, slot = a.slots - 1 - (int)(blockIdx.x / a.kv.heads), split = blockIdx.y;
+  Tile t;
+  if (!tile_at<ROWS>(a, slot, lane, t)) return;
+  const int ns = splits_of(t.begin, t.end, a.chunk);
+  if (split >= ns) return;
+  const int group = a.q_heads / a.kv.heads, D = a.kv.dim;
+  const int k_begin = t.begin + split * a.chunk, k_end = t.end > k_begin ? k_begin + min(a.chunk, t.end - k_begin) : k_begin;
+  const int steps = (k_end - k_begin + KT - 1) / KT;
+  const float inf = __builtin_huge_valf(), nan = __builtin_nanf("");
+  const int kw = wave % KW, rw = wave / KW, n = lane & 31, hh = lane >> 5;
+  const int own = rw * 32 + n;                   // of the tile's rows
+  const bool live = own < t.rows;
+  const Row row = row_of(a, t, t.row0 + (live ? own : 0));
+  // scores of zero are those of queries of zero: a key that is not seen has -inf, which no factor may make NaN
+  const float factor = a.scale * (a.kv.k_scale ? fabsf(a.kv.k_scale[kvh]) : 1.f), scale = factor == 0.f ? 1.f : factor;
+  const uint32_t sign = a.sign ^ (a.kv.k_scale && a.kv.k_scale[kvh] < 0.f ? 0x80008000u : 0u);
+
+  v4u q[NM];
+  {
+    const int head = kvh * group + (t.row0 + (live ? own : 0)) % group;
+    const T* qp = (const T*)a.q + (int64_t)(t.start + row.token) * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      const int d = i * 16 + hh * 8;
+      q[i] = d < D ? *(const v4u*)(qp + d) : v4u{0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) q[i][w] = live && d < D && factor != 0.f ? q[i][w] ^ sign : 0u;
+    }
+  }
+
+  v16f acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = v16f{};
+  float m = -inf, l = 0.f;
+  bool bad = false;
+  if (tid < KT / 32) odd[0][tid] = odd[1][tid] = odd[2][tid] = 0;
+  if (tid == 0) wrong = 0;
+  __syncthreads();
+
+  // staging: thread's chunk i of a step is dims 8 (tid % CPK) .. of key tid / CPK + i KPR
+  const int c = tid % CPK, c_key = tid / CPK, ps = a.kv.page_size;
+  const bool c_live = c * 8 < D;
+  const int32_t* table = a.table + (int64_t)t.b * a.table_row;
+  const C* const kb = (const C*)a.kv.k + kvh * a.kv.k_head + (c_live ? c * 8 : 0);
+  const C* const vb = (const C*)a.kv.v + kvh * a.kv.v_head + (c_live ? c * 8 : 0);
+  struct Raw { uint32_t w[F8 ? 2 : 4]; };
+  Raw kr[NCH], vr[NCH];
+  int page[NCH];
+  auto look = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int key = base + c_key + i * KPR;
+      page[i] = key < k_end ? table[__umulhi(2u * (uint32_t)key, a.magic) >> a.shift] : 0;
+    }
+  };
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int key = base + c_key + i * KPR;
+      const bool out = (uint32_t)page[i] >= (uint32_t)a.kv.pages;   // a page outside of the cache is not read
+      bad |= out;
+      const int at = (int)(__umulhi(2u * (uint32_t)key, a.magic) >> a.shift);
+      const int64_t p = out ? 0 : page[i], o = key - at * ps;
+      Raw k{}, v{};
+      if (c_live && key < k_end && !out) {
+        __builtin_memcpy(&k, __builtin_assume_aligned(kb + p * a.kv.k_page + o * a.kv.k_token, sizeof(Raw)), sizeof(Raw));
+        __builtin_memcpy(&v, __builtin_assume_aligned(vb + p * a.kv.v_page + o * a.kv.v_token, sizeof(Raw)), sizeof(Raw));
+      }
+      kr[i] = k;
+      vr[i] = v;
+    }
+  };
+  auto wide = [&](const Raw& r) {
+    if constexpr (F8) return widen8<T>(r.w[0], r.w[1]);
+    else return v4u{r.w[0], r.w[1], r.w[2], r.w[3]};
+  };
+  // rows of the tile that see all keys below `whole`, and none that the window takes
+  const int whole = a.mask ? t.context : t.context + t.row0 / group + 1;
+  const int open = a.window > 0 ? t.end - a.window : 0;   // from here on the window takes nothing (a row sees at most the keys up to end)
+  auto mixed = [&](int base, int keys) { return base + keys > whole || base < open; };
+  auto stage = [&](int base, int buf, int third) {
+    char* const at = lds + buf * 2 * TB;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int key = c_key + i * KPR, to = key * DP * 2 + place_of<DP>(key, c) * 16;
+      *(v4u*)(at + to) = wide(kr[i]);
+      *(v4u*)(at + TB + to) = wide(vr[i]);
+    }
+    if (mixed(base, KT)) {
+      constexpr uint32_t e = __is_same(T, f16_t) ? 0x7c00u : 0x7f80u;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const v4u v = wide(vr[i]);
+        bool any = false;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) any |= (v[w] & e) == e || (v[w] >> 16 & e) == e;
+        const int key = c_key + i * KPR;
+        if (any) atomicOr(&odd[third][key >> 5], 1u << (key & 31));
+      }
+    }
+  };
+
+  if (steps > 0) {
+    look(k_begin);
+    fetch(k_begin);
+    stage(k_begin, 0, 0);
+    look(k_begin + KT);
+  }
+  __syncthreads();
+  int third = 0;
+  for (int s = 0; s < steps; ++s) {
+    const int base = k_begin + s * KT, buf = s & 1, third_next = third == 2 ? 0 : third + 1, third_free = third_next == 2 ? 0 : third_next + 1;
+    const bool more = s + 1 < steps;
+    if (more) {
+      fetch(base + KT);
+      look(base + 2 * KT);
+    }
+    if (tid < KT / 32) odd[third_free][tid] = 0;   // last read a step ago, written next a step from now
+    const char* const K = lds + buf * 2 * TB;
+    const char* const V = K + TB;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      const int block = kw * KB + b, first = base + block * 32;
+      if (first >= k_end) continue;
+      v16f sc{};
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        const int key = block * 32 + n;
+        sc = mfma32(*(const v4u*)(K + key * DP * 2 + place_of<DP>(key, 2 * i + hh) * 16), q[i], sc, T{});
+      }
+      const bool some = mixed(first, 32);
+      if (some) {
+        const uint32_t seen = seen_of(a, t, row, first) >> (4 * hh);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = seen >> ((i & 3) + 8 * (i >> 2)) & 1 ? sc[i] : -inf;
+      }
+      float top = fmaxf(sc[0], sc[1]);
+#pragma unroll
+      for (int i = 2; i < 16; ++i) top = fmaxf(top, sc[i]);
+      top = fmaxf(top, __shfl_xor(top, 32)) * scale;
+      const float mn = fmaxf(m, top), mb = base_of(mn);
+      if (__any(mn != m)) {   // rarely, once the first keys were seen
+        const float f = __builtin_amdgcn_exp2f(m - mb);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= f;
+      }
+      m = mn;
+      const float pb = kLift<T> - mb;
+      float p[16], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(sc[i] * scale + pb);
+        sum += p[i];
+      }
+      l += sum;
+      v4u pt[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        pt[k] = v4u{pack2<T>(p[8 * k], p[8 * k + 1]), pack2<T>(p[8 * k + 2], p[8 * k + 3]), pack2<T>(p[8 * k + 4], p[8 * k + 5]),
+                    pack2<T>(p[8 * k + 6], p[8 * k + 7])};
+      // values that are not finite at keys that some rows see and some do not: a weight of 0 does not silence them
+      const uint32_t not_finite = some ? __builtin_amdgcn_readfirstlane(odd[third][block]) : 0u;
+      typedef __attribute__((address_space(3))) v4s* Lds;
+      const int r4 = (lane & 15) >> 2, half = lane >> 4 & 1;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          // lane: four dims of key r4 of a group of four; after the transposition four keys of dim lane % 16
+          const int key = block * 32 + 16 * k + 4 * hh + r4, chunk = d * 4 + half * 2 + ((lane & 3) >> 1), in = (lane & 1) * 8;
+          const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(V + key * DP * 2 + place_of<DP>(key, chunk) * 16 + in));
+          const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(V + (key + 8) * DP * 2 + place_of<DP>(key + 8, chunk) * 16 + in));
+          const v2u x = __builtin_bit_cast(v2u, lo), y = __builtin_bit_cast(v2u, hi);
+          v4u v{x.x, x.y, y.x, y.y};
+          if (not_finite) {
+            const uint32_t bits = not_finite >> (16 * k + 4 * hh);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int at = (w & 1) * 2 + (w >> 1) * 8;
+              v[w] &= (bits >> at & 1 ? 0u : 0xffffu) | (bits >> (at + 1) & 1 ? 0u : 0xffff0000u);
+            }
+          }
+          acc[d] = mfma32(v, pt[k], acc[d], T{});
+        }
+      for (uint32_t rest = not_finite; rest; rest &= rest - 1) {   // one key at a time, for the rows that see it
+        const int key = __ffs(rest) - 1, i = (key >> 3) * 4 + (key & 3);
+        float w = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w = j == i ? p[j] : w;
+        w = __shfl(w, n + 32 * (key >> 2 & 1));
+        const char* from = V + (block * 32 + key) * DP * 2;
+        if (w != 0.f)
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              T x[4];
+              __builtin_memcpy(x, from + place_of<DP>(block * 32 + key, d * 4 + j) * 16 + hh * 8, 8);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[d][4 * j + e] += w * to_f(x[e]);
+            }
+      }
+    }
+    if (more) stage(base + KT, buf ^ 1, third_next);
+    third = third_next;
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32);
+  if (bad) wrong = 1;
+
+  // the waves' sums, joined: lane (n, hh) holds dims 32 d + 8 j + 4 hh + e of row n in acc[d][4 j + e]
+  float* const red = (float*)lds;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *(v4f*)(red + (wave * 32 + n) * RS + d * 32 + j * 8 + hh * 4) = v4f{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+  if (hh == 0) {
+    stat[wave * 32 + n][0] = m;
+    stat[wave * 32 + n][1] = l;
+  }
+  __syncthreads();
+  const bool lost = wrong || t.bad;
+  const float v_scale = a.kv.v_scale ? a.kv.v_scale[kvh] : 1.f;
+  const int quads = D / 4;
+  float* const part = a.partials + ((int64_t)slot * a.kv.heads + kvh) * a.splits * ROWS * (D + 4);   // [splits][ROWS][D], then [splits][ROWS][2]
+  for (int x = tid; x < t.rows * quads; x += 256) {
+    const int r = x / quads, d = (x - r * quads) * 4, w0 = (r >> 5) * KW;
+    float M = -inf, L = 0.f;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) M = fmaxf(M, stat[(w0 + k) * 32 + (r & 31)][0]);
+    const float Mb = base_of(M);
+    v4f o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const int w = (w0 + k) * 32 + (r & 31);
+      const float f = __builtin_amdgcn_exp2f(stat[w][0] - Mb);
+      L += stat[w][1] * f;
+      o += *(const v4f*)(red + w * RS + d) * f;
+    }
+    if (lost) L = nan;
+    if (ns > 1) {
+      *(v4f*)(part + ((int64_t)split * ROWS + r) * D + d) = o;
+      if (d == 0) {
+        float* st = part + (int64_t)a.splits * ROWS * D + ((int64_t)split * ROWS + r) * 2;
+        st[0] = M;
+        st[1] = L;
+      }
+      continue;
+    }
+    const int token = (t.row0 + r) / group, head = kvh * group + (t.row0 + r) % group;
+    const float f = L == 0.f ? 0.f : v_scale / L;
+    T* to = (T*)a.out + (int64_t)(t.start + token) * a.out_row + head * a.out_head + d;
+    *(v2u*)to = v2u{pack2<T>(o[0] * f, o[1] * f), pack2<T>(o[2] * f, o[3] * f)};
+    if (a.lse && d == 0)
+      a.lse[(int64_t)(t.start + token) * a.q_heads + head] = L == 0.f ? -inf : (M - kLift<T> + __builtin_amdgcn_logf(L)) * kLn2;
+  }
+}
+
+// The join of a row tile's splits, in their order: a workgroup for eight rows of it.
+template <typename T, int ROWS>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
+  constexpr int kRows = 8, kBatch = 8;
+  const int tid = threadIdx.x, parts = ROWS / kRows, D = a.kv.dim, quads = D / 4, group = a.q_heads / a.kv.heads;
+  const int kvh = blockIdx.x % a.kv.heads, rest = blockIdx.x / a.kv.heads, slot = rest / parts, r0 = (rest - slot * parts) * kRows;
+  Tile t;
+  if (!tile_at<ROWS>(a, slot, tid & 63, t)) return;
+  const int ns = splits_of(t.begin, t.end, a.chunk);
+  if (ns == 1) return;   // written already
+  const float* part = a.partials + ((int64_t)slot * a.kv.heads + kvh) * a.splits * ROWS * (D + 4);
+  const float* stat = part + (int64_t)a.splits * ROWS * D;
+  for (int x = tid; x < kRows * quads; x += 256) {
+    const int r = r0 + x / quads, d = x % quads * 4;
+    if (r >= t.rows) continue;
+    Joined j;
+    for (int s0 = 0; s0 < ns; s0 += kBatch) {
+      v2u st[kBatch];
+      v4u y[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int64_t s = min(s0 + k, ns - 1);
+        st[k] = *(const v2u*)(stat + (s * ROWS + r) * 2);
+        y[k] = *(const v4u*)(part + (s * ROWS + r) * D + d);
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        if (s0 + k < ns) j.add(st[k], y[k]);
+    }
+    const int token = (t.row0 + r) / group, head = kvh * group + (t.row0 + r) % group;
+    const float f = j.l == 0.f ? 0.f : (a.kv.v_scale ? a.kv.v_scale[kvh] : 1.f) / j.l;
+    T* to = (T*)a.out + (int64_t)(t.start + token) * a.out_row + head * a.out_head + d;
+    *(v2u*)to = v2u{pack2<T>(j.o[0] * f, j.o[1] * f), pack2<T>(j.o[2] * f, j.o[3] * f)};
+    if (a.lse && d == 0)
+      a.lse[(int64_t)(t.start + token) * a.q_heads + head] = j.l == 0.f ? -__builtin_huge_valf() : (j.m - kLift<T> + __builtin_amdgcn_logf(j.l)) * kLn2;
+  }
+}
+
+// How a call is cut: rows of a tile, keys of a step, places for tiles, splits of `chunk` keys.
+struct Cut { int key_waves, rows, step, slots, splits, chunk; };
+
+Cut cut_of(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_tokens, int max_length, int window, int64_t workspace_bytes) {
+  const int group = q_heads / kv_heads;
+  const int64_t most = (int64_t)std::min(tokens, max_tokens) * group;   // rows of a sequence
+  Cut c;
+  c.key_waves = most <= 32 && dim <= 128 ? 4 : most <= 64 ? 2 : 1;   // (of 256 dims 128 keys do not fit LDS)
+  c.rows = 32 * 4 / c.key_waves;
+  c.step = c.key_waves == 4 ? 128 : 64;
+  const int64_t slots = (int64_t)tokens * group / c.rows + batch;
+  c.slots = (int)slots;
+  // keys that a row tile can see, from a multiple of 32
+  const int64_t sees = std::min<int64_t>((int64_t)std::min(tokens, max_tokens), c.rows / group + 1);
+  const int64_t span = std::min<int64_t>(max_length, window > 0 ? (int64_t)window + sees + std::min(tokens, max_tokens) + 31 : max_length);
+  const int64_t units = slots * kv_heads, wanted = 2LL * device_cus();
+  int64_t splits = std::max<int64_t>(1, std::min((wanted + units - 1) / std::max<int64_t>(1, units), (span + c.step - 1) / c.step));
+  splits = std::min<int64_t>(splits, kMostSplits);
+  const int64_t each = units * c.rows * (dim + 4) * 4;   // bytes of one split of all units
+  if (workspace_bytes < GQK_CTR_BYTES) splits = 1;
+  else splits = std::max<int64_t>(1, std::min(splits, (workspace_bytes - GQK_CTR_BYTES) / std::max<int64_t>(1, each)));
+  c.chunk = (int)std::min<int64_t>(0x7fffff80, std::max<int64_t>(c.step, ((span + splits - 1) / splits + c.step - 1) / c.step * c.step));
+  c.splits = (int)std::max<int64_t>(1, (span + c.chunk - 1) / c.chunk);
+  return c;
+}
+
+template <typename T, typename C, int DP>
+void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)c.slots * a.kv.heads), c.splits);
+  if constexpr (DP < 256)
+    if (c.key_waves == 4) {
+      tree_kernel<T, C, DP, 4, 128><<<grid, 256, 0, st>>>(a);
+      return;
+    }
+  if (c.key_waves == 2) tree_kernel<T, C, DP, 2, 64><<<grid, 256, 0, st>>>(a);
+  else tree_kernel<T, C, DP, 1, 64><<<grid, 256, 0, st>>>(a);
+}
+
+template <typename T, typename C>
+void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
+  if (a.kv.dim <= 64) launch<T, C, 64>(a, c, st);
+  else if (a.kv.dim <= 128) launch<T, C, 128>(a, c, st);
+  else launch<T, C, 256>(a, c, st);
+}
+
+template <typename T>
+void join(const TreeArgs& a, const Cut& c, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)c.slots * a.kv.heads * (c.rows / 8)));
+  if (c.rows == 32) tree_join_kernel<T, 32><<<grid, 256, 0, st>>>(a);
+  else if (c.rows == 64) tree_join_kernel<T, 64><<<grid, 256, 0, st>>>(a);
+  else tree_join_kernel<T, 128><<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace gqk
+
+using namespace gqk;
+
+extern "C" {
+
+int64_t gqk_tree_attention_workspace_bytes(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_tokens, int max_length,
+                                           int window) {
+  if (tokens < 0 || tokens > GQK_MAX_TOKENS || batch < 0 || batch > 65535 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads ||
+      q_heads / kv_heads > GQK_MAX_GROUP || dim < 8 || dim > 256 || dim % 8 || max_tokens < 0 || max_length < 0 || max_length > GQK_MAX_KEYS || window < 0)
+    return decode_fail(GQK_ERR_SHAPE, "tree_attention: %d tokens of %d sequences, %d / %d heads of %d, max_tokens %d, max_length %d, window %d",
+                       tokens, batch, q_heads, kv_heads, dim, max_tokens, max_length, window);
+  if (tokens == 0 || batch == 0) return 0;
+  const Cut c = cut_of(tokens, batch, q_heads, kv_heads, dim, max_tokens, max_length, window, INT64_MAX);
+  return c.splits > 1 ? GQK_CTR_BYTES + (int64_t)c.slots * kv_heads * c.rows * c.splits * (dim + 4) * 4 : 0;
+}
+
+int gqk_tree_attention(const void* q, int64_t q_row, int64_t q_head, int dtype, int tokens, int batch, int q_heads,
+                       const gqk_pages* pages, const int32_t* table, int64_t table_row, int table_width, const int32_t* lengths,
+                       const int32_t* starts, const int32_t* mask, int mask_words, int max_length, int max_tokens, int window, float scale,
+                       void* out, int64_t out_row, int64_t out_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "tree_attention";
+  if (dtype != GQK_DTYPE_BF16 && dtype != GQK_DTYPE_F16) return decode_fail(GQK_ERR_ARG, "%s: dtype %d", what, dtype);
+  if (const int rc = check_pages(what, pages, dtype)) return rc;
+  if (tokens < 0 || tokens > GQK_MAX_TOKENS || batch < 0 || batch > 65535 || q_heads < 1 || q_heads % pages->heads ||
+      q_heads / pages->heads > GQK_MAX_GROUP)
+    return decode_fail(GQK_ERR_SHAPE, "%s: %d tokens of %d sequences, %d query heads over %d", what, tokens, batch, q_heads, pages->heads);
+  if (window < 0 || max_tokens < 0 || max_length < 0 || max_length > GQK_MAX_KEYS || table_width < 0 ||
+      (int64_t)max_length > (int64_t)table_width * pages->page_size)
+    return decode_fail(GQK_ERR_SHAPE, "%s: window %d, up to %d tokens, lengths up to %d in %d pages of %d tokens", what, window, max_tokens,
+                       max_length, table_width, pages->page_size);
+  if (mask && mask_words < 1) return decode_fail(GQK_ERR_SHAPE, "%s: a mask of %d words", what, mask_words);
+  if (tokens == 0 || batch == 0) return GQK_OK;
+  if (!q || !out || !lengths || !starts || (!table && max_length > 0)) return decode_fail(GQK_ERR_ARG, "%s: null pointer", what);
+  if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_row | q_head | out_row | out_head) & 7)
+    return decode_fail(GQK_ERR_SHAPE, "%s: q and out are 16-byte aligned with strides that are multiples of 8", what);
+  const Cut c = cut_of(tokens, batch, q_heads, pages->heads, pages->dim, max_tokens, max_length, window, workspace ? workspace_bytes : 0);
+  if ((uintptr_t)workspace & 255) return decode_fail(GQK_ERR_SHAPE, "%s: workspace is not 256-byte aligned", what);
+  if ((int64_t)c.slots * pages->heads * (c.rows / 8) > 0x7fffffff)
+    return decode_fail(GQK_ERR_SHAPE, "%s: %d tokens of %d heads are more than a launch takes", what, tokens, q_heads);
+  TreeArgs a{};
+  a.q = q; a.q_row = q_row; a.q_head = q_head; a.kv = *pages; a.table = table; a.table_row = table_row; a.lengths = lengths; a.starts = starts;
+  a.mask = mask; a.words = mask_words; a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.tokens = tokens; a.batch = batch;
+  a.q_heads = q_heads; a.max_length = max_length; a.max_tokens = max_tokens; a.window = window; a.scale = fabsf(scale) * kLog2e; a.sign = scale < 0.f ? 0x80008000u : 0u;
+  a.chunk = c.chunk; a.splits = c.splits; a.slots = c.slots;
+  a.partials = workspace ? (float*)((char*)workspace + GQK_CTR_BYTES) : nullptr;
+  const PageDivisor by = page_divisor(pages->page_size);
+  a.magic = by.magic;
+  a.shift = by.shift;
+  const hipStream_t st = (hipStream_t)stream;
+  const bool bf = dtype == GQK_DTYPE_BF16;
+  if (pages->dtype == GQK_DTYPE_FP8) {
+    if (bf) launch<bf16_t, fp8_t>(a, c, st);
+    else launch<f16_t, fp8_t>(a, c, st);
+  } else if (bf) {
+    launch<bf16_t, bf16_t>(a, c, st);
+  } else {
+    launch<f16_t, f16_t>(a, c, st);
+  }
+  if (c.splits > 1) {
+    if (bf) join<bf16_t>(a, c, st);
+    else join<f16_t>(a, c, st);
+  }
+  return decode_launched(what);
+}
+
+}  // extern "C"

@@ -27,6 +27,8 @@ GQK_NOALLOC_SCRATCH_BYTES = GQK_CTR_BYTES + (32 << 20)   # gqk_linear_noalloc's 
 GQK_DTYPE_F32, GQK_DTYPE_BF16, GQK_DTYPE_F16, GQK_DTYPE_FP8 = 0, 1, 2, 3
 GQK_MAX_KEYS = 0x7ffffc00
 GQK_ROPE_UNIT_OFFSET, GQK_ROPE_INTERLEAVED = 1, 2
+GQK_MAX_TREE, GQK_NORM_MAX_DIM = 1024, 32768
+GQK_MAX_TOKENS, GQK_MAX_GROUP = 1 << 20, 1024
 
 # every entry point include/gguf_hip.h declares
 EXPORTS = ("gqk_last_error", "gqk_version", "gqk_type_info", "gqk_dequantize", "gqk_dequantize_tiles",
@@ -35,7 +37,9 @@ EXPORTS = ("gqk_last_error", "gqk_version", "gqk_type_info", "gqk_dequantize", "
            "gqk_gguf_open", "gqk_gguf_close", "gqk_gguf_info", "gqk_gguf_tensor_at", "gqk_gguf_find_tensor",
            "gqk_gguf_kv_at", "gqk_gguf_find_kv", "gqk_gguf_kv_string", "gqk_gguf_upload_tiles", "gqk_read_floor",
            "gqk_lora_workspace_bytes", "gqk_lora_add", "gqk_qk_norm_rope", "gqk_paged_attention_workspace_bytes",
-           "gqk_paged_attention", "gqk_copy_pages")
+           "gqk_paged_attention", "gqk_copy_pages", "gqk_paged_attention_heads", "gqk_step_tables", "gqk_add_rms_norm",
+           "gqk_tree_attention_workspace_bytes", "gqk_tree_attention", "gqk_page_bounds", "gqk_select_pages_workspace_bytes",
+           "gqk_select_pages")
 
 
 class GqkShard(ctypes.Structure):
@@ -133,6 +137,17 @@ def _load() -> ctypes.CDLL:
         "gqk_paged_attention": (i32, [vp, i64, i64, i32, i32, i32, vp, vp, i64, i32, vp, i32, i32, ctypes.c_float, vp, i64,
                                       i64, vp, vp, i64, vp]),
         "gqk_copy_pages": (i32, [vp, i64, i64, i64, i64, i64, vp, vp, i64, vp]),
+        "gqk_paged_attention_heads": (i32, [vp, i64, i64, i32, i32, i32, vp, vp, i64, i64, i32, vp, i32, i32, ctypes.c_float, vp,
+                                            i64, i64, vp, vp, i64, vp]),
+        "gqk_step_tables": (i32, [vp, i64, i32, i32, vp, i32, vp, vp, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "gqk_add_rms_norm": (i32, [vp, i64, vp, i64, i32, i64, i32, vp, i32, ctypes.c_float, i32, vp, i64, i32, vp, i32, vp, i64, vp]),
+        "gqk_tree_attention_workspace_bytes": (i64, [i32] * 8),
+        "gqk_tree_attention": (i32, [vp, i64, i64, i32, i32, i32, i32, vp, vp, i64, i32, vp, vp, vp, i32, i32, i32, i32, ctypes.c_float,
+                                     vp, i64, i64, vp, vp, i64, vp]),
+        "gqk_page_bounds": (i32, [vp, vp, i64, i32, vp, i32, i32, vp, vp]),
+        "gqk_select_pages_workspace_bytes": (i64, [i32] * 4),
+        "gqk_select_pages": (i32, [vp, i64, i64, i32, i32, i32, vp, i32, i32, i32, i32, vp, i64, i32, vp, i32, i32, i32, i32, i32, vp,
+                                   vp, vp, i64, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

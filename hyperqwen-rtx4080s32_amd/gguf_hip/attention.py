@@ -1,7 +1,7 @@
 """Attention around the linear path: the heads that qkv's output holds, normalized, rotated and stored into
 the pages of a key-value cache (``qk_norm_rope``), and the attention of each new token over those pages
-(``paged_attention``).  Both run on the current stream (one launch; a second where a
-sequence's keys are cut into more than 16 splits, or heads that share one of keys are many), allocate their outputs alone, do not synchronise the host
+(``paged_attention``), or of several new tokens per sequence (``tree_attention``).  They run on the current stream (one launch; a second where a
+sequence's keys are cut into more than 16 splits, or heads that share one of keys are many; of several tokens where they are cut at all), allocate their outputs alone, do not synchronise the host
 and can be captured in a HIP graph; under tracing they are custom ops with fakes.
 
 Layouts: heads are [tokens, heads, dim] views with any strides (column ranges of qkv's output as they are);
@@ -100,11 +100,12 @@ def _attention_into(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                                    out, lse, workspace)
     ws = ops.shared_workspace(device) if workspace is None else workspace
     qs, os = _strides(q), _strides(out)
-    check(lib.gqk_paged_attention(q.data_ptr(), qs[0], qs[1], _TYPES[q.dtype], batch, heads,
-                                  _lib.byref(_c_pages(k_pages, v_pages, k_scale, v_scale)), block_table.data_ptr(),
-                                  block_table.stride(0), block_table.shape[1], lengths.data_ptr(), max_length, window, scale,
-                                  out.data_ptr(), os[0], os[1], None if lse is None else lse.data_ptr(), ws.data_ptr(),
-                                  ws.numel() * ws.element_size(), _stream(device)), "paged_attention")
+    check(lib.gqk_paged_attention_heads(q.data_ptr(), qs[0], qs[1], _TYPES[q.dtype], batch, heads,
+                                        _lib.byref(_c_pages(k_pages, v_pages, k_scale, v_scale)), block_table.data_ptr(),
+                                        block_table.stride(0), block_table.stride(1) if block_table.dim() == 3 else 0,
+                                        block_table.shape[-1], lengths.data_ptr(), max_length, window, scale, out.data_ptr(), os[0],
+                                        os[1], None if lse is None else lse.data_ptr(), ws.data_ptr(),
+                                        ws.numel() * ws.element_size(), _stream(device)), "paged_attention")
 
 
 @torch.library.custom_op("gguf_hip::paged_attention", mutates_args=("out", "lse", "workspace"))
@@ -128,7 +129,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Attention of one new token per sequence over its pages: q [batch, query heads, dim] (bf16 or fp16), pages
     [pages, page_size, heads, dim] of q's type or float8_e4m3fn (times ``k_scale`` / ``v_scale`` fp32 [heads]), query
     heads a multiple of the pages' heads, dim a multiple of 8 up to 256.  Key j of sequence b lies in page
-    block_table[b, j // page_size] (int32); lengths int32 [batch] counts the keys, the new token's among them;
+    block_table[b, j // page_size] (int32), or with a table for each of the pages' heads, [batch, heads, pages] (as ``select_pages``
+    makes it), in block_table[b, head, j // page_size]; lengths int32 [batch] counts the keys, the new token's among them;
     ``window`` > 0 keeps the last ``window`` of them.  A sequence without a key gets zeros.  ``scale``: dim ** -0.5
     by default.  ``max_length``: an upper bound on lengths known to the host (default: what the table holds); the work
     is split by it, so a tight one is faster.  A sequence above it, or with a page outside of the cache, gets NaN.
@@ -148,14 +150,16 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     batch, heads, dim = q.shape
     if heads == 0 or heads % k_pages.shape[2]:
         raise ValueError(f"paged_attention: {heads} query heads over {k_pages.shape[2]}")
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch
-            or block_table.device != q.device or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-        raise ValueError(f"paged_attention: block_table is int32 [{batch}, pages] on {q.device}, its columns side by side")
+    if (block_table.dtype != torch.int32 or block_table.dim() not in (2, 3) or block_table.shape[0] != batch
+            or (block_table.dim() == 3 and block_table.shape[1] != k_pages.shape[2])
+            or block_table.device != q.device or (block_table.shape[-1] > 1 and block_table.stride(-1) != 1)):
+        raise ValueError(f"paged_attention: block_table is int32 [{batch}, pages] or [{batch}, {k_pages.shape[2]}, pages] on {q.device}, "
+                         f"its columns side by side")
     if (lengths.dtype != torch.int32 or lengths.shape != (batch,) or lengths.device != q.device
             or not lengths.is_contiguous()):
         raise ValueError(f"paged_attention: lengths is contiguous int32 [{batch}] on {q.device}")
     ops.check_workspace(workspace, q.device, "paged_attention")
-    room = min(block_table.shape[1] * k_pages.shape[1], _lib.GQK_MAX_KEYS)
+    room = min(block_table.shape[-1] * k_pages.shape[1], _lib.GQK_MAX_KEYS)
     max_length = room if max_length is None else int(max_length)
     if not 0 <= max_length <= room or window < 0:
         raise ValueError(f"paged_attention: max_length {max_length} (the table holds {room} keys), window {window}")
@@ -173,6 +177,110 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _attention_op(*args)
     for t in (out, lse):
         no_backward("paged_attention", t, q, k_pages, v_pages, k_scale, v_scale)
+    return (out, lse) if return_lse else out
+
+
+# ---- attention of several new tokens -----------------------------------------------------------
+
+def _tree_into(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+               starts: torch.Tensor, mask: torch.Tensor | None, scale: float, window: int, k_scale: torch.Tensor | None,
+               v_scale: torch.Tensor | None, max_length: int, max_tokens: int, out: torch.Tensor, lse: torch.Tensor | None,
+               workspace: torch.Tensor | None) -> None:
+    tokens, heads, dim = q.shape
+    batch = lengths.shape[0]
+    if tokens == 0 or batch == 0:
+        return
+    device = q.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _tree_into(q, k_pages, v_pages, block_table, lengths, starts, mask, scale, window, k_scale, v_scale, max_length,
+                              max_tokens, out, lse, workspace)
+    ws = ops.shared_workspace(device) if workspace is None else workspace
+    qs, os = _strides(q), _strides(out)
+    check(lib.gqk_tree_attention(q.data_ptr(), qs[0], qs[1], _TYPES[q.dtype], tokens, batch, heads,
+                                 _lib.byref(_c_pages(k_pages, v_pages, k_scale, v_scale)), block_table.data_ptr(),
+                                 block_table.stride(0), block_table.shape[1], lengths.data_ptr(), starts.data_ptr(),
+                                 None if mask is None else mask.data_ptr(), 0 if mask is None else mask.shape[1], max_length, max_tokens,
+                                 window, scale, out.data_ptr(), os[0], os[1], None if lse is None else lse.data_ptr(), ws.data_ptr(),
+                                 ws.numel() * ws.element_size(), _stream(device)), "tree_attention")
+
+
+@torch.library.custom_op("gguf_hip::tree_attention", mutates_args=("out", "lse", "workspace"))
+def _tree_op(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+             starts: torch.Tensor, mask: torch.Tensor | None, scale: float, window: int, k_scale: torch.Tensor | None,
+             v_scale: torch.Tensor | None, max_length: int, max_tokens: int, out: torch.Tensor, lse: torch.Tensor | None,
+             workspace: torch.Tensor | None) -> None:
+    _tree_into(q, k_pages, v_pages, block_table, lengths, starts, mask, scale, window, k_scale, v_scale, max_length, max_tokens, out, lse,
+               workspace)
+
+
+@_tree_op.register_fake
+def _(q, k_pages, v_pages, block_table, lengths, starts, mask, scale, window, k_scale, v_scale, max_length, max_tokens, out, lse, workspace):
+    return None
+
+
+def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                   starts: torch.Tensor, mask: torch.Tensor | None = None, *, scale: float | None = None, window: int = 0,
+                   k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None, max_length: int | None = None,
+                   max_tokens: int | None = None, out: torch.Tensor | None = None, return_lse: bool = False,
+                   workspace: torch.Tensor | None = None):
+    """Attention of several new tokens per sequence over its pages: drafted trees and chains, chunks of prompts.  q [tokens, query heads,
+    dim] (bf16 or fp16): sequence b's new tokens are its rows starts[b] .. starts[b + 1] (int32 [batch + 1]); pages, block_table int32 [batch,
+    pages], scales, ``scale`` as paged_attention's; lengths int32 [batch] counts the keys, the new tokens' among them, which
+    are the last ones in the tokens' order.  A new token sees the keys before the new ones and those of the new ones that ``mask`` names: bit
+    j % 32 of mask[row, j // 32] (int32 [tokens, words], as ``step_tables`` makes it) is new token j of its sequence.  Without a mask it sees
+    its own and the earlier ones'.  ``window`` > 0 keeps the last ``window`` of the keys that a token sees; one that sees none gets zeros.
+    ``max_length``, ``max_tokens``: upper bounds on lengths and on a sequence's new tokens known to the host (default: what the table and q
+    hold); the work is divided by them, so tight ones are faster.  A sequence above them, with fewer keys than new tokens, or with more of these
+    than the mask has bits gets NaN; tokens whose keys lie in a page outside of the cache get NaN, and others of their
+    sequence may.  Rows of q that belong to no sequence are left as they were in ``out``.  Returns out [tokens, query heads, dim], with
+    ``return_lse`` also the log-sum-exp of the scores (fp32 [tokens, query heads], -inf without a key).  ``workspace``: as
+    mul_mat_grouped's (its own for calls on concurrent streams).  No backward pass."""
+    what = "tree_attention"
+    if _fast is not None and _unwatched():
+        got = _fast.tree_attention(q, k_pages, v_pages, block_table, lengths, starts, mask, scale, window, k_scale, v_scale, max_length,
+                                   max_tokens, out, return_lse, workspace)
+        if got is not None:
+            return got
+    ops._require_gpu(q, what)
+    if q.dtype not in _TYPES:
+        raise ValueError(f"{what}: q is bf16 or fp16, not {q.dtype}")
+    q = _heads_view(q, what)
+    _check_pages(k_pages, v_pages, k_scale, v_scale, q, what)
+    tokens, heads, dim = q.shape
+    if heads == 0 or heads % k_pages.shape[2] or heads // k_pages.shape[2] > _lib.GQK_MAX_GROUP or tokens > _lib.GQK_MAX_TOKENS:
+        raise ValueError(f"{what}: {tokens} tokens, {heads} query heads over {k_pages.shape[2]}")
+    if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.device != q.device or not lengths.is_contiguous():
+        raise ValueError(f"{what}: lengths is contiguous int32 [batch] on {q.device}")
+    batch = lengths.shape[0]
+    if starts.dtype != torch.int32 or starts.shape != (batch + 1,) or starts.device != q.device or not starts.is_contiguous():
+        raise ValueError(f"{what}: starts is contiguous int32 [{batch + 1}] on {q.device}")
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch
+            or block_table.device != q.device or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        raise ValueError(f"{what}: block_table is int32 [{batch}, pages] on {q.device}, its columns side by side")
+    if mask is not None and (mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[0] != tokens or mask.shape[1] < 1
+                             or mask.device != q.device or not mask.is_contiguous()):
+        raise ValueError(f"{what}: mask is contiguous int32 [{tokens}, words] on {q.device}")
+    ops.check_workspace(workspace, q.device, what)
+    room = min(block_table.shape[1] * k_pages.shape[1], _lib.GQK_MAX_KEYS)
+    max_length = room if max_length is None else int(max_length)
+    max_tokens = tokens if max_tokens is None else min(int(max_tokens), tokens)
+    if not 0 <= max_length <= room or window < 0 or max_tokens < 0:
+        raise ValueError(f"{what}: max_length {max_length} (the table holds {room} keys), max_tokens {max_tokens}, window {window}")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        _out_heads(out, q, what)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    args = (q, k_pages, v_pages, block_table, lengths, starts, mask, dim ** -0.5 if scale is None else float(scale), int(window), k_scale,
+            v_scale, max_length, max_tokens, out, lse, workspace)
+    if _direct(q, k_pages, v_pages, block_table, lengths, starts, mask, k_scale, v_scale, out, workspace):
+        _tree_into(*args)
+        torch.autograd.graph.increment_version(out)
+    else:
+        _tree_op(*args)
+    for t in (out, lse):
+        no_backward(what, t, q, k_pages, v_pages, k_scale, v_scale)
     return (out, lse) if return_lse else out
 
 

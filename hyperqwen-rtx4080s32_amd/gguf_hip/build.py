@@ -21,7 +21,7 @@ SOURCES = (("gqk_api.hip", (), "gqk_api.o"), ("gqk_codec.hip", (), "gqk_codec.o"
            ("gqk_mid.hip", (), "gqk_mid.o"), ("gqk_gemm_plan.hip", (), "gqk_gemm_plan.o"),
            *(("gqk_gemm.hip", (f"-DGQK_GEMM_MB={mb}",), f"gqk_gemm{mb}.o") for mb in (2, 4, 8)),
            ("gqk_gguf.cpp", (), "gqk_gguf.o"),
-           *((f"gqk_{n}.hip", (), f"gqk_{n}.o") for n in ("lora", "rope", "attention", "pages")))
+           *((f"gqk_{n}.hip", (), f"gqk_{n}.o") for n in ("lora", "rope", "attention", "pages", "norm", "tables", "tree", "select")))
 ARCH = os.environ.get("GQK_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 MODULE = os.path.join(PKG, "_fast.so")   # the CPython module of the eager calls (gqk_torch.cpp)

@@ -257,6 +257,87 @@ int gqk_paged_attention(const void* q, int64_t q_row, int64_t q_head, int dtype,
                         const int32_t* lengths, int max_length, int window, float scale, void* out, int64_t out_row,
                         int64_t out_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* gqk_paged_attention with a table for each key head: key j of sequence b, for the query heads of key head h, lies in page
+ * table[b, h, j / page_size], the rows of one sequence's heads table_head apart (0: one for all).  lengths[b] counts the keys that each head's row lists. */
+int gqk_paged_attention_heads(const void* q, int64_t q_row, int64_t q_head, int dtype, int batch, int q_heads,
+                              const gqk_pages* pages, const int32_t* table, int64_t table_row, int64_t table_head, int table_width,
+                              const int32_t* lengths, int max_length, int window, float scale, void* out, int64_t out_row,
+                              int64_t out_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- steps of several new tokens per sequence ------------------------------------------------- */
+
+/* What a step needs to know of its tokens, from the sequences' lengths.  Sequence b of the batch is request requests[b] (int32, or int64
+ * with requests_64; negative: no sequence), whose pages are lists[requests[b], :] (int32 [lists_n, width], rows list_row apart); it has
+ * lengths[b] keys in the cache and brings counts[b] new tokens, which are rows starts[b] .. starts[b + 1] of the step's `tokens` rows
+ * (one sequence's after another's).  Written:
+ *   table [batch, width]      the pages of lengths[b] + counts[b] keys, -1 behind them
+ *   totals [batch]            lengths[b] + counts[b]
+ *   starts [batch + 1]
+ *   sequences [tokens]        the row's sequence, -1 behind the last
+ *   positions [tokens]        lengths[b] + i for new token i; in a tree lengths[b] + the number of its ancestors (0 behind the last)
+ *   slots [tokens] (int64)    page * page_size + place of key lengths[b] + i (-1 behind the last, and where the list has a negative page)
+ *   mask [tokens, (tree + 31) / 32]   with parents: the bits of the token's ancestors and its own
+ * parents: NULL (a chain), or int32 [tokens], the number of each new token's parent among its sequence's (-1: the cache's last key), which comes before
+ * it; tree: the most new tokens of a sequence then (at most GQK_MAX_TREE), else 0.  What cannot be (a request that has no list, lengths beyond
+ * its width or negative, more tokens than rows or than `tree`): totals 2^31 - 1, for which the attention answers NaN, no slots, positions -1;
+ * a parent that does not come before its child: an empty mask and position -1 for the token and those below it. */
+#define GQK_MAX_TREE 1024
+int gqk_step_tables(const int32_t* lists, int64_t list_row, int lists_n, int width, const void* requests, int requests_64,
+                    const int32_t* lengths, const int32_t* counts, int batch, int tokens, int page_size, const int32_t* parents, int tree,
+                    int32_t* table, int32_t* totals, int32_t* starts, int32_t* sequences, int32_t* positions, int64_t* slots, int32_t* mask,
+                    void* stream);
+
+/* The residual's addition and the RMS norm of rows x [rows, dim] (bf16 or fp16, rows x_row elements apart, any dim up to
+ * GQK_NORM_MAX_DIM):
+ *   s = x + residual,  out_residual = s,  out = s rsqrt(mean(s^2) + eps) * weight
+ * residual NULL: s = x; out_residual NULL: not written; weight NULL: 1, else [dim] of x's type or fp32, 1 + weight with
+ * GQK_ROPE_UNIT_OFFSET.  Arithmetic is in fp32, the norm that of s before it is rounded.  out_dtype: x's, or
+ * GQK_DTYPE_FP8: out = the values divided by scale, which is fp32 [rows], or [rows, dim / group] with a group (a power of two from 32
+ * to 512 that divides dim): the largest size of a value (2^-100 at least) / 448.  out, out_residual may be x, residual (whole, with their row strides);
+ * out in 8 bits shares no memory with the inputs. */
+#define GQK_NORM_MAX_DIM 32768
+int gqk_add_rms_norm(const void* x, int64_t x_row, const void* residual, int64_t residual_row, int dtype, int64_t rows, int dim,
+                     const void* weight, int weight_dtype, float eps, int flags, void* out, int64_t out_row, int out_dtype, float* scale,
+                     int group, void* out_residual, int64_t out_residual_row, void* stream);
+
+/* Attention of several new tokens per sequence over its pages.  q, out: [tokens, q_heads, dim], sequence b's tokens the rows starts[b] ..
+ * starts[b + 1] (int32 [batch + 1]; rows outside of them, and a sequence whose rows are not within q's, are not written); lengths[b] counts its
+ * keys, the new tokens' among them, which are its last ones in their order.  New token i sees the keys before the new
+ * ones, and of those the ones that its mask names: bit j % 32 of mask[starts[b] + i, j / 32] (int32 [tokens, mask_words]) is new token j; mask
+ * NULL: new tokens 0 .. i.  window > 0: of the keys that it sees the last `window`.  No key: zeros, lse -inf.  A length above max_length or below the
+ * sequence's new tokens, more of them than max_tokens or the mask's bits: NaN for the sequence; a page outside of the cache: NaN for the tokens whose
+ * keys it would hold, and maybe for others of the sequence.  Values that are not finite at keys that a token does not see do not reach it.  Everything else as gqk_paged_attention (one launch, a second where
+ * the keys are split). */
+#define GQK_MAX_TOKENS 1048576
+#define GQK_MAX_GROUP 1024 /* query heads of a key head */
+int64_t gqk_tree_attention_workspace_bytes(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_tokens, int max_length,
+                                           int window);
+int gqk_tree_attention(const void* q, int64_t q_row, int64_t q_head, int dtype, int tokens, int batch, int q_heads,
+                       const gqk_pages* pages, const int32_t* table, int64_t table_row, int table_width, const int32_t* lengths,
+                       const int32_t* starts, const int32_t* mask, int mask_words, int max_length, int max_tokens, int window, float scale,
+                       void* out, int64_t out_row, int64_t out_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- the pages of a long cache that are worth reading ------------------------------------------ */
+
+/* Bounds of the keys in the pages that hold each sequence's last `count` keys, [pages, 2, heads, dim] of the pages' type (contiguous, aligned to 8 elements): the
+ * smallest and the largest of the page's keys of this sequence, per head and dim (NaN for both where one is NaN).  Only pages->k and its strides are read.  Pages
+ * that several sequences hold must hold the same keys of each; a length or page out of its range writes nothing. */
+int gqk_page_bounds(const gqk_pages* pages, const int32_t* table, int64_t table_row, int table_width, const int32_t* lengths, int batch,
+                    int count, void* bounds, void* stream);
+
+/* For each sequence and key head the `keep` pages of its table to attend to: the first `sink`, the last `recent` (one at least), and of the others
+ * those with the largest  max over the key head's query heads of sum_d max(q_d lo_d, q_d hi_d), which no key of the page exceeds; among equals the first.
+ * out [batch, heads, keep]: their pages in the table's order (-1 behind them, where a sequence has fewer), out_lengths [batch]: the keys in them (the last
+ * page alone may be partial), for gqk_paged_attention_heads.  The order is that of the scores in 64 bits; a score that is NaN counts as infinity.
+ * Positive scales of 8-bit keys do not change it.  A page outside of the cache is taken (the attention then answers NaN), a length above max_length
+ * gives 2^31 - 1.  workspace: gqk_select_pages_workspace_bytes bytes, 256-byte aligned, or less, down to one sequence's (they then go in
+ * turns); its first GQK_CTR_BYTES are left alone. */
+int64_t gqk_select_pages_workspace_bytes(int batch, int heads, int page_size, int max_length);
+int gqk_select_pages(const void* q, int64_t q_row, int64_t q_head, int dtype, int batch, int q_heads, const void* bounds, int bounds_dtype,
+                     int pages, int heads, int dim, const int32_t* table, int64_t table_row, int table_width, const int32_t* lengths,
+                     int max_length, int page_size, int keep, int sink, int recent, int32_t* out, int32_t* out_lengths, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 /* Page src[i] to page dst[i] in each of `planes` planes (a layer's keys, a layer's values, ...), for n pairs: page p of
  * plane l is the page_bytes bytes at base + l * plane_stride + p * page_stride.  src and dst are host arrays, read
  * before the call returns (a captured graph copies the pairs of its capture).  A page outside of
