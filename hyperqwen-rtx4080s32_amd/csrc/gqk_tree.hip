@@ -140,8 +140,8 @@ template <int DP> __device__ __forceinline__ int place_of(int key, int c) {
 }
 
 // A workgroup takes one row tile of one key head and one split of its keys.  Its four waves are 4 / KW groups of 32 rows by KW
-// groups of 32 keys of each step; keys and values of a step of KT keys go through LDS (the next step's are on their way in registers
-// meanwhile), so that a page's row is read once by the workgroup, in whole lines, whatever its type and layout.
+// groups of 32 or 64 keys of each step; keys and values of a step of KT keys go through LDS, the next step's on their way
+// meanwhile, so that a page's row is read once by the workgroup, in whole lines, whatever its type and layout.
 //
 // Both products run on 32 x 32 x 16 matrix instructions with the keys (then the dims) as the rows and the tile's rows as the
 // columns: S^T = K Q^T, lane l has row l % 32's scores of keys 8 (i / 4) + 4 (l / 32) + i % 4 of 32, and as O^T += V^T P^T may take the
@@ -149,9 +149,12 @@ template <int DP> __device__ __forceinline__ int place_of(int key, int c) {
 // maximum crosses lanes.
 //
 // Scores, statistics and sums are in 32 bits; the weights become T for the second product, as in the attention of single tokens.
-template <typename T, typename C, int DP, int KW, int KT>
+//
+// RUNS: pages hold whole runs of the keys of one round of loads, and heads all dims: a run's page is one number for the whole workgroup,
+// and a chunk's place in it the thread's own, so that nothing is computed per chunk.  16-bit pages then go to LDS directly.
+template <typename T, typename C, int DP, int KW, int KT, bool RUNS>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {
-  constexpr bool F8 = sizeof(C) == 1;
+  constexpr bool F8 = sizeof(C) == 1, DIRECT = RUNS && !F8;
   constexpr int RW = 4 / KW, ROWS = 32 * RW;
   constexpr int NM = DP / 16, ND = DP / 32, CPK = DP / 8;
   constexpr int NCH = KT * CPK / 256;            // chunks of a thread's share of a step
@@ -160,10 +163,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   constexpr int TB = KT * DP * 2;                // bytes of a step's keys, or values
   constexpr int RS = DP + 4;                     // row stride of the sums
   constexpr int LDS = std::max(4 * TB, 4 * 32 * RS * 4);
-  __shared__ __align__(16) char lds[LDS];
+  __shared__ __align__(1024) char lds[LDS];      // (addresses are made by xor: rows begin at multiples of their size)
   __shared__ float stat[4 * 32][2];
   __shared__ uint32_t odd[3][KT / 32];           // of three steps: keys with a value that is not finite
   __shared__ int wrong;
+  typedef __attribute__((address_space(3))) char* Lds;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % a.kv.heads, slot = a.slots - 1 - (int)(blockIdx.x / a.kv.heads), split = blockIdx.y;
@@ -205,37 +209,66 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   if (tid == 0) wrong = 0;
   __syncthreads();
 
-  // staging: thread's chunk i of a step is dims 8 (tid % CPK) .. of key tid / CPK + i KPR
-  const int c = tid % CPK, c_key = tid / CPK, ps = a.kv.page_size;
-  const bool c_live = c * 8 < D;
+  // A step's chunk i KPR CPK + tid: 16 bytes of LDS, at place tid % CPK of key tid / CPK + i KPR's row, where one chunk of dims lies
+  // (place_of is its own inverse).  A thread loads the chunk that belongs there.
+  const int c_key = tid / CPK, ps = a.kv.page_size;
+  auto dims_of = [&](int i) { return place_of<DP>(c_key + i * KPR, tid % CPK) * 8; };
+  typedef const __attribute__((address_space(4))) int32_t* Uniform;
   const int32_t* table = a.table + (int64_t)t.b * a.table_row;
-  const C* const kb = (const C*)a.kv.k + kvh * a.kv.k_head + (c_live ? c * 8 : 0);
-  const C* const vb = (const C*)a.kv.v + kvh * a.kv.v_head + (c_live ? c * 8 : 0);
+  const C* const kb = (const C*)a.kv.k + kvh * a.kv.k_head;
+  const C* const vb = (const C*)a.kv.v + kvh * a.kv.v_head;
+  auto page_of = [&](int key) { return (int)(__umulhi(2u * (uint32_t)key, a.magic) >> a.shift); };
   struct Raw { uint32_t w[F8 ? 2 : 4]; };
-  Raw kr[NCH], vr[NCH];
+  constexpr int HELD = DIRECT ? 1 : NCH;
+  Raw kr[HELD], vr[HELD];
   int page[NCH];
   auto look = [&](int base) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int key = base + c_key + i * KPR;
-      page[i] = key < k_end ? table[__umulhi(2u * (uint32_t)key, a.magic) >> a.shift] : 0;
+      const int key = RUNS ? base + i * KPR : base + c_key + i * KPR;
+      if constexpr (RUNS) page[i] = key < k_end ? ((Uniform)table)[page_of(key)] : 0;
+      else page[i] = key < k_end ? table[page_of(key)] : 0;
     }
   };
-  auto fetch = [&](int base) {
+  // The chunks of a step's keys and values: on their way to LDS (DIRECT) or to registers.
+  auto fetch = [&](int base, int buf) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int key = base + c_key + i * KPR;
+      const int key = RUNS ? base + i * KPR : base + c_key + i * KPR;
       const bool out = (uint32_t)page[i] >= (uint32_t)a.kv.pages;   // a page outside of the cache is not read
       bad |= out;
-      const int at = (int)(__umulhi(2u * (uint32_t)key, a.magic) >> a.shift);
-      const int64_t p = out ? 0 : page[i], o = key - at * ps;
-      Raw k{}, v{};
-      if (c_live && key < k_end && !out) {
-        __builtin_memcpy(&k, __builtin_assume_aligned(kb + p * a.kv.k_page + o * a.kv.k_token, sizeof(Raw)), sizeof(Raw));
-        __builtin_memcpy(&v, __builtin_assume_aligned(vb + p * a.kv.v_page + o * a.kv.v_token, sizeof(Raw)), sizeof(Raw));
+      const int64_t p = out ? 0 : page[i], o = key - page_of(key) * ps;
+      const C *kp = kb + p * a.kv.k_page + o * a.kv.k_token, *vp = vb + p * a.kv.v_page + o * a.kv.v_token;
+      if constexpr (RUNS) {   // (of a run that the keys end in, the page has the rest)
+        const uint32_t k_own = (uint32_t)(c_key * (int)a.kv.k_token + dims_of(i)) * sizeof(C);
+        const uint32_t v_own = (uint32_t)(c_key * (int)a.kv.v_token + dims_of(i)) * sizeof(C);
+        if constexpr (DIRECT) {
+          if (key < k_end && !out) {
+#ifdef __HIP_DEVICE_COMPILE__   // the host pass rejects 16-byte direct-to-LDS loads
+            const auto kr_ = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, 0xFFFFFFFFu, 0x00020000);
+            const auto vr_ = __builtin_amdgcn_make_buffer_rsrc((void*)vp, 0, 0xFFFFFFFFu, 0x00020000);
+            char* const to = lds + buf * 2 * TB + i * 4096 + wave * 1024;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr_, (__attribute__((address_space(3))) void*)to, 16, k_own, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr_, (__attribute__((address_space(3))) void*)(to + TB), 16, v_own, 0, 0, 0);
+#endif
+          }
+          continue;
+        }
+        kp = (const C*)((const char*)kp + k_own);
+        vp = (const C*)((const char*)vp + v_own);
+      } else {
+        kp += dims_of(i);
+        vp += dims_of(i);
       }
-      kr[i] = k;
-      vr[i] = v;
+      if constexpr (!DIRECT) {
+        Raw k{}, v{};
+        if ((RUNS || dims_of(i) < D) && key < k_end && !out) {
+          __builtin_memcpy(&k, __builtin_assume_aligned(kp, sizeof(Raw)), sizeof(Raw));
+          __builtin_memcpy(&v, __builtin_assume_aligned(vp, sizeof(Raw)), sizeof(Raw));
+        }
+        kr[i] = k;
+        vr[i] = v;
+      }
     }
   };
   auto wide = [&](const Raw& r) {
@@ -246,65 +279,103 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   const int whole = a.mask ? t.context : t.context + t.row0 / group + 1;
   const int open = a.window > 0 ? t.end - a.window : 0;   // from here on the window takes nothing (a row sees at most the keys up to end)
   auto mixed = [&](int base, int keys) { return base + keys > whole || base < open; };
-  auto stage = [&](int base, int buf, int third) {
-    char* const at = lds + buf * 2 * TB;
+  // A weight of 0 does not silence a value that is not finite: where some rows see a key and some do not, such values are put aside.
+  auto put_aside = [&](v4u& v, int key, int third) {
+    constexpr uint32_t e = __is_same(T, f16_t) ? 0x7c00u : 0x7f80u;
+    bool any = false;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      const int key = c_key + i * KPR, to = key * DP * 2 + place_of<DP>(key, c) * 16;
-      *(v4u*)(at + to) = wide(kr[i]);
-      *(v4u*)(at + TB + to) = wide(vr[i]);
+    for (int w = 0; w < 4; ++w) {
+      const bool lo = (v[w] & e) == e, hi = (v[w] >> 16 & e) == e;
+      any |= lo | hi;
+      v[w] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
     }
-    if (mixed(base, KT)) {
-      constexpr uint32_t e = __is_same(T, f16_t) ? 0x7c00u : 0x7f80u;
+    if (any) atomicOr(&odd[third][key >> 5], 1u << (key & 31));
+    return any;
+  };
+  auto stage = [&](int base, int buf, int third) {
+    char* const at = lds + buf * 2 * TB + tid * 16;
+    if constexpr (DIRECT) {   // what has come, where it does not stay as it is
+      if (!mixed(base, KT)) return;   // (the last key is in none but a mixed step)
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const v4u v = wide(vr[i]);
-        bool any = false;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) any |= (v[w] & e) == e || (v[w] >> 16 & e) == e;
         const int key = c_key + i * KPR;
-        if (any) atomicOr(&odd[third][key >> 5], 1u << (key & 31));
+        v4u* const v = (v4u*)(at + TB + i * 4096);
+        if (base + key >= k_end) {
+          *(v4u*)(at + i * 4096) = v4u{0, 0, 0, 0};
+          *v = v4u{0, 0, 0, 0};
+        } else {
+          v4u x = *v;
+          if (put_aside(x, key, third)) *v = x;
+        }
+      }
+    } else {
+      const bool some = mixed(base, KT);
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        v4u k = wide(kr[i]), v = wide(vr[i]);
+        if (some) {
+          if (base + c_key + i * KPR >= k_end) k = v = v4u{0, 0, 0, 0};
+          put_aside(v, c_key + i * KPR, third);
+        }
+        *(v4u*)(at + i * 4096) = k;
+        *(v4u*)(at + TB + i * 4096) = v;
       }
     }
   };
 
+  // A wave's operands in LDS: of keys, chunk 2 i + hh of key n is at (n's row, chunk hh) ^ 32 i; of values a lane reads four dims of key r4 of
+  // a group of four, and has four keys of dim lane % 16 after the transposition: chunk 4 d + .. of the row at ^ 64 d, the group eight keys on at ^ 32.
+  const int r4 = (lane & 15) >> 2;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(Lds)lds + kw * KB * 32 * DP * 2;
+  const uint32_t k_at = lds0 + n * DP * 2 + place_of<DP>(n, hh) * 16;
+  const uint32_t v_at = lds0 + TB + (4 * hh + r4) * DP * 2 + place_of<DP>(4 * hh + r4, (lane >> 4 & 1) * 2 + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+
   if (steps > 0) {
     look(k_begin);
-    fetch(k_begin);
-    stage(k_begin, 0, 0);
+    fetch(k_begin, 0);
+    if constexpr (!DIRECT) stage(k_begin, 0, 0);
     look(k_begin + KT);
   }
-  __syncthreads();
+  if constexpr (!DIRECT) __syncthreads();
   int third = 0;
   for (int s = 0; s < steps; ++s) {
     const int base = k_begin + s * KT, buf = s & 1, third_next = third == 2 ? 0 : third + 1, third_free = third_next == 2 ? 0 : third_next + 1;
     const bool more = s + 1 < steps;
+    if constexpr (DIRECT) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      stage(base, buf, third);
+      __syncthreads();
+    }
     if (more) {
-      fetch(base + KT);
+      fetch(base + KT, buf ^ 1);
       look(base + 2 * KT);
     }
     if (tid < KT / 32) odd[third_free][tid] = 0;   // last read a step ago, written next a step from now
-    const char* const K = lds + buf * 2 * TB;
-    const char* const V = K + TB;
+    const int first = base + kw * KB * 32;
+    if (first < k_end) {
+      uint32_t ka = k_at + buf * 2 * TB, va = v_at + buf * 2 * TB;
+      asm volatile("" : "+v"(ka), "+v"(va));   // their variants are made anew in each step, not kept
+      v16f sc[KB];
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      const int block = kw * KB + b, first = base + block * 32;
-      if (first >= k_end) continue;
-      v16f sc{};
+      for (int b = 0; b < KB; ++b) sc[b] = v16f{};
 #pragma unroll
-      for (int i = 0; i < NM; ++i) {
-        const int key = block * 32 + n;
-        sc = mfma32(*(const v4u*)(K + key * DP * 2 + place_of<DP>(key, 2 * i + hh) * 16), q[i], sc, T{});
+      for (int i = 0; i < NM; ++i)
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+          sc[b] = mfma32(*(const __attribute__((address_space(3))) v4u*)((Lds)(uintptr_t)(ka ^ (i * 32)) + b * 32 * DP * 2), q[i], sc[b], T{});
+      if (mixed(first, 32 * KB)) {
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          const uint32_t mine = seen_of(a, t, row, first + b * 32) >> (4 * hh);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[b][i] = mine >> ((i & 3) + 8 * (i >> 2)) & 1 ? sc[b][i] : -inf;
+        }
       }
-      const bool some = mixed(first, 32);
-      if (some) {
-        const uint32_t seen = seen_of(a, t, row, first) >> (4 * hh);
+      float top = sc[0][0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = seen >> ((i & 3) + 8 * (i >> 2)) & 1 ? sc[i] : -inf;
-      }
-      float top = fmaxf(sc[0], sc[1]);
+      for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int i = 2; i < 16; ++i) top = fmaxf(top, sc[i]);
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[b][i]);
       top = fmaxf(top, __shfl_xor(top, 32)) * scale;
       const float mn = fmaxf(m, top), mb = base_of(mn);
       if (__any(mn != m)) {   // rarely, once the first keys were seen
@@ -314,66 +385,66 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
         for (int d = 0; d < ND; ++d) acc[d] *= f;
       }
       m = mn;
-      const float pb = kLift<T> - mb;
-      float p[16], sum = 0.f;
+      if (mixed(first, 32 * KB)) {
+        // the values that were put aside reach the rows that see them: as they are, whatever their weight
+#pragma unroll 1
+        for (int b = 0; b < KB; ++b)
+#pragma unroll 1
+          for (uint32_t rest = __builtin_amdgcn_readfirstlane(odd[third][kw * KB + b]); rest; rest &= rest - 1) {
+            const int bit = __ffs(rest) - 1, key = first + b * 32 + bit, at = page_of(key);
+            const bool sees = seen_of(a, t, row, first + b * 32) >> bit & 1;
+            const C* from = vb + table[at] * a.kv.v_page + (int64_t)(key - at * ps) * a.kv.v_token;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(sc[i] * scale + pb);
-        sum += p[i];
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int dim = d * 32 + 8 * j + 4 * hh;
+                const bool some = sees && dim < D;
+                C x[4];
+                __builtin_memcpy(x, __builtin_assume_aligned(from + (some ? dim : 0), 4 * sizeof(C)), 4 * sizeof(C));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float y = to_f(x[e]);
+                  acc[d][4 * j + e] += !some || y - y == 0.f ? 0.f : y;
+                }
+              }
+          }
       }
-      l += sum;
-      v4u pt[2];
+      const float pb = kLift<T> - mb;
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        pt[k] = v4u{pack2<T>(p[8 * k], p[8 * k + 1]), pack2<T>(p[8 * k + 2], p[8 * k + 3]), pack2<T>(p[8 * k + 4], p[8 * k + 5]),
-                    pack2<T>(p[8 * k + 6], p[8 * k + 7])};
-      // values that are not finite at keys that some rows see and some do not: a weight of 0 does not silence them
-      const uint32_t not_finite = some ? __builtin_amdgcn_readfirstlane(odd[third][block]) : 0u;
-      typedef __attribute__((address_space(3))) v4s* Lds;
-      const int r4 = (lane & 15) >> 2, half = lane >> 4 & 1;
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
+      for (int b = 0; b < KB; ++b) {
+        v4u pt[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          // lane: four dims of key r4 of a group of four; after the transposition four keys of dim lane % 16
-          const int key = block * 32 + 16 * k + 4 * hh + r4, chunk = d * 4 + half * 2 + ((lane & 3) >> 1), in = (lane & 1) * 8;
-          const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(V + key * DP * 2 + place_of<DP>(key, chunk) * 16 + in));
-          const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(V + (key + 8) * DP * 2 + place_of<DP>(key + 8, chunk) * 16 + in));
-          const v2u x = __builtin_bit_cast(v2u, lo), y = __builtin_bit_cast(v2u, hi);
-          v4u v{x.x, x.y, y.x, y.y};
-          if (not_finite) {
-            const uint32_t bits = not_finite >> (16 * k + 4 * hh);
+          float p[8];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const int at = (w & 1) * 2 + (w >> 1) * 8;
-              v[w] &= (bits >> at & 1 ? 0u : 0xffffu) | (bits >> (at + 1) & 1 ? 0u : 0xffff0000u);
-            }
+          for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(sc[b][8 * k + i] * scale + pb);
+            l += p[i];
           }
-          acc[d] = mfma32(v, pt[k], acc[d], T{});
+          pt[k] = v4u{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
         }
-      for (uint32_t rest = not_finite; rest; rest &= rest - 1) {   // one key at a time, for the rows that see it
-        const int key = __ffs(rest) - 1, i = (key >> 3) * 4 + (key & 3);
-        float w = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w = j == i ? p[j] : w;
-        w = __shfl(w, n + 32 * (key >> 2 & 1));
-        const char* from = V + (block * 32 + key) * DP * 2;
-        if (w != 0.f)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              T x[4];
-              __builtin_memcpy(x, from + place_of<DP>(block * 32 + key, d * 4 + j) * 16 + hh * 8, 8);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[d][4 * j + e] += w * to_f(x[e]);
-            }
+          for (int k = 0; k < 2; ++k) {
+            typedef const __attribute__((address_space(3))) char* From;
+            typedef __attribute__((address_space(3))) v4s* Four;
+            const int rows = (b * 32 + 16 * k) * DP * 2;
+            const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Four)((From)(uintptr_t)(va ^ (d * 64)) + rows));
+            const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Four)((From)(uintptr_t)(va ^ (d * 64) ^ 32) + rows + 8 * DP * 2));
+            const v2u x = __builtin_bit_cast(v2u, lo), y = __builtin_bit_cast(v2u, hi);
+            acc[d] = mfma32(v4u{x.x, x.y, y.x, y.y}, pt[k], acc[d], T{});
+          }
       }
     }
-    if (more) stage(base + KT, buf ^ 1, third_next);
+    if constexpr (!DIRECT) {
+      if (more) stage(base + KT, buf ^ 1, third_next);
+      __syncthreads();
+    }
     third = third_next;
-    __syncthreads();
   }
+  if constexpr (DIRECT) __syncthreads();
   l += __shfl_xor(l, 32);
   if (bad) wrong = 1;
 
@@ -490,16 +561,23 @@ Cut cut_of(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_to
   return c;
 }
 
-template <typename T, typename C, int DP>
+template <typename T, typename C, int DP, bool RUNS>
 void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)c.slots * a.kv.heads), c.splits);
   if constexpr (DP < 256)
     if (c.key_waves == 4) {
-      tree_kernel<T, C, DP, 4, 128><<<grid, 256, 0, st>>>(a);
+      tree_kernel<T, C, DP, 4, 128, RUNS><<<grid, 256, 0, st>>>(a);
       return;
     }
-  if (c.key_waves == 2) tree_kernel<T, C, DP, 2, 64><<<grid, 256, 0, st>>>(a);
-  else tree_kernel<T, C, DP, 1, 64><<<grid, 256, 0, st>>>(a);
+  if (c.key_waves == 2) tree_kernel<T, C, DP, 2, 64, RUNS><<<grid, 256, 0, st>>>(a);
+  else tree_kernel<T, C, DP, 1, 64, RUNS><<<grid, 256, 0, st>>>(a);
+}
+
+template <typename T, typename C, int DP>
+void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
+  constexpr int run = 256 * 8 / DP;   // keys of a round of loads
+  if (a.kv.dim == DP && a.kv.page_size % run == 0) launch<T, C, DP, true>(a, c, st);
+  else launch<T, C, DP, false>(a, c, st);
 }
 
 template <typename T, typename C>
