@@ -43,6 +43,16 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c, f16_t) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// 16 bytes of every lane from base + own to LDS, the lanes' side by side from `to` on, while the wave goes on: it waits for vmcnt itself before
+// anyone reads them.  (Of the builtin the compiler waits for all of these loads before the next read of LDS, whichever it reads: 680 us where
+// this takes 480.)
+__device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t own, uint32_t to) {
+  const v4u from{(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, 0xFFFFFFFFu, 0x00020000u};
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(own), "s"(from), "s"(to) : "memory", "m0");
+#endif
+}
+
 // A row tile: `rows` (token, query head) pairs of one sequence and key head, tokens outermost, from row row0 of the sequence's on.
 struct Tile {
   int b, start, tokens;   // the sequence, its first row of q, its new tokens
@@ -175,7 +185,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   if (!tile_at<ROWS>(a, slot, lane, t)) return;
   const int ns = splits_of(t.begin, t.end, a.chunk);
   if (split >= ns) return;
-  const int group = a.q_heads / a.kv.heads, D = a.kv.dim;
+  const int group = a.q_heads / a.kv.heads, D = RUNS ? DP : a.kv.dim;
   const int k_begin = t.begin + split * a.chunk, k_end = t.end > k_begin ? k_begin + min(a.chunk, t.end - k_begin) : k_begin;
   const int steps = (k_end - k_begin + KT - 1) / KT;
   const float inf = __builtin_huge_valf(), nan = __builtin_nanf("");
@@ -204,7 +214,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = v16f{};
   float m = -inf, l = 0.f;
-  bool bad = false;
+  uint32_t top_page = 0;
   if (tid < KT / 32) odd[0][tid] = odd[1][tid] = odd[2][tid] = 0;
   if (tid == 0) wrong = 0;
   __syncthreads();
@@ -221,50 +231,53 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   struct Raw { uint32_t w[F8 ? 2 : 4]; };
   constexpr int HELD = DIRECT ? 1 : NCH;
   Raw kr[HELD], vr[HELD];
-  int page[NCH];
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(Lds)lds + wave * 1024;
+  int page[NCH], place[NCH];   // of a step that is fetched next: its runs' pages, and the places of their first keys (RUNS)
+  int run_at = page_of(k_begin), run_place = k_begin - run_at * ps;
+  const int run_last = k_end > 0 ? page_of(k_end - 1) : 0;
   auto look = [&](int base) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int key = RUNS ? base + i * KPR : base + c_key + i * KPR;
-      if constexpr (RUNS) page[i] = key < k_end ? ((Uniform)table)[page_of(key)] : 0;
-      else page[i] = key < k_end ? table[page_of(key)] : 0;
+      if constexpr (RUNS) {   // runs follow one another; one behind the last key is read as any other, and not used
+        page[i] = ((Uniform)table)[min(run_at, run_last)];
+        place[i] = run_place;
+        run_place += KPR;
+        if (run_place == ps) run_place = 0, ++run_at;
+      } else {
+        const int key = base + c_key + i * KPR;
+        page[i] = key < k_end ? table[page_of(key)] : 0;
+      }
     }
   };
   // The chunks of a step's keys and values: on their way to LDS (DIRECT) or to registers.
+  const uint32_t k_page = (uint32_t)a.kv.k_page * sizeof(C), v_page = (uint32_t)a.kv.v_page * sizeof(C);
+  const uint32_t k_tok = (uint32_t)a.kv.k_token * sizeof(C), v_tok = (uint32_t)a.kv.v_token * sizeof(C);
+  const bool alike = k_page == v_page && k_tok == v_tok;
   auto fetch = [&](int base, int buf) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int key = RUNS ? base + i * KPR : base + c_key + i * KPR;
       const bool out = (uint32_t)page[i] >= (uint32_t)a.kv.pages;   // a page outside of the cache is not read
-      bad |= out;
-      const int64_t p = out ? 0 : page[i], o = key - page_of(key) * ps;
-      const C *kp = kb + p * a.kv.k_page + o * a.kv.k_token, *vp = vb + p * a.kv.v_page + o * a.kv.v_token;
-      if constexpr (RUNS) {   // (of a run that the keys end in, the page has the rest)
-        const uint32_t k_own = (uint32_t)(c_key * (int)a.kv.k_token + dims_of(i)) * sizeof(C);
-        const uint32_t v_own = (uint32_t)(c_key * (int)a.kv.v_token + dims_of(i)) * sizeof(C);
+      top_page = max(top_page, (uint32_t)page[i]);
+      if constexpr (RUNS) {
+        const uint32_t p = out ? 0 : page[i];
+        const uint64_t ko = (uint64_t)p * k_page + (uint32_t)place[i] * k_tok, vo = alike ? ko : (uint64_t)p * v_page + (uint32_t)place[i] * v_tok;
+        const char *kp = (const char*)kb + ko, *vp = (const char*)vb + vo;
+        const uint32_t k_own = c_key * k_tok + dims_of(i) * (uint32_t)sizeof(C), v_own = c_key * v_tok + dims_of(i) * (uint32_t)sizeof(C);
         if constexpr (DIRECT) {
-          if (key < k_end && !out) {
-#ifdef __HIP_DEVICE_COMPILE__   // the host pass rejects 16-byte direct-to-LDS loads
-            const auto kr_ = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, 0xFFFFFFFFu, 0x00020000);
-            const auto vr_ = __builtin_amdgcn_make_buffer_rsrc((void*)vp, 0, 0xFFFFFFFFu, 0x00020000);
-            char* const to = lds + buf * 2 * TB + i * 4096 + wave * 1024;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr_, (__attribute__((address_space(3))) void*)to, 16, k_own, 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr_, (__attribute__((address_space(3))) void*)(to + TB), 16, v_own, 0, 0, 0);
-#endif
-          }
-          continue;
+          const uint32_t to = lds_at + buf * 2 * TB + i * 4096;
+          load_to_lds((uint64_t)kp, k_own, to);
+          load_to_lds((uint64_t)vp, v_own, to + TB);
+        } else {
+          __builtin_memcpy(&kr[i], __builtin_assume_aligned(kp + k_own, sizeof(Raw)), sizeof(Raw));
+          __builtin_memcpy(&vr[i], __builtin_assume_aligned(vp + v_own, sizeof(Raw)), sizeof(Raw));
         }
-        kp = (const C*)((const char*)kp + k_own);
-        vp = (const C*)((const char*)vp + v_own);
       } else {
-        kp += dims_of(i);
-        vp += dims_of(i);
-      }
-      if constexpr (!DIRECT) {
+        const int key = base + c_key + i * KPR;
+        const int64_t p = out ? 0 : page[i], o = key - page_of(key) * ps;
         Raw k{}, v{};
-        if ((RUNS || dims_of(i) < D) && key < k_end && !out) {
-          __builtin_memcpy(&k, __builtin_assume_aligned(kp, sizeof(Raw)), sizeof(Raw));
-          __builtin_memcpy(&v, __builtin_assume_aligned(vp, sizeof(Raw)), sizeof(Raw));
+        if (dims_of(i) < D && key < k_end && !out) {
+          __builtin_memcpy(&k, __builtin_assume_aligned(kb + p * a.kv.k_page + o * a.kv.k_token + dims_of(i), sizeof(Raw)), sizeof(Raw));
+          __builtin_memcpy(&v, __builtin_assume_aligned(vb + p * a.kv.v_page + o * a.kv.v_token + dims_of(i), sizeof(Raw)), sizeof(Raw));
         }
         kr[i] = k;
         vr[i] = v;
@@ -350,19 +363,31 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
       fetch(base + KT, buf ^ 1);
       look(base + 2 * KT);
     }
-    if (tid < KT / 32) odd[third_free][tid] = 0;   // last read a step ago, written next a step from now
+    if (mixed(base - KT, KT) && tid < KT / 32) odd[third_free][tid] = 0;   // the last step's: written again two steps from now at the earliest
     const int first = base + kw * KB * 32;
     if (first < k_end) {
       uint32_t ka = k_at + buf * 2 * TB, va = v_at + buf * 2 * TB;
       asm volatile("" : "+v"(ka), "+v"(va));   // their variants are made anew in each step, not kept
+      typedef const __attribute__((address_space(3))) char* From;
+      auto keys = [&](int i, int b) { return *(const __attribute__((address_space(3))) v4u*)((From)(uintptr_t)(ka ^ (i * 32)) + b * 32 * DP * 2); };
+      auto values = [&](int b, int x) {   // of dims 32 (x / 2) on and sixteen keys
+        typedef __attribute__((address_space(3))) v4s* Four;
+        const uint32_t at = va ^ (x >> 1) * 64;
+        const int rows = (b * 32 + 16 * (x & 1)) * DP * 2;
+        const v2u lo = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Four)((From)(uintptr_t)at + rows)));
+        const v2u hi = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Four)((From)(uintptr_t)(at ^ 32) + rows + 8 * DP * 2)));
+        return v4u{lo.x, lo.y, hi.x, hi.y};
+      };
       v16f sc[KB];
 #pragma unroll
       for (int b = 0; b < KB; ++b) sc[b] = v16f{};
 #pragma unroll
       for (int i = 0; i < NM; ++i)
 #pragma unroll
-        for (int b = 0; b < KB; ++b)
-          sc[b] = mfma32(*(const __attribute__((address_space(3))) v4u*)((Lds)(uintptr_t)(ka ^ (i * 32)) + b * 32 * DP * 2), q[i], sc[b], T{});
+        for (int b = 0; b < KB; ++b) sc[b] = mfma32(keys(i, b), q[i], sc[b], T{});
+      v4u vf[2 * ND];
+#pragma unroll
+      for (int x = 0; x < 2 * ND; ++x) vf[x] = values(0, x);
       if (mixed(first, 32 * KB)) {
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
@@ -425,17 +450,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
           pt[k] = v4u{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
         }
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            typedef const __attribute__((address_space(3))) char* From;
-            typedef __attribute__((address_space(3))) v4s* Four;
-            const int rows = (b * 32 + 16 * k) * DP * 2;
-            const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Four)((From)(uintptr_t)(va ^ (d * 64)) + rows));
-            const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Four)((From)(uintptr_t)(va ^ (d * 64) ^ 32) + rows + 8 * DP * 2));
-            const v2u x = __builtin_bit_cast(v2u, lo), y = __builtin_bit_cast(v2u, hi);
-            acc[d] = mfma32(v4u{x.x, x.y, y.x, y.y}, pt[k], acc[d], T{});
-          }
+        for (int x = 0; x < 2 * ND; ++x) {
+          acc[x >> 1] = mfma32(vf[x], pt[x & 1], acc[x >> 1], T{});
+          if (b + 1 < KB) vf[x] = values(b + 1, x);
+        }
       }
     }
     if constexpr (!DIRECT) {
@@ -446,7 +464,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   }
   if constexpr (DIRECT) __syncthreads();
   l += __shfl_xor(l, 32);
-  if (bad) wrong = 1;
+  if (top_page >= (uint32_t)a.kv.pages) wrong = 1;
 
   // the waves' sums, joined: lane (n, hh) holds dims 32 d + 8 j + 4 hh + e of row n in acc[d][4 j + e]
   float* const red = (float*)lds;
@@ -576,7 +594,8 @@ void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
 template <typename T, typename C, int DP>
 void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
   constexpr int run = 256 * 8 / DP;   // keys of a round of loads
-  if (a.kv.dim == DP && a.kv.page_size % run == 0) launch<T, C, DP, true>(a, c, st);
+  const int64_t far = (int64_t)a.kv.page_size * std::max(a.kv.k_token, a.kv.v_token) * (int64_t)sizeof(C);   // bytes of a page, from its first key's
+  if (a.kv.dim == DP && a.kv.page_size % run == 0 && far <= 0x7fffffff) launch<T, C, DP, true>(a, c, st);
   else launch<T, C, DP, false>(a, c, st);
 }
 
