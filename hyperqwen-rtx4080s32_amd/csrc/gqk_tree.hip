@@ -43,9 +43,17 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c, f16_t) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// the larger of lane and lane ^ 32
+__device__ __forceinline__ float over_halves(float x) {
+  float y = x;
+  asm("" : "+v"(y));   // (of the same value twice the compiler keeps one half)
+  const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)both[0]), __builtin_bit_cast(float, (uint32_t)both[1]));
+}
+
 // 16 bytes of every lane from base + own to LDS, the lanes' side by side from `to` on, while the wave goes on: it waits for vmcnt itself before
-// anyone reads them.  (Of the builtin the compiler waits for all of these loads before the next read of LDS, whichever it reads: 680 us where
-// this takes 480.)
+// anyone reads them.  (Of the builtin the compiler waits for all of these loads before the next read of LDS, whichever it reads: 680 us for a chunk of
+// 4096 tokens behind 4096 where this took 593.)
 __device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t own, uint32_t to) {
   const v4u from{(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, 0xFFFFFFFFu, 0x00020000u};
 #ifdef __HIP_DEVICE_COMPILE__
@@ -167,8 +175,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   constexpr bool F8 = sizeof(C) == 1, DIRECT = RUNS && !F8;
   constexpr int RW = 4 / KW, ROWS = 32 * RW;
   constexpr int NM = DP / 16, ND = DP / 32, CPK = DP / 8;
-  constexpr int NCH = KT * CPK / 256;            // chunks of a thread's share of a step
-  constexpr int KPR = 256 / CPK;                 // keys of a round of them
+  constexpr int RL = 16, NR = KT / RL / 4;       // keys of a run, runs of a wave's share of a step
+  constexpr int NI = RL * CPK / 64, KPI = 64 / CPK;   // loads of a run, keys of a load
   constexpr int KB = KT / 32 / KW;               // 32-key blocks of a wave
   constexpr int TB = KT * DP * 2;                // bytes of a step's keys, or values
   constexpr int RS = DP + 4;                     // row stride of the sums
@@ -219,65 +227,69 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   if (tid == 0) wrong = 0;
   __syncthreads();
 
-  // A step's chunk i KPR CPK + tid: 16 bytes of LDS, at place tid % CPK of key tid / CPK + i KPR's row, where one chunk of dims lies
-  // (place_of is its own inverse).  A thread loads the chunk that belongs there.
-  const int c_key = tid / CPK, ps = a.kv.page_size;
-  auto dims_of = [&](int i) { return place_of<DP>(c_key + i * KPR, tid % CPK) * 8; };
+  // A step's keys come as runs of sixteen, NR to a wave; a load brings KPI keys of one, each lane 16 bytes of LDS: at place lane % CPK of
+  // its key's row, where one chunk of dims lies (place_of is its own inverse).
+  const int ps = a.kv.page_size, key0 = wave * NR * RL;
+  auto key_of = [&](int r, int j) { return key0 + r * RL + j * KPI + lane / CPK; };   // of the step
+  auto dims_of = [&](int j) { return place_of<DP>(j * KPI + lane / CPK, lane % CPK) * 8; };
+  auto at_of = [&](int r, int j) { return (key0 + r * RL) * DP * 2 + j * 1024; };     // of lane 0's bytes
   typedef const __attribute__((address_space(4))) int32_t* Uniform;
   const int32_t* table = a.table + (int64_t)t.b * a.table_row;
   const C* const kb = (const C*)a.kv.k + kvh * a.kv.k_head;
   const C* const vb = (const C*)a.kv.v + kvh * a.kv.v_head;
   auto page_of = [&](int key) { return (int)(__umulhi(2u * (uint32_t)key, a.magic) >> a.shift); };
   struct Raw { uint32_t w[F8 ? 2 : 4]; };
-  constexpr int HELD = DIRECT ? 1 : NCH;
+  constexpr int HELD = DIRECT ? 1 : NR * NI;
   Raw kr[HELD], vr[HELD];
-  const uint32_t lds_at = (uint32_t)(uintptr_t)(Lds)lds + wave * 1024;
-  int page[NCH], place[NCH];   // of a step that is fetched next: its runs' pages, and the places of their first keys (RUNS)
-  int run_at = page_of(k_begin), run_place = k_begin - run_at * ps;
-  const int run_last = k_end > 0 ? page_of(k_end - 1) : 0;
-  auto look = [&](int base) {
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(Lds)lds;
+  constexpr int PAGES = RUNS ? NR : NR * NI;
+  int page[PAGES], place[PAGES];   // of the step that is fetched next: pages, and places in them
+  const int last = max(0, k_end - 1);
+  auto look = [&](int base) {      // a key behind the last is read as the last one's page, and not used
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      if constexpr (RUNS) {   // runs follow one another; one behind the last key is read as any other, and not used
-        page[i] = ((Uniform)table)[min(run_at, run_last)];
-        place[i] = run_place;
-        run_place += KPR;
-        if (run_place == ps) run_place = 0, ++run_at;
-      } else {
-        const int key = base + c_key + i * KPR;
-        page[i] = key < k_end ? table[page_of(key)] : 0;
-      }
+    for (int i = 0; i < PAGES; ++i) {
+      const int key = min(base + (RUNS ? key0 + i * RL : key_of(i / NI, i % NI)), RUNS ? last & ~(RL - 1) : last), at = page_of(key);
+      if constexpr (RUNS) page[i] = ((Uniform)table)[at];
+      else page[i] = table[at];
+      place[i] = key - at * ps;
     }
   };
   // The chunks of a step's keys and values: on their way to LDS (DIRECT) or to registers.
   const uint32_t k_page = (uint32_t)a.kv.k_page * sizeof(C), v_page = (uint32_t)a.kv.v_page * sizeof(C);
   const uint32_t k_tok = (uint32_t)a.kv.k_token * sizeof(C), v_tok = (uint32_t)a.kv.v_token * sizeof(C);
-  const bool alike = k_page == v_page && k_tok == v_tok;
-  auto fetch = [&](int base, int buf) {
+  uint32_t k_own[RUNS ? NI : 1], v_own[RUNS ? NI : 1];   // a lane's bytes of a run, from its first key's
+  if constexpr (RUNS)
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
+    for (int j = 0; j < NI; ++j) {
+      k_own[j] = (j * KPI + lane / CPK) * k_tok + dims_of(j) * (uint32_t)sizeof(C);
+      v_own[j] = (j * KPI + lane / CPK) * v_tok + dims_of(j) * (uint32_t)sizeof(C);
+    }
+  auto fetch = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < PAGES; ++i) {
       const bool out = (uint32_t)page[i] >= (uint32_t)a.kv.pages;   // a page outside of the cache is not read
       top_page = max(top_page, (uint32_t)page[i]);
+      const uint32_t p = out ? 0 : page[i];
       if constexpr (RUNS) {
-        const uint32_t p = out ? 0 : page[i];
-        const uint64_t ko = (uint64_t)p * k_page + (uint32_t)place[i] * k_tok, vo = alike ? ko : (uint64_t)p * v_page + (uint32_t)place[i] * v_tok;
-        const char *kp = (const char*)kb + ko, *vp = (const char*)vb + vo;
-        const uint32_t k_own = c_key * k_tok + dims_of(i) * (uint32_t)sizeof(C), v_own = c_key * v_tok + dims_of(i) * (uint32_t)sizeof(C);
-        if constexpr (DIRECT) {
-          const uint32_t to = lds_at + buf * 2 * TB + i * 4096;
-          load_to_lds((uint64_t)kp, k_own, to);
-          load_to_lds((uint64_t)vp, v_own, to + TB);
-        } else {
-          __builtin_memcpy(&kr[i], __builtin_assume_aligned(kp + k_own, sizeof(Raw)), sizeof(Raw));
-          __builtin_memcpy(&vr[i], __builtin_assume_aligned(vp + v_own, sizeof(Raw)), sizeof(Raw));
+        const char* const kp = (const char*)kb + ((uint64_t)p * k_page + (uint32_t)place[i] * k_tok);
+        const char* const vp = (const char*)vb + ((uint64_t)p * v_page + (uint32_t)place[i] * v_tok);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          if constexpr (DIRECT) {
+            const uint32_t to = lds_at + buf * 2 * TB + at_of(i, j);
+            load_to_lds((uint64_t)kp, k_own[j], to);
+            load_to_lds((uint64_t)vp, v_own[j], to + TB);
+          } else {
+            __builtin_memcpy(&kr[i * NI + j], __builtin_assume_aligned(kp + k_own[j], sizeof(Raw)), sizeof(Raw));
+            __builtin_memcpy(&vr[i * NI + j], __builtin_assume_aligned(vp + v_own[j], sizeof(Raw)), sizeof(Raw));
+          }
         }
       } else {
-        const int key = base + c_key + i * KPR;
-        const int64_t p = out ? 0 : page[i], o = key - page_of(key) * ps;
         Raw k{}, v{};
-        if (dims_of(i) < D && key < k_end && !out) {
-          __builtin_memcpy(&k, __builtin_assume_aligned(kb + p * a.kv.k_page + o * a.kv.k_token + dims_of(i), sizeof(Raw)), sizeof(Raw));
-          __builtin_memcpy(&v, __builtin_assume_aligned(vb + p * a.kv.v_page + o * a.kv.v_token + dims_of(i), sizeof(Raw)), sizeof(Raw));
+        const int d = dims_of(i % NI);
+        if (d < D) {
+          __builtin_memcpy(&k, __builtin_assume_aligned(kb + (int64_t)p * a.kv.k_page + (int64_t)place[i] * a.kv.k_token + d, sizeof(Raw)), sizeof(Raw));
+          __builtin_memcpy(&v, __builtin_assume_aligned(vb + (int64_t)p * a.kv.v_page + (int64_t)place[i] * a.kv.v_token + d, sizeof(Raw)), sizeof(Raw));
         }
         kr[i] = k;
         vr[i] = v;
@@ -306,32 +318,23 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
     return any;
   };
   auto stage = [&](int base, int buf, int third) {
-    char* const at = lds + buf * 2 * TB + tid * 16;
-    if constexpr (DIRECT) {   // what has come, where it does not stay as it is
-      if (!mixed(base, KT)) return;   // (the last key is in none but a mixed step)
+    const bool some = mixed(base, KT);
+    if (DIRECT && !some) return;   // what has come stays as it is (the last key is in none but a mixed step)
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        const int key = c_key + i * KPR;
-        v4u* const v = (v4u*)(at + TB + i * 4096);
-        if (base + key >= k_end) {
-          *(v4u*)(at + i * 4096) = v4u{0, 0, 0, 0};
-          *v = v4u{0, 0, 0, 0};
-        } else {
-          v4u x = *v;
-          if (put_aside(x, key, third)) *v = x;
-        }
-      }
-    } else {
-      const bool some = mixed(base, KT);
-#pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        v4u k = wide(kr[i]), v = wide(vr[i]);
-        if (some) {
-          if (base + c_key + i * KPR >= k_end) k = v = v4u{0, 0, 0, 0};
-          put_aside(v, c_key + i * KPR, third);
-        }
-        *(v4u*)(at + i * 4096) = k;
-        *(v4u*)(at + TB + i * 4096) = v;
+    for (int i = 0; i < NR * NI; ++i) {
+      const int key = key_of(i / NI, i % NI);
+      v4u* const to = (v4u*)(lds + buf * 2 * TB + at_of(i / NI, i % NI) + lane * 16);
+      v4u *const k = to, *const v = (v4u*)((char*)to + TB);
+      v4u x = v4u{0, 0, 0, 0};
+      if constexpr (DIRECT) {
+        if (base + key >= k_end) *k = *v = x;   // behind the last key: whatever there was
+        else if (x = *v, put_aside(x, key, third)) *v = x;
+      } else {
+        const bool there = !some || base + key < k_end;
+        *k = there ? wide(kr[i]) : x;
+        x = there ? wide(vr[i]) : x;
+        if (some) put_aside(x, key, third);
+        *v = x;
       }
     }
   };
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
 
   if (steps > 0) {
     look(k_begin);
-    fetch(k_begin, 0);
+    fetch(0);
     if constexpr (!DIRECT) stage(k_begin, 0, 0);
     look(k_begin + KT);
   }
@@ -360,7 +363,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
       __syncthreads();
     }
     if (more) {
-      fetch(base + KT, buf ^ 1);
+      fetch(buf ^ 1);
       look(base + 2 * KT);
     }
     if (mixed(base - KT, KT) && tid < KT / 32) odd[third_free][tid] = 0;   // the last step's: written again two steps from now at the earliest
@@ -388,6 +391,18 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
       v4u vf[2 * ND];
 #pragma unroll
       for (int x = 0; x < 2 * ND; ++x) vf[x] = values(0, x);
+      // six reads ahead of the products (of the compiler two: 592 -> 577 us for a chunk of 4096 tokens behind 4096)
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+      for (int i = 0; i < NM * KB - 6; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 6; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      }
       if (mixed(first, 32 * KB)) {
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
@@ -396,12 +411,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
           for (int i = 0; i < 16; ++i) sc[b][i] = mine >> ((i & 3) + 8 * (i >> 2)) & 1 ? sc[b][i] : -inf;
         }
       }
-      float top = sc[0][0];
+      // (a median with infinity is the larger; of fmaxf the compiler makes two instructions for a product's result)
+      float top = -inf;
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[b][i]);
-      top = fmaxf(top, __shfl_xor(top, 32)) * scale;
+        for (int i = 0; i < 16; ++i) top = __builtin_amdgcn_fmed3f(top, sc[b][i], inf);
+      top = over_halves(top) * scale;
       const float mn = fmaxf(m, top), mb = base_of(mn);
       if (__any(mn != m)) {   // rarely, once the first keys were seen
         const float f = __builtin_amdgcn_exp2f(m - mb);
@@ -450,7 +466,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
           pt[k] = v4u{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
         }
 #pragma unroll
-        for (int x = 0; x < 2 * ND; ++x) {
+        for (int y = 0; y < 2 * ND; ++y) {   // all dims of sixteen keys, then of the others: no product waits for the one before
+          const int x = (y % ND) * 2 + y / ND;
           acc[x >> 1] = mfma32(vf[x], pt[x & 1], acc[x >> 1], T{});
           if (b + 1 < KB) vf[x] = values(b + 1, x);
         }
@@ -593,9 +610,8 @@ void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
 
 template <typename T, typename C, int DP>
 void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
-  constexpr int run = 256 * 8 / DP;   // keys of a round of loads
-  const int64_t far = (int64_t)a.kv.page_size * std::max(a.kv.k_token, a.kv.v_token) * (int64_t)sizeof(C);   // bytes of a page, from its first key's
-  if (a.kv.dim == DP && a.kv.page_size % run == 0 && far <= 0x7fffffff) launch<T, C, DP, true>(a, c, st);
+  const int64_t page_bytes = (int64_t)a.kv.page_size * std::max(a.kv.k_token, a.kv.v_token) * (int64_t)sizeof(C);   // from its first key to the next's
+  if (a.kv.dim == DP && a.kv.page_size % 16 == 0 && page_bytes <= 0x7fffffff) launch<T, C, DP, true>(a, c, st);
   else launch<T, C, DP, false>(a, c, st);
 }
 
