@@ -24,28 +24,37 @@ struct NormArgs {
 };
 
 // Up to eight values of a row: 16 bytes at any address of the type (unaligned 16-byte accesses are the hardware's own), the row's last
-// ones one by one.
-template <typename T> __device__ __forceinline__ void load_some(const T* p, int n, T* v) {
+// ones one by one.  STREAM: lines that leave the caches first.
+typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
+template <bool STREAM, typename T> __device__ __forceinline__ void load_some(const T* p, int n, T* v) {
   if (n >= 8) {
-    __builtin_memcpy(v, p, 8 * sizeof(T));
+    if constexpr (STREAM && sizeof(T) == 2) {
+      const any4 x = __builtin_nontemporal_load((const any4*)p);
+      __builtin_memcpy(v, &x, 16);
+    } else {
+      __builtin_memcpy(v, p, 8 * sizeof(T));
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : (T)0.f;
   }
 }
-template <typename T> __device__ __forceinline__ void store_some(T* p, int n, const float* x) {
+template <bool STREAM, typename T> __device__ __forceinline__ void store_some(T* p, int n, const float* x) {
   T v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = from_f<T>(x[e]);
   if (n >= 8) {
-    __builtin_memcpy(p, v, 8 * sizeof(T));
+    any4 y;
+    __builtin_memcpy(&y, v, 16);
+    if constexpr (STREAM) __builtin_nontemporal_store(y, (any4*)p);
+    else *(any4*)p = y;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e < n) p[e] = v[e];
   }
 }
-template <> __device__ __forceinline__ void store_some(fp8_t* p, int n, const float* x) {
+template <bool STREAM> __device__ __forceinline__ void store_some(fp8_t* p, int n, const float* x) {
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = x[e] != x[e] ? x[e] : fminf(fmaxf(x[e], -kFp8Max), kFp8Max);
@@ -72,26 +81,27 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x, int lanes) {
 // What the type's largest value stands for: a maximum below 2^-100 counts as that (a row of zeros is zeros times it).
 __device__ __forceinline__ float top_of(uint32_t bits) { return __builtin_bit_cast(float, max(bits, 27u << 23)); }
 
-// TR threads take a row, eight columns of it at a time; a row stays in registers from its one load to its store.
-template <typename T, typename O, int TR, int NC>
-__global__ __launch_bounds__(TR == 64 ? 256 : TR) void add_norm_kernel(NormArgs a) {
+// TR threads take a row, eight columns of it at a time; a row stays in registers from its one load to its store.  One pass over the bytes,
+// which bound it: 8191 rows of 5120, 336 MB in 61 us (5.5 TB/s; with lines that stay in the caches 85, with a wave for a row 78 and 109);
+// 96 rows of 17408 8 us, of one row 3: a launch and three trips to memory.
+template <typename T, typename O, int TR, int NC, bool STREAM>
+__global__ __launch_bounds__(TR) void add_norm_kernel(NormArgs a) {
   constexpr bool F8 = sizeof(O) == 1;
   constexpr int W = TR / 64;   // waves of a row
   __shared__ float part[2][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = TR == 64 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-  if (row >= a.rows) return;
-  const int tid = TR == 64 ? threadIdx.x & 63 : threadIdx.x, dim = a.dim;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, dim = a.dim;
   const T* x = (const T*)a.x + row * a.x_row;
   const T* r = (const T*)a.r + row * a.r_row;
   float s[NC][8];
   {
     T vx[NC][8], vr[NC][8];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) load_some(x + (int64_t)(i * TR + tid) * 8, dim - (i * TR + tid) * 8, vx[i]);
+    for (int i = 0; i < NC; ++i) load_some<STREAM>(x + (int64_t)(i * TR + tid) * 8, dim - (i * TR + tid) * 8, vx[i]);
     if (a.r)
 #pragma unroll
-      for (int i = 0; i < NC; ++i) load_some(r + (int64_t)(i * TR + tid) * 8, dim - (i * TR + tid) * 8, vr[i]);
+      for (int i = 0; i < NC; ++i) load_some<STREAM>(r + (int64_t)(i * TR + tid) * 8, dim - (i * TR + tid) * 8, vr[i]);
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -105,7 +115,7 @@ __global__ __launch_bounds__(TR == 64 ? 256 : TR) void add_norm_kernel(NormArgs 
   if (a.out_r)   // after the row's loads, before any of its threads' other stores: it may be x or r
 #pragma unroll
     for (int i = 0; i < NC; ++i)
-      store_some((T*)a.out_r + row * a.or_row + (int64_t)(i * TR + tid) * 8, dim - (i * TR + tid) * 8, s[i]);
+      store_some<STREAM>((T*)a.out_r + row * a.or_row + (int64_t)(i * TR + tid) * 8, dim - (i * TR + tid) * 8, s[i]);
   ss = lane_sum<32>(ss);
   ss += __shfl_xor(ss, 32);
   if constexpr (W > 1) {
@@ -125,10 +135,10 @@ __global__ __launch_bounds__(TR == 64 ? 256 : TR) void add_norm_kernel(NormArgs 
     for (int e = 0; e < 8; ++e) w[e] = 1.f;
     if (a.w) {
       if (a.weight_f32) {
-        load_some((const float*)a.w + d, n, w);
+        load_some<false>((const float*)a.w + d, n, w);
       } else {
         T t[8];
-        load_some((const T*)a.w + d, n, t);
+        load_some<false>((const T*)a.w + d, n, t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = to_f(t[e]);
       }
@@ -138,7 +148,7 @@ __global__ __launch_bounds__(TR == 64 ? 256 : TR) void add_norm_kernel(NormArgs 
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[i][e] = e < n ? s[i][e] * f * w[e] : 0.f;
-    if constexpr (!F8) store_some((O*)a.out + row * a.out_row + d, n, s[i]);
+    if constexpr (!F8) store_some<STREAM>((O*)a.out + row * a.out_row + d, n, s[i]);
   }
   if constexpr (F8) {
     uint32_t top[NC], all = 0;
@@ -177,37 +187,33 @@ __global__ __launch_bounds__(TR == 64 ? 256 : TR) void add_norm_kernel(NormArgs 
       const float inv = kFp8Max / top_of(top[i]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[i][e] *= inv;
-      store_some((O*)a.out + row * a.out_row + d, n, s[i]);
+      store_some<STREAM>((O*)a.out + row * a.out_row + d, n, s[i]);
     }
   }
 }
 
-template <typename T, typename O, int TR>
-void launch(const NormArgs& a, int nc, hipStream_t st) {
-  const dim3 grid((unsigned)(TR == 64 ? (a.rows + 3) / 4 : a.rows));
-  constexpr int TB = TR == 64 ? 256 : TR;
-#define GQK_NC(N) add_norm_kernel<T, O, TR, N><<<grid, TB, 0, st>>>(a)
-  if (nc <= 1) GQK_NC(1);
-  else if (nc == 2) GQK_NC(2);
-  else if (nc == 3) GQK_NC(3);
-  else if (nc == 4) GQK_NC(4);
-  if constexpr (TR < 1024) {
-    if (nc > 4 && nc <= 6) GQK_NC(6);
-    else if (nc > 6 && nc <= 8) GQK_NC(8);
-    else if (nc > 8) GQK_NC(10);
-  }
-#undef GQK_NC
+template <typename T, typename O, int TR, bool STREAM>
+void launch(const NormArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)a.rows);
+  const int nc = (a.dim + 8 * TR - 1) / (8 * TR);
+  if (nc <= 1) add_norm_kernel<T, O, TR, 1, STREAM><<<grid, TR, 0, st>>>(a);
+  else if (nc == 2) add_norm_kernel<T, O, TR, 2, STREAM><<<grid, TR, 0, st>>>(a);
+  else if (nc == 3) add_norm_kernel<T, O, TR, 3, STREAM><<<grid, TR, 0, st>>>(a);
+  else add_norm_kernel<T, O, TR, 4, STREAM><<<grid, TR, 0, st>>>(a);
 }
 
-constexpr int kMostChunks = 10;   // of a thread: what fits its registers
-
+// 1024 threads to a row where a thread of 256 would have more than four chunks of it, or in short batches more than one (512 rows of 5120: 8.0
+// -> 7.2 us).  What passes the caches by far leaves them first (2048 rows of 5120, 84 MB: 22.0 -> 19.6; 1024 rows the same either way).
 template <typename T, typename O>
 void launch(const NormArgs& a, hipStream_t st) {
-  auto nc = [&](int threads) { return (a.dim + 8 * threads - 1) / (8 * threads); };
-  if (a.rows >= 2048 && nc(64) <= kMostChunks) launch<T, O, 64>(a, nc(64), st);
-  else if (a.rows >= 512 && nc(256) <= kMostChunks) launch<T, O, 256>(a, nc(256), st);
-  else if (nc(256) == 1) launch<T, O, 256>(a, 1, st);
-  else launch<T, O, 1024>(a, nc(1024), st);
+  const bool wide = a.dim > 8192 || (a.rows < 1024 && a.dim > 2048);
+  if (a.rows * a.dim >= 8 << 20) {
+    if (wide) launch<T, O, 1024, true>(a, st);
+    else launch<T, O, 256, true>(a, st);
+  } else {
+    if (wide) launch<T, O, 1024, false>(a, st);
+    else launch<T, O, 256, false>(a, st);
+  }
 }
 
 }  // namespace
