@@ -107,11 +107,30 @@ __global__ __launch_bounds__(TR) void add_norm_kernel(NormArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[i][e] = to_f(vx[i][e]) + (a.r ? to_f(vr[i][e]) : 0.f);
   }
+  float w[NC][8];   // on their way while the row is summed up
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int d = (i * TR + tid) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[i][e] = 1.f;
+    if (!a.w) continue;
+    if (a.weight_f32) {
+      load_some<false>((const float*)a.w + d, dim - d, w[i]);
+    } else {
+      T t[8];
+      load_some<false>((const T*)a.w + d, dim - d, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[i][e] = to_f(t[e]);
+    }
+  }
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < NC; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += s[i][e] * s[i][e];
+    for (int e = 0; e < 8; ++e) {
+      ss += s[i][e] * s[i][e];
+      w[i][e] += a.unit_offset ? 1.f : 0.f;
+    }
   if (a.out_r)   // after the row's loads, before any of its threads' other stores: it may be x or r
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -130,24 +149,8 @@ __global__ __launch_bounds__(TR) void add_norm_kernel(NormArgs a) {
   for (int i = 0; i < NC; ++i) {
     const int d = (i * TR + tid) * 8, n = dim - d;
     if (n <= 0) continue;
-    float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = 1.f;
-    if (a.w) {
-      if (a.weight_f32) {
-        load_some<false>((const float*)a.w + d, n, w);
-      } else {
-        T t[8];
-        load_some<false>((const T*)a.w + d, n, t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = to_f(t[e]);
-      }
-      if (a.unit_offset)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] += 1.f;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s[i][e] = e < n ? s[i][e] * f * w[e] : 0.f;
+    for (int e = 0; e < 8; ++e) s[i][e] = e < n ? s[i][e] * f * w[i][e] : 0.f;
     if constexpr (!F8) store_some<STREAM>((O*)a.out + row * a.out_row + d, n, s[i]);
   }
   if constexpr (F8) {
