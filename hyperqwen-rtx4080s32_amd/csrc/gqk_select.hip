@@ -56,11 +56,13 @@ struct BoundsArgs {
   int pages, page_size, heads, dim, width, count;
 };
 
-// A workgroup takes one page of one key head: its threads the page's keys, eight dims of one at a time.
+// A workgroup takes one page of one key head: its threads the page's keys, eight dims of one at a time.  Everything is in the trips to memory
+// that follow one another: the length, the table, the keys, the store.  (One page of 64 keys of 8 heads: 14 us where one thread of a dim
+// went through the 16 keys that the others had left, 6 with the waves' own sums first.)
 template <typename C, int DP>
 __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
   constexpr int LPK = DP / 8, KPW = 256 / LPK;   // lanes of a key, keys at once
-  __shared__ float ends[2][KPW][DP];
+  __shared__ float ends[2][4][DP];
   const int b = blockIdx.x, h = blockIdx.z, len = a.lengths[b];
   if (len <= 0 || len > (int64_t)a.width * a.page_size) return;
   const int first = max(0, len - a.count) / a.page_size, j = first + blockIdx.y;
@@ -68,45 +70,52 @@ __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
   const int page = a.table[(int64_t)b * a.table_row + j];
   if ((uint32_t)page >= (uint32_t)a.pages) return;
   const int keys = min(a.page_size, len - j * a.page_size);
-  const int at = threadIdx.x / LPK, d = (threadIdx.x % LPK) * 8;
+  const int at = threadIdx.x / LPK, d = (threadIdx.x % LPK) * 8, wave = threadIdx.x >> 6;
   const bool live = d < a.dim;
   const C* base = (const C*)a.k + page * a.k_page + h * a.k_head + (live ? d : 0);
   const float inf = __builtin_huge_valf(), nan = __builtin_nanf("");
-  float lo[8], hi[8];
+  float lo[8], hi[8];   // a dim with a NaN has NaN for both
 #pragma unroll
   for (int e = 0; e < 8; ++e) { lo[e] = inf; hi[e] = -inf; }
-  bool bad[8] = {};
-  for (int i = at; i < keys; i += KPW) {
-    float x[8];
-    load8(base + (int64_t)i * a.k_token, x);
+  auto lower = [&](float x, float y) { return x != x || y != y ? nan : fminf(x, y); };
+  auto upper = [&](float x, float y) { return x != x || y != y ? nan : fmaxf(x, y); };
+  for (int i = at; i < keys; i += 4 * KPW) {
+    float x[4][8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) load8(base + (int64_t)min(i + k * KPW, keys - 1) * a.k_token, x[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        lo[e] = lower(lo[e], x[k][e]);
+        hi[e] = upper(hi[e], x[k][e]);
+      }
+  }
+#pragma unroll
+  for (int o = LPK; o < 64; o <<= 1)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      lo[e] = fminf(lo[e], x[e]);
-      hi[e] = fmaxf(hi[e], x[e]);
-      bad[e] |= x[e] != x[e];
+      lo[e] = lower(lo[e], __shfl_xor(lo[e], o));
+      hi[e] = upper(hi[e], __shfl_xor(hi[e], o));
     }
-  }
+  if ((threadIdx.x & 63) < LPK)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {   // a dim with a NaN has NaN for both bounds
-    ends[0][at][d + e] = bad[e] ? nan : lo[e];
-    ends[1][at][d + e] = bad[e] ? nan : hi[e];
-  }
+    for (int e = 0; e < 8; ++e) {
+      ends[0][wave][d + e] = lo[e];
+      ends[1][wave][d + e] = hi[e];
+    }
   __syncthreads();
   // one thread for each eight dims of a bound
-  if (threadIdx.x >= 2 * LPK) return;
-  const int which = threadIdx.x / LPK, dd = (threadIdx.x % LPK) * 8;
-  if (dd >= a.dim) return;
+  if (threadIdx.x >= 2 * LPK || !live) return;
+  const int which = threadIdx.x / LPK;
   float y[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    float m = ends[which][0][dd + e];
-    for (int i = 1; i < min(KPW, keys); ++i) {
-      const float x = ends[which][i][dd + e];
-      m = m != m || x != x ? nan : which ? fmaxf(m, x) : fminf(m, x);
-    }
-    y[e] = m;
+    y[e] = ends[which][0][d + e];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) y[e] = which ? upper(y[e], ends[1][w][d + e]) : lower(y[e], ends[0][w][d + e]);
   }
-  store8((C*)a.bounds + (((int64_t)page * 2 + which) * a.heads + h) * a.dim + dd, y);
+  store8((C*)a.bounds + (((int64_t)page * 2 + which) * a.heads + h) * a.dim + d, y);
 }
 
 // ---- scores ----------------------------------------------------------------------------------
@@ -137,8 +146,26 @@ __device__ __forceinline__ int pages_of(const SelectArgs& a, int len) {
   return len > a.max_length ? -1 : len <= 0 ? 0 : (len - 1) / a.page_size + 1;
 }
 
+template <int CTRL> __device__ __forceinline__ double dpp_add(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+  return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// the sum over 8, 16 or 32 neighbouring lanes
+template <int LANES> __device__ __forceinline__ double lane_sum(double x) {
+  x = dpp_add<0xB1>(x);    // quad_perm 1, 0, 3, 2
+  x = dpp_add<0x4E>(x);    // quad_perm 2, 3, 0, 1
+  x = dpp_add<0x141>(x);   // row_half_mirror
+  if constexpr (LANES >= 16) x = dpp_add<0x140>(x);   // row_mirror
+  if constexpr (LANES >= 32) x += __shfl_xor(x, 16);
+  return x;
+}
+
 // Eight dims of a page's bounds to a lane; products in 32 bits (exact: two factors of 16-bit types), sums in 64, as the comparison of near
-// equals decides which pages are read.
+// equals decides which pages are read.  The 64-bit sums bound it in a batch: up to 500 pages of 48 sequences, 8 heads, 40 of queries (31 MB in 8
+// bits) 29 us; 2048 pages of one (8 MB) 7.  (Sums in 32 bits first, and those in 64 of the heads within their error of the largest alone: 29 and 10, as
+// the queries' norms, the registers that hold them and the second reading of a query cost what it saves.)
 template <typename T, typename C, int DP>
 __global__ __launch_bounds__(256) void score_kernel(SelectArgs a) {
   constexpr int LPP = DP / 8, PPW = 256 / LPP;   // lanes of a page, pages at once
@@ -167,8 +194,7 @@ __global__ __launch_bounds__(256) void score_kernel(SelectArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum += (double)(x[e] * (x[e] >= 0.f ? hi[e] : lo[e]));
         if (!live) sum = 0.0;
-#pragma unroll
-        for (int o = 1; o < LPP; o <<= 1) sum += __shfl_xor(sum, o);
+        sum = lane_sum<LPP>(sum);
         bad |= sum != sum;
         best = fmax(best, sum);
       }
@@ -180,16 +206,21 @@ __global__ __launch_bounds__(256) void score_kernel(SelectArgs a) {
 
 // ---- the choice ------------------------------------------------------------------------------
 
-constexpr int kSelect = 1024, kSelectWaves = kSelect / 64, kHeld = 8;
+constexpr int kHeld = 8;
 
-// A workgroup chooses for one key head of one sequence: the keep-th largest key by its digits from the highest in which the keys differ,
-// until a digit's bin holds just what is left to take, then the pages above it in their order.  A wave's keys are neighbours; up to
-// eight to a lane stay in registers.
-__global__ __launch_bounds__(kSelect) void select_kernel(SelectArgs a) {
+// A workgroup chooses for one key head of one sequence: the keep-th largest key by its digits of eight bits, from the highest in which the keys
+// differ, until the digit's bin holds just what is left to take, or few enough keys to be compared with each other by one wave; then the pages
+// above it in their order.  A wave's keys are neighbours; up to eight to a lane stay in registers.  500 pages of 8 heads of 48 sequences 8.6 us, of
+// 256 threads each (22 of 1024, digit by digit to the end), 2048 pages of 8 heads of one 9 (13): a launch, four trips to memory and some ten barriers.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void select_kernel(SelectArgs a) {
+  constexpr int WAVES = THREADS / 64;
   __shared__ int bins[256];
-  __shared__ uint64_t ends[2][kSelectWaves];
-  __shared__ int counts[2][kSelectWaves];
-  __shared__ int found[2];
+  __shared__ uint32_t ends[2][WAVES];
+  __shared__ int counts[2][WAVES];
+  __shared__ uint64_t near[64];
+  __shared__ int some, found[2];
+  __shared__ uint64_t edge;
   const int b = a.batch0 + blockIdx.y, h = blockIdx.x, len = a.lengths[b], n = pages_of(a, len);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t* table = a.table + (int64_t)b * a.table_row;
@@ -199,11 +230,11 @@ __global__ __launch_bounds__(kSelect) void select_kernel(SelectArgs a) {
     a.out_lengths[b] = n < 0 ? 0x7fffffff : over <= 0 ? max(0, len) : len - over * a.page_size;
   }
   if (n <= a.keep) {
-    for (int j = tid; j < a.keep; j += kSelect) out[j] = j < n ? table[j] : -1;
+    for (int j = tid; j < a.keep; j += THREADS) out[j] = j < n ? table[j] : -1;
     return;
   }
   const uint64_t* keys = a.keys + ((int64_t)blockIdx.y * a.heads + h) * a.most;
-  const int each = ((n + kSelect - 1) / kSelect) * 64, begin = wave * each;   // of a wave
+  const int each = ((n + THREADS - 1) / THREADS) * 64, begin = wave * each;   // of a wave
   const int rounds = each / 64;
   uint64_t held[kHeld];
   auto load = [&](int r0) {
@@ -215,42 +246,44 @@ __global__ __launch_bounds__(kSelect) void select_kernel(SelectArgs a) {
   };
   load(0);
   const bool all = rounds <= kHeld;
-  // where the keys begin to differ
-  uint64_t low = ~0ull, high = 0;
+  // where the keys begin to differ: by their upper halves
+  uint32_t low = ~0u, high = 0;
   for (int r0 = 0; r0 < rounds; r0 += kHeld) {
     if (!all) load(r0);
 #pragma unroll
     for (int r = 0; r < kHeld; ++r)
       if (held[r]) {
-        low = min(low, held[r]);
-        high = max(high, held[r] == kTaken ? 0 : held[r]);
+        const uint32_t up = held[r] >> 32;
+        low = min(low, up);
+        high = max(high, held[r] == kTaken ? 0u : up);
       }
   }
   for (int o = 32; o > 0; o >>= 1) {
-    low = min(low, (uint64_t)__shfl_xor((unsigned long long)low, o));
-    high = max(high, (uint64_t)__shfl_xor((unsigned long long)high, o));
+    low = min(low, (uint32_t)__shfl_xor((int)low, o));
+    high = max(high, (uint32_t)__shfl_xor((int)high, o));
   }
   if (lane == 0) { ends[0][wave] = low; ends[1][wave] = high; }
+  if (tid < 256) bins[tid] = 0;
+  if (tid == 0) some = 0;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kSelectWaves; ++k) { low = min(low, ends[0][k]); high = max(high, ends[1][k]); }
-  // those always taken are above all others: a difference that they do not widen
-  auto rank_of = [&](uint64_t key) { return key == 0 ? 0 : key == kTaken ? high - low + 2 : key - low + 1; };
-  int left = a.keep, bits = 64 - __builtin_clzll(high - low + 2);
+  for (int k = 0; k < WAVES; ++k) { low = min(low, ends[0][k]); high = max(high, ends[1][k]); }
+  high = max(low, high);
+  // keys less what they have in common; those always taken are above all others, by as little as there is
+  const uint64_t base = (uint64_t)low << 32, top = ((uint64_t)(high - low) + 1) << 32;
+  auto rank_of = [&](uint64_t key) { return key == kTaken ? top : key - base; };
+  int left = a.keep, bits = 64 - __builtin_clzll(top);
   uint64_t prefix = 0;   // of the keep-th largest rank, its bits above `bits`
   bool exact = false;    // everything at or above prefix is taken
-  while (bits > 0 && !exact) {
+  while (bits > 0) {
     const int digit = min(8, bits);
     bits -= digit;
-    if (tid < 256) bins[tid] = 0;
-    __syncthreads();
     for (int r0 = 0; r0 < rounds; r0 += kHeld) {
       if (!all) load(r0);
 #pragma unroll
       for (int r = 0; r < kHeld; ++r) {
         const uint64_t x = rank_of(held[r]);
-        // (the shift by all of its 64 bits is none)
-        if (held[r] && (bits + digit >= 64 || x >> (bits + digit) == prefix >> (bits + digit))) atomicAdd(&bins[(x >> bits) & 255], 1);
+        if (held[r] && x >> bits >> digit == prefix >> bits >> digit) atomicAdd(&bins[(x >> bits) & 255], 1);
       }
     }
     __syncthreads();
@@ -271,10 +304,38 @@ __global__ __launch_bounds__(kSelect) void select_kernel(SelectArgs a) {
       }
     }
     __syncthreads();
-    const int bin = found[0];
+    const int bin = found[0], held_by = bins[bin];
     left -= found[1];
     prefix |= (uint64_t)bin << bits;
-    exact = bins[bin] == left;
+    exact = held_by == left;
+    if (exact || bits == 0) break;
+    if (held_by <= 64) {
+      for (int r0 = 0; r0 < rounds; r0 += kHeld) {
+        if (!all) load(r0);
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+          const uint64_t x = rank_of(held[r]);
+          if (held[r] && x >> bits == prefix >> bits) near[atomicAdd(&some, 1)] = x;
+        }
+      }
+      __syncthreads();
+      if (wave == 0) {   // the left-th largest of them, and how many of its equals are to be taken
+        const uint64_t mine = lane < held_by ? near[lane] : 0;
+        int more = 0, same = 0;
+        for (int k = 0; k < held_by; ++k) {
+          const uint64_t x = near[k];
+          more += x > mine;
+          same += x == mine;
+        }
+        if (lane < held_by && more < left && more + same >= left) { edge = mine; found[1] = left - more; }   // (equals write the same)
+      }
+      __syncthreads();
+      prefix = edge;
+      left = found[1];
+      break;
+    }
+    __syncthreads();
+    if (tid < 256) bins[tid] = 0;
     __syncthreads();
   }
   // What is above is taken, and of the equal ones the first `left` (all, where exact).
@@ -301,7 +362,7 @@ __global__ __launch_bounds__(kSelect) void select_kernel(SelectArgs a) {
       const uint64_t up = __ballot(above_of(held[r])), eq = __ballot(equal_to(held[r]));
       const int rank = same + __popcll(eq & under);
       const bool mine = (up >> lane & 1) || ((eq >> lane & 1) && rank < left);
-      const int place = more + __popcll(up & under) + min(rank, exact ? 0 : left);
+      const int place = more + __popcll(up & under) + (exact ? 0 : min(rank, left));
       if (mine && place < a.keep) out[place] = table[begin + (r0 + r) * 64 + lane];
       more += __popcll(up);
       same += __popcll(eq);
@@ -421,7 +482,9 @@ int gqk_select_pages(const void* q, int64_t q_row, int64_t q_head, int dtype, in
         score<f16_t, f16_t>(a, grid, st);
       }
     }
-    select_kernel<<<dim3(heads, n), kSelect, 0, st>>>(a);
+    // what 256 threads hold in registers, they choose of fastest: fewer waves meet at the barriers
+    if (a.most <= 256 * kHeld) select_kernel<256><<<dim3(heads, n), 256, 0, st>>>(a);
+    else select_kernel<1024><<<dim3(heads, n), 1024, 0, st>>>(a);
   }
   return decode_launched(what);
 }
