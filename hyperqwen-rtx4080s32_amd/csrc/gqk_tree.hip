@@ -15,6 +15,7 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 constexpr int kMostSplits = 256;
+constexpr int kStep = 64;   // keys of a step
 
 struct TreeArgs {
   const void* q;
@@ -32,6 +33,7 @@ struct TreeArgs {
   uint32_t sign;
   int chunk, splits;    // keys of a split, and the most splits of a row tile
   int slots;            // places for row tiles
+  bool once;            // a sequence has one: nobody else reads its keys, which leave the caches first
   uint32_t magic;       // key / page_size = 2 key magic >> 32 >> shift, exact below 2^31
   int shift;
 };
@@ -54,10 +56,13 @@ __device__ __forceinline__ float over_halves(float x) {
 // 16 bytes of every lane from base + own to LDS, the lanes' side by side from `to` on, while the wave goes on: it waits for vmcnt itself before
 // anyone reads them.  (Of the builtin the compiler waits for all of these loads before the next read of LDS, whichever it reads: 680 us for a chunk of
 // 4096 tokens behind 4096 where this took 593.)
+// ONCE: they leave the caches first (64 sequences of up to 4000 keys, 655 MB: 153 -> 146 us).
+template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t own, uint32_t to) {
   const v4u from{(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, 0xFFFFFFFFu, 0x00020000u};
 #ifdef __HIP_DEVICE_COMPILE__
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(own), "s"(from), "s"(to) : "memory", "m0");
+  if constexpr (ONCE) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(own), "s"(from), "s"(to) : "memory", "m0");
+  else asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(own), "s"(from), "s"(to) : "memory", "m0");
 #endif
 }
 
@@ -168,11 +173,20 @@ template <int DP> __device__ __forceinline__ int place_of(int key, int c) {
 //
 // Scores, statistics and sums are in 32 bits; the weights become T for the second product, as in the attention of single tokens.
 //
+// What bounds it (bf16, 40 heads over 8 of 128 dims).  Chunks of prompts, the matrix instructions and what the vector units do between them: 4096
+// tokens behind 4096, 516 GFLOP, 522 us, 988 TFLOP/s.  Trees, memory: 32 of up to 16 tokens behind up to 4000, 337 MB, 89 us, 3.8 TB/s, where loads
+// without the products take as long (partial sums of two splits move another 43 MB); 64 of 4, 655 MB, 136 us, 4.8 TB/s.  8-bit pages are widened on
+// the way to LDS, in every workgroup that reads them: four trees of up to 61 tokens behind 32768, 197 MB, 93 GFLOP, 164 us.  Workgroups of eight
+// waves and 256 rows were slower (581 us for the chunk, when this took 540), and so were three steps on their way (584), steps of 32 keys
+// (640), and halves of steps with a wait each (no faster for trees, 573 for the chunk).  Shares of equal steps, dealt over the tiles from
+// what the lengths are, gave 172 us for the four trees and 107 for the windows of cut_of, and 16 for the smallest call in place of 11.
+//
 // RUNS: pages hold whole runs of the keys of one round of loads, and heads all dims: a run's page is one number for the whole workgroup,
 // and a chunk's place in it the thread's own, so that nothing is computed per chunk.  16-bit pages then go to LDS directly.
-template <typename T, typename C, int DP, int KW, int KT, bool RUNS>
+template <typename T, typename C, int DP, int KW, bool RUNS>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {
   constexpr bool F8 = sizeof(C) == 1, DIRECT = RUNS && !F8;
+  constexpr int KT = kStep;
   constexpr int RW = 4 / KW, ROWS = 32 * RW;
   constexpr int NM = DP / 16, ND = DP / 32, CPK = DP / 8;
   constexpr int RL = 16, NR = KT / RL / 4;       // keys of a run, runs of a wave's share of a step
@@ -273,13 +287,20 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
       if constexpr (RUNS) {
         const char* const kp = (const char*)kb + ((uint64_t)p * k_page + (uint32_t)place[i] * k_tok);
         const char* const vp = (const char*)vb + ((uint64_t)p * v_page + (uint32_t)place[i] * v_tok);
+        auto load = [&]<bool ONCE>() {
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          if constexpr (DIRECT) {
+          for (int j = 0; j < NI; ++j) {
             const uint32_t to = lds_at + buf * 2 * TB + at_of(i, j);
-            load_to_lds((uint64_t)kp, k_own[j], to);
-            load_to_lds((uint64_t)vp, v_own[j], to + TB);
-          } else {
+            load_to_lds<ONCE>((uint64_t)kp, k_own[j], to);
+            load_to_lds<ONCE>((uint64_t)vp, v_own[j], to + TB);
+          }
+        };
+        if constexpr (DIRECT) {
+          if (a.once) load.template operator()<true>();
+          else load.template operator()<false>();
+        } else {
+#pragma unroll
+          for (int j = 0; j < NI; ++j) {
             __builtin_memcpy(&kr[i * NI + j], __builtin_assume_aligned(kp + k_own[j], sizeof(Raw)), sizeof(Raw));
             __builtin_memcpy(&vr[i * NI + j], __builtin_assume_aligned(vp + v_own[j], sizeof(Raw)), sizeof(Raw));
           }
@@ -570,28 +591,37 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
   }
 }
 
-// How a call is cut: rows of a tile, keys of a step, places for tiles, splits of `chunk` keys.
-struct Cut { int key_waves, rows, step, slots, splits, chunk; };
+// How a call is cut: waves that share a row's keys, rows of a tile, places for tiles, splits of `chunk` keys.
+struct Cut { int key_waves, rows, slots, splits, chunk; };
 
+// Up to 64 rows of a sequence are a tile of 64, in which two waves share the keys (16 sequences of up to 8000 8-bit keys and 8 tokens of 5 heads: 68 us, in
+// tiles of 128 rows 86; 64 of up to 4000 and 4 tokens 136 and 162; tiles of 32 rows with four waves to the keys, 128 a step: 146).
+//
+// Where the tiles that a batch is likely to have are fewer than the workgroups that stay resident, their keys are split, into as many
+// splits as still stay all at once: a few more would run on their own at the end (24 sequences of a window of 4096 keys, heads of 256 dims: 2
+// splits 85.6 us, 3 111, 4 94; one of 100000 keys: 64 splits 89 us, 128 109; 16 of up to 8000 8-bit keys: 4 splits 68, 5 83).  Tiles of prompts see
+// different lengths, so that a tenth more than stay do not run on their own (two prompts of 320 and 512 tokens behind 8000: 2 splits 171 us, none 211).
 Cut cut_of(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_tokens, int max_length, int window, int64_t workspace_bytes) {
   const int group = q_heads / kv_heads;
   const int64_t most = (int64_t)std::min(tokens, max_tokens) * group;   // rows of a sequence
   Cut c;
-  c.key_waves = most <= 32 && dim <= 128 ? 4 : most <= 64 ? 2 : 1;   // (of 256 dims 128 keys do not fit LDS)
+  c.key_waves = most <= 64 ? 2 : 1;
   c.rows = 32 * 4 / c.key_waves;
-  c.step = c.key_waves == 4 ? 128 : 64;
   const int64_t slots = (int64_t)tokens * group / c.rows + batch;
   c.slots = (int)slots;
   // keys that a row tile can see, from a multiple of 32
   const int64_t sees = std::min<int64_t>((int64_t)std::min(tokens, max_tokens), c.rows / group + 1);
   const int64_t span = std::min<int64_t>(max_length, window > 0 ? (int64_t)window + sees + std::min(tokens, max_tokens) + 31 : max_length);
-  const int64_t units = slots * kv_heads, wanted = 2LL * device_cus();
-  int64_t splits = std::max<int64_t>(1, std::min((wanted + units - 1) / std::max<int64_t>(1, units), (span + c.step - 1) / c.step));
+  const int64_t units = slots * kv_heads;
+  const int64_t stay = (int64_t)device_cus() * (dim <= 128 ? 2 : 1);   // workgroups, by their LDS
+  const bool one = most <= c.rows;
+  const int64_t tiles = std::max<int64_t>(1, one ? std::min(batch, tokens) : (int64_t)tokens * group / c.rows + batch / 2) * kv_heads;
+  int64_t splits = std::max<int64_t>(1, std::min((one ? stay : stay + stay / 10) / tiles, (span + kStep - 1) / kStep));
   splits = std::min<int64_t>(splits, kMostSplits);
   const int64_t each = units * c.rows * (dim + 4) * 4;   // bytes of one split of all units
   if (workspace_bytes < GQK_CTR_BYTES) splits = 1;
   else splits = std::max<int64_t>(1, std::min(splits, (workspace_bytes - GQK_CTR_BYTES) / std::max<int64_t>(1, each)));
-  c.chunk = (int)std::min<int64_t>(0x7fffff80, std::max<int64_t>(c.step, ((span + splits - 1) / splits + c.step - 1) / c.step * c.step));
+  c.chunk = (int)std::min<int64_t>(0x7fffff80, std::max<int64_t>(kStep, ((span + splits - 1) / splits + kStep - 1) / kStep * kStep));
   c.splits = (int)std::max<int64_t>(1, (span + c.chunk - 1) / c.chunk);
   return c;
 }
@@ -599,13 +629,8 @@ Cut cut_of(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_to
 template <typename T, typename C, int DP, bool RUNS>
 void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)c.slots * a.kv.heads), c.splits);
-  if constexpr (DP < 256)
-    if (c.key_waves == 4) {
-      tree_kernel<T, C, DP, 4, 128, RUNS><<<grid, 256, 0, st>>>(a);
-      return;
-    }
-  if (c.key_waves == 2) tree_kernel<T, C, DP, 2, 64, RUNS><<<grid, 256, 0, st>>>(a);
-  else tree_kernel<T, C, DP, 1, 64, RUNS><<<grid, 256, 0, st>>>(a);
+  if (c.key_waves == 2) tree_kernel<T, C, DP, 2, RUNS><<<grid, 256, 0, st>>>(a);
+  else tree_kernel<T, C, DP, 1, RUNS><<<grid, 256, 0, st>>>(a);
 }
 
 template <typename T, typename C, int DP>
@@ -625,8 +650,7 @@ void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
 template <typename T>
 void join(const TreeArgs& a, const Cut& c, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)c.slots * a.kv.heads * (c.rows / 8)));
-  if (c.rows == 32) tree_join_kernel<T, 32><<<grid, 256, 0, st>>>(a);
-  else if (c.rows == 64) tree_join_kernel<T, 64><<<grid, 256, 0, st>>>(a);
+  if (c.rows == 64) tree_join_kernel<T, 64><<<grid, 256, 0, st>>>(a);
   else tree_join_kernel<T, 128><<<grid, 256, 0, st>>>(a);
 }
 
@@ -675,7 +699,7 @@ int gqk_tree_attention(const void* q, int64_t q_row, int64_t q_head, int dtype, 
   a.q = q; a.q_row = q_row; a.q_head = q_head; a.kv = *pages; a.table = table; a.table_row = table_row; a.lengths = lengths; a.starts = starts;
   a.mask = mask; a.words = mask_words; a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.tokens = tokens; a.batch = batch;
   a.q_heads = q_heads; a.max_length = max_length; a.max_tokens = max_tokens; a.window = window; a.scale = fabsf(scale) * kLog2e; a.sign = scale < 0.f ? 0x80008000u : 0u;
-  a.chunk = c.chunk; a.splits = c.splits; a.slots = c.slots;
+  a.chunk = c.chunk; a.splits = c.splits; a.slots = c.slots; a.once = (int64_t)std::min(tokens, max_tokens) * (q_heads / pages->heads) <= c.rows;
   a.partials = workspace ? (float*)((char*)workspace + GQK_CTR_BYTES) : nullptr;
   const PageDivisor by = page_divisor(pages->page_size);
   a.magic = by.magic;
