@@ -1051,3 +1051,20 @@ def test_eight_bit_output_of_shared_memory_is_refused():
     x = _randn(_gen(1), 4, 256, dtype=BF)
     with pytest.raises(ValueError, match="memory of its own"):
         gguf_hip.add_rms_norm_fp8(x, None, out=x.view(F8)[:, :256])
+
+
+# ---- all together ----------------------------------------------------------------------------
+
+def test_draft_step_example():
+    """examples/draft_step.py: chunks of prompts, trees and sparse steps by graphs over a padded batch.  Per layer a token's value is
+    rounded at most ten times on its way (norm, projection, adapter, heads, cache, probabilities, attention, projection, adapter, residual),
+    weights once, each at most 2^-8 of it, and once by the last norm: two layers stay within 23 * 2^-8."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "draft_step.py")
+    spec = importlib.util.spec_from_file_location("draft_step", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    got = module.run(steps=5)
+    assert sorted(got["errors"]) == ["a", "b", "c"] and got["outputs"] > 150 and got["pages"] > got["keep"]
+    assert max(got["errors"].values()) < 23 * 2.0 ** -8, got
