@@ -63,9 +63,9 @@ template <typename C, int DP>
 __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
   constexpr int LPK = DP / 8, KPW = 256 / LPK;   // lanes of a key, keys at once
   __shared__ float ends[2][4][DP];
-  const int b = blockIdx.x, h = blockIdx.z, len = a.lengths[b];
+  const int b = blockIdx.y, h = blockIdx.z, len = a.lengths[b];
   if (len <= 0 || len > (int64_t)a.width * a.page_size) return;
-  const int first = max(0, len - a.count) / a.page_size, j = first + blockIdx.y;
+  const int first = max(0, len - a.count) / a.page_size, j = first + blockIdx.x;
   if (j > (len - 1) / a.page_size) return;
   const int page = a.table[(int64_t)b * a.table_row + j];
   if ((uint32_t)page >= (uint32_t)a.pages) return;
@@ -417,8 +417,7 @@ int gqk_page_bounds(const gqk_pages* pages, const int32_t* table, int64_t table_
   a.dim = pages->dim; a.width = table_width; a.count = count;
   const int most = (int)std::min<int64_t>(table_width, ((int64_t)count + pages->page_size - 2) / pages->page_size + 1);
   const hipStream_t st = (hipStream_t)stream;
-  if (most > 65535) return decode_fail(GQK_ERR_SHAPE, "%s: the last %d keys are in more than 65535 pages", what, count);
-  const dim3 grid(batch, most, a.heads);
+  const dim3 grid(most, batch, a.heads);
   if (pages->dtype == GQK_DTYPE_FP8) bounds<fp8_t>(a, grid, st);
   else if (pages->dtype == GQK_DTYPE_BF16) bounds<bf16_t>(a, grid, st);
   else bounds<f16_t>(a, grid, st);
