@@ -268,6 +268,12 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (w && (w->dim() != 1 || w->size(0) != dim || (w->scalar_type() != x->scalar_type() && w->scalar_type() != at::kFloat) ||
             !w->is_contiguous() || !same_device(*x, w)))
     return none();
+  // outputs that share memory with another tensor, unless row by row the same as an input: the Python path looks
+  for (const Tensor* o : {out, rout})
+    for (const Tensor* t : {x, r, w, rout})
+      if (o && t && o != t && o->storage().data() == t->storage().data() &&
+          (t == w || (o == out && t == rout) || o->data_ptr() != t->data_ptr() || (rows > 1 && o->stride(0) != t->stride(0))))
+        return none();
   Tensor made, scale, made_r;
   if (!out) made = at::empty({rows, dim}, f8 ? x->options().dtype(at::kFloat8_e4m3fn) : x->options());
   if (f8) scale = at::empty({rows, group ? dim / group : 1}, x->options().dtype(at::kFloat));

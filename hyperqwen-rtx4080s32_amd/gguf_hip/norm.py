@@ -22,6 +22,20 @@ def _rows(t: torch.Tensor) -> bool:
     return (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
 
 
+def _shared(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.untyped_storage()._cdata == b.untyped_storage()._cdata
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one type and shape, rows as above, share memory otherwise than row by row the same."""
+    (n, dim), row, at, to = a.shape, _row(a), a.storage_offset(), b.storage_offset()
+    if not _shared(a, b) or at + (n - 1) * row + dim <= to or to + (n - 1) * _row(b) + dim <= at:
+        return False
+    if row != _row(b):
+        return True
+    return at != to and (n == 1 or not dim <= (to - at) % row <= row - dim)   # (columns of one tensor lie between each other's rows)
+
+
 def _norm_into(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor | None, eps: float, flags: int, group: int,
                out: torch.Tensor, scale: torch.Tensor | None, out_residual: torch.Tensor | None) -> None:
     rows, dim = x.shape
@@ -81,17 +95,23 @@ def _call(what: str, x: torch.Tensor, residual: torch.Tensor | None, weight: tor
         if t is not None and t.numel() and not _rows(t):
             raise ValueError(f"{what}: an output's columns must lie side by side, got strides {t.stride()}")
     if f8 and out is not None and out.numel():
-        at = lambda t: t.untyped_storage().data_ptr()  # noqa: E731
-        if any(t is not None and at(t) == at(out) for t in (x, residual, weight, out_residual)):
+        if any(t is not None and _shared(t, out) for t in (x, residual, weight, out_residual)):
             raise ValueError(f"{what}: out in 8 bits is memory of its own")
+    both = [t for t in (out, out_residual) if t is not None and t.numel()]
+    if not f8 and len(both) == 2 and ((_shared(*both) and both[0].storage_offset() == both[1].storage_offset()) or _meet(*both)):
+        raise ValueError(f"{what}: out and out_residual share memory")
     new_out, new_residual = out is None, residual is not None and out_residual is None
     if new_out:
         out = torch.empty((rows, dim), dtype=F8 if f8 else x.dtype, device=x.device)
     if new_residual:
         out_residual = torch.empty((rows, dim), dtype=x.dtype, device=x.device)
     scale = torch.empty((rows, dim // group if group else 1), dtype=torch.float32, device=x.device) if f8 else None
-    # an input that a kernel cannot read as it is, or that overlaps an output of another layout, is copied
-    a, b = ((t if t is None or t.numel() == 0 or _rows(t) else t.clone(memory_format=torch.contiguous_format)) for t in (x, residual))
+    # an input that a kernel cannot read as it is, or that shares memory with an output of another layout, is copied
+    both = [t for t in both if t.dtype == x.dtype]
+    a, b = (t if t is None or t.numel() == 0 or (_rows(t) and not any(_meet(t, o) for o in both)) else
+            t.clone(memory_format=torch.contiguous_format) for t in (x, residual))
+    if weight is not None and any(_shared(weight, o) for o in both):
+        weight = weight.clone()
     args = (a, b, weight, float(eps), flags, int(group), out, scale, out_residual)
     if _direct(x, residual, weight, out, out_residual):
         _norm_into(*args)
@@ -119,7 +139,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
     """s = x + residual and its RMS norm, s rsqrt(mean(s ** 2) + eps) * weight, of rows x [rows, dim] (bf16 or fp16, any strides between rows,
     dim up to 32768).  ``weight`` [dim] of x's type or fp32 (``unit_offset``: 1 + weight; None: no weight); residual None: of x alone.  Sums are
     in 32 bits, the norm is of s before it is rounded.  Returns (normed rows, s), s None without a residual: new tensors, or ``out`` /
-    ``out_residual``, which may be x or residual themselves.  No backward pass."""
+    ``out_residual``, which may be x or residual themselves, but share no memory with each other.  No backward pass."""
     return _call("add_rms_norm", x, residual, weight, eps, unit_offset, False, 0, out, out_residual)
 
 

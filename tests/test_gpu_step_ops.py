@@ -1053,6 +1053,67 @@ def test_eight_bit_output_of_shared_memory_is_refused():
         gguf_hip.add_rms_norm_fp8(x, None, out=x.view(F8)[:, :256])
 
 
+def test_norm_outputs_that_share_memory():
+    """An output may be an input, lie between its rows, or reach over other rows of it; the outputs share nothing with each other."""
+    gen, dim = _gen(7), 192
+    buf, r, w = _randn(gen, 65, 2 * dim, dtype=BF), _randn(gen, 64, dim, dtype=BF), _randn(gen, dim, dtype=BF)
+    start = buf.clone()
+
+    def views(t):
+        return {"rows before": (t[1:, :dim], t[:-1, :dim]), "rows behind": (t[:-1, :dim], t[1:, :dim]), "columns": (t[1:, :dim], t[1:, dim:]),
+                "columns across": (t[:-1, dim // 2:dim // 2 + dim], t[:-1, :dim]), "the same": (t[:-1, :dim], t[:-1, :dim])}
+
+    for name in views(buf):
+        for as_residual in (False, True):
+            for to_residual in (False, True):
+                buf.copy_(start)
+                x, out = views(buf)[name]
+                a, b = (r, x) if as_residual else (x, r)
+                want, want_s = gguf_hip.add_rms_norm(a.clone(), b.clone(), w)
+                got = gguf_hip.add_rms_norm(a, b, w, **{"out_residual" if to_residual else "out": out})
+                assert _same(got, (want, want_s)), (name, as_residual, to_residual)
+                assert got[to_residual].data_ptr() == out.data_ptr()
+    for o, p in ((buf[1:, :dim], buf[1:, :dim]), (buf[1:, :dim], buf[:-1, :dim]), (buf[:-1, dim - 8:2 * dim - 8], buf[:-1, :dim])):
+        with pytest.raises(ValueError, match="share memory"):
+            gguf_hip.add_rms_norm(r, r, w, out=o, out_residual=p)
+    want = gguf_hip.add_rms_norm(r, r, w)
+    got = gguf_hip.add_rms_norm(r, r, w, out=buf[1:, :dim], out_residual=buf[1:, dim:])   # side by side
+    assert _same(got, want)
+    rows = r.clone()
+    want = gguf_hip.add_rms_norm(rows, r, rows[3].clone())
+    assert _same(gguf_hip.add_rms_norm(rows, r, rows[3], out=rows), want)
+
+
+def test_bounds_of_more_pages_than_a_grid_has_rows():
+    gen = _gen(8)
+    k = _randn(gen, 70, 1, 2, 64, dtype=BF)
+    table = torch.randint(0, 70, (2, 70_000), dtype=torch.int32, device="cuda", generator=gen)
+    bounds = torch.zeros((70, 2, 2, 64), dtype=BF, device="cuda")
+    gguf_hip.page_bounds(k, table, _i32([70_000, 3]), bounds, count=70_000)
+    assert torch.equal(bounds, k.expand(70, 2, 2, 64))
+
+
+def test_as_many_sequences_as_a_batch_holds():
+    """65535 sequences of a token each: tables, attention in both forms, and the choice of pages."""
+    gen, n = _gen(9), 65535
+    k, v = (_randn(gen, 40, 8, 1, 64, dtype=BF) for _ in range(2))
+    lists = torch.randint(0, 40, (50, 3), dtype=torch.int32, device="cuda", generator=gen)
+    request = torch.randint(0, 50, (n,), dtype=torch.int32, device="cuda", generator=gen)
+    old = torch.randint(0, 23, (n,), dtype=torch.int32, device="cuda", generator=gen)
+    t = gguf_hip.step_tables(lists, request, old, torch.ones_like(old), n, 8)
+    assert torch.equal(t.lengths, old + 1) and torch.equal(t.starts, torch.arange(n + 1, device="cuda", dtype=torch.int32))
+    assert torch.equal(t.sequences, t.starts[:-1]) and torch.equal(t.positions, old)
+    q = _randn(gen, n, 2, 64, dtype=BF)
+    one = gguf_hip.paged_attention(q, k, v, t.block_table, t.lengths)
+    many = gguf_hip.tree_attention(q, k, v, t.block_table, t.lengths, t.starts, max_tokens=1)
+    assert (one.float() - many.float()).abs().max() <= 2 * 2.0 ** -7 * v.abs().max()   # two roundings of weights and outputs each
+    bounds = gguf_hip.page_bounds(k, t.block_table, t.lengths, torch.zeros((40, 2, 1, 64), dtype=BF, device="cuda"), count=24)
+    table, lengths = gguf_hip.select_pages(q, bounds, t.block_table, t.lengths, 2, 8)
+    pages = (old + 8) // 8
+    assert torch.equal(table[:, 0, 0], t.block_table[:, 0])
+    assert torch.equal(lengths, torch.where(pages > 2, old + 1 - 8, old + 1))
+
+
 # ---- all together ----------------------------------------------------------------------------
 
 def test_draft_step_example():
