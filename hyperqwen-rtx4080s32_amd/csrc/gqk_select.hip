@@ -162,7 +162,7 @@ template <int LANES> __device__ __forceinline__ double lane_sum(double x) {
   return x;
 }
 
-// Eight dims of a page's bounds to a lane; products in 32 bits (exact: two factors of 16-bit types), sums in 64, as the comparison of near
+// Eight dims of a page's bounds to a lane; products in 32 bits (exact within their range, as both factors have 11 bits at most), sums in 64, as the comparison of near
 // equals decides which pages are read.  The 64-bit sums bound it in a batch: up to 500 pages of 48 sequences, 8 heads, 40 of queries (31 MB in 8
 // bits) 29 us; 2048 pages of one (8 MB) 7.  (Sums in 32 bits first, and those in 64 of the heads within their error of the largest alone: 29 and 10, as
 // the queries' norms, the registers that hold them and the second reading of a query cost what it saves.)
