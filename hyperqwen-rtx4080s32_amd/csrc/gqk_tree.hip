@@ -66,6 +66,15 @@ __device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t own, uint32_
 #endif
 }
 
+// The same from an address of each lane.
+template <bool ONCE>
+__device__ __forceinline__ void load_lanes_to_lds(const void* from, uint32_t to) {
+#ifdef __HIP_DEVICE_COMPILE__
+  if constexpr (ONCE) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(from), "s"(to) : "memory", "m0");
+  else asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+#endif
+}
+
 // A row tile: `rows` (token, query head) pairs of one sequence and key head, tokens outermost, from row row0 of the sequence's on.
 struct Tile {
   int b, start, tokens;   // the sequence, its first row of q, its new tokens
@@ -185,7 +194,7 @@ template <int DP> __device__ __forceinline__ int place_of(int key, int c) {
 // and a chunk's place in it the thread's own, so that nothing is computed per chunk.  16-bit pages then go to LDS directly.
 template <typename T, typename C, int DP, int KW, bool RUNS>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {
-  constexpr bool F8 = sizeof(C) == 1, DIRECT = RUNS && !F8;
+  constexpr bool F8 = sizeof(C) == 1, DIRECT = !F8;
   constexpr int KT = kStep;
   constexpr int RW = 4 / KW, ROWS = 32 * RW;
   constexpr int NM = DP / 16, ND = DP / 32, CPK = DP / 8;
@@ -239,6 +248,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   uint32_t top_page = 0;
   if (tid < KT / 32) odd[0][tid] = odd[1][tid] = odd[2][tid] = 0;
   if (tid == 0) wrong = 0;
+  if (DIRECT && !RUNS && D < DP)   // dims that no load brings
+    for (int x = tid * 16; x < 4 * TB; x += 256 * 16) *(v4u*)(lds + x) = v4u{0, 0, 0, 0};
   __syncthreads();
 
   // A step's keys come as runs of sixteen, NR to a wave; a load brings KPI keys of one, each lane 16 bytes of LDS: at place lane % CPK of
@@ -308,12 +319,27 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
       } else {
         Raw k{}, v{};
         const int d = dims_of(i % NI);
-        if (d < D) {
-          __builtin_memcpy(&k, __builtin_assume_aligned(kb + (int64_t)p * a.kv.k_page + (int64_t)place[i] * a.kv.k_token + d, sizeof(Raw)), sizeof(Raw));
-          __builtin_memcpy(&v, __builtin_assume_aligned(vb + (int64_t)p * a.kv.v_page + (int64_t)place[i] * a.kv.v_token + d, sizeof(Raw)), sizeof(Raw));
+        if (d < D) {   // (a lane that does not load does not write to LDS)
+          const C* const kp = kb + (int64_t)p * a.kv.k_page + (int64_t)place[i] * a.kv.k_token + d;
+          const C* const vp = vb + (int64_t)p * a.kv.v_page + (int64_t)place[i] * a.kv.v_token + d;
+          if constexpr (DIRECT) {
+            const uint32_t to = lds_at + buf * 2 * TB + at_of(i / NI, i % NI);
+            if (a.once) {
+              load_lanes_to_lds<true>(kp, to);
+              load_lanes_to_lds<true>(vp, to + TB);
+            } else {
+              load_lanes_to_lds<false>(kp, to);
+              load_lanes_to_lds<false>(vp, to + TB);
+            }
+          } else {
+            __builtin_memcpy(&k, __builtin_assume_aligned(kp, sizeof(Raw)), sizeof(Raw));
+            __builtin_memcpy(&v, __builtin_assume_aligned(vp, sizeof(Raw)), sizeof(Raw));
+          }
         }
-        kr[i] = k;
-        vr[i] = v;
+        if constexpr (!DIRECT) {
+          kr[i] = k;
+          vr[i] = v;
+        }
       }
     }
   };
