@@ -24,7 +24,8 @@ constexpr int kThreads = 256;
 
 // Sequence blockIdx.x, a part (blockIdx.y) of its table's columns and of its tokens; the sequence after the last is the rows without one.
 // Everything is in the trips to memory that follow one another: counts, the list, (the tree's parents,) the stores.  A workgroup adds up
-// the counts before its own by itself, which needs no second launch.
+// the counts before its own by itself, which needs no second launch.  32 trees of up to 16 tokens, tables of 256 pages: 4.8 us; 512 chunks of up to
+// 63, tables of 2048 (4.2 MB written): 5.3.  A call takes the host 10, half of it the seven or eight tensors that it returns.
 __global__ __launch_bounds__(kThreads) void tables_kernel(TablesArgs a) {
   __shared__ int64_t sums[kThreads / 64];
   __shared__ int32_t parent[GQK_MAX_TREE];

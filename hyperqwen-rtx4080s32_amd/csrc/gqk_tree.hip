@@ -183,16 +183,18 @@ template <int DP> __device__ __forceinline__ int place_of(int key, int c) {
 // Scores, statistics and sums are in 32 bits; the weights become T for the second product, as in the attention of single tokens.
 //
 // What bounds it (bf16, 40 heads over 8 of 128 dims).  Chunks of prompts, the matrix instructions and what the vector units do between them: 4096
-// tokens behind 4096, 516 GFLOP, 522 us, 988 TFLOP/s.  Trees, memory: 32 of up to 16 tokens behind up to 4000, 337 MB, 89 us, 3.8 TB/s, where loads
+// tokens behind 4096, 516 GFLOP, 530 us, 974 TFLOP/s.  Trees, memory: 32 of up to 16 tokens behind up to 4000, 337 MB, 84 us, 4.0 TB/s, where loads
 // without the products take as long (partial sums of two splits move another 43 MB); 64 of 4, 655 MB, 136 us, 4.8 TB/s.  8-bit pages are widened on
 // the way to LDS, in every workgroup that reads them: four trees of up to 61 tokens behind 32768, 197 MB, 93 GFLOP, 164 us.  Workgroups of eight
 // waves and 256 rows were slower (581 us for the chunk, when this took 540), and so were three steps on their way (584), steps of 32 keys
 // (640), and halves of steps with a wait each (no faster for trees, 573 for the chunk).  Shares of equal steps, dealt over the tiles from
 // what the lengths are, gave 172 us for the four trees and 107 for the windows of cut_of, and 16 for the smallest call in place of 11.
 //
-// RUNS: pages hold whole runs of the keys of one round of loads, and heads all dims: a run's page is one number for the whole workgroup,
-// and a chunk's place in it the thread's own, so that nothing is computed per chunk.  16-bit pages then go to LDS directly.
-template <typename T, typename C, int DP, int KW, bool RUNS>
+// RUNS: pages hold whole runs of the keys of one round of loads: a run's page is one number for the whole workgroup, and a chunk's place
+// in it the thread's own, so that nothing is computed per chunk (32 trees in pages of 16 tokens 84 us, of 7 137).  FULL: heads have all DP dims; else
+// those behind the last stay the zeros that LDS begins with (80 dims 88 us, addressed chunk by chunk 132).  16-bit pages go to LDS directly
+// (by way of registers: 197 and, of 7 tokens, 232).
+template <typename T, typename C, int DP, int KW, bool RUNS, bool FULL>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {
   constexpr bool F8 = sizeof(C) == 1, DIRECT = !F8;
   constexpr int KT = kStep;
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   if (!tile_at<ROWS>(a, slot, lane, t)) return;
   const int ns = splits_of(t.begin, t.end, a.chunk);
   if (split >= ns) return;
-  const int group = a.q_heads / a.kv.heads, D = RUNS ? DP : a.kv.dim;
+  const int group = a.q_heads / a.kv.heads, D = FULL ? DP : a.kv.dim;
   const int k_begin = t.begin + split * a.chunk, k_end = t.end > k_begin ? k_begin + min(a.chunk, t.end - k_begin) : k_begin;
   const int steps = (k_end - k_begin + KT - 1) / KT;
   const float inf = __builtin_huge_valf(), nan = __builtin_nanf("");
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   uint32_t top_page = 0;
   if (tid < KT / 32) odd[0][tid] = odd[1][tid] = odd[2][tid] = 0;
   if (tid == 0) wrong = 0;
-  if (DIRECT && !RUNS && D < DP)   // dims that no load brings
+  if (DIRECT && !FULL && D < DP)   // dims that no load brings
     for (int x = tid * 16; x < 4 * TB; x += 256 * 16) *(v4u*)(lds + x) = v4u{0, 0, 0, 0};
   __syncthreads();
 
@@ -302,6 +304,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
 #pragma unroll
           for (int j = 0; j < NI; ++j) {
             const uint32_t to = lds_at + buf * 2 * TB + at_of(i, j);
+            if (!FULL && dims_of(j) >= D) continue;   // (a lane that does not load does not write to LDS)
             load_to_lds<ONCE>((uint64_t)kp, k_own[j], to);
             load_to_lds<ONCE>((uint64_t)vp, v_own[j], to + TB);
           }
@@ -312,6 +315,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
         } else {
 #pragma unroll
           for (int j = 0; j < NI; ++j) {
+            kr[i * NI + j] = vr[i * NI + j] = Raw{};
+            if (!FULL && dims_of(j) >= D) continue;
             __builtin_memcpy(&kr[i * NI + j], __builtin_assume_aligned(kp + k_own[j], sizeof(Raw)), sizeof(Raw));
             __builtin_memcpy(&vr[i * NI + j], __builtin_assume_aligned(vp + v_own[j], sizeof(Raw)), sizeof(Raw));
           }
@@ -319,7 +324,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
       } else {
         Raw k{}, v{};
         const int d = dims_of(i % NI);
-        if (d < D) {   // (a lane that does not load does not write to LDS)
+        if (d < D) {
           const C* const kp = kb + (int64_t)p * a.kv.k_page + (int64_t)place[i] * a.kv.k_token + d;
           const C* const vp = vb + (int64_t)p * a.kv.v_page + (int64_t)place[i] * a.kv.v_token + d;
           if constexpr (DIRECT) {
@@ -655,18 +660,19 @@ Cut cut_of(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_to
   return c;
 }
 
-template <typename T, typename C, int DP, bool RUNS>
+template <typename T, typename C, int DP, bool RUNS, bool FULL>
 void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)c.slots * a.kv.heads), c.splits);
-  if (c.key_waves == 2) tree_kernel<T, C, DP, 2, RUNS><<<grid, 256, 0, st>>>(a);
-  else tree_kernel<T, C, DP, 1, RUNS><<<grid, 256, 0, st>>>(a);
+  if (c.key_waves == 2) tree_kernel<T, C, DP, 2, RUNS, FULL><<<grid, 256, 0, st>>>(a);
+  else tree_kernel<T, C, DP, 1, RUNS, FULL><<<grid, 256, 0, st>>>(a);
 }
 
 template <typename T, typename C, int DP>
 void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
   const int64_t page_bytes = (int64_t)a.kv.page_size * std::max(a.kv.k_token, a.kv.v_token) * (int64_t)sizeof(C);   // from its first key to the next's
-  if (a.kv.dim == DP && a.kv.page_size % 16 == 0 && page_bytes <= 0x7fffffff) launch<T, C, DP, true>(a, c, st);
-  else launch<T, C, DP, false>(a, c, st);
+  if (a.kv.page_size % 16 || page_bytes > 0x7fffffff) launch<T, C, DP, false, false>(a, c, st);
+  else if (a.kv.dim == DP) launch<T, C, DP, true, true>(a, c, st);
+  else launch<T, C, DP, true, false>(a, c, st);
 }
 
 template <typename T, typename C>
