@@ -634,7 +634,7 @@ struct Cut { int key_waves, rows, slots, splits, chunk; };
 // Where the tiles that a batch is likely to have are fewer than the workgroups that stay resident, their keys are split, into as many
 // splits as still stay all at once: a few more would run on their own at the end (24 sequences of a window of 4096 keys, heads of 256 dims: 2
 // splits 85.6 us, 3 111, 4 94; one of 100000 keys: 64 splits 89 us, 128 109; 16 of up to 8000 8-bit keys: 4 splits 68, 5 83).  Tiles of prompts see
-// different lengths, so that a tenth more than stay do not run on their own (two prompts of 320 and 512 tokens behind 8000: 2 splits 171 us, none 211).
+// different lengths, so that a tenth more than stay do not run on their own (320 and 512 tokens of two prompts behind 5000 and 8000: 2 splits 171 us, none 211).
 Cut cut_of(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_tokens, int max_length, int window, int64_t workspace_bytes) {
   const int group = q_heads / kv_heads;
   const int64_t most = (int64_t)std::min(tokens, max_tokens) * group;   // rows of a sequence

@@ -294,7 +294,8 @@ int gqk_step_tables(const int32_t* lists, int64_t list_row, int lists_n, int wid
  * GQK_ROPE_UNIT_OFFSET.  Arithmetic is in fp32, the norm that of s before it is rounded.  out_dtype: x's, or
  * GQK_DTYPE_FP8: out = the values divided by scale, which is fp32 [rows], or [rows, dim / group] with a group (a power of two from 32
  * to 512 that divides dim): the largest size of a value (2^-100 at least) / 448.  out, out_residual may be x, residual (whole, with their row strides);
- * out in 8 bits shares no memory with the inputs. */
+ * out in 8 bits shares no memory with the inputs,
+ * and the outputs none with each other. */
 #define GQK_NORM_MAX_DIM 32768
 int gqk_add_rms_norm(const void* x, int64_t x_row, const void* residual, int64_t residual_row, int dtype, int64_t rows, int dim,
                      const void* weight, int weight_dtype, float eps, int flags, void* out, int64_t out_row, int out_dtype, float* scale,
