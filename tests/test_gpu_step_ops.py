@@ -596,6 +596,39 @@ def test_tree_what_is_not_seen_does_not_matter(qt, ct, dim, kind):
     assert out[sees3].isnan().all()
 
 
+@pytest.mark.parametrize("dim", [8, 40, 72, 80, 96, 120, 136, 200, 248])
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("qt,ct", [(BF, BF), (F16, F16), (F16, F8)])
+@pytest.mark.parametrize("counts", [[3, 7, 1], [40, 9, 33]])
+def test_tree_dims_that_a_tile_does_not_fill(dim, page, qt, ct, counts):
+    """What an earlier call left in shared memory, infinities and NaN here, is nothing to the dims behind the last."""
+    q, k, v, table, lens, starts, _, _, _ = _tree_case(1, [600, 600, 600], counts, 8, 2, 256, 16, BF, BF, "chain")
+    k.fill_(INF)
+    v.fill_(NAN)
+    gguf_hip.tree_attention(q, k, v, table, lens, starts)
+    _tree_check(dim + page, [130, 0, 61], counts, 6, 2, dim, page, qt, ct, kind="any", scaled=ct == F8)
+
+
+@pytest.mark.parametrize("dim,page", [(80, 16), (80, 7), (128, 7), (200, 48), (248, 1), (256, 5)])
+@pytest.mark.parametrize("qt,ct", [(BF, BF), (F16, F16), (BF, F8)])
+def test_tree_not_seen_in_every_form(dim, page, qt, ct):
+    """Keys and values that are not finite, at places that only some tokens see, and a page outside of the cache."""
+    context, counts = [70, 3, 40], [50, 20, 4]
+    q, k, v, table, lens, starts, mask, _, _ = _tree_case(dim, context, counts, 6, 2, dim, page, qt, ct, "tree")
+    want, _, tol, _ = _attend_exact(q, k, v, table, context, counts, mask, dim ** -0.5, 0)
+    touched = torch.zeros(74, dtype=torch.bool, device="cuda")
+    for j, t in ((75, k), (99, v), (110, v)):
+        _bytes(t)[int(table[0, j // page]), j % page] = 0x7F if ct == F8 else NAN
+        touched[:50] |= _sees(mask, 0, 70, 50, 0)[:, j]
+    table = table.clone()
+    table[2, 40 // page] = k.shape[0]
+    for workspace in (None, torch.zeros(65536, dtype=torch.int32, device="cuda")):
+        out = gguf_hip.tree_attention(q, k, v, table, lens, starts, mask, workspace=workspace)
+        assert out[70:].isnan().any(2).all()
+        _within(out[:70][~touched[:70]], want[:70][~touched[:70]], tol[:70][~touched[:70]], "not seen")
+        assert touched.any() and out[touched].isnan().any(2).all()
+
+
 def test_tree_extreme_scores_and_scales():
     """Scores far apart, negative and zero scales, negative key scales, keys of score -inf."""
     context, counts = [150, 80], [9, 20]
