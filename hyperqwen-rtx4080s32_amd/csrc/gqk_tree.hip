@@ -382,11 +382,16 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
         if (base + key >= k_end) *k = *v = x;   // behind the last key: whatever there was
         else if (x = *v, put_aside(x, key, third)) *v = x;
       } else {
-        const bool there = !some || base + key < k_end;
-        *k = there ? wide(kr[i]) : x;
-        x = there ? wide(vr[i]) : x;
-        if (some) put_aside(x, key, third);
-        *v = x;
+        if (some) {
+          const bool there = base + key < k_end;
+          *k = there ? wide(kr[i]) : x;
+          x = there ? wide(vr[i]) : x;
+          put_aside(x, key, third);
+          *v = x;
+        } else {
+          *k = wide(kr[i]);
+          *v = wide(vr[i]);
+        }
       }
     }
   };
