@@ -185,9 +185,10 @@ template <int DP> __device__ __forceinline__ int place_of(int key, int c) {
 // What bounds it (bf16, 40 heads over 8 of 128 dims).  Chunks of prompts, the matrix instructions and what the vector units do between them: 4096
 // tokens behind 4096, 516 GFLOP, 530 us, 974 TFLOP/s.  Trees, memory: 32 of up to 16 tokens behind up to 4000, 337 MB, 84 us, 4.0 TB/s, where loads
 // without the products take as long (partial sums of two splits move another 43 MB); 64 of 4, 655 MB, 136 us, 4.8 TB/s.  8-bit pages are widened on
-// the way to LDS, in every workgroup that reads them: four trees of up to 61 tokens behind 32768, 197 MB, 93 GFLOP, 164 us.  Workgroups of eight
+// the way to LDS, in every workgroup that reads them: four trees of up to 61 tokens behind 32768, 197 MB, 93 GFLOP, 160 us.  Workgroups of eight
 // waves and 256 rows were slower (581 us for the chunk, when this took 540), and so were three steps on their way (584), steps of 32 keys
-// (640), and halves of steps with a wait each (no faster for trees, 573 for the chunk).  Shares of equal steps, dealt over the tiles from
+// (640), halves of steps with a wait each (no faster for trees, 573 for the chunk), and the next step's scores
+// among a step's exponentials (540 where this took 517).  Shares of equal steps, dealt over the tiles from
 // what the lengths are, gave 172 us for the four trees and 107 for the windows of cut_of, and 16 for the smallest call in place of 11.
 //
 // RUNS: pages hold whole runs of the keys of one round of loads: a run's page is one number for the whole workgroup, and a chunk's place
