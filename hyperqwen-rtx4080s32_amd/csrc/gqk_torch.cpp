@@ -229,6 +229,8 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* space;
   int64_t bytes;
   if (!workspace_of(ws, *q, &space, &bytes) || (out && (!like(*out, *q) || !heads_of(out, &oh)))) return none();
+  if (out && out->storage().data() == q->storage().data() && (out->data_ptr() != q->data_ptr() || out->strides() != q->strides()))
+    return none();   // q is copied
   Tensor made, lse;
   if (!out) {
     made = at::empty({tokens, heads, dim}, q->options());
@@ -269,10 +271,11 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
             !w->is_contiguous() || !same_device(*x, w)))
     return none();
   // outputs that share memory with another tensor, unless row by row the same as an input: the Python path looks
+  if (out && rout && out->storage().data() == rout->storage().data()) return none();
   for (const Tensor* o : {out, rout})
-    for (const Tensor* t : {x, r, w, rout})
-      if (o && t && o != t && o->storage().data() == t->storage().data() &&
-          (t == w || (o == out && t == rout) || o->data_ptr() != t->data_ptr() || (rows > 1 && o->stride(0) != t->stride(0))))
+    for (const Tensor* t : {x, r, w})
+      if (o && t && o->storage().data() == t->storage().data() &&
+          (t == w || o->data_ptr() != t->data_ptr() || (rows > 1 && o->stride(0) != t->stride(0))))
         return none();
   Tensor made, scale, made_r;
   if (!out) made = at::empty({rows, dim}, f8 ? x->options().dtype(at::kFloat8_e4m3fn) : x->options());

@@ -1109,12 +1109,29 @@ def test_norm_outputs_that_share_memory():
     for o, p in ((buf[1:, :dim], buf[1:, :dim]), (buf[1:, :dim], buf[:-1, :dim]), (buf[:-1, dim - 8:2 * dim - 8], buf[:-1, :dim])):
         with pytest.raises(ValueError, match="share memory"):
             gguf_hip.add_rms_norm(r, r, w, out=o, out_residual=p)
+    for o in (torch.empty_like(r), r):   # one tensor for both
+        with pytest.raises(ValueError, match="share memory"):
+            gguf_hip.add_rms_norm(r, r, w, out=o, out_residual=o)
     want = gguf_hip.add_rms_norm(r, r, w)
     got = gguf_hip.add_rms_norm(r, r, w, out=buf[1:, :dim], out_residual=buf[1:, dim:])   # side by side
     assert _same(got, want)
     rows = r.clone()
     want = gguf_hip.add_rms_norm(rows, r, rows[3].clone())
     assert _same(gguf_hip.add_rms_norm(rows, r, rows[3], out=rows), want)
+
+
+def test_tree_out_over_q():
+    """Into q itself, and into rows and heads of it that other tokens' q lie in."""
+    for counts in ([30, 1, 9], [3, 0, 2]):
+        q, k, v, table, lens, starts, mask, _, _ = _tree_case(3, [40, 9, 0], counts, 8, 2, 64, 16, BF, BF, "tree")
+        n = sum(counts)
+        buf = torch.zeros((n + 1, 16, 64), dtype=BF, device="cuda")
+        few = torch.zeros(64, dtype=torch.int32, device="cuda")   # holds no partial sums: one split
+        want = gguf_hip.tree_attention(q, k, v, table, lens, starts, mask, workspace=few)
+        for at, to in ((buf[:n, :8], buf[:n, :8]), (buf[:n, :8], buf[1:, :8]), (buf[1:, :8], buf[:n, :8]), (buf[:n, :8], buf[:n, 4:12])):
+            at.copy_(q)
+            got = gguf_hip.tree_attention(at, k, v, table, lens, starts, mask, out=to, workspace=few)
+            assert got is to and torch.equal(got, want)
 
 
 def test_bounds_of_more_pages_than_a_grid_has_rows():
