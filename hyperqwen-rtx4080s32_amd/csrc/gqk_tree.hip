@@ -491,20 +491,22 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
 #pragma unroll 1
           for (uint32_t rest = __builtin_amdgcn_readfirstlane(odd[third][kw * KB + b]); rest; rest &= rest - 1) {
             const int bit = __ffs(rest) - 1, key = first + b * 32 + bit, at = page_of(key);
+            const int from_page = table[at];
+            if ((uint32_t)from_page >= (uint32_t)a.kv.pages) continue;   // what was put aside is another page's, and the result NaN anyway
             const bool sees = seen_of(a, t, row, first + b * 32) >> bit & 1;
-            const C* from = vb + table[at] * a.kv.v_page + (int64_t)(key - at * ps) * a.kv.v_token;
+            const C* from = vb + from_page * a.kv.v_page + (int64_t)(key - at * ps) * a.kv.v_token;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int dim = d * 32 + 8 * j + 4 * hh;
-                const bool some = sees && dim < D;
+                if (!sees || dim >= D) continue;
                 C x[4];
-                __builtin_memcpy(x, __builtin_assume_aligned(from + (some ? dim : 0), 4 * sizeof(C)), 4 * sizeof(C));
+                __builtin_memcpy(x, __builtin_assume_aligned(from + dim, 4 * sizeof(C)), 4 * sizeof(C));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const float y = to_f(x[e]);
-                  acc[d][4 * j + e] += !some || y - y == 0.f ? 0.f : y;
+                  acc[d][4 * j + e] += y - y == 0.f ? 0.f : y;
                 }
               }
           }

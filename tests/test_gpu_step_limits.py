@@ -1,0 +1,55 @@
+"""The operators of steps of several new tokens and of long caches where a mask, a window, a table or a size ends, on the GPU: what a row sees reaches it
+whatever it holds, what no row sees is not looked at, no page outside of the cache is read.  Definitions in 64 bits and tolerances per value are
+those of test_gpu_step_ops.py."""
+import pytest
+import torch
+
+import gguf_hip
+from test_gpu_step_ops import BF, F8, F16, INF, NAN, _attend_exact, _bytes, _i32, _sees, _tree_case, _within
+
+pytestmark = pytest.mark.gpu
+
+# rows of a sequence and key head that one tile of 64 rows holds, whose keys two waves share, and that tiles of 128 rows hold
+FEW, MANY = [4, 9, 5], [50, 21, 30]
+
+
+def _behind_a_page(t, fill):
+    """The cache with another page in front of its first, in the same layout."""
+    first = torch.zeros_like(t[:1])
+    _bytes(first)[:] = fill
+    heads = t.stride(1) < t.stride(2)     # a head's tokens lie together
+    parts = [x.transpose(1, 2) if heads else x for x in (first, t)]
+    got = torch.cat([_bytes(x.contiguous()) for x in parts])
+    got = got.view(F8) if t.dtype == F8 else got
+    return got.transpose(1, 2) if heads else got
+
+
+@pytest.mark.parametrize("qt,ct", [(BF, BF), (F16, F16), (BF, F8)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (128, 7), (80, 16), (256, 48)])
+@pytest.mark.parametrize("counts", [FEW, MANY])
+@pytest.mark.parametrize("kind", ["tree", "chain"])
+def test_tree_bad_pages_where_the_first_page_is_not_finite(qt, ct, dim, page, counts, kind):
+    """A page outside of the cache gives NaN to those that see its keys and is not read, among the new tokens' keys, the last of the cache
+    and far from both, whatever the cache's first page holds (as one that was never written may)."""
+    context = [100, 230, 45]
+    q, k, v, table, lens, starts, mask, _, _ = _tree_case(dim + page, context, counts, 6, 2, dim, page, qt, ct, kind)
+    want, _, tol, _ = _attend_exact(q, k, v, table, context, counts, mask, dim ** -0.5, 0)
+    k, v = (_behind_a_page(t, 0x7F if ct == F8 else NAN) for t in (k, v))
+    assert _bytes(v[:1]).float().isnan().all() or ct == F8
+    sound = table + 1                                   # (the entries that no sequence uses become -2^31)
+    ends = [0, counts[0], counts[0] + counts[1], sum(counts)]
+    out = gguf_hip.tree_attention(q, k, v, sound, lens, starts, mask)
+    _within(out, want, tol, "sound")
+    for bad in (-1, 2 ** 30, 2 ** 31 - 1, k.shape[0], -2 ** 31):
+        for where in (3, context[1] - 1, context[1]):   # keys of the second sequence
+            table = sound.clone()
+            table[1, where // page] = bad
+            for window in (0, 200):
+                out = gguf_hip.tree_attention(q, k, v, table, lens, starts, mask, window=window)
+                sees = _sees(mask, ends[1], context[1], counts[1], window)
+                hit = sees[:, where // page * page:(where // page + 1) * page].any(1)
+                assert window or hit.any()
+                assert out[ends[1]:ends[2]][hit].isnan().all(), (bad, where, window)
+                if not window:
+                    for lo, hi in ((ends[0], ends[1]), (ends[2], ends[3])):
+                        _within(out[lo:hi], want[lo:hi], tol[lo:hi], "the sound ones")
