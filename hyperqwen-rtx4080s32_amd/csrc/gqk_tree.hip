@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
         for (int d = 0; d < ND; ++d) acc[d] *= f;
       }
       m = mn;
-      if (mixed(first, 32 * KB)) {
+      if (mixed(base, KT)) {   // (the step, as where they were put aside: this wave's keys may be seen by all rows)
         // the values that were put aside reach the rows that see them: as they are, whatever their weight
 #pragma unroll 1
         for (int b = 0; b < KB; ++b)

@@ -53,3 +53,34 @@ def test_tree_bad_pages_where_the_first_page_is_not_finite(qt, ct, dim, page, co
                 if not window:
                     for lo, hi in ((ends[0], ends[1]), (ends[2], ends[3])):
                         _within(out[lo:hi], want[lo:hi], tol[lo:hi], "the sound ones")
+
+
+@pytest.mark.parametrize("qt,ct,x", [(BF, BF, NAN), (F16, F16, INF), (BF, BF, -INF), (BF, F8, NAN), (F16, F8, NAN)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (128, 7), (256, 16), (80, 32)])
+@pytest.mark.parametrize("counts", [FEW, MANY])
+@pytest.mark.parametrize("kind", ["tree", "chain", "any"])
+@pytest.mark.parametrize("window", [0, 90])
+def test_tree_what_is_seen_counts_whatever_it_holds(qt, ct, x, dim, page, counts, kind, window):
+    """One value that is not finite makes that dim of its head not finite for every token that sees its key, and changes nothing else: keys of the
+    cache's last steps in either half of them, at the window's edge in either half, and the new tokens' own."""
+    context = [40, 185, 64]                             # 40 of 64, 57 of 64 and 0 of 64 keys in the step where the new ones begin
+    q, k, v, table, lens, starts, mask, _, _ = _tree_case(dim, context, counts, 6, 2, dim, page, qt, ct, kind)
+    want, _, tol, _ = _attend_exact(q, k, v, table, context, counts, mask, dim ** -0.5, window)
+    t0 = 0
+    for b, (m, n) in enumerate(zip(context, counts)):
+        sees = _sees(mask, t0, m, n, window)
+        for j in sorted({0, 5, 31, 32, 39, *range(m - window - 20, m - window + 45, 7), *range(m - 65, m + n, 9), m, m + n - 1}):
+            if not 0 <= j < m + n:
+                continue
+            h, d, at = j % 2, j * 5 % dim, int(table[b, j // page])
+            bad = v.clone()
+            if ct == F8:
+                _bytes(bad)[at, j % page, h, d] = 0x7F
+            else:
+                bad[at, j % page, h, d] = x
+            out = gguf_hip.tree_attention(q, k, bad, table, lens, starts, mask, window=window)
+            hit = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+            hit[t0:t0 + n, 3 * h:3 * h + 3, d] = sees[:, j, None]
+            assert not torch.isfinite(out[hit].float()).any(), (b, j)
+            _within(out[~hit], want[~hit], tol[~hit], (b, j))
+        t0 += n
