@@ -80,7 +80,7 @@ struct Tile {
   int b, start, tokens;   // the sequence, its first row of q, its new tokens
   int row0, rows;
   int context, length;    // keys before the new tokens', and with them
-  int begin, end;         // the keys that its rows can see lie in [begin, end)
+  int begin, end;         // the keys that its rows can see lie in [begin, end); begin is a multiple of 32
   bool bad;               // lengths or a mask that cannot be: NaN
 };
 
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   __shared__ __align__(1024) char lds[LDS];      // (addresses are made by xor: rows begin at multiples of their size)
   __shared__ float stat[4 * 32][2];
   __shared__ uint32_t odd[3][KT / 32];           // of three steps: keys with a value that is not finite
-  __shared__ int wrong;
+  __shared__ int wrong, lows[4];
   typedef __attribute__((address_space(3))) char* Lds;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -227,6 +227,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   const int own = rw * 32 + n;                   // of the tile's rows
   const bool live = own < t.rows;
   const Row row = row_of(a, t, t.row0 + (live ? own : 0));
+  // The first key that any of the rows sees: what lies behind all windows is not looked up, as a server may have given up its pages.
+  int low = a.window > 0 ? max(0, t.context + t.row0 / group + 1 - a.window) : 0;
+  if (a.mask && a.window > 0) {
+    low = row.first;
+    for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor(low, o));
+    if (lane == 0) lows[wave] = low;
+  }
   // scores of zero are those of queries of zero: a key that is not seen has -inf, which no factor may make NaN
   const float factor = a.scale * (a.kv.k_scale ? fabsf(a.kv.k_scale[kvh]) : 1.f), scale = factor == 0.f ? 1.f : factor;
   const uint32_t sign = a.sign ^ (a.kv.k_scale && a.kv.k_scale[kvh] < 0.f ? 0x80008000u : 0u);
@@ -254,6 +261,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   if (DIRECT && !FULL && D < DP)   // dims that no load brings
     for (int x = tid * 16; x < 4 * TB; x += 256 * 16) *(v4u*)(lds + x) = v4u{0, 0, 0, 0};
   __syncthreads();
+  if (a.mask && a.window > 0) low = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
+  low = __builtin_amdgcn_readfirstlane(low);
 
   // A step's keys come as runs of sixteen, NR to a wave; a load brings KPI keys of one, each lane 16 bytes of LDS: at place lane % CPK of
   // its key's row, where one chunk of dims lies (place_of is its own inverse).
@@ -273,10 +282,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a
   constexpr int PAGES = RUNS ? NR : NR * NI;
   int page[PAGES], place[PAGES];   // of the step that is fetched next: pages, and places in them
   const int last = max(0, k_end - 1);
-  auto look = [&](int base) {      // a key behind the last is read as the last one's page, and not used
+  auto look = [&](int base) {      // a key behind the last is read as the last one's page, one before the first as the first one's, and not used
 #pragma unroll
     for (int i = 0; i < PAGES; ++i) {
-      const int key = min(base + (RUNS ? key0 + i * RL : key_of(i / NI, i % NI)), RUNS ? last & ~(RL - 1) : last), at = page_of(key);
+      const int key = max(min(base + (RUNS ? key0 + i * RL : key_of(i / NI, i % NI)), RUNS ? last & ~(RL - 1) : last), RUNS ? low & ~(RL - 1) : low);
+      const int at = page_of(key);
       if constexpr (RUNS) page[i] = ((Uniform)table)[at];
       else page[i] = table[at];
       place[i] = key - at * ps;

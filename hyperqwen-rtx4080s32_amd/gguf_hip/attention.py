@@ -233,7 +233,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ``max_length``, ``max_tokens``: upper bounds on lengths and on a sequence's new tokens known to the host (default: what the table and q
     hold); the work is divided by them, so tight ones are faster.  A sequence above them, with fewer keys than new tokens, or with more of these
     than the mask has bits gets NaN; tokens whose keys lie in a page outside of the cache get NaN, and others of their
-    sequence may.  Rows of q that belong to no sequence are left as they were in ``out``, which may be q.  Returns out [tokens, query heads, dim], with
+    sequence may; entries of pages behind the windows of all of them are not looked at.  Rows of q that belong to no sequence are left as they were in ``out``, which may be q.  Returns out [tokens, query heads, dim], with
     ``return_lse`` also the log-sum-exp of the scores (fp32 [tokens, query heads], -inf without a key).  ``workspace``: as
     mul_mat_grouped's (its own for calls on concurrent streams).  No backward pass."""
     what = "tree_attention"

@@ -307,7 +307,8 @@ int gqk_add_rms_norm(const void* x, int64_t x_row, const void* residual, int64_t
  * ones, and of those the ones that its mask names: bit j % 32 of mask[starts[b] + i, j / 32] (int32 [tokens, mask_words]) is new token j; mask
  * NULL: new tokens 0 .. i.  window > 0: of the keys that it sees the last `window`.  No key: zeros, lse -inf.  A length above max_length or below the
  * sequence's new tokens, more of them than max_tokens or the mask's bits: NaN for the sequence; a page outside of the cache: NaN for the tokens whose
- * keys it would hold, and maybe for others of the sequence.  Values that are not finite at keys that a token does not see do not reach it.  Everything else as gqk_paged_attention (one launch, a second where
+ * keys it would hold, and maybe for others of the sequence; entries of pages that lie behind the windows of all the sequence's tokens are not looked
+ * at.  Values that are not finite at keys that a token does not see do not reach it.  Everything else as gqk_paged_attention (one launch, a second where
  * the keys are split). */
 #define GQK_MAX_TOKENS 1048576
 #define GQK_MAX_GROUP 1024 /* query heads of a key head */

@@ -84,3 +84,34 @@ def test_tree_what_is_seen_counts_whatever_it_holds(qt, ct, x, dim, page, counts
             assert not torch.isfinite(out[hit].float()).any(), (b, j)
             _within(out[~hit], want[~hit], tol[~hit], (b, j))
         t0 += n
+
+
+@pytest.mark.parametrize("qt,ct", [(BF, BF), (BF, F8)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 1), (128, 7), (128, 16), (80, 8), (80, 16), (256, 48), (64, 64), (256, 20)])
+@pytest.mark.parametrize("counts", [FEW, MANY])
+@pytest.mark.parametrize("kind", ["tree", "chain", "any"])
+def test_tree_pages_behind_the_window_may_be_given_up(qt, ct, dim, page, counts, kind):
+    """What no token of a sequence sees under the window is not looked up: entries outside of the cache there change nothing, in one split and in many.
+    The first page that a token does see is looked up: such an entry in its place gives it NaN."""
+    context = [700, 90, 1301]
+    q, k, v, table, lens, starts, mask, _, _ = _tree_case(dim + page, context, counts, 6, 2, dim, page, qt, ct, kind)
+    few = torch.zeros(64, dtype=torch.int32, device="cuda")   # holds no partial sums: one split
+    for window in (1, 2, 17, 33, 64, 200, 641):
+        want, _, tol, _ = _attend_exact(q, k, v, table, context, counts, mask, dim ** -0.5, window)
+        given_up, t0, ends = table.clone(), 0, []
+        for b, (m, n) in enumerate(zip(context, counts)):
+            sees = _sees(mask, t0, m, n, window)
+            first = int(sees.any(0).nonzero()[0])
+            given_up[b, :first // page] = torch.tensor([-1, 2 ** 30, k.shape[0]], device="cuda").to(torch.int32).repeat(first // page)[:first // page]
+            ends.append((t0, b, first // page, sees[:, :(first // page + 1) * page].any(1)))
+            t0 += n
+        for workspace in (None, few):
+            out = gguf_hip.tree_attention(q, k, v, given_up, lens, starts, mask, window=window, workspace=workspace)
+            _within(out, want, tol, window)
+            again = gguf_hip.tree_attention(q, k, v, table, lens, starts, mask, window=window, workspace=workspace)
+            assert torch.equal(out, again)
+        t0, b, at, hit = ends[2]
+        given_up[b, at] = -1
+        out = gguf_hip.tree_attention(q, k, v, given_up, lens, starts, mask, window=window)
+        assert out[t0:][hit].isnan().all() and hit.any()
+        _within(out[:t0], want[:t0], tol[:t0], "the other sequences")
