@@ -17,7 +17,7 @@ struct NormArgs {
   int64_t x_row, r_row, out_row, or_row;
   void *out, *out_r;
   float* scale;
-  int64_t rows;
+  int64_t rows, row0;   // row0: the launch's first
   int dim, group;       // group 0: the row
   int weight_f32, unit_offset;
   float eps;
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(TR) void add_norm_kernel(NormArgs a) {
   constexpr int W = TR / 64;   // waves of a row
   __shared__ float part[2][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.row0 + blockIdx.x;
   const int tid = threadIdx.x, dim = a.dim;
   const T* x = (const T*)a.x + row * a.x_row;
   const T* r = (const T*)a.r + row * a.r_row;
@@ -195,14 +195,19 @@ __global__ __launch_bounds__(TR) void add_norm_kernel(NormArgs a) {
   }
 }
 
+// A launch has fewer than 2^32 threads: more rows than that go in turns.
 template <typename T, typename O, int TR, bool STREAM>
-void launch(const NormArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.rows);
-  const int nc = (a.dim + 8 * TR - 1) / (8 * TR);
-  if (nc <= 1) add_norm_kernel<T, O, TR, 1, STREAM><<<grid, TR, 0, st>>>(a);
-  else if (nc == 2) add_norm_kernel<T, O, TR, 2, STREAM><<<grid, TR, 0, st>>>(a);
-  else if (nc == 3) add_norm_kernel<T, O, TR, 3, STREAM><<<grid, TR, 0, st>>>(a);
-  else add_norm_kernel<T, O, TR, 4, STREAM><<<grid, TR, 0, st>>>(a);
+void launch(const NormArgs& all, hipStream_t st) {
+  constexpr int64_t most = 0xffffffffll / TR;
+  const int nc = (all.dim + 8 * TR - 1) / (8 * TR);
+  NormArgs a = all;
+  for (; a.row0 < a.rows; a.row0 += most) {
+    const dim3 grid((unsigned)std::min(most, a.rows - a.row0));
+    if (nc <= 1) add_norm_kernel<T, O, TR, 1, STREAM><<<grid, TR, 0, st>>>(a);
+    else if (nc == 2) add_norm_kernel<T, O, TR, 2, STREAM><<<grid, TR, 0, st>>>(a);
+    else if (nc == 3) add_norm_kernel<T, O, TR, 3, STREAM><<<grid, TR, 0, st>>>(a);
+    else add_norm_kernel<T, O, TR, 4, STREAM><<<grid, TR, 0, st>>>(a);
+  }
 }
 
 // 1024 threads to a row where a thread of 256 would have more than four chunks of it, or in short batches more than one (512 rows of 5120: 8.0

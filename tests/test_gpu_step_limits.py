@@ -115,3 +115,17 @@ def test_tree_pages_behind_the_window_may_be_given_up(qt, ct, dim, page, counts,
         out = gguf_hip.tree_attention(q, k, v, given_up, lens, starts, mask, window=window)
         assert out[t0:][hit].isnan().all() and hit.any()
         _within(out[:t0], want[:t0], tol[:t0], "the other sequences")
+
+
+def test_norm_of_more_rows_than_a_launch_has_workgroups():
+    """2^24 and more rows, in 16 bits and in 8: the first, those about the limit and the last are their own batch's."""
+    rows, dim = (1 << 24) + 77, 8
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x, r = (torch.randint(-99, 100, (rows, dim), device="cuda", generator=gen, dtype=torch.int8).to(BF) for _ in range(2))
+    out, res = gguf_hip.add_rms_norm(x, r)
+    out8, scale, _ = gguf_hip.add_rms_norm_fp8(x, r)
+    for lo, hi in ((0, 500), ((1 << 24) - 300, (1 << 24) + 60), (rows - 20, rows), (5_000_000, 5_000_100)):
+        want, want_r = gguf_hip.add_rms_norm(x[lo:hi], r[lo:hi])
+        want8, want_s, _ = gguf_hip.add_rms_norm_fp8(x[lo:hi], r[lo:hi])
+        assert torch.equal(out[lo:hi], want) and torch.equal(res[lo:hi], want_r) and want.any()
+        assert torch.equal(_bytes(out8[lo:hi]), _bytes(want8)) and torch.equal(scale[lo:hi], want_s)
