@@ -15,6 +15,7 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 constexpr int kMostSplits = 256;
+constexpr int kMostGroups = 0xffffff;   // workgroups of 256 threads in a launch, whose threads are counted in 32 bits
 constexpr int kStep = 64;   // keys of a step
 
 struct TreeArgs {
@@ -671,7 +672,7 @@ Cut cut_of(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_to
   int64_t splits = std::max<int64_t>(1, std::min((one ? stay : stay + stay / 10) / tiles, (span + kStep - 1) / kStep));
   splits = std::min<int64_t>(splits, kMostSplits);
   const int64_t each = units * c.rows * (dim + 4) * 4;   // bytes of one split of all units
-  if (workspace_bytes < GQK_CTR_BYTES) splits = 1;
+  if (workspace_bytes < GQK_CTR_BYTES || units * (c.rows / 32) > kMostGroups) splits = 1;   // (the join has a workgroup for 32 rows at least)
   else splits = std::max<int64_t>(1, std::min(splits, (workspace_bytes - GQK_CTR_BYTES) / std::max<int64_t>(1, each)));
   c.chunk = (int)std::min<int64_t>(0x7fffff80, std::max<int64_t>(kStep, ((span + splits - 1) / splits + kStep - 1) / kStep * kStep));
   c.splits = (int)std::max<int64_t>(1, (span + c.chunk - 1) / c.chunk);
@@ -702,7 +703,7 @@ void launch(const TreeArgs& a, const Cut& c, hipStream_t st) {
 
 template <typename T, int ROWS>
 void join(const TreeArgs& a, const Cut& c, hipStream_t st) {
-  const int64_t eights = (int64_t)c.slots * a.kv.heads * (ROWS / 8);
+  const int64_t eights = (int64_t)c.slots * a.kv.heads * (ROWS / 8);   // (at most 4 kMostGroups, by the count of splits)
   if (eights > 8 * device_cus()) tree_join_kernel<T, ROWS, 32><<<dim3((unsigned)(eights / 4)), 256, 0, st>>>(a);
   else tree_join_kernel<T, ROWS, 8><<<dim3((unsigned)eights), 256, 0, st>>>(a);
 }
@@ -746,8 +747,9 @@ int gqk_tree_attention(const void* q, int64_t q_row, int64_t q_head, int dtype, 
     return decode_fail(GQK_ERR_SHAPE, "%s: q and out are 16-byte aligned with strides that are multiples of 8", what);
   const Cut c = cut_of(tokens, batch, q_heads, pages->heads, pages->dim, max_tokens, max_length, window, workspace ? workspace_bytes : 0);
   if ((uintptr_t)workspace & 255) return decode_fail(GQK_ERR_SHAPE, "%s: workspace is not 256-byte aligned", what);
-  if ((int64_t)c.slots * pages->heads * (c.rows / 8) > 0x7fffffff)
-    return decode_fail(GQK_ERR_SHAPE, "%s: %d tokens of %d heads are more than a launch takes", what, tokens, q_heads);
+  if ((int64_t)c.slots * pages->heads > kMostGroups)
+    return decode_fail(GQK_ERR_SHAPE, "%s: %d tokens of %d sequences, %d heads over %d are more than a launch takes", what, tokens, batch, q_heads,
+                       pages->heads);
   TreeArgs a{};
   a.q = q; a.q_row = q_row; a.q_head = q_head; a.kv = *pages; a.table = table; a.table_row = table_row; a.lengths = lengths; a.starts = starts;
   a.mask = mask; a.words = mask_words; a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.tokens = tokens; a.batch = batch;

@@ -309,7 +309,8 @@ int gqk_add_rms_norm(const void* x, int64_t x_row, const void* residual, int64_t
  * sequence's new tokens, more of them than max_tokens or the mask's bits: NaN for the sequence; a page outside of the cache: NaN for the tokens whose
  * keys it would hold, and maybe for others of the sequence; entries of pages that lie behind the windows of all the sequence's tokens are not looked
  * at.  Values that are not finite at keys that a token does not see do not reach it.  Everything else as gqk_paged_attention (one launch, a second where
- * the keys are split). */
+ * the keys are split).  Refused: tokens q_heads / 64 + batch heads of 2^24 or more (128 for 64 where a sequence may have more than 64 rows
+ * of a key head), which are more than a launch takes. */
 #define GQK_MAX_TOKENS 1048576
 #define GQK_MAX_GROUP 1024 /* query heads of a key head */
 int64_t gqk_tree_attention_workspace_bytes(int tokens, int batch, int q_heads, int kv_heads, int dim, int max_tokens, int max_length,
