@@ -53,7 +53,7 @@ struct BoundsArgs {
   int64_t table_row;
   const int32_t* lengths;
   void* bounds;
-  int pages, page_size, heads, dim, width, count;
+  int pages, page_size, heads, dim, width, count, page0;   // page0: of a sequence's, the launch's first
 };
 
 // A workgroup takes one page of one key head: its threads the page's keys, eight dims of one at a time.  Everything is in the trips to memory
@@ -65,8 +65,9 @@ __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
   __shared__ float ends[2][4][DP];
   const int b = blockIdx.y, h = blockIdx.z, len = a.lengths[b];
   if (len <= 0 || len > (int64_t)a.width * a.page_size) return;
-  const int first = max(0, len - a.count) / a.page_size, j = first + blockIdx.x;
-  if (j > (len - 1) / a.page_size) return;
+  const int64_t first = max(0, len - a.count) / a.page_size, at_page = first + a.page0 + blockIdx.x;
+  if (at_page > (len - 1) / a.page_size) return;
+  const int j = (int)at_page;
   const int page = a.table[(int64_t)b * a.table_row + j];
   if ((uint32_t)page >= (uint32_t)a.pages) return;
   const int keys = min(a.page_size, len - j * a.page_size);
@@ -417,10 +418,14 @@ int gqk_page_bounds(const gqk_pages* pages, const int32_t* table, int64_t table_
   a.dim = pages->dim; a.width = table_width; a.count = count;
   const int most = (int)std::min<int64_t>(table_width, ((int64_t)count + pages->page_size - 2) / pages->page_size + 1);
   const hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(most, batch, a.heads);
-  if (pages->dtype == GQK_DTYPE_FP8) bounds<fp8_t>(a, grid, st);
-  else if (pages->dtype == GQK_DTYPE_BF16) bounds<bf16_t>(a, grid, st);
-  else bounds<f16_t>(a, grid, st);
+  constexpr int turn = 0xffffff;   // pages of a launch, which has fewer than 2^32 threads
+  for (int64_t p0 = 0; p0 < most; p0 += turn) {
+    a.page0 = (int)p0;
+    const dim3 grid((unsigned)std::min<int64_t>(turn, most - p0), batch, a.heads);
+    if (pages->dtype == GQK_DTYPE_FP8) bounds<fp8_t>(a, grid, st);
+    else if (pages->dtype == GQK_DTYPE_BF16) bounds<bf16_t>(a, grid, st);
+    else bounds<f16_t>(a, grid, st);
+  }
   return decode_launched(what);
 }
 

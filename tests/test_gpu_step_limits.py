@@ -129,3 +129,17 @@ def test_norm_of_more_rows_than_a_launch_has_workgroups():
         want8, want_s, _ = gguf_hip.add_rms_norm_fp8(x[lo:hi], r[lo:hi])
         assert torch.equal(out[lo:hi], want) and torch.equal(res[lo:hi], want_r) and want.any()
         assert torch.equal(_bytes(out8[lo:hi]), _bytes(want8)) and torch.equal(scale[lo:hi], want_s)
+
+
+def test_bounds_of_more_pages_than_a_launch_has_workgroups():
+    """A sequence of 2^24 and more pages of one token: the first and the last of them too."""
+    n = (1 << 24) + 1000
+    k = torch.randn((90, 1, 1, 8), device="cuda", generator=torch.Generator(device="cuda").manual_seed(6)).to(BF)
+    table = torch.full((1, n), 7, dtype=torch.int32, device="cuda")
+    table[0, :10], table[0, -10:], table[0, (1 << 24) - 20:(1 << 24) + 20] = _i32(list(range(10, 20))), _i32(list(range(20, 30))), _i32(list(range(30, 70)))
+    bounds = torch.zeros((90, 2, 1, 8), dtype=BF, device="cuda")
+    gguf_hip.page_bounds(k, table, _i32([n]), bounds, count=n)
+    used = torch.tensor([7, *range(10, 70)], device="cuda")
+    assert torch.equal(bounds[used], k.expand(90, 2, 1, 8)[used])
+    bounds[used] = 0
+    assert not bounds.any()
