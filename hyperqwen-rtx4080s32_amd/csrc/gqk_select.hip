@@ -163,8 +163,8 @@ template <int LANES> __device__ __forceinline__ double lane_sum(double x) {
   return x;
 }
 
-// Eight dims of a page's bounds to a lane; products in 32 bits (exact within their range, as both factors have 11 bits at most), sums in 64, as the comparison of near
-// equals decides which pages are read.  The 64-bit sums bound it in a batch: up to 500 pages of 48 sequences, 8 heads, 40 of queries (31 MB in 8
+// Eight dims of a page's bounds to a lane; products (exact) and sums in 64 bits, as the comparison of near equals decides which pages are read.  (Products in
+// 32 bits are as exact within their range, which bf16's squares pass: a batch took 107 us with them where it takes 109.)  The 64-bit sums bound it in a batch: up to 500 pages of 48 sequences, 8 heads, 40 of queries (31 MB in 8
 // bits) 29 us; 2048 pages of one (8 MB) 7.  (Sums in 32 bits first, and those in 64 of the heads within their error of the largest alone: 29 and 10, as
 // the queries' norms, the registers that hold them and the second reading of a query cost what it saves.)
 template <typename T, typename C, int DP>
@@ -183,9 +183,12 @@ __global__ __launch_bounds__(256) void score_kernel(SelectArgs a) {
     const bool sound = (uint32_t)page < (uint32_t)a.pages;
     if (sound) {
       const C* from = (const C*)a.bounds + ((int64_t)page * 2 * a.heads + h) * a.dim + (live ? d : 0);
-      float lo[8], hi[8];
-      load8(from, lo);
-      load8(from + (int64_t)a.heads * a.dim, hi);
+      float lo32[8], hi32[8];
+      load8(from, lo32);
+      load8(from + (int64_t)a.heads * a.dim, hi32);
+      double lo[8], hi[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { lo[e] = lo32[e]; hi[e] = hi32[e]; }
       double best = -__builtin_huge_val();
       bool bad = false;
       for (int g = 0; g < a.group; ++g) {
@@ -193,7 +196,7 @@ __global__ __launch_bounds__(256) void score_kernel(SelectArgs a) {
         load8(q + g * a.q_head, x);
         double sum = 0.0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += (double)(x[e] * (x[e] >= 0.f ? hi[e] : lo[e]));
+        for (int e = 0; e < 8; ++e) sum = __builtin_fma((double)x[e], x[e] >= 0.f ? hi[e] : lo[e], sum);
         if (!live) sum = 0.0;
         sum = lane_sum<LPP>(sum);
         bad |= sum != sum;

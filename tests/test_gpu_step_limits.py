@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import gguf_hip
-from test_gpu_step_ops import BF, F8, F16, INF, NAN, _attend_exact, _bytes, _i32, _sees, _tree_case, _within
+from test_gpu_step_ops import BF, F8, F16, INF, NAN, _attend_exact, _bytes, _i32, _sees, _select_exact, _tree_case, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +143,17 @@ def test_bounds_of_more_pages_than_a_launch_has_workgroups():
     assert torch.equal(bounds[used], k.expand(90, 2, 1, 8)[used])
     bounds[used] = 0
     assert not bounds.any()
+
+
+@pytest.mark.parametrize("size", [2.0 ** 70, 2.0 ** -80])
+def test_select_scores_beyond_32_bits(size):
+    """Products that a 32-bit number cannot hold are told apart in 64 bits: of bounds and queries of a size whose square is above or below its range."""
+    pages, keep = 200, 12
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    k = (torch.randn((pages, 4, 2, 16), device="cuda", generator=gen) * size).to(BF)
+    q = (torch.randn((1, 4, 16), device="cuda", generator=gen) * size).to(BF)
+    table = torch.randperm(pages, device="cuda", generator=gen).to(torch.int32)[None]
+    bounds = gguf_hip.page_bounds(k, table, _i32([4 * pages]), torch.zeros((pages, 2, 2, 16), dtype=BF, device="cuda"), count=4 * pages)
+    got, kept = gguf_hip.select_pages(q, bounds, table, _i32([4 * pages]), keep, 4)
+    want, want_n = _select_exact(q, bounds, table, [4 * pages], keep, 4, 1, 1)
+    assert torch.equal(got.cpu(), want) and kept.tolist() == want_n
