@@ -26,14 +26,19 @@ def _shared(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.untyped_storage()._cdata == b.untyped_storage()._cdata
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether rows as above, of any two types, have bytes in common."""
+    n, own, other = a.shape[0], a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+    row, far = _row(a) * a.element_size(), _row(b) * b.element_size()
+    at, to = a.storage_offset() * a.element_size(), b.storage_offset() * b.element_size()
+    if not _shared(a, b) or at + (n - 1) * row + own <= to or to + (b.shape[0] - 1) * far + other <= at:
+        return False
+    return n == 1 or row != far or not own <= (to - at) % row <= row - other   # (columns of one tensor lie between each other's rows)
+
+
 def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors of one type and shape, rows as above, share memory otherwise than row by row the same."""
-    (n, dim), row, at, to = a.shape, _row(a), a.storage_offset(), b.storage_offset()
-    if not _shared(a, b) or at + (n - 1) * row + dim <= to or to + (n - 1) * _row(b) + dim <= at:
-        return False
-    if row != _row(b):
-        return True
-    return at != to and (n == 1 or not dim <= (to - at) % row <= row - dim)   # (columns of one tensor lie between each other's rows)
+    return (a.storage_offset(), _row(a)) != (b.storage_offset(), _row(b)) and _overlap(a, b)
 
 
 def _norm_into(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor | None, eps: float, flags: int, group: int,
@@ -95,7 +100,8 @@ def _call(what: str, x: torch.Tensor, residual: torch.Tensor | None, weight: tor
         if t is not None and t.numel() and not _rows(t):
             raise ValueError(f"{what}: an output's columns must lie side by side, got strides {t.stride()}")
     if f8 and out is not None and out.numel():
-        if any(t is not None and _shared(t, out) for t in (x, residual, weight, out_residual)):
+        # (an input that is not rows is copied before)
+        if any(t is not None and _rows(t) and _overlap(t, out) for t in (x, residual, None if weight is None else weight[None], out_residual)):
             raise ValueError(f"{what}: out in 8 bits is memory of its own")
     both = [t for t in (out, out_residual) if t is not None and t.numel()]
     if not f8 and len(both) == 2 and ((_shared(*both) and both[0].storage_offset() == both[1].storage_offset()) or _meet(*both)):
@@ -148,5 +154,5 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: tor
                      out_residual: torch.Tensor | None = None):
     """``add_rms_norm`` with the normed rows in float8_e4m3fn and their scales: (values, scales, s), values * scales being the rows.
     Scales are fp32 [rows, 1], or [rows, dim / group] for each ``group`` columns (a power of two from 32 to 512 that divides dim): the largest
-    size of a value (2 ** -100 at least) / 448.  ``out``: float8_e4m3fn [rows, dim], memory of its own.  No backward pass."""
+    size of a value (2 ** -100 at least) / 448.  ``out``: float8_e4m3fn [rows, dim], bytes of its own.  No backward pass."""
     return _call("add_rms_norm_fp8", x, residual, weight, eps, unit_offset, True, group, out, out_residual)

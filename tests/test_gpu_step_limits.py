@@ -157,3 +157,18 @@ def test_select_scores_beyond_32_bits(size):
     got, kept = gguf_hip.select_pages(q, bounds, table, _i32([4 * pages]), keep, 4)
     want, want_n = _select_exact(q, bounds, table, [4 * pages], keep, 4, 1, 1)
     assert torch.equal(got.cpu(), want) and kept.tolist() == want_n
+
+
+def test_eight_bit_output_beside_its_inputs():
+    """In the bytes behind each row of the input, and of the residual."""
+    buf = torch.randn((300, 200), device="cuda", generator=torch.Generator(device="cuda").manual_seed(8)).to(BF)
+    for lo in (0, 1):
+        x, out = buf[:, 64 * lo:64 * lo + 64], buf.view(F8)[:, 256:320]
+        before = buf.clone()
+        for kw in (dict(x=x, residual=None), dict(x=x, residual=buf[:, 160:200].repeat(1, 2)[:, :64]), dict(x=buf[:, :64].clone(), residual=x, out_residual=x)):
+            copies = {n: None if t is None else t.clone() for n, t in kw.items() if n != "out_residual"}
+            want, scale, res = gguf_hip.add_rms_norm_fp8(**copies)
+            got, scale2, res2 = gguf_hip.add_rms_norm_fp8(**kw, out=out)
+            assert got is out and torch.equal(_bytes(out), _bytes(want)) and torch.equal(scale, scale2)
+            assert res is None and res2 is None or torch.equal(res, res2)
+        assert torch.equal(buf[:, 160:], before[:, 160:]) and torch.equal(buf[:, 64 * (1 - lo):64 * (1 - lo) + 64], before[:, 64 * (1 - lo):64 * (1 - lo) + 64])
