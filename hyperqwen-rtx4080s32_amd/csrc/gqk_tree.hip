@@ -141,7 +141,7 @@ __device__ __forceinline__ Row row_of(const TreeArgs& a, const Tile& t, int row)
         r.first = t.context + w * 32 + __ffs(bits) - 1;
         left = 0;
       }
-      if (left > 0) r.first = max(0, t.context - left);
+      if (left > 0) r.first = t.context > 0 || left < a.window ? max(0, t.context - left) : t.length - 1;   // (the last: it sees none at all)
     }
   }
   return r;

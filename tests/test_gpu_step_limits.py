@@ -172,3 +172,24 @@ def test_eight_bit_output_beside_its_inputs():
             assert got is out and torch.equal(_bytes(out), _bytes(want)) and torch.equal(scale, scale2)
             assert res is None and res2 is None or torch.equal(res, res2)
         assert torch.equal(buf[:, 160:], before[:, 160:]) and torch.equal(buf[:, 64 * (1 - lo):64 * (1 - lo) + 64], before[:, 64 * (1 - lo):64 * (1 - lo) + 64])
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 4), (256, 7)])
+@pytest.mark.parametrize("counts", [[20], [90]])
+def test_tree_rows_that_see_nothing_hold_no_page(dim, page, counts):
+    """Without a cache a row whose mask is empty sees no key, and under the window the others see the last ones: the pages before them are not
+    looked up for its sake."""
+    n, window = counts[0], 3
+    q, k, v, table, lens, starts, mask, _, _ = _tree_case(dim, [0], counts, 6, 2, dim, page, BF, BF, "tree")
+    j = torch.arange(n, device="cuda")
+    mask[:] = 0
+    for i in range(n):                                   # the last three of the sequence, or nothing
+        if i % 3:
+            for bit in range(n - 3, n):
+                mask[i, bit // 32] |= 1 << bit % 32 if bit % 32 < 31 else -2 ** 31
+    want, _, tol, _ = _attend_exact(q, k, v, table, [0], counts, mask, dim ** -0.5, window)
+    table[0, :(n - 3) // page] = -1
+    assert (table[0] == -1).any()
+    out = gguf_hip.tree_attention(q, k, v, table, lens, starts, mask, window=window)
+    _within(out, want, tol, "out")
+    assert not out[j % 3 == 0].any() and out[j % 3 > 0].any()
