@@ -10,8 +10,6 @@
 namespace gqk {
 namespace {
 
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-
 struct NormArgs {
   const void *x, *r, *w;
   int64_t x_row, r_row, out_row, or_row;
@@ -82,8 +80,8 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x, int lanes) {
 __device__ __forceinline__ float top_of(uint32_t bits) { return __builtin_bit_cast(float, max(bits, 27u << 23)); }
 
 // TR threads take a row, eight columns of it at a time; a row stays in registers from its one load to its store.  One pass over the bytes,
-// which bound it: 8191 rows of 5120, 336 MB in 61 us (5.5 TB/s; with lines that stay in the caches 85, with a wave for a row 78 and 109);
-// 96 rows of 17408 8 us, of one row 3: a launch and three trips to memory.
+// which bound it: 8191 rows of 5120, 336 MB in 58 us (5.8 TB/s; with lines that stay in the caches 85, with a wave for a row 78 and 109),
+// to 8 bits 294 MB in 52 (5.7); 96 rows of 17408 8 us, of one row 3: a launch and three trips to memory.
 template <typename T, typename O, int TR, int NC, bool STREAM>
 __global__ __launch_bounds__(TR) void add_norm_kernel(NormArgs a) {
   constexpr bool F8 = sizeof(O) == 1;

@@ -11,8 +11,6 @@
 namespace gqk {
 namespace {
 
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-
 // x of eight values of a page
 __device__ __forceinline__ void load8(const bf16_t* p, float* x) {
   bf16_t v[8];
@@ -165,8 +163,8 @@ template <int LANES> __device__ __forceinline__ double lane_sum(double x) {
 
 // Eight dims of a page's bounds to a lane; products (exact) and sums in 64 bits, as the comparison of near equals decides which pages are read.  (Products in
 // 32 bits are as exact within their range, which bf16's squares pass: a batch took 107 us with them where it takes 109.)  The 64-bit sums bound it in a batch: up to 500 pages of 48 sequences, 8 heads, 40 of queries (31 MB in 8
-// bits) 29 us; 2048 pages of one (8 MB) 7.  (Sums in 32 bits first, and those in 64 of the heads within their error of the largest alone: 29 and 10, as
-// the queries' norms, the registers that hold them and the second reading of a query cost what it saves.)
+// bits) 31 us; 2048 pages of one (8 MB) 7.  (Sums in 32 bits first, and those in 64 of the heads within their error of the largest alone: 29 and 10 where this
+// took 29 and 7 with products in 32 bits, as the queries' norms, the registers that hold them and the second reading of a query cost what it saves.)
 template <typename T, typename C, int DP>
 __global__ __launch_bounds__(256) void score_kernel(SelectArgs a) {
   constexpr int LPP = DP / 8, PPW = 256 / LPP;   // lanes of a page, pages at once

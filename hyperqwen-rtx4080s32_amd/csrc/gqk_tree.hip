@@ -181,12 +181,14 @@ template <int DP> __device__ __forceinline__ int place_of(int key, int c) {
 // keys in any order, these are its operand as they are; V's operand comes transposed out of LDS in the same order.  Only the
 // maximum crosses lanes.
 //
-// Scores, statistics and sums are in 32 bits; the weights become T for the second product, as in the attention of single tokens.
+// Scores, statistics and sums are in 32 bits; the weights become T for the second product, as in the attention of single tokens, because the matrix
+// instructions of 32-bit operands run at a sixteenth of the rate (error against 64 bits 2.1e-3 in bf16 and 2.5e-4 in fp16, of which the result's own rounding
+// is 1.7e-3 and 2.1e-4).
 //
 // What bounds it (bf16, 40 heads over 8 of 128 dims).  Chunks of prompts, the matrix instructions and what the vector units do between them: 4096
-// tokens behind 4096, 516 GFLOP, 530 us, 974 TFLOP/s.  Trees, memory: 32 of up to 16 tokens behind up to 4000, 337 MB, 84 us, 4.0 TB/s, where loads
+// tokens behind 4096, 516 GFLOP, 524 to 552 us from one card to another, 930 to 980 TFLOP/s.  Trees, memory: 32 of up to 16 tokens behind up to 4000, 337 MB, 84 us, 4.0 TB/s, where loads
 // without the products take as long (partial sums of two splits move another 43 MB); 64 of 4, 655 MB, 136 us, 4.8 TB/s.  8-bit pages are widened on
-// the way to LDS, in every workgroup that reads them: four trees of up to 61 tokens behind 32768, 197 MB, 93 GFLOP, 160 us.  Workgroups of eight
+// the way to LDS, in every workgroup that reads them: four trees of up to 61 tokens behind 32768, 197 MB, 93 GFLOP, 158 us.  Workgroups of eight
 // waves and 256 rows were slower (581 us for the chunk, when this took 540), and so were three steps on their way (584), steps of 32 keys
 // (640), halves of steps with a wait each (no faster for trees, 573 for the chunk), and the next step's scores
 // among a step's exponentials (540 where this took 517).  Shares of equal steps, dealt over the tiles from
@@ -194,7 +196,7 @@ template <int DP> __device__ __forceinline__ int place_of(int key, int c) {
 //
 // RUNS: pages hold whole runs of the keys of one round of loads: a run's page is one number for the whole workgroup, and a chunk's place
 // in it the thread's own, so that nothing is computed per chunk (32 trees in pages of 16 tokens 84 us, of 7 137).  FULL: heads have all DP dims; else
-// those behind the last stay the zeros that LDS begins with (80 dims 88 us, addressed chunk by chunk 132).  16-bit pages go to LDS directly
+// those behind the last stay the zeros that LDS begins with (80 dims 85 us, addressed chunk by chunk 132).  16-bit pages go to LDS directly
 // (by way of registers: 197 and, of 7 tokens, 232).
 template <typename T, typename C, int DP, int KW, bool RUNS, bool FULL>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {

@@ -5,7 +5,7 @@ sequence's keys are cut into more than 16 splits, or heads that share one of key
 and can be captured in a HIP graph; under tracing they are custom ops with fakes.
 
 Layouts: heads are [tokens, heads, dim] views with any strides (column ranges of qkv's output as they are);
-pages are [pages, page_size, heads, dim] with any strides, so a cache may keep a token's heads or a head's tokens
+pages are [pages, page_size, heads, dim] with any strides that are multiples of 8, so a cache may keep a token's heads or a head's tokens
 together (the latter reads faster: a head's page is then one run of memory)."""
 from __future__ import annotations
 
@@ -233,9 +233,10 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ``max_length``, ``max_tokens``: upper bounds on lengths and on a sequence's new tokens known to the host (default: what the table and q
     hold); the work is divided by them, so tight ones are faster.  A sequence above them, with fewer keys than new tokens, or with more of these
     than the mask has bits gets NaN; tokens whose keys lie in a page outside of the cache get NaN, and others of their
-    sequence may; entries of pages behind the windows of all of them are not looked at.  Rows of q that belong to no sequence are left as they were in ``out``, which may be q.  Returns out [tokens, query heads, dim], with
-    ``return_lse`` also the log-sum-exp of the scores (fp32 [tokens, query heads], -inf without a key).  ``workspace``: as
-    mul_mat_grouped's (its own for calls on concurrent streams).  No backward pass."""
+    sequence may; entries of pages behind the windows of all of them are not looked at.  Rows of q that belong to no sequence are left as they
+    were in ``out``, which may be q.  Scores, softmax and sums are in 32 bits; the weights that multiply v are rounded to q's type.  Returns out
+    [tokens, query heads, dim], with ``return_lse`` also the log-sum-exp of the scores (fp32 [tokens, query heads], -inf without a key).
+    ``workspace``: as mul_mat_grouped's (its own for calls on concurrent streams).  No backward pass."""
     what = "tree_attention"
     if _fast is not None and _unwatched():
         got = _fast.tree_attention(q, k_pages, v_pages, block_table, lengths, starts, mask, scale, window, k_scale, v_scale, max_length,

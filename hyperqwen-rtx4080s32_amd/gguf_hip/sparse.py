@@ -50,7 +50,7 @@ def page_bounds(k_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch
                 count: int = 1) -> torch.Tensor:
     """Brings ``bounds`` up to date for the pages that hold each sequence's last ``count`` keys (the step's new ones): bounds[p, 0] and
     bounds[p, 1] [heads, dim] are the smallest and the largest of page p's keys of that sequence, exactly (NaN where one is).  k_pages [pages, page_size,
-    heads, dim] (bf16, fp16 or float8_e4m3fn, any strides), bounds [pages, 2, heads, dim] of its type, contiguous; block_table int32 [batch, pages] and
+    heads, dim] (bf16, fp16 or float8_e4m3fn, strides that are multiples of 8), bounds [pages, 2, heads, dim] of its type, contiguous; block_table int32 [batch, pages] and
     lengths int32 [batch] as paged_attention's.  Keys that were taken back are forgotten, as a page is read anew.  A page that
     several sequences hold must hold the same keys of each.  ``copy_pages`` on bounds follows a fork or a compaction.  Returns bounds."""
     what = "page_bounds"
